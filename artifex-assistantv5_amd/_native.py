@@ -63,6 +63,23 @@ SIGNATURES = {
     "gguf_hip_argmax_workspace": (_i64, []),
 }
 
+# Every symbol include/gguf_hip_kv4.h declares (the 4-bit KV cache)
+KV4_TILE, KV4_MAX_SLOTS, KV4_MAX_ROWS = 32, 1 << 20, 64
+KV4_WEIGHTS_NONE, KV4_WEIGHTS_STORE, KV4_WEIGHTS_ADD = 0, 1, 2
+KV4_SIGNATURES = {
+    "gguf_hip_kv4_bytes": (_i64, [_i32, _i32, _i32, _i64]),
+    "gguf_hip_kv4_append": (_i32, [_fp, _i64, _i64, _vp, _vp, _vp, _fp, _fp, _i64, _vp, _vp, _fp,
+                                   _i32, _i32, _i32, _i32, _i64, _vp]),
+    "gguf_hip_kv4_attention": (_i32, [_fp, _i64, _i32, _vp, _vp, _fp, _fp, _i64, _vp, _i32, _vp,
+                                      _fp, _i32, _fp, _i64, _i32, _i32, _i32, _i32, _i64, _vp,
+                                      _i64, _vp]),
+    "gguf_hip_kv4_attention_workspace": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i64]),
+    "gguf_hip_kv4_load": (_i32, [_vp, _vp, _fp, _fp, _i64, _i32, _i32, _i32, _i32, _i64, _vp]),
+    "gguf_hip_kv4_evict": (_i32, [_vp, _fp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _fp, _vp, _vp,
+                                  _i32, _i32, _i32, _i32, _i64, _vp, _i64, _vp]),
+    "gguf_hip_kv4_evict_workspace": (_i64, [_i32, _i32, _i32, _i32, _i64]),
+}
+
 
 class GGUFHipError(RuntimeError):
     """A HIP runtime or launch failure reported by the library."""
@@ -101,7 +118,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
             f"{p} is not built; run `python artifex-assistantv5_amd/build.py` "
             "(the GGUF HIP path has no CPU fallback)")
     lib = ctypes.CDLL(p, mode=ctypes.RTLD_GLOBAL)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **KV4_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

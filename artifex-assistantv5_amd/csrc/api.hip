@@ -9,7 +9,8 @@
 #include <stdio.h>
 
 #include "common.hpp"
-#include "gguf_hip.h"
+#include "gguf_hip_kv4.h"
+#include "kv4.hpp"
 
 namespace {
 
@@ -498,6 +499,191 @@ int gguf_hip_matmul(const void *x, int x_type, int64_t ldx, const void *tiles, i
                     int64_t n, int64_t k, float *y, int64_t ldy, int64_t m, void *stream) {
   return gguf_hip_matmul_variant(x, x_type, ldx, tiles, ggml_type, n, k, y, ldy, m,
                                  GGUF_HIP_VARIANT_AUTO, stream);
+}
+
+// ---------------------------------------------------------------------------
+// The 4-bit KV cache (gguf_hip_kv4.h).
+// ---------------------------------------------------------------------------
+namespace {
+
+int check_kv4(int n_layers, int n_seq, int n_kv_heads, int head_dim, int64_t slots) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] kv4: head_dim %d not 64, 128 or 256", head_dim);
+  if (slots <= 0 || slots > GGUF_HIP_KV4_MAX_SLOTS || slots % GGUF_HIP_KV4_TILE)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] kv4: slots %lld not a multiple of %d in 1..%d",
+                (long long)slots, GGUF_HIP_KV4_TILE, GGUF_HIP_KV4_MAX_SLOTS);
+  if (n_layers <= 0 || n_seq <= 0 || n_kv_heads <= 0 ||
+      (int64_t)n_layers * n_seq > 65535 / n_kv_heads)
+    return fail(GGUF_HIP_ERR_SHAPE,
+                "[gguf-hip] kv4: %d layers of %d sequences of %d KV heads (1..65535 lists)",
+                n_layers, n_seq, n_kv_heads);
+  return GGUF_HIP_OK;
+}
+
+int check_kv4_rows(int n_seq, int n_heads, int n_kv_heads, int head_dim, int64_t slots,
+                   int64_t ldqkv, int64_t rope_rows) {
+  const int rc = check_kv4(1, n_seq, n_kv_heads, head_dim, slots);
+  if (rc) return rc;
+  if (n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 8)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] kv4: n_heads %d must be 1..8 times n_kv_heads %d",
+                n_heads, n_kv_heads);
+  const int64_t row = (int64_t)(n_heads + 2 * n_kv_heads) * head_dim;
+  if (ldqkv < row || ldqkv % 4)
+    return fail(GGUF_HIP_ERR_SHAPE,
+                "[gguf-hip] kv4: ldqkv %lld must hold a row of %lld and be a multiple of 4",
+                (long long)ldqkv, (long long)row);
+  if (rope_rows <= 0 || rope_rows > ((int64_t)1 << 31) - 1)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] kv4: rope_rows %lld out of range",
+                (long long)rope_rows);
+  return GGUF_HIP_OK;
+}
+
+int check_kv4_rows_buffers(const float *qkv, const int64_t *lengths, const int64_t *pos,
+                           const float *cs, const float *sn, const void *kv,
+                           const int32_t *positions, const float *weights) {
+  if (!qkv || !lengths || !pos || !cs || !sn || !kv)
+    return fail(GGUF_HIP_ERR_NULL, "[gguf-hip] null pointer");
+  if (!aligned(qkv, 16) || !aligned(lengths, 8) || !aligned(pos, 8) || !aligned(cs, 16) ||
+      !aligned(sn, 16) || !aligned(kv, 16) || !aligned(positions, 4) || !aligned(weights, 4))
+    return fail(GGUF_HIP_ERR_ALIGN, "[gguf-hip] kv4 buffers misaligned");
+  return GGUF_HIP_OK;
+}
+
+}  // namespace
+
+int64_t gguf_hip_kv4_bytes(int n_seq, int n_kv_heads, int head_dim, int64_t slots) {
+  const int rc = check_kv4(1, n_seq, n_kv_heads, head_dim, slots);
+  if (rc) return rc;
+  ok();
+  return (int64_t)n_seq * n_kv_heads * (slots / GGUF_HIP_KV4_TILE) * 36 * head_dim;
+}
+
+int gguf_hip_kv4_append(const float *qkv, int64_t ldqkv, int64_t n_rows, const int64_t *starts,
+                        const int64_t *lengths, const int64_t *pos, const float *cos_table,
+                        const float *sin_table, int64_t rope_rows, void *kv, int32_t *positions,
+                        float *weights, int n_seq, int n_heads, int n_kv_heads, int head_dim,
+                        int64_t slots, void *stream) {
+  int rc = check_kv4_rows(n_seq, n_heads, n_kv_heads, head_dim, slots, ldqkv, rope_rows);
+  if (rc) return rc;
+  if (n_rows < 0 || n_rows > ((int64_t)1 << 31) / n_kv_heads)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] kv4_append: %lld rows out of range",
+                (long long)n_rows);
+  if (!starts && n_rows % n_seq)
+    return fail(GGUF_HIP_ERR_SHAPE,
+                "[gguf-hip] kv4_append: %lld rows are not the same number for each of %d sequences",
+                (long long)n_rows, n_seq);
+  if (n_rows == 0) return ok();
+  if ((rc = check_kv4_rows_buffers(qkv, lengths, pos, cos_table, sin_table, kv, positions, weights)))
+    return rc;
+  if (!aligned(starts, 8)) return fail(GGUF_HIP_ERR_ALIGN, "[gguf-hip] kv4 buffers misaligned");
+  const gguf::Kv4Cache c{(uint8_t *)kv, lengths,   pos,   cos_table, sin_table,  positions, weights,
+                         rope_rows,     n_seq,     n_heads, n_kv_heads, head_dim, (int)slots};
+  return hip_status(gguf::launch_kv4_append(c, qkv, ldqkv, n_rows, starts, (hipStream_t)stream),
+                    "kv4_append launch");
+}
+
+int64_t gguf_hip_kv4_attention_workspace(int rows, int weights_mode, int n_seq, int n_heads,
+                                         int n_kv_heads, int head_dim, int64_t slots) {
+  const int64_t row = (int64_t)(n_heads + 2 * (int64_t)n_kv_heads) * head_dim;
+  const int rc = check_kv4_rows(n_seq, n_heads, n_kv_heads, head_dim, slots, (row + 3) / 4 * 4, 1);
+  if (rc) return rc;
+  if (rows < 1 || rows > GGUF_HIP_KV4_MAX_ROWS)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] kv4_attention: %d rows per sequence not in 1..%d",
+                rows, GGUF_HIP_KV4_MAX_ROWS);
+  if (weights_mode < GGUF_HIP_KV4_WEIGHTS_NONE || weights_mode > GGUF_HIP_KV4_WEIGHTS_ADD)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] kv4_attention: unknown weights mode %d",
+                weights_mode);
+  ok();
+  return gguf::kv4_attention_work_bytes(rows, weights_mode != 0, n_seq, n_heads, n_kv_heads,
+                                        head_dim, (int)slots);
+}
+
+int gguf_hip_kv4_attention(const float *qkv, int64_t ldqkv, int rows, const int64_t *lengths,
+                           const int64_t *pos, const float *cos_table, const float *sin_table,
+                           int64_t rope_rows, void *kv, int store, int32_t *positions,
+                           float *weights, int weights_mode, float *out, int64_t ldo, int n_seq,
+                           int n_heads, int n_kv_heads, int head_dim, int64_t slots, void *work,
+                           int64_t work_bytes, void *stream) {
+  const int64_t need = gguf_hip_kv4_attention_workspace(rows, weights_mode, n_seq, n_heads,
+                                                        n_kv_heads, head_dim, slots);
+  if (need < 0) return (int)need;
+  int rc = check_kv4_rows(n_seq, n_heads, n_kv_heads, head_dim, slots, ldqkv, rope_rows);
+  if (rc) return rc;
+  if (ldo < (int64_t)n_heads * head_dim || ldo % 4)
+    return fail(GGUF_HIP_ERR_SHAPE,
+                "[gguf-hip] kv4_attention: ldo %lld must hold a row of %lld and be a multiple of 4",
+                (long long)ldo, (long long)n_heads * head_dim);
+  if ((rc = check_kv4_rows_buffers(qkv, lengths, pos, cos_table, sin_table, kv, positions, weights)))
+    return rc;
+  if (!out || !work || (weights_mode && !weights))
+    return fail(GGUF_HIP_ERR_NULL, "[gguf-hip] null pointer");
+  if (!aligned(out, 16) || !aligned(work, 16))
+    return fail(GGUF_HIP_ERR_ALIGN, "[gguf-hip] kv4 buffers misaligned");
+  if (work_bytes < need)
+    return fail(GGUF_HIP_ERR_BYTES, "[gguf-hip] kv4_attention: workspace of %lld bytes, needs %lld",
+                (long long)work_bytes, (long long)need);
+  const gguf::Kv4Cache c{(uint8_t *)kv, lengths,   pos,   cos_table, sin_table,  positions, weights,
+                         rope_rows,     n_seq,     n_heads, n_kv_heads, head_dim, (int)slots};
+  const gguf::Kv4Attn a{qkv, ldqkv, rows, store != 0, weights_mode, out, ldo, work};
+  return hip_status(gguf::launch_kv4_attention(c, a, (hipStream_t)stream), "kv4_attention launch");
+}
+
+int gguf_hip_kv4_load(const void *kv, const int64_t *lengths, float *k_out, float *v_out,
+                      int64_t out_slots, int n_layers, int n_seq, int n_kv_heads, int head_dim,
+                      int64_t slots, void *stream) {
+  const int rc = check_kv4(n_layers, n_seq, n_kv_heads, head_dim, slots);
+  if (rc) return rc;
+  if (out_slots < 0)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] kv4_load: out_slots %lld", (long long)out_slots);
+  if (out_slots == 0) return ok();
+  if (!kv || !lengths || !k_out || !v_out)
+    return fail(GGUF_HIP_ERR_NULL, "[gguf-hip] null pointer");
+  if (!aligned(kv, 16) || !aligned(lengths, 8) || !aligned(k_out, 16) || !aligned(v_out, 16))
+    return fail(GGUF_HIP_ERR_ALIGN, "[gguf-hip] kv4 buffers misaligned");
+  return hip_status(gguf::launch_kv4_load((const uint8_t *)kv, lengths, k_out, v_out, out_slots,
+                                          n_layers, n_seq, n_kv_heads, head_dim, (int)slots,
+                                          (hipStream_t)stream),
+                    "kv4_load launch");
+}
+
+int64_t gguf_hip_kv4_evict_workspace(int n_layers, int n_seq, int n_kv_heads, int head_dim,
+                                     int64_t slots) {
+  const int rc = check_kv4(n_layers, n_seq, n_kv_heads, head_dim, slots);
+  if (rc) return rc;
+  ok();
+  return gguf::kv4_evict_work_bytes((int64_t)n_layers * n_seq * n_kv_heads, (int)slots);
+}
+
+int gguf_hip_kv4_evict(void *kv, const float *weights, const int32_t *positions,
+                       const int64_t *lengths, const int64_t *pos, int64_t keep, int64_t trigger,
+                       int64_t recent, int64_t sinks, float *weights_out, int32_t *positions_out,
+                       int64_t *lengths_out, int n_layers, int n_seq, int n_kv_heads, int head_dim,
+                       int64_t slots, void *work, int64_t work_bytes, void *stream) {
+  const int64_t need =
+      gguf_hip_kv4_evict_workspace(n_layers, n_seq, n_kv_heads, head_dim, slots);
+  if (need < 0) return (int)need;
+  if (keep < 1 || keep > slots)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] kv4_evict: keep %lld not in 1..%lld slots",
+                (long long)keep, (long long)slots);
+  if (recent < 0 || sinks < 0 || recent > keep || sinks > keep - recent)
+    return fail(GGUF_HIP_ERR_SHAPE,
+                "[gguf-hip] kv4_evict: recent %lld and sinks %lld do not fit keep %lld",
+                (long long)recent, (long long)sinks, (long long)keep);
+  if (!kv || !weights || !positions || !lengths || !pos || !weights_out || !positions_out ||
+      !lengths_out || !work)
+    return fail(GGUF_HIP_ERR_NULL, "[gguf-hip] null pointer");
+  if (!aligned(kv, 16) || !aligned(weights, 4) || !aligned(positions, 4) || !aligned(lengths, 8) ||
+      !aligned(pos, 8) || !aligned(weights_out, 4) || !aligned(positions_out, 4) ||
+      !aligned(lengths_out, 8) || !aligned(work, 16))
+    return fail(GGUF_HIP_ERR_ALIGN, "[gguf-hip] kv4 buffers misaligned");
+  if (work_bytes < need)
+    return fail(GGUF_HIP_ERR_BYTES, "[gguf-hip] kv4_evict: workspace of %lld bytes, needs %lld",
+                (long long)work_bytes, (long long)need);
+  const gguf::Kv4Cache c{(uint8_t *)kv, lengths, pos,        nullptr,  nullptr,   nullptr, nullptr, 0,
+                         n_seq,         0,       n_kv_heads, head_dim, (int)slots};
+  const gguf::Kv4Evict e{keep,        trigger,       recent,      sinks, weights, positions,
+                         weights_out, positions_out, lengths_out, work,  n_layers};
+  return hip_status(gguf::launch_kv4_evict(c, e, (hipStream_t)stream), "kv4_evict launch");
 }
 
 }  // extern "C"
