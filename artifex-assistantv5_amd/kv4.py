@@ -23,6 +23,7 @@ from typing import Optional
 import torch
 
 from . import _native
+from .linear import _stream
 
 TILE = _native.KV4_TILE
 MAX_ROWS = _native.KV4_MAX_ROWS
@@ -90,6 +91,18 @@ def _common(qkv, lengths, pos, cos, sin, kv, n_heads, positions, weights):
             None if weights is None else _tensor("weights", weights, torch.float32, slot, dev))
 
 
+def _launch(fn, dev: torch.device, *args) -> None:
+    """``fn`` on the current stream of ``dev``, which need not be the current device."""
+    stream = _stream(dev)
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        _native.check(rc)
+
+
 def append(qkv: torch.Tensor, lengths: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor,
            sin: torch.Tensor, kv: torch.Tensor, n_heads: int,
            starts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
@@ -105,12 +118,9 @@ def append(qkv: torch.Tensor, lengths: torch.Tensor, pos: torch.Tensor, cos: tor
     n_seq, n_kv, hd, slots, ld, lp, pp, cp, sp, posp, wp = _common(
         qkv, lengths, pos, cos, sin, kv, n_heads, positions, weights)
     st = None if starts is None else _tensor("starts", starts, torch.int64, (n_seq + 1,), kv.device)
-    lib = _native.load_library()
-    with torch.cuda.device(kv.device):
-        _native.check(lib.gguf_hip_kv4_append(
-            qkv.data_ptr(), ld, qkv.shape[0], st, lp, pp, cp, sp, cos.shape[0], kv.data_ptr(), posp,
-            wp, n_seq, n_heads, n_kv, hd, slots,
-            torch.cuda.current_stream(kv.device).cuda_stream), lib)
+    _launch(_native.load_library().gguf_hip_kv4_append, kv.device, qkv.data_ptr(), ld,
+            qkv.shape[0], st, lp, pp, cp, sp, cos.shape[0], kv.data_ptr(), posp, wp, n_seq, n_heads,
+            n_kv, hd, slots)
     return kv
 
 
@@ -150,13 +160,10 @@ def attention(qkv: torch.Tensor, lengths: torch.Tensor, pos: torch.Tensor, cos: 
         raise ValueError("kv4: the workspace must be a contiguous tensor on the cache's device")
     mode = 0 if weights is None else (_native.KV4_WEIGHTS_ADD if accumulate
                                       else _native.KV4_WEIGHTS_STORE)
-    lib = _native.load_library()
-    with torch.cuda.device(kv.device):
-        _native.check(lib.gguf_hip_kv4_attention(
-            qkv.data_ptr(), ld, rows, lp, pp, cp, sp, cos.shape[0], kv.data_ptr(), int(store), posp,
-            wp, mode, out.data_ptr(), ldo, n_seq, n_heads, n_kv, hd, slots, work.data_ptr(),
-            work.numel() * work.element_size(),
-            torch.cuda.current_stream(kv.device).cuda_stream), lib)
+    _launch(_native.load_library().gguf_hip_kv4_attention, kv.device, qkv.data_ptr(), ld, rows,
+            lp, pp, cp, sp, cos.shape[0], kv.data_ptr(), int(store), posp, wp, mode, out.data_ptr(),
+            ldo, n_seq, n_heads, n_kv, hd, slots, work.data_ptr(),
+            work.numel() * work.element_size())
     return out
 
 
@@ -171,11 +178,8 @@ def load(kv: torch.Tensor, lengths: torch.Tensor, k_out: torch.Tensor,
     kp = _tensor("k_out", k_out, torch.float32, shape, kv.device)
     vp = _tensor("v_out", v_out, torch.float32, shape, kv.device)
     lp = _tensor("lengths", lengths, torch.int64, (n_seq,), kv.device)
-    lib = _native.load_library()
-    with torch.cuda.device(kv.device):
-        _native.check(lib.gguf_hip_kv4_load(kv.data_ptr(), lp, kp, vp, shape[-2], n_layers, n_seq,
-                                            n_kv, hd, slots,
-                                            torch.cuda.current_stream(kv.device).cuda_stream), lib)
+    _launch(_native.load_library().gguf_hip_kv4_load, kv.device, kv.data_ptr(), lp, kp, vp,
+            shape[-2], n_layers, n_seq, n_kv, hd, slots)
 
 
 def evict_workspace(kv: torch.Tensor) -> torch.Tensor:
@@ -215,9 +219,6 @@ def evict(kv: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor, leng
     lo = _tensor("lengths_out", lengths_out, torch.int64, (n_seq,), dev)
     if work.device != dev or not work.is_contiguous():
         raise ValueError("kv4: the workspace must be a contiguous tensor on the cache's device")
-    lib = _native.load_library()
-    with torch.cuda.device(dev):
-        _native.check(lib.gguf_hip_kv4_evict(
-            kv.data_ptr(), wp, pp, lp, np_, keep, keep + 1 if trigger is None else trigger, recent,
-            sinks, wo, po, lo, n_layers, n_seq, n_kv, hd, slots, work.data_ptr(),
-            work.numel() * work.element_size(), torch.cuda.current_stream(dev).cuda_stream), lib)
+    _launch(_native.load_library().gguf_hip_kv4_evict, kv.device, kv.data_ptr(), wp, pp, lp, np_,
+            keep, keep + 1 if trigger is None else trigger, recent, sinks, wo, po, lo, n_layers,
+            n_seq, n_kv, hd, slots, work.data_ptr(), work.numel() * work.element_size())
