@@ -8,24 +8,30 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------------------
-// Storing rows: a wave per (row, KV head, K or V).
+// Storing rows: a wave per row and KV head (K and V), four neighbouring rows per workgroup, which
+// mostly share the four slots that V's words hold, so that their bytes meet in one L2.  (A wave
+// per row, KV head and K or V, its row found with vector loads: 29 us for 3700 packed rows of
+// 8 heads of 128, five sequences.)
 // ---------------------------------------------------------------------------
 template <int HD>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
                                                               const float *__restrict__ qkv,
-                                                              int64_t ldq, int64_t n_rows,
+                                                              int64_t ldq, uint32_t n_rows,
                                                               const int64_t *__restrict__ starts) {
-  const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  const int64_t r = unit / (2 * c.nkv);
+  const int lane = threadIdx.x & 63, h = blockIdx.y;
+  const uint32_t r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   if (r >= n_rows) return;
-  const int hv = (int)(unit - r * 2 * c.nkv), h = hv >> 1;
-  int64_t s, i;
+  const float *x = qkv + r * ldq + (int64_t)(c.nh + h) * HD;
+  Kv4Row<HD> k, v;
+  k.load(x, lane);
+  v.load(x + (int64_t)c.nkv * HD, lane);
+  uint32_t s;
+  int64_t i;
   if (starts) {
     if (r < starts[0] || r >= starts[c.n_seq]) return;
-    int lo = 0, hi = c.n_seq;  // starts[lo] <= r < starts[hi]
+    uint32_t lo = 0, hi = c.n_seq;  // starts[lo] <= r < starts[hi]
     while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
+      const uint32_t mid = (lo + hi) >> 1;
       if (starts[mid] <= r)
         lo = mid;
       else
@@ -34,23 +40,20 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
     s = lo;
     i = r - starts[lo];
   } else {
-    const int64_t per = n_rows / c.n_seq;
+    const uint32_t per = n_rows / (uint32_t)c.n_seq;
     s = r / per;
     i = r - s * per;
   }
   const int64_t slot = c.lengths[s] + i, p = c.pos[s] + i;
   if (slot < 0 || slot >= c.slots || p < 0 || p >= c.rope_rows) return;
-  const int64_t list = s * c.nkv + h;
+  k.load_turn(c.cs + p * (HD / 2), c.sn + p * (HD / 2), lane);
+  const int64_t list = (int64_t)s * c.nkv + h;
   uint8_t *base = kv4_list(c.kv, list, c.slots, Kv4<HD>::TB);
-  const float *x = qkv + r * ldq + (int64_t)(c.nh + (hv & 1) * c.nkv + h) * HD;
-  if (hv & 1) {
-    kv4_store_row<HD, false>(base, (int)slot, x, nullptr, nullptr, lane);
-    if (lane == 0) {
-      if (c.positions) c.positions[list * c.slots + slot] = (int32_t)p;
-      if (c.weights) c.weights[list * c.slots + slot] = 0.f;
-    }
-  } else {
-    kv4_store_row<HD, true>(base, (int)slot, x, c.cs + p * (HD / 2), c.sn + p * (HD / 2), lane);
+  kv4_put_row<HD, false>(base, (int)slot, v, lane);
+  kv4_put_row<HD, true>(base, (int)slot, k, lane);
+  if (lane == 0) {
+    if (c.positions) c.positions[list * c.slots + slot] = (int32_t)p;
+    if (c.weights) c.weights[list * c.slots + slot] = 0.f;
   }
 }
 
@@ -111,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void kv4_load_kernel(const uint8_t *__res
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 
 // The order of the slots: larger is kept first.  NaN is 0, -0 equals +0.
-__device__ __forceinline__ uint32_t evict_key(float w, int32_t p, int64_t from, int64_t sinks) {
+__device__ __forceinline__ uint32_t evict_key(float w, int32_t p, int32_t from, int32_t sinks) {
   if (p >= from || p < sinks) w = INFINITY;
   if (!(w == w)) return 0u;
   const uint32_t u = __float_as_uint(w + 0.f);
@@ -124,30 +127,51 @@ __device__ __forceinline__ int32_t *evict_holes(void *work, int64_t lists, int64
   return (int32_t *)work + (lists + 3) / 4 * 4 + list * 2 * half;
 }
 
-// Sum over the workgroup of one bit per thread below this thread; `all` gets the total.
-__device__ __forceinline__ int block_rank(bool bit, int *part, int &all) {
+// The sum of v over the threads below this one, and over all of them.
+__device__ __forceinline__ int block_before(int v, int *part, int &all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint64_t m = __ballot(bit);
-  __syncthreads();
-  if (lane == 0) part[wave] = __popcll(m);
-  __syncthreads();
-  int before = 0;
-  all = 0;
-  for (int w = 0; w < kSelWaves; ++w) {
-    before += w < wave ? part[w] : 0;
-    all += part[w];
+  int run = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(run, o);
+    if (lane >= o) run += x;
   }
-  return before + __popcll(m & ((1ull << lane) - 1ull));
+  __syncthreads();  // the last use of `part` is over
+  if (lane == 63) part[wave] = run;
+  __syncthreads();
+  int x = part[lane & (kSelWaves - 1)];
+#pragma unroll
+  for (int o = 1; o < kSelWaves; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if ((lane & (kSelWaves - 1)) >= o) x += y;
+  }
+  all = __shfl(x, kSelWaves - 1);
+  return run - v + (wave ? __shfl(x, wave - 1) : 0);
 }
 
-// One workgroup per list: the keep-th largest key by four 8-bit digits (a histogram each),
-// then one pass in slot order that writes the lists.
+// The same number, not known to be: what is computed from it is computed where it is used, and
+// not kept for all the turns of an unrolled loop.
+__device__ __forceinline__ int again(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// One workgroup per list; thread t holds the keys of slots t, t + 1024, ... (KPT of them; a
+// longer list is read again, segment by segment, for every pass).
+// - The keep-th largest key by digits of 11, 11 and 10 bits: a histogram in LDS (four copies
+//   for the first digit, where most keys share a few bins), then a scan from the top.
+// - The ranks within a list need the counts of all waves' turns before one's own: every wave
+//   leaves the count of each turn, and one scan of the workgroup over them gives all ranks.
+// Bound: latency of these passes; 16000 slots are read in 3 us and take ten barriers.
+template <int KPT>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, Kv4Evict e, int half) {
-  __shared__ int hist[256], part[kSelWaves], found[2];
+  constexpr int kBins = 2048, kSeg = KPT * kSelThreads;
+  __shared__ int hist[4][kBins], cnt[2][KPT * kSelWaves], part[kSelWaves], found[2];
   const int64_t list = blockIdx.x, lists = gridDim.x;
   const int64_t s = list / c.nkv % c.n_seq;
   const int64_t n64 = c.lengths[s];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint64_t below = (1ull << lane) - 1ull;
   int32_t *count = (int32_t *)e.work + list;
   const float *w = e.weights + list * c.slots;
   const int32_t *p = e.positions + list * c.slots;
@@ -163,75 +187,149 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
     }
     return;
   }
-  const int64_t from = c.pos[s] - e.recent;
+  // positions are below 2^31 - 1 (the tables' rows)
+  const int64_t from64 = c.pos[s] - e.recent;
+  const int32_t from = (int32_t)(from64 < -1 ? -1 : (from64 > INT32_MAX ? INT32_MAX : from64));
+  const int32_t sinks = (int32_t)e.sinks;
+  uint32_t key[KPT];
+  int held = -1;  // the segment in `key`
+  auto read = [&](int s0) {
+    if (held == s0) return;
+    held = s0;
+    const int tid = again(threadIdx.x);
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) {
+      const float *wk = w + s0 + k * kSelThreads;  // uniform
+      const int32_t *pk = p + s0 + k * kSelThreads;
+      key[k] = s0 + k * kSelThreads + tid < n ? evict_key(wk[tid], pk[tid], from, sinks) : 0u;
+      if (k % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // 16 loads in flight are enough
+    }
+  };
   uint32_t prefix = 0;
   int need = keep;  // of the keys that share the prefix, this many stay
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kSelThreads) {
-      const uint32_t k = evict_key(w[i], p[i], from, e.sinks);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&hist[(k >> shift) & 255u], 1);
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < kBins; i += kSelThreads) {
+      hist[0][i] = 0;
+      if (pass == 0) hist[1][i] = hist[2][i] = hist[3][i] = 0;
     }
     __syncthreads();
-    if (tid < 64) {  // the digit: from the top, the first whose running count reaches `need`
-      int h[4], sum = 0;
+    for (int s0 = 0; s0 < n; s0 += kSeg) {
+      read(s0);
+      const int tid = again(threadIdx.x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += h[i] = hist[255 - (4 * tid + i)];
-      int run = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(run, o);
-        if (tid >= o) run += v;
+      for (int k = 0; k < KPT; ++k) {
+        if (s0 + k * kSelThreads >= n) break;
+        const bool in = s0 + k * kSelThreads + tid < n &&
+                        (pass == 0 || (key[k] >> (shift + bits)) == (prefix >> (shift + bits)));
+        if (in) atomicAdd(&hist[pass == 0 ? wave & 3 : 0][(key[k] >> shift) & (kBins - 1) &
+                                                          ((1u << bits) - 1u)], 1);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      int before = run - sum;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (before < need && before + h[i] >= need) {
-          found[0] = 255 - (4 * tid + i);
-          found[1] = need - before;
-        }
-        before += h[i];
-      }
+    }
+    __syncthreads();
+    // bins from the top, two per thread: the first whose running count reaches `need`
+    const int b0 = kBins - 1 - 2 * tid;
+    int h0 = hist[0][b0], h1 = hist[0][b0 - 1];
+    if (pass == 0) {
+      h0 += hist[1][b0] + hist[2][b0] + hist[3][b0];
+      h1 += hist[1][b0 - 1] + hist[2][b0 - 1] + hist[3][b0 - 1];
+    }
+    int all;
+    const int before = block_before(h0 + h1, part, all);
+    if (before < need && before + h0 >= need) {
+      found[0] = b0;
+      found[1] = need - before;
+    } else if (before + h0 < need && before + h0 + h1 >= need) {
+      found[0] = b0 - 1;
+      found[1] = need - before - h0;
     }
     __syncthreads();
     prefix |= (uint32_t)found[0] << shift;
     need = found[1];
-    __syncthreads();
   }
   int32_t *holes = evict_holes(e.work, lists, list, half), *late = holes + half;
-  int ties = 0, nh = 0, nl = 0;
-  for (int i0 = 0; i0 < n; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    const bool in = i < n;
-    const float wi = in ? w[i] : 0.f;
-    const int32_t pi = in ? p[i] : 0;
-    const uint32_t k = in ? evict_key(wi, pi, from, e.sinks) : 0u;
-    int all;
-    const int rank = ties + block_rank(in && k == prefix, part, all);
-    ties += all;
-    const bool stays = in && (k > prefix || (k == prefix && rank < need));
-    const bool hole = in && !stays && i < keep, moves = stays && i >= keep;
-    const int hr = nh + block_rank(hole, part, all);
-    nh += all;
-    if (hole) holes[hr] = i;
-    const int lr = nl + block_rank(moves, part, all);
-    nl += all;
-    if (moves) late[lr] = i;
-    if (stays && i < keep) {
-      if (wo != w) wo[i] = wi;
-      if (po != p) po[i] = pi;
+  int ties = 0, nh = 0, nl = 0;  // of the segments before
+  for (int s0 = 0; s0 < n; s0 += kSeg) {
+    read(s0);
+    uint64_t stays = 0;
+    int t = again(tid);
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) {
+      const uint64_t m = __ballot(s0 + k * kSelThreads + t < n && key[k] == prefix);
+      if (lane == 0) cnt[0][k * kSelWaves + wave] = __popcll(m);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    __syncthreads();
+    int all;
+    {
+      const int v = tid < KPT * kSelWaves ? cnt[0][tid] : 0;
+      const int b = block_before(v, part, all);
+      if (tid < KPT * kSelWaves) cnt[0][tid] = ties + b;
+      ties += all;
+    }
+    __syncthreads();
+    t = again(tid);
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) {
+      const bool in = s0 + k * kSelThreads + t < n, tie = in && key[k] == prefix;
+      const uint64_t m = __ballot(tie);
+      const bool st = in && (key[k] > prefix ||
+                             (tie && cnt[0][k * kSelWaves + wave] + __popcll(m & below) < need));
+      stays |= (uint64_t)st << k;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+    t = again(tid);
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) {
+      const int i = s0 + k * kSelThreads + t;
+      const bool st = (stays >> k) & 1u;
+      const uint64_t mh = __ballot(i < keep && !st), mm = __ballot(i >= keep && st);
+      if (lane == 0) {
+        cnt[0][k * kSelWaves + wave] = __popcll(mh);
+        cnt[1][k * kSelWaves + wave] = __popcll(mm);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int v = tid < KPT * kSelWaves ? cnt[j][tid] : 0;
+      const int b = block_before(v, part, all);
+      if (tid < KPT * kSelWaves) cnt[j][tid] = (j ? nl : nh) + b;
+      (j ? nl : nh) += all;
+    }
+    __syncthreads();
+    t = again(tid);
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) {
+      if (s0 + k * kSelThreads >= n) break;
+      const int i = s0 + k * kSelThreads + t;  // keep < n: every hole is in use
+      const bool st = (stays >> k) & 1u, hole = i < keep && !st, moves = i >= keep && st;
+      const uint64_t mh = __ballot(hole), mm = __ballot(moves);
+      if (hole) holes[cnt[0][k * kSelWaves + wave] + __popcll(mh & below)] = i;
+      if (moves) late[cnt[1][k * kSelWaves + wave] + __popcll(mm & below)] = i;
+      if (i < keep && st) {
+        if (wo != w) wo[i] = w[i];
+        if (po != p) po[i] = p[i];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
   }
   if (tid == 0) *count = nl;
 }
 
-// One wave per move: the bytes of slot `late[i]` to slot `holes[i]`.
+// A wave takes 16 moves at a time, slot late[i] to slot holes[i]: all their loads are issued
+// before the first store (a slot from `keep` on is never written, so the order of the waves
+// does not matter).  V's bytes are four apart, a lane takes one; K goes in 16 bytes a lane.
 template <int HD>
 __global__ __launch_bounds__(kThreads) void evict_move_kernel(Kv4Cache c, Kv4Evict e, int half) {
   using L = Kv4<HD>;
-  constexpr int NB = L::NB;
+  constexpr int NB = L::NB, M = 16;
+  constexpr int VN = M * HD / 2 / 64, KN = (M * NB + 63) / 64, SN = M * 2 * NB / 64;
   const int64_t list = blockIdx.y, lists = gridDim.y;
   const int lane = threadIdx.x & 63;
   if (blockIdx.x == 0 && threadIdx.x == 0 && list < (int64_t)c.n_seq * c.nkv && list % c.nkv == 0) {
@@ -241,25 +339,56 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(Kv4Cache c, Kv4Evi
   const int count = ((const int32_t *)e.work)[list];
   const int32_t *holes = evict_holes(e.work, lists, list, half), *late = holes + half;
   uint8_t *base = kv4_list(c.kv, list, c.slots, L::TB);
-  for (int i = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); i < count;
-       i += gridDim.x * (kThreads / 64)) {
-    const int dst = holes[i], src = late[i];
-    uint8_t *to = base + (int64_t)(dst / kKv4Tile) * L::TB;
-    const uint8_t *from = base + (int64_t)(src / kKv4Tile) * L::TB;
-    const int jd = dst % kKv4Tile, js = src % kKv4Tile;
-    if (lane < HD / 8)
-      ((uint32_t *)(to + jd * (HD / 2)))[lane] = ((const uint32_t *)(from + js * (HD / 2)))[lane];
-    for (int b = lane; b < HD / 2; b += 64)
-      to[L::VO + (jd >> 2) * (2 * HD) + b * 4 + (jd & 3)] =
-          from[L::VO + (js >> 2) * (2 * HD) + b * 4 + (js & 3)];
-    if (lane < 2 * NB) {
-      const int o = (lane < NB ? L::KS : L::VS) + (lane % NB) * 8;
-      *(half_t *)(to + o + (jd >> 2) * NB * 8 + (jd & 3) * 2) =
-          *(const half_t *)(from + o + (js >> 2) * NB * 8 + (js & 3) * 2);
+  const float *wi = e.weights + list * c.slots;
+  const int32_t *pi = e.positions + list * c.slots;
+  // byte offset of the tile of slot x, and of a slot within the V codes and the scales
+  auto tile = [](int x) { return (uint32_t)(x / kKv4Tile) * (uint32_t)L::TB; };
+  for (int i0 = (blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)) * M; i0 < count;
+       i0 += gridDim.x * (kThreads / 64) * M) {
+    const int nm = min(M, count - i0), at = i0 + min(lane & (M - 1), nm - 1);
+    const int dst = holes[at], src = late[at];  // past the last move: the last one again
+    uint8_t v[VN];
+    uint4 k[KN];
+    uint16_t sc[SN];
+#pragma unroll
+    for (int j = 0; j < VN; ++j) {
+      const int x = j * 64 + lane, f = __shfl(src, x / (HD / 2)), b = x % (HD / 2);
+      v[j] = base[tile(f) + L::VO + (f % kKv4Tile >> 2) * (2 * HD) + b * 4 + (f & 3)];
     }
-    if (lane == 0) {
-      e.weights_out[list * c.slots + dst] = e.weights[list * c.slots + src];
-      e.positions_out[list * c.slots + dst] = e.positions[list * c.slots + src];
+#pragma unroll
+    for (int j = 0; j < KN; ++j) {
+      const int x = j * 64 + lane, f = __shfl(src, x / NB % M);
+      k[j] = *(const uint4 *)(base + tile(f) + f % kKv4Tile * (HD / 2) + x % NB * 16);
+    }
+#pragma unroll
+    for (int j = 0; j < SN; ++j) {
+      const int x = j * 64 + lane, f = __shfl(src, x / (2 * NB)), b = x % (2 * NB);
+      sc[j] = *(const uint16_t *)(base + tile(f) + (b < NB ? L::KS : L::VS) +
+                                  ((f % kKv4Tile >> 2) * NB + b % NB) * 8 + (f & 3) * 2);
+    }
+    const float wv = wi[src];
+    const int32_t pv = pi[src];
+#pragma unroll
+    for (int j = 0; j < VN; ++j) {
+      const int x = j * 64 + lane, t = __shfl(dst, x / (HD / 2)), b = x % (HD / 2);
+      if (x / (HD / 2) < nm)
+        base[tile(t) + L::VO + (t % kKv4Tile >> 2) * (2 * HD) + b * 4 + (t & 3)] = v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < KN; ++j) {
+      const int x = j * 64 + lane, t = __shfl(dst, x / NB % M);
+      if (x / NB < nm) *(uint4 *)(base + tile(t) + t % kKv4Tile * (HD / 2) + x % NB * 16) = k[j];
+    }
+#pragma unroll
+    for (int j = 0; j < SN; ++j) {
+      const int x = j * 64 + lane, t = __shfl(dst, x / (2 * NB)), b = x % (2 * NB);
+      if (x / (2 * NB) < nm)
+        *(uint16_t *)(base + tile(t) + (b < NB ? L::KS : L::VS) +
+                      ((t % kKv4Tile >> 2) * NB + b % NB) * 8 + (t & 3) * 2) = sc[j];
+    }
+    if (lane < nm) {
+      e.weights_out[list * c.slots + dst] = wv;
+      e.positions_out[list * c.slots + dst] = pv;
     }
   }
 }
@@ -286,10 +415,9 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(Kv4Cache c, Kv4Evi
 
 hipError_t launch_kv4_append(const Kv4Cache &c, const float *qkv, int64_t ldq, int64_t n_rows,
                              const int64_t *starts, hipStream_t s) {
-  const int64_t units = n_rows * c.nkv * 2;
-  const dim3 grid((unsigned)((units + kThreads / 64 - 1) / (kThreads / 64)));
+  const dim3 grid((unsigned)((n_rows + 3) / 4), (unsigned)c.nkv);
   KV4_DISPATCH(c.hd, hipLaunchKernelGGL(kv4_append_kernel<HD>, grid, dim3(kThreads), 0, s, c, qkv,
-                                        ldq, n_rows, starts));
+                                        ldq, (uint32_t)n_rows, starts));
   return hipGetLastError();
 }
 
@@ -310,12 +438,17 @@ int64_t kv4_evict_work_bytes(int64_t lists, int slots) {
 hipError_t launch_kv4_evict(const Kv4Cache &c, const Kv4Evict &e, hipStream_t s) {
   const int64_t lists = (int64_t)e.n_layers * c.n_seq * c.nkv;
   const int half = c.slots / 2;  // at most min(keep, slots - keep) slots move
-  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)lists), dim3(kSelThreads), 0, s, c, e,
-                     half);
+  const dim3 sel((unsigned)lists), st(kSelThreads);
+  if (c.slots <= 4 * kSelThreads)
+    hipLaunchKernelGGL(evict_select_kernel<4>, sel, st, 0, s, c, e, half);
+  else if (c.slots <= 16 * kSelThreads)
+    hipLaunchKernelGGL(evict_select_kernel<16>, sel, st, 0, s, c, e, half);
+  else
+    hipLaunchKernelGGL(evict_select_kernel<64>, sel, st, 0, s, c, e, half);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   const int64_t most = e.keep < c.slots - e.keep ? e.keep : c.slots - e.keep;
-  int64_t bx = (most + 3) / 4;
+  int64_t bx = (most + 63) / 64;  // four waves of 16 moves
   bx = bx < 1 ? 1 : (bx > 1024 ? 1024 : bx);
   const dim3 grid((unsigned)bx, (unsigned)lists);
   KV4_DISPATCH(c.hd, hipLaunchKernelGGL(evict_move_kernel<HD>, grid, dim3(kThreads), 0, s, c, e,

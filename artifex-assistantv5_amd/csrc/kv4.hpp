@@ -30,66 +30,106 @@ __device__ __forceinline__ uint8_t *kv4_list(uint8_t *kv, int64_t list, int slot
   return kv + list * (int64_t)(slots / kKv4Tile) * tile_bytes;
 }
 
-// One row of K (roped with the table rows c, s) or V into slot `slot` of a list, by one
-// wave: lane l holds channels l, l + 64, ...  The rounding of every step is fixed (no
-// contraction), so that the codes can be restated bit for bit.
-template <int HD, bool IS_K>
-__device__ __forceinline__ void kv4_store_row(uint8_t *list, int slot, const float *__restrict__ x,
-                                              const float *__restrict__ c,
-                                              const float *__restrict__ s, int lane) {
-#pragma clang fp contract(off)
-  using L = Kv4<HD>;
-  constexpr int R = HD / 64, half = HD / 2;
-  float y[R];
+// Lane l's channels l, l + 64, ... of a row, and for a K row its cos / sin.
+template <int HD>
+struct Kv4Row {
+  static constexpr int R = HD / 64, T = HD == 64 ? 1 : R / 2;
+  float y[R], c[T], s[T];
+  __device__ __forceinline__ void load(const float *__restrict__ x, int lane) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) y[r] = x[lane + 64 * r];
+    for (int r = 0; r < R; ++r) y[r] = x[lane + 64 * r];
+  }
+  __device__ __forceinline__ void load_turn(const float *__restrict__ cr,
+                                            const float *__restrict__ sr, int lane) {
+#pragma unroll
+    for (int r = 0; r < T; ++r) {
+      const int i = HD == 64 ? lane & 31 : lane + 64 * r;
+      c[r] = cr[i];
+      s[r] = sr[i];
+    }
+  }
+};
+
+// The value of lane l ^ 16 / l ^ 32 (the two results of a swap are both lanes' values).
+__device__ __forceinline__ uint32_t from_xor16(uint32_t v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return r[0] ^ r[1] ^ v;
+}
+__device__ __forceinline__ uint32_t from_xor32(uint32_t v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return r[0] ^ r[1] ^ v;
+}
+
+// A row's codes and scales, by one wave.  The rounding of every step is fixed (no contraction),
+// so that they can be restated bit for bit.  For the 64 channels of each r: K: lanes with
+// (lane & 7) < 4 hold the byte at ((lane >> 3) & 3, block, lane & 3) of the slot's K codes; V:
+// lanes with (lane & 31) < 16 the byte at (lane & 15, block) of its V codes; the block is 2 r +
+// (lane >> 5), and d its scale.
+template <int HD, bool IS_K>
+__device__ __forceinline__ void kv4_quantize(Kv4Row<HD> &x, int lane, uint8_t (&byte)[HD / 64],
+                                             half_t (&scale)[HD / 64]) {
+#pragma clang fp contract(off)
+  constexpr int R = HD / 64;
   if constexpr (IS_K) {
     if constexpr (HD == 64) {
-      const float o = __shfl_xor(y[0], 32), cv = c[lane & 31], sv = s[lane & 31];
-      const float a = y[0] * cv, b = o * sv;
-      y[0] = lane < 32 ? a - b : a + b;
+      const float o = __uint_as_float(from_xor32(__float_as_uint(x.y[0])));
+      const float a = x.y[0] * x.c[0], b = o * x.s[0];
+      x.y[0] = lane < 32 ? a - b : a + b;
     } else {
 #pragma unroll
       for (int r = 0; r < R / 2; ++r) {
-        const float cv = c[lane + 64 * r], sv = s[lane + 64 * r];
-        const float a = y[r], b = y[r + R / 2];
-        const float ac = a * cv, bs = b * sv, bc = b * cv, as = a * sv;
-        y[r] = ac - bs;
-        y[r + R / 2] = bc + as;
+        const float a = x.y[r], b = x.y[r + R / 2];
+        const float ac = a * x.c[r], bs = b * x.s[r], bc = b * x.c[r], as = a * x.s[r];
+        x.y[r] = ac - bs;
+        x.y[r + R / 2] = bc + as;
       }
     }
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float y = x.y[r], a = fabsf(y), m = max_xor16(max_lanes16(a));
+    const uint64_t eq = __ballot(a == m);
+    const uint32_t e0 = (uint32_t)eq, e1 = (uint32_t)(eq >> 32);
+    // the first of the largest in each block (none where every element is NaN)
+    const int i0 = e0 ? __builtin_ctz(e0) : 0, i1 = 32 + (e1 ? __builtin_ctz(e1) : 0);
+    const float t0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(y), i0));
+    const float t1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(y), i1));
+    float d32 = (lane < 32 ? t0 : t1) * -0.125f;
+    // the product by itself: fused into the conversion it is added to +0, and -0 is lost
+    asm volatile("" : "+v"(d32));
+    scale[r] = (half_t)d32;
+    const float df = (float)scale[r];
+    const float q = df != 0.f ? rintf(y / df) + 8.f : 8.f;
+    const uint32_t code = (uint32_t)fminf(fmaxf(q, 0.f), 15.f);
+    const uint32_t hi = IS_K ? (uint32_t)__builtin_amdgcn_update_dpp(0, (int)code, 0x104, 0xF, 0xF,
+                                                                     true)  // lane + 4
+                             : from_xor16(code);
+    byte[r] = (uint8_t)(code | (hi << 4));
+  }
+}
+
+// Quantize a row into slot `slot` of a list.
+template <int HD, bool IS_K>
+__device__ __forceinline__ void kv4_put_row(uint8_t *list, int slot, Kv4Row<HD> &x, int lane) {
+  using L = Kv4<HD>;
+  uint8_t byte[HD / 64];
+  half_t scale[HD / 64];
+  kv4_quantize<HD, IS_K>(x, lane, byte, scale);
   uint8_t *tile = list + (int64_t)(slot / kKv4Tile) * L::TB;
   const int j = slot % kKv4Tile;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const float a = fabsf(y[r]);
-    float m = a;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    const uint32_t eq = (uint32_t)(__ballot(a == m) >> (lane & 32));
-    const int first = eq ? __builtin_ctz(eq) : 0;  // none: every element is NaN
-    float d32 = __shfl(y[r], (lane & 32) + first) * -0.125f;
-    // the product by itself: fused into the conversion it is added to +0, and -0 is lost
-    asm volatile("" : "+v"(d32));
-    const half_t d = (half_t)d32;
-    const float df = (float)d;
-    const float q = df != 0.f ? rintf(y[r] / df) + 8.f : 8.f;
-    const int code = (int)fminf(fmaxf(q, 0.f), 15.f);
+  for (int r = 0; r < HD / 64; ++r) {
     const int b = 2 * r + (lane >> 5);
     if constexpr (IS_K) {
-      const int hi = __shfl(code, lane + 4);
       if ((lane & 7) < 4)
-        tile[j * half + (((lane >> 3) & 3) * L::NB + b) * 4 + (lane & 3)] =
-            (uint8_t)(code | (hi << 4));
+        tile[j * (HD / 2) + (((lane >> 3) & 3) * L::NB + b) * 4 + (lane & 3)] = byte[r];
     } else {
-      const int hi = __shfl(code, lane + 16);
       if ((lane & 31) < 16)
-        tile[L::VO + (j >> 2) * (2 * HD) + ((lane & 15) * L::NB + b) * 4 + (j & 3)] =
-            (uint8_t)(code | (hi << 4));
+        tile[L::VO + (j >> 2) * (2 * HD) + ((lane & 15) * L::NB + b) * 4 + (j & 3)] = byte[r];
     }
     if ((lane & 31) == 0)
-      *(half_t *)(tile + (IS_K ? L::KS : L::VS) + ((j >> 2) * L::NB + b) * 8 + (j & 3) * 2) = d;
+      *(half_t *)(tile + (IS_K ? L::KS : L::VS) + ((j >> 2) * L::NB + b) * 8 + (j & 3) * 2) =
+          scale[r];
   }
 }
 

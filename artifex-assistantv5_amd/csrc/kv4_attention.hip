@@ -20,22 +20,91 @@ constexpr int record_floats() {
   return HD + 2 * (HD / 32);
 }
 
-// The splits of a sequence that sees `vis` slots: `per` tiles each (whole turns of the W waves
-// of a workgroup), `n` of them.
-struct Splits {
-  int per, n;
-};
-__device__ __forceinline__ Splits kv4_splits(int vis, int S, int W) {
-  const int tiles = (vis + kKv4Tile - 1) / kKv4Tile;
-  int per = (tiles + S - 1) / S;
-  per = (per + W - 1) / W * W;
-  return {per, (tiles + per - 1) / per};
-}
-
 // The slots in use before the call, or -1 if the sequence takes no part.
 __device__ __forceinline__ int kv4_filled(const Kv4Cache &c, int64_t s, int rows) {
   const int64_t n = c.lengths[s], p = c.pos[s];
   return n < 0 || n + rows > c.slots || p < 0 || p + rows > c.rope_rows ? -1 : (int)n;
+}
+
+// How the tiles of a list are cut: `per` for each workgroup, `n` of them at most S.  Every
+// workgroup of the call gets about the same number, whatever the sequences' lengths: all lists'
+// tiles over `wgs` workgroups, in whole turns of a workgroup's W waves.
+struct Cut {
+  int S, wgs, W;
+};
+struct Splits {
+  int per, n;
+};
+__device__ __forceinline__ int kv4_tiles(int filled, int rows) {
+  return filled < 0 ? 0 : (filled + rows + kKv4Tile - 1) / kKv4Tile;
+}
+__device__ __forceinline__ Splits kv4_splits(int tiles, int fair, const Cut &k) {
+  const int per = (max(max(fair, 1), (tiles + k.S - 1) / k.S) + k.W - 1) / k.W * k.W;
+  return {per, (tiles + per - 1) / per};
+}
+// The fair share: a wave's lanes add the sequences.
+__device__ __forceinline__ int kv4_fair(const Kv4Cache &c, int rows, const Cut &k) {
+  int sum = 0;
+  if (c.n_seq == 1) {
+    sum = kv4_tiles(kv4_filled(c, 0, rows), rows);
+  } else {
+    for (int s = threadIdx.x & 63; s < c.n_seq; s += 64) sum += kv4_tiles(kv4_filled(c, s, rows), rows);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    sum = __builtin_amdgcn_readfirstlane(sum);
+  }
+  return (int)(((int64_t)sum * c.nkv + k.wgs - 1) / k.wgs);
+}
+// Workgroup `item` of the call: sequences in order, within one the splits in order, each for
+// every KV head.  Only the last workgroups of a launch are left without an item, so that the
+// dies, which take workgroups in turn, get the same number of items.
+struct Item {
+  int s, kvh, split, filled;
+  Splits sp;
+};
+__device__ __forceinline__ bool kv4_item(const Kv4Cache &c, int rows, int item, const Cut &k,
+                                         Item &it) {
+  const int fair = kv4_fair(c, rows, k);
+  if (c.n_seq == 1) {
+    it.s = 0;
+    it.filled = kv4_filled(c, 0, rows);
+    it.sp = kv4_splits(kv4_tiles(it.filled, rows), fair, k);
+    it.split = item / c.nkv;
+    it.kvh = item - it.split * c.nkv;
+    return it.filled >= 0 && it.split < it.sp.n;
+  }
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
+    const int filled = s0 + lane < c.n_seq ? kv4_filled(c, s0 + lane, rows) : -1;
+    const Splits sp = kv4_splits(kv4_tiles(filled, rows), fair, k);
+    int run = sp.n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(run, o);
+      if (lane >= o) run += x;
+    }
+    const uint64_t hit = __ballot(item < (before + run) * c.nkv);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      it.s = s0 + at;
+      it.filled = __builtin_amdgcn_readlane(filled, at);
+      it.sp.per = __builtin_amdgcn_readlane(sp.per, at);
+      it.sp.n = __builtin_amdgcn_readlane(sp.n, at);
+      const int first = before + __builtin_amdgcn_readlane(run, at) - it.sp.n;
+      it.split = (item - first * c.nkv) / c.nkv;
+      it.kvh = item - first * c.nkv - it.split * c.nkv;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(run, 63);
+  }
+  return false;
+}
+
+// The stride of a query row's scores: an odd number of 256-byte lines, so that the rows that
+// workgroups write side by side do not fall on one memory channel.
+__host__ __device__ __forceinline__ int64_t score_stride(int slots) {
+  return (int64_t)(((slots + 63) / 64) | 1) * 64;
 }
 
 // Eight 4-bit codes (element 0..3 in the low nibbles of bytes 0..3, 4..7 in the high ones) as
@@ -49,24 +118,38 @@ __device__ __forceinline__ half8_t k_codes(uint32_t w) {
       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true))};
   return __builtin_bit_cast(half8_t, r);
 }
-// Codes in bits 0-3 and 16-19 of w as f16 integers code - 8 (1024 + code, less 1032); `magic`
+// Codes of V as f16 integers: bits 0-3 and 16-19 of w give code - 8 (1024 + code, less 1032),
+// bits 4-7 and 20-23 give 16 (code - 8) (1024 + 16 code, less 1152) without a shift.  `magic`
 // holds 1024.0 twice in a vector register, so that mask and OR are one instruction.
+template <int SCALE>
 __device__ __forceinline__ half2_t v_codes(uint32_t w, uint32_t magic) {
-  const half2_t c = __builtin_bit_cast(half2_t, (w & 0x000F000Fu) | magic);
-  return c - half2_t{(half_t)1032.f, (half_t)1032.f};
+  const half2_t c = __builtin_bit_cast(half2_t, (w & (0x000F000Fu * SCALE)) | magic);
+  return c - half2_t{(half_t)(1024.f + 8.f * SCALE), (half_t)(1024.f + 8.f * SCALE)};
 }
-__device__ __forceinline__ half8_t v_frag(uint32_t w0, uint32_t w1, uint32_t magic) {
-  const half2_t r[4] = {v_codes(w0, magic), v_codes(w0 >> 8, magic), v_codes(w1, magic),
-                        v_codes(w1 >> 8, magic)};
+template <int SCALE>
+__device__ __forceinline__ half8_t v_frag(uint32_t w0, uint32_t h0, uint32_t w1, uint32_t h1,
+                                          uint32_t magic) {
+  const half2_t r[4] = {v_codes<SCALE>(w0, magic), v_codes<SCALE>(h0, magic),
+                        v_codes<SCALE>(w1, magic), v_codes<SCALE>(h1, magic)};
   return __builtin_bit_cast(half8_t, r);
 }
 __device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+// x * (float)h in one instruction: a product alone is converted and multiplied in two, and one
+// that is added to something would be fused into that.
+__device__ __forceinline__ float mul_f16(float x, half_t h) { return fmaf(x, (float)h, 0.f); }
+
 // v plus that of the lane N to the left in its 16, cyclically.
 template <int N>
 __device__ __forceinline__ float add_ror16(float v) {
   return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
+}
+
+template <int N>
+__device__ __forceinline__ float max_ror16(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF,
+                                                             true)));
 }
 
 // What a wave reads of a tile.  Lane (r = lane % 16, g = lane / 16), halves t = 0, 1: K codes of
@@ -81,14 +164,42 @@ struct TileRegs {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       words(tile + (uint32_t)((16 * t + r) * (HD / 2) + g * NB * 4), k[t]);
-      ks[t] = *(const uint2 *)(tile + (uint32_t)(Kv4<HD>::KS + ((4 * t + g) * NB + b) * 8));
+      const uint8_t *sp = tile + (uint32_t)(Kv4<HD>::KS + ((4 * t + g) * NB + b) * 8);
+      ks[t] = *(const uint2 *)sp;
+      vs[t] = *(const uint2 *)(sp + 2 * HD);
     }
   }
-  __device__ __forceinline__ void load_v(const uint8_t *tile, int r, int g, int b) {
+  __device__ __forceinline__ void load_v(const uint8_t *tile, int r, int g) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       words(tile + (uint32_t)(Kv4<HD>::VO + (4 * t + g) * (2 * HD) + r * NB * 4), v[t]);
-      vs[t] = *(const uint2 *)(tile + (uint32_t)(Kv4<HD>::VS + ((4 * t + g) * NB + b) * 8));
+    }
+  }
+  // Slot j of the tile from its bytes and scales.
+  __device__ __forceinline__ void patch(const uint8_t (&fresh)[2][HD / 2],
+                                        const half_t (&fscale)[2][NB], int j, int r, int g, int b) {
+    const int sh = 8 * (j & 3), ss = 16 * (j & 1);
+    const uint32_t kd = __builtin_bit_cast(uint16_t, fscale[0][b]);
+    const uint32_t vd = __builtin_bit_cast(uint16_t, fscale[1][b]);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (j == 16 * t + r)
+#pragma unroll
+        for (int i = 0; i < NB; ++i) k[t][i] = *(const uint32_t *)(fresh[0] + (g * NB + i) * 4);
+      if (j >> 2 == 4 * t + g) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+          v[t][i] = (v[t][i] & ~(0xFFu << sh)) | ((uint32_t)fresh[1][r * NB + i] << sh);
+        // by value: a reference to one of two words would put the registers in memory
+        const uint32_t keep = ~(0xFFFFu << ss), kn = kd << ss, vn = vd << ss;
+        if (j & 2) {
+          ks[t].y = (ks[t].y & keep) | kn;
+          vs[t].y = (vs[t].y & keep) | vn;
+        } else {
+          ks[t].x = (ks[t].x & keep) | kn;
+          vs[t].x = (vs[t].x & keep) | vn;
+        }
+      }
     }
   }
   static __device__ __forceinline__ void words(const uint8_t *p, uint32_t (&w)[NB]) {
@@ -131,11 +242,11 @@ struct TileRegs {
 // - K's registers take the next tile as soon as its scores are made, V's after its products:
 //   one tile in flight per wave, four waves per SIMD.
 // Bound: HBM, 9/8 head_dim bytes per slot and list.
-template <int HD, int NSUB, int W>
-__global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4Attn a,
+template <int HD, int NSUB, int W, int WPS>
+__global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, Kv4Attn a,
                                                                float *__restrict__ rec,
                                                                float *__restrict__ lse,
-                                                               float *__restrict__ scores, int S,
+                                                               float *__restrict__ scores, Cut cut,
                                                                bool store) {
   using L = Kv4<HD>;
   constexpr int NB = L::NB, HPS = 16 / NB, half = HD / 2, RS = record_floats<HD>();
@@ -144,27 +255,33 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
   __shared__ float2 lm[W][NSUB][16];           // and the 16 rows' (m, sum of p)
   __shared__ half8_t q_[NSUB][NB][2][64];      // queries: per block, hi and lo part, a B operand
   __shared__ float2 qc[NSUB][16];              // per row: initial value, log2 units per unit
-  const int64_t list = blockIdx.y, s = list / c.nkv;
-  const int kvh = (int)(list - s * c.nkv), grp = c.nh / c.nkv, V = a.rows * grp;
+  __shared__ __align__(16) uint8_t fresh[2][half];  // the stored row's K and V code bytes,
+  __shared__ half_t fscale[2][NB];                  // and scales
+  Item it;
+  if (!kv4_item(c, a.rows, blockIdx.x, cut, it)) return;
+  it.s = __builtin_amdgcn_readfirstlane(it.s);  // all known uniform from here on
+  it.kvh = __builtin_amdgcn_readfirstlane(it.kvh);
+  it.split = __builtin_amdgcn_readfirstlane(it.split);
+  it.filled = __builtin_amdgcn_readfirstlane(it.filled);
+  it.sp.per = __builtin_amdgcn_readfirstlane(it.sp.per);
+  it.sp.n = __builtin_amdgcn_readfirstlane(it.sp.n);
+  const int64_t s = it.s, list = s * c.nkv + it.kvh;
+  const int kvh = it.kvh, grp = c.nh / c.nkv, V = a.rows * grp, filled = it.filled;
+  const Splits sp = it.sp;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // known uniform: scalar addresses
   const int b = r / HPS, h = r % HPS;
-  const int filled = kv4_filled(c, s, a.rows);
-  if (filled < 0) return;
-  const Splits sp = kv4_splits(filled + a.rows, S, W);
-  if ((int)blockIdx.x >= sp.n) return;
-  const int tile0 = blockIdx.x * sp.per;
-  const int tile1 = min(tile0 + sp.per, (filled + a.rows + kKv4Tile - 1) / kKv4Tile);
+  const int tile0 = it.split * sp.per, tile1 = min(tile0 + sp.per, kv4_tiles(filled, a.rows));
   uint8_t *base = kv4_list(c.kv, list, c.slots, L::TB);
   const int v0 = blockIdx.z * NSUB * HPS;
   // the workgroup whose range has the one new row stores it (a call of more rows stores them
-  // beforehand) and reads its tiles afterwards; the others request theirs now
+  // beforehand) and keeps its bytes in LDS, for the wave whose first tile has the slot stale
   const bool stores = store && filled / kKv4Tile >= tile0 && filled / kKv4Tile < tile1;
   TileRegs<HD> d;
   int tile = tile0 + wave;
-  if (!stores && tile < tile1) {
+  if (tile < tile1) {
     d.load_k(base + (int64_t)tile * L::TB, r, g, b);
-    d.load_v(base + (int64_t)tile * L::TB, r, g, b);
+    d.load_v(base + (int64_t)tile * L::TB, r, g);
   }
   if (wave < NSUB) {
     // queries of group `wave`: lane (r, g) holds channels 32 b + 8 g + 0..7 of its row
@@ -187,8 +304,9 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
     float mx = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(y[j]));
-#pragma unroll
-    for (int o = HPS; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    if constexpr (NB > 4) mx = max_ror16<2>(mx);
+    if constexpr (NB > 2) mx = max_ror16<4>(mx);
+    mx = max_xor32(max_xor16(max_ror16<8>(mx)));
     const int e = stage_exp(mx);
     const float up = pow2f(e);
     half8_t hi, lo;
@@ -200,8 +318,7 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
       lo[j] = (half_t)(t - (float)hi[j]);
       sum += (float)hi[j] + (float)lo[j];
     }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
+    sum = sum_xor32(sum_xor16(sum));
     if (g == 0) qc[wave][r] = make_float2(-8.f * sum, pow2f(-e) * (kLog2e / sqrtf((float)HD)));
     const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
@@ -209,23 +326,45 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
       q_[wave][k][0][lane] = b == k ? hi : zero;
       q_[wave][k][1][lane] = b == k ? lo : zero;
     }
-  } else if (stores && wave < NSUB + 3) {
+  } else if (stores && wave < NSUB + 2) {
     const float *x = a.qkv + s * a.ldq + (int64_t)(c.nh + kvh) * HD;
     const int64_t p = c.pos[s];
+    const int j = filled % kKv4Tile;
+    Kv4Row<HD> row;
+    uint8_t byte[HD / 64];
+    half_t scale[HD / 64];
+    uint8_t *to = base + (int64_t)(filled / kKv4Tile) * L::TB;
     if (wave == NSUB) {
-      kv4_store_row<HD, true>(base, filled, x, c.cs + p * half, c.sn + p * half, lane);
-    } else if (wave == NSUB + 1) {
-      kv4_store_row<HD, false>(base, filled, x + (int64_t)c.nkv * HD, nullptr, nullptr, lane);
-    } else if (lane == 0) {
-      if (c.positions) c.positions[list * c.slots + filled] = (int32_t)p;
-      if (c.weights) c.weights[list * c.slots + filled] = 0.f;
+      row.load(x, lane);
+      row.load_turn(c.cs + p * half, c.sn + p * half, lane);
+      kv4_quantize<HD, true>(row, lane, byte, scale);
+#pragma unroll
+      for (int k = 0; k < HD / 64; ++k) {
+        const int blk = 2 * k + (lane >> 5), at = (((lane >> 3) & 3) * NB + blk) * 4 + (lane & 3);
+        if ((lane & 7) < 4) to[j * half + at] = fresh[0][at] = byte[k];
+        if ((lane & 31) == 0)
+          *(half_t *)(to + L::KS + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = fscale[0][blk] =
+              scale[k];
+      }
+    } else {
+      row.load(x + (int64_t)c.nkv * HD, lane);
+      kv4_quantize<HD, false>(row, lane, byte, scale);
+#pragma unroll
+      for (int k = 0; k < HD / 64; ++k) {
+        const int blk = 2 * k + (lane >> 5), at = (lane & 15) * NB + blk;
+        if ((lane & 31) < 16)
+          to[L::VO + (j >> 2) * (2 * HD) + at * 4 + (j & 3)] = fresh[1][at] = byte[k];
+        if ((lane & 31) == 0)
+          *(half_t *)(to + L::VS + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = fscale[1][blk] =
+              scale[k];
+      }
+      if (lane == 0) {
+        if (c.positions) c.positions[list * c.slots + filled] = (int32_t)p;
+        if (c.weights) c.weights[list * c.slots + filled] = 0.f;
+      }
     }
   }
   __syncthreads();
-  if (stores && tile < tile1) {
-    d.load_k(base + (int64_t)tile * L::TB, r, g, b);
-    d.load_v(base + (int64_t)tile * L::TB, r, g, b);
-  }
   float q0[NSUB], f[NSUB];  // the accumulators' initial value; log2 units per accumulated unit
   int vis[NSUB];            // slots that the row sees
 #pragma unroll
@@ -249,6 +388,10 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
 
   uint32_t magic;
   asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(magic));
+  float minus1 = -1.f;  // not known to be: x - (float)h stays one fused instruction
+  asm volatile("" : "+s"(minus1));
+  // a tile requested before the barrier may lack the new slot; a later one has it
+  if (stores && tile == filled / kKv4Tile) d.patch(fresh, fscale, filled % kKv4Tile, r, g, b);
   int ql = lane;  // made anew every turn: the queries are read from LDS there, not kept
   for (; tile < tile1; tile += W) {
     const uint8_t *next = base + (int64_t)min(tile + W, tile1 - 1) * L::TB;  // the last one: unused
@@ -276,10 +419,10 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float ks = (float)__builtin_bit_cast(half4_t, d.ks[i >> 2])[i & 3];
+        const half_t ks = __builtin_bit_cast(half4_t, d.ks[i >> 2])[i & 3];
 #pragma unroll
         for (int u = 0; u < NSUB; ++u) {
-          float x = sc[u][i >> 2][i & 3] * ks;
+          float x = mul_f16(sc[u][i >> 2][i & 3], ks);
           if constexpr (NB > 1) x = add_ror16<8>(x);
           if constexpr (NB > 2) x = add_ror16<4>(x);
           if constexpr (NB > 4) x = add_ror16<2>(x);
@@ -287,12 +430,13 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
         }
       }
     }
+    const half4_t dv[2] = {__builtin_bit_cast(half4_t, d.vs[0]), __builtin_bit_cast(half4_t, d.vs[1])};
     d.load_k(next, r, g, b);
     if (scores) {
 #pragma unroll
       for (int u = 0; u < NSUB; ++u)
         if (r < HPS && v0 + u * HPS + r < V) {
-          float *o = scores + (list * V + v0 + u * HPS + r) * c.slots + slot0;
+          float *o = scores + (list * V + v0 + u * HPS + r) * score_stride(c.slots) + slot0;
           *(float4 *)o = make_float4(y[u][0] * f[u], y[u][1] * f[u], y[u][2] * f[u], y[u][3] * f[u]);
           *(float4 *)(o + 16) =
               make_float4(y[u][4] * f[u], y[u][5] * f[u], y[u][6] * f[u], y[u][7] * f[u]);
@@ -302,38 +446,36 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
     half8_t wh[NSUB], wl[NSUB];
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) {
-      float p[8], w[8];
-      float most_w, most_p;
+      float p[8], w[8], sum, most;
+      // the first slot past those that the row sees, from slot0: hides i from there on (unrolled
+      // turns share nothing of this but where a tile is masked)
+      auto hidden = [&](int i) { return slot0 + (i < 4 ? i : 12 + i) >= vis[u]; };
       auto weigh = [&]() {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           p[i] = __builtin_amdgcn_exp2f(fmaf(y[u][i], f[u], -m[u]));
-          w[i] = p[i] * (float)__builtin_bit_cast(half4_t, d.vs[i >> 2])[i & 3];
+          w[i] = mul_f16(p[i], dv[i >> 2][i & 3]);
         }
         if (masked) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (slot0 + (i < 4 ? i : 12 + i) >= vis[u]) p[i] = w[i] = 0.f;
+            if (hidden(i)) p[i] = w[i] = 0.f;
         }
-        most_w = fmaxf(fabsf(w[0]), fabsf(w[1]));
-        most_p = fmaxf(p[0], p[1]);
+        sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        most = fabsf(w[0]);
 #pragma unroll
-        for (int i = 2; i < 8; i += 2) {
-          most_w = fmaxf(fmaxf(most_w, fabsf(w[i])), fabsf(w[i + 1]));
-          most_p = fmaxf(fmaxf(most_p, p[i]), p[i + 1]);
-        }
+        for (int i = 1; i < 7; i += 2) most = fmaxf(fmaxf(most, fabsf(w[i])), fabsf(w[i + 1]));
+        most = fmaxf(most, fabsf(w[7]));
       };
       weigh();
-      if (__any(most_w > kMostW || most_p > kMostP)) {
+      if (__any(most > kMostW || sum > kMostP)) {
         float n = m[u];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint32_t bits =
-              __float_as_uint((float)__builtin_bit_cast(half4_t, d.vs[i >> 2])[i & 3]) & 0x7FFFFFFFu;
+          const uint32_t bits = __float_as_uint((float)dv[i >> 2][i & 3]) & 0x7FFFFFFFu;
           const float lg =  // of at least 2^-24
               fmaf((float)(int)(bits < 0x33800000u ? 0x33800000u : bits), 0x1p-23f, -127.f - kLift);
-          if (!masked || slot0 + (i < 4 ? i : 12 + i) < vis[u])
-            n = fmaxf(n, fmaf(y[u][i], f[u], lg));
+          if (!masked || !hidden(i)) n = fmaxf(n, fmaf(y[u][i], f[u], lg));
         }
         n = max_xor16(n);
         n = max_xor32(n);
@@ -349,24 +491,24 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
           for (int i = 0; i < 4; ++i) acc[u][t][i] *= ar[i];
         weigh();
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) l[u] += p[i];
+      l[u] += sum;
       half2_t hp[4], lp[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {  // V's pairs: slots (0, 2), (1, 3) of each half
         const int i = (k & 1) + (k >> 1) * 4;
         hp[k] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(w[i], w[i + 2]));
         lp[k] = __builtin_bit_cast(half2_t,
-                                   __builtin_amdgcn_cvt_pkrtz(fmaf((float)hp[k][0], -1.f, w[i]),
-                                                              fmaf((float)hp[k][1], -1.f, w[i + 2])));
+                                   __builtin_amdgcn_cvt_pkrtz(fmaf((float)hp[k][0], minus1, w[i]),
+                                                              fmaf((float)hp[k][1], minus1, w[i + 2])));
       }
       wh[u] = __builtin_bit_cast(half8_t, hp);
       wl[u] = __builtin_bit_cast(half8_t, lp);
     }
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
-      const half8_t va = v_frag(d.v[0][k], d.v[1][k], magic);
-      const half8_t vb = v_frag(d.v[0][k] >> 4, d.v[1][k] >> 4, magic);
+      const uint32_t w0 = d.v[0][k], h0 = w0 >> 8, w1 = d.v[1][k], h1 = w1 >> 8;
+      const half8_t va = v_frag<1>(w0, h0, w1, h1, magic);
+      const half8_t vb = v_frag<16>(w0, h0, w1, h1, magic);  // channels 16..31 of the block
 #pragma unroll
       for (int u = 0; u < NSUB; ++u) {
         acc[u][2 * k] = mfma(wh[u], va, acc[u][2 * k]);
@@ -375,7 +517,7 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
         acc[u][2 * k + 1] = mfma(wl[u], vb, acc[u][2 * k + 1]);
       }
     }
-    d.load_v(next, r, g, b);
+    d.load_v(next, r, g);
   }
 
   // the waves' sums: lane (r, g), register i holds row 4 g + i, channel 16 t + r
@@ -388,11 +530,12 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
       const int row = 4 * g + i, rb = row / HPS;
 #pragma unroll
       for (int t = 0; t < 2 * NB; ++t)
-        if (rb == t / 2) lo_[wave][u][row % HPS * HD + 16 * t + r] = acc[u][t][i];
+        if (rb == t / 2)
+          lo_[wave][u][row % HPS * HD + 16 * t + r] = acc[u][t][i] * (t & 1 ? 0.0625f : 1.f);
     }
   }
   __syncthreads();
-  float *out = rec + (list * S + blockIdx.x) * V * RS;
+  float *out = rec + (list * cut.S + it.split) * V * RS;
   for (int e = tid; e < NSUB * 512; e += 64 * W) {
     const int u = e >> 9, hh = (e & 511) / HD, ch = e & (HD - 1), row = (ch >> 5) * HPS + hh;
     const int v = v0 + u * HPS + hh;
@@ -422,7 +565,7 @@ __global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4Cache c, Kv4At
 template <int HD>
 __global__ __launch_bounds__(kThreads) void kv4_merge_kernel(Kv4Cache c, Kv4Attn a,
                                                              const float *__restrict__ rec,
-                                                             float *__restrict__ lse, int S, int W) {
+                                                             float *__restrict__ lse, Cut cut) {
   constexpr int RS = record_floats<HD>(), Q = HD / 4, G = kThreads / Q;
   __shared__ float4 o_[G][Q];
   __shared__ float2 ml_[G][Q];
@@ -431,9 +574,9 @@ __global__ __launch_bounds__(kThreads) void kv4_merge_kernel(Kv4Cache c, Kv4Attn
   const int q = threadIdx.x % Q, gi = threadIdx.x / Q;
   const int filled = kv4_filled(c, s, a.rows);
   if (filled < 0) return;
-  const Splits sp = kv4_splits(filled + a.rows, S, W);
+  const Splits sp = kv4_splits(kv4_tiles(filled, a.rows), kv4_fair(c, a.rows, cut), cut);
   if (sp.n == 1) return;
-  const float *r = rec + (list * S * V + v) * RS;
+  const float *r = rec + (list * cut.S * V + v) * RS;
   const int64_t step = (int64_t)V * RS;
   const int at = HD + 2 * (q / 8);
   float m = -INFINITY, l = 0.f;
@@ -473,28 +616,65 @@ __global__ __launch_bounds__(kThreads) void kv4_merge_kernel(Kv4Cache c, Kv4Attn
   if (lse && q == 0) lse[list * V + v] = m + log2f(l);
 }
 
-// The attention weights of a list's slots, a thread per slot: the scores of every query row
-// against the row's log-sum-exp.
+// The attention weights of a list's slots: 64 threads of four slots each times four shares of
+// the query rows, whose scores are taken against the rows' log-sum-exp; shares joined in order.
+constexpr int kWeightSlots = 256;
 __global__ __launch_bounds__(kThreads) void kv4_weights_kernel(Kv4Cache c, Kv4Attn a,
                                                                const float *__restrict__ lse,
                                                                const float *__restrict__ scores) {
+  __shared__ float4 part[3][64];
   const int64_t list = blockIdx.y, s = list / c.nkv;
-  const int grp = c.nh / c.nkv, V = a.rows * grp;
+  const int grp = c.nh / c.nkv, V = a.rows * grp, x = threadIdx.x & 63;
+  const int share = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int filled = kv4_filled(c, s, a.rows);
-  const int t = blockIdx.x * kThreads + threadIdx.x;
-  if (filled < 0 || t >= filled + a.rows) return;
-  const float *e = lse + list * V, *x = scores + list * V * c.slots + t;
-  float sum = 0.f;
+  const int t = blockIdx.x * kWeightSlots + 4 * x;
+  if (filled < 0 || (int)(blockIdx.x * kWeightSlots) >= filled + a.rows) return;
+  const int64_t step = score_stride(c.slots);
+  const float *e = lse + list * V, *sc = scores + list * V * step + t;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (t < filled + a.rows) {
+    if (t + 3 <= filled) {  // every row sees the four slots
 #pragma unroll 8
-  for (int v = 0; v < V; ++v)
-    if (t <= filled + v / grp) sum += __builtin_amdgcn_exp2f(x[(int64_t)v * c.slots] - e[v]);
-  float *w = c.weights + list * c.slots + t;
-  *w = a.weights_mode == 2 ? *w + sum : sum;
+      for (int v = share; v < V; v += 4) {
+        const float4 y = *(const float4 *)(sc + v * step);
+        const float z = e[v];
+        sum.x += __builtin_amdgcn_exp2f(y.x - z);
+        sum.y += __builtin_amdgcn_exp2f(y.y - z);
+        sum.z += __builtin_amdgcn_exp2f(y.z - z);
+        sum.w += __builtin_amdgcn_exp2f(y.w - z);
+      }
+    } else {
+      for (int v = share; v < V; v += 4) {
+        const int last = filled + v / grp;  // the last slot that row v sees
+        const float4 y = *(const float4 *)(sc + v * step);
+        const float z = e[v];
+        if (t <= last) sum.x += __builtin_amdgcn_exp2f(y.x - z);
+        if (t + 1 <= last) sum.y += __builtin_amdgcn_exp2f(y.y - z);
+        if (t + 2 <= last) sum.z += __builtin_amdgcn_exp2f(y.z - z);
+        if (t + 3 <= last) sum.w += __builtin_amdgcn_exp2f(y.w - z);
+      }
+    }
+  }
+  if (share) part[share - 1][x] = sum;
+  __syncthreads();
+  if (share) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const float4 y = part[k][x];
+    sum.x += y.x, sum.y += y.y, sum.z += y.z, sum.w += y.w;
+  }
+  const float w[4] = {sum.x, sum.y, sum.z, sum.w};
+  float *to = c.weights + list * c.slots + t;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (t + k < filled + a.rows) to[k] = a.weights_mode == 2 ? to[k] + w[k] : w[k];
 }
 
-// How a call is cut: NSUB groups of HPS query rows per workgroup of W waves, S splits at most.
+// How a call is cut: NSUB groups of HPS query rows per workgroup of W waves, `wgs` workgroups
+// at a time on the GPU for each group of rows, a list in S of them at most.
 struct Plan {
-  int V, nsub, W, nz, S;
+  int V, nsub, nz;
+  Cut cut;
   int64_t lists;
 };
 Plan plan(int rows, int n_seq, int nh, int nkv, int hd, int slots) {
@@ -502,18 +682,22 @@ Plan plan(int rows, int n_seq, int nh, int nkv, int hd, int slots) {
   const int hps = 512 / hd;
   p.V = rows * (nh / nkv);
   p.nsub = hd < 256 && p.V > hps ? 2 : 1;
-  p.W = hd < 256 && p.nsub == 1 ? 16 : 8;
+  p.cut.W = 8;
   p.nz = (p.V + p.nsub * hps - 1) / (p.nsub * hps);
   p.lists = (int64_t)n_seq * nkv;
-  const int64_t most = (slots / kKv4Tile + p.W - 1) / p.W;
-  const int64_t want = (4096 / p.W + p.lists * p.nz - 1) / (p.lists * p.nz);
-  p.S = (int)(want < most ? want : most);
+  const int resident = hd < 256 && p.nsub == 1 ? 512 : 256;
+  p.cut.wgs = (resident + p.nz - 1) / p.nz;
+  // a list is not cut below two turns of a workgroup's waves: one launch, and nothing to join
+  const int64_t tiles = slots / kKv4Tile, most = tiles <= 2 * p.cut.W ? 1 : (tiles + p.cut.W - 1) / p.cut.W;
+  // sequences of different lengths: up to four times the workgroups that equal ones would take
+  const int64_t want = (4 * p.cut.wgs + p.lists - 1) / p.lists;
+  p.cut.S = (int)(want < most ? want : most);
   return p;
 }
 
 // Work: records (several splits), then per query row its log-sum-exp and its scores (weights).
 int64_t record_bytes(const Plan &p, int hd) {
-  return p.S > 1 ? p.lists * p.S * p.V * (int64_t)(hd + hd / 16) * 4 : 0;
+  return p.cut.S > 1 ? p.lists * p.cut.S * p.V * (int64_t)(hd + hd / 16) * 4 : 0;
 }
 int64_t lse_bytes(const Plan &p) { return (p.lists * p.V * 4 + 15) / 16 * 16; }
 
@@ -531,28 +715,31 @@ hipError_t launch(const Kv4Cache &c, const Kv4Attn &a, hipStream_t s) {
         launch_kv4_append(c, a.qkv, a.ldq, (int64_t)c.n_seq * a.rows, nullptr, s);
     if (e != hipSuccess) return e;
   }
-  const dim3 grid((unsigned)p.S, (unsigned)p.lists, (unsigned)p.nz), block(64 * p.W);
+  // No call has more items than wgs + lists (every list but for its last workgroup gets whole
+  // shares).  A multiple of the dies: one item's groups of rows meet in one L2.
+  const int64_t most = p.lists * p.cut.S, items = most < p.cut.wgs + p.lists ? most : p.cut.wgs + p.lists;
+  const dim3 grid((unsigned)((items + 7) / 8 * 8), 1, (unsigned)p.nz), block(64 * p.cut.W);
   if constexpr (HD == 256) {
-    hipLaunchKernelGGL((kv4_attention_kernel<HD, 1, 8>), grid, block, 0, s, c, a, rec, lse, scores,
-                       p.S, inside);
+    hipLaunchKernelGGL((kv4_attention_kernel<HD, 1, 8, 2>), grid, block, 0, s, c, a, rec, lse,
+                       scores, p.cut, inside);
   } else if (p.nsub == 2) {
-    hipLaunchKernelGGL((kv4_attention_kernel<HD, 2, 8>), grid, block, 0, s, c, a, rec, lse, scores,
-                       p.S, inside);
+    hipLaunchKernelGGL((kv4_attention_kernel<HD, 2, 8, 2>), grid, block, 0, s, c, a, rec, lse,
+                       scores, p.cut, inside);
   } else {
-    hipLaunchKernelGGL((kv4_attention_kernel<HD, 1, 16>), grid, block, 0, s, c, a, rec, lse, scores,
-                       p.S, inside);
+    hipLaunchKernelGGL((kv4_attention_kernel<HD, 1, 8, 4>), grid, block, 0, s, c, a, rec, lse,
+                       scores, p.cut, inside);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (p.S > 1) {
+  if (p.cut.S > 1) {
     hipLaunchKernelGGL(kv4_merge_kernel<HD>, dim3((unsigned)p.V, (unsigned)p.lists), dim3(kThreads),
-                       0, s, c, a, rec, lse, p.S, p.W);
+                       0, s, c, a, rec, lse, p.cut);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   if (!a.weights_mode) return hipSuccess;
   hipLaunchKernelGGL(kv4_weights_kernel,
-                     dim3((unsigned)((c.slots + kThreads - 1) / kThreads), (unsigned)p.lists),
+                     dim3((unsigned)((c.slots + kWeightSlots - 1) / kWeightSlots), (unsigned)p.lists),
                      dim3(kThreads), 0, s, c, a, lse, scores);
   return hipGetLastError();
 }
@@ -562,7 +749,7 @@ hipError_t launch(const Kv4Cache &c, const Kv4Attn &a, hipStream_t s) {
 int64_t kv4_attention_work_bytes(int rows, bool weights, int n_seq, int nh, int nkv, int hd,
                                  int slots) {
   const Plan p = plan(rows, n_seq, nh, nkv, hd, slots);
-  return record_bytes(p, hd) + 16 + (weights ? lse_bytes(p) + p.lists * p.V * (int64_t)slots * 4 : 0);
+  return record_bytes(p, hd) + 16 + (weights ? lse_bytes(p) + p.lists * p.V * score_stride(slots) * 4 : 0);
 }
 
 hipError_t launch_kv4_attention(const Kv4Cache &c, const Kv4Attn &a, hipStream_t s) {
