@@ -274,32 +274,53 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
   const int tile0 = it.split * sp.per, tile1 = min(tile0 + sp.per, kv4_tiles(filled, a.rows));
   uint8_t *base = kv4_list(c.kv, list, c.slots, L::TB);
   const int v0 = blockIdx.z * NSUB * HPS;
-  // the workgroup whose range has the one new row stores it (a call of more rows stores them
-  // beforehand) and keeps its bytes in LDS, for the wave whose first tile has the slot stale
+  // the workgroups whose range has the one new row (a call of more rows stores them beforehand)
+  // make its bytes in LDS, for the wave whose first tile lacks them; those of the first group of
+  // query rows store them
   const bool stores = store && filled / kKv4Tile >= tile0 && filled / kKv4Tile < tile1;
+  const float *row0 = a.qkv + s * a.rows * a.ldq;  // the sequence's first row
+  const float *kx = row0 + (int64_t)(c.nh + kvh) * HD, *vx = kx + (int64_t)c.nkv * HD;
+  const int64_t pos0 = c.pos[s];
+
+  // What comes before the barrier is requested before the tile, since loads return in order:
+  // behind a full chip's tiles the queries took 5.6 us (130000 slots).
+  float4 xo[2], xp[2], cv[2], sv[2];  // wave < NSUB: the queries of group `wave`: lane (r, g)
+  Kv4Row<HD> row;                     // holds channels 32 b + 8 g + 0..7 of its row
+  if (wave < NSUB) {
+    const int v = v0 + wave * HPS + h, i = v < V ? v / grp : 0;
+    const float *x = row0 + i * a.ldq + (int64_t)(kvh * grp + (v < V ? v % grp : 0)) * HD;
+    const int e0 = 32 * b + 8 * g, ep = b < NB / 2 ? e0 + half : e0 - half;
+    const int64_t p = (pos0 + i) * half + (b < NB / 2 ? e0 : ep);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      xo[j] = *(const float4 *)(x + e0 + 4 * j);
+      xp[j] = *(const float4 *)(x + ep + 4 * j);
+      cv[j] = *(const float4 *)(c.cs + p + 4 * j);
+      sv[j] = *(const float4 *)(c.sn + p + 4 * j);
+    }
+  } else if (stores && wave == NSUB) {
+    row.load(kx, lane);
+    row.load_turn(c.cs + pos0 * half, c.sn + pos0 * half, lane);
+  } else if (stores && wave == NSUB + 1) {
+    row.load(vx, lane);
+  }
+  __builtin_amdgcn_sched_barrier(0);
   TileRegs<HD> d;
-  int tile = tile0 + wave;
-  if (tile < tile1) {
+  // from the last tile down: the new row's is some wave's first
+  int tile = tile1 - 1 - wave;
+  if (tile >= tile0) {
     d.load_k(base + (int64_t)tile * L::TB, r, g, b);
     d.load_v(base + (int64_t)tile * L::TB, r, g);
   }
+  __builtin_amdgcn_sched_barrier(0);
   if (wave < NSUB) {
-    // queries of group `wave`: lane (r, g) holds channels 32 b + 8 g + 0..7 of its row
-    const int v = v0 + wave * HPS + h, i = v < V ? v / grp : 0;
-    const float *x = a.qkv + (s * a.rows + i) * a.ldq + (int64_t)(kvh * grp + v - v / grp * grp) * HD;
-    const int e0 = 32 * b + 8 * g, ep = b < NB / 2 ? e0 + half : e0 - half;
-    const int64_t p = (c.pos[s] + i) * half + (b < NB / 2 ? e0 : ep);
+    const bool on = v0 + wave * HPS + h < V;  // past the last query row: zeros
     const float sign = b < NB / 2 ? -1.f : 1.f;
     float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; j += 4) {
-      const float4 xo = v < V ? *(const float4 *)(x + e0 + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 xp = v < V ? *(const float4 *)(x + ep + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 cv = *(const float4 *)(c.cs + p + j), sv = *(const float4 *)(c.sn + p + j);
-      y[j] = xo.x * cv.x + sign * (xp.x * sv.x);
-      y[j + 1] = xo.y * cv.y + sign * (xp.y * sv.y);
-      y[j + 2] = xo.z * cv.z + sign * (xp.z * sv.z);
-      y[j + 3] = xo.w * cv.w + sign * (xp.w * sv.w);
+    for (int j = 0; j < 8; ++j) {
+      const float o = (&xo[j >> 2].x)[j & 3], t = (&xp[j >> 2].x)[j & 3];
+      y[j] = on ? o * (&cv[j >> 2].x)[j & 3] + sign * (t * (&sv[j >> 2].x)[j & 3]) : 0.f;
     }
     float mx = 0.f;
 #pragma unroll
@@ -327,39 +348,41 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
       q_[wave][k][1][lane] = b == k ? lo : zero;
     }
   } else if (stores && wave < NSUB + 2) {
-    const float *x = a.qkv + s * a.ldq + (int64_t)(c.nh + kvh) * HD;
-    const int64_t p = c.pos[s];
+    const bool writes = blockIdx.z == 0;
     const int j = filled % kKv4Tile;
-    Kv4Row<HD> row;
     uint8_t byte[HD / 64];
     half_t scale[HD / 64];
     uint8_t *to = base + (int64_t)(filled / kKv4Tile) * L::TB;
     if (wave == NSUB) {
-      row.load(x, lane);
-      row.load_turn(c.cs + p * half, c.sn + p * half, lane);
       kv4_quantize<HD, true>(row, lane, byte, scale);
 #pragma unroll
       for (int k = 0; k < HD / 64; ++k) {
         const int blk = 2 * k + (lane >> 5), at = (((lane >> 3) & 3) * NB + blk) * 4 + (lane & 3);
-        if ((lane & 7) < 4) to[j * half + at] = fresh[0][at] = byte[k];
-        if ((lane & 31) == 0)
-          *(half_t *)(to + L::KS + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = fscale[0][blk] =
-              scale[k];
+        if ((lane & 7) < 4) {
+          fresh[0][at] = byte[k];
+          if (writes) to[j * half + at] = byte[k];
+        }
+        if ((lane & 31) == 0) {
+          fscale[0][blk] = scale[k];
+          if (writes) *(half_t *)(to + L::KS + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = scale[k];
+        }
       }
     } else {
-      row.load(x + (int64_t)c.nkv * HD, lane);
       kv4_quantize<HD, false>(row, lane, byte, scale);
 #pragma unroll
       for (int k = 0; k < HD / 64; ++k) {
         const int blk = 2 * k + (lane >> 5), at = (lane & 15) * NB + blk;
-        if ((lane & 31) < 16)
-          to[L::VO + (j >> 2) * (2 * HD) + at * 4 + (j & 3)] = fresh[1][at] = byte[k];
-        if ((lane & 31) == 0)
-          *(half_t *)(to + L::VS + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = fscale[1][blk] =
-              scale[k];
+        if ((lane & 31) < 16) {
+          fresh[1][at] = byte[k];
+          if (writes) to[L::VO + (j >> 2) * (2 * HD) + at * 4 + (j & 3)] = byte[k];
+        }
+        if ((lane & 31) == 0) {
+          fscale[1][blk] = scale[k];
+          if (writes) *(half_t *)(to + L::VS + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = scale[k];
+        }
       }
-      if (lane == 0) {
-        if (c.positions) c.positions[list * c.slots + filled] = (int32_t)p;
+      if (lane == 0 && writes) {
+        if (c.positions) c.positions[list * c.slots + filled] = (int32_t)pos0;
         if (c.weights) c.weights[list * c.slots + filled] = 0.f;
       }
     }
@@ -390,11 +413,10 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
   asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(magic));
   float minus1 = -1.f;  // not known to be: x - (float)h stays one fused instruction
   asm volatile("" : "+s"(minus1));
-  // a tile requested before the barrier may lack the new slot; a later one has it
   if (stores && tile == filled / kKv4Tile) d.patch(fresh, fscale, filled % kKv4Tile, r, g, b);
   int ql = lane;  // made anew every turn: the queries are read from LDS there, not kept
-  for (; tile < tile1; tile += W) {
-    const uint8_t *next = base + (int64_t)min(tile + W, tile1 - 1) * L::TB;  // the last one: unused
+  for (; tile >= tile0; tile -= W) {
+    const uint8_t *next = base + (int64_t)max(tile - W, tile0) * L::TB;  // the last one: unused
     const int slot0 = tile * kKv4Tile + 4 * g;  // of half 0, i = 0
     asm volatile("" : "+v"(ql));
     float y[NSUB][8];  // scores / f
@@ -682,10 +704,24 @@ Plan plan(int rows, int n_seq, int nh, int nkv, int hd, int slots) {
   const int hps = 512 / hd;
   p.V = rows * (nh / nkv);
   p.nsub = hd < 256 && p.V > hps ? 2 : 1;
-  p.cut.W = 8;
   p.nz = (p.V + p.nsub * hps - 1) / (p.nsub * hps);
   p.lists = (int64_t)n_seq * nkv;
-  const int resident = hd < 256 && p.nsub == 1 ? 512 : 256;
+  // Waves per workgroup and workgroups at a time, measured (us; 32 / 8 heads of 128 unless said):
+  // many lists of different lengths balance better in small workgroups (16 sequences of up to
+  // 4095 slots: 8 x 512 24.8, 4 x 768 21.2); few lists leave fewer records with large ones (6000
+  // slots: 11.1 against 12.7; 130000: 40.2 against 40.8).  Two groups of rows take 182 registers:
+  // two workgroups of four waves (32 rows over 20000 slots: 4 x 512 133, 8 x 512 142, 8 x 256 218,
+  // where ten of the 256 CUs get two); 256 channels 160 (4 sequences of 9000 slots, 16 / 2 heads:
+  // 8 x 256 32.3, 4 x 768 34.2).
+  const bool many = p.lists * p.nz >= 32;
+  int resident;
+  if (p.nsub == 2) {
+    p.cut.W = 4, resident = 512;
+  } else if (hd == 256) {
+    p.cut.W = 8, resident = 256;
+  } else {
+    p.cut.W = many ? 4 : 8, resident = many ? 768 : 512;
+  }
   p.cut.wgs = (resident + p.nz - 1) / p.nz;
   // a list is not cut below two turns of a workgroup's waves: one launch, and nothing to join
   const int64_t tiles = slots / kKv4Tile, most = tiles <= 2 * p.cut.W ? 1 : (tiles + p.cut.W - 1) / p.cut.W;
@@ -709,7 +745,7 @@ hipError_t launch(const Kv4Cache &c, const Kv4Attn &a, hipStream_t s) {
     lse = (float *)((char *)a.work + record_bytes(p, HD));
     scores = (float *)((char *)lse + lse_bytes(p));
   }
-  const bool inside = a.store && a.rows == 1 && p.nz == 1;  // one workgroup stores the one row
+  const bool inside = a.store && a.rows == 1;  // the one row is stored by the workgroups
   if (a.store && !inside) {
     const hipError_t e =
         launch_kv4_append(c, a.qkv, a.ldq, (int64_t)c.n_seq * a.rows, nullptr, s);
@@ -719,16 +755,17 @@ hipError_t launch(const Kv4Cache &c, const Kv4Attn &a, hipStream_t s) {
   // shares).  A multiple of the dies: one item's groups of rows meet in one L2.
   const int64_t most = p.lists * p.cut.S, items = most < p.cut.wgs + p.lists ? most : p.cut.wgs + p.lists;
   const dim3 grid((unsigned)((items + 7) / 8 * 8), 1, (unsigned)p.nz), block(64 * p.cut.W);
-  if constexpr (HD == 256) {
-    hipLaunchKernelGGL((kv4_attention_kernel<HD, 1, 8, 2>), grid, block, 0, s, c, a, rec, lse,
-                       scores, p.cut, inside);
-  } else if (p.nsub == 2) {
-    hipLaunchKernelGGL((kv4_attention_kernel<HD, 2, 8, 2>), grid, block, 0, s, c, a, rec, lse,
-                       scores, p.cut, inside);
-  } else {
-    hipLaunchKernelGGL((kv4_attention_kernel<HD, 1, 8, 4>), grid, block, 0, s, c, a, rec, lse,
-                       scores, p.cut, inside);
-  }
+  auto go = [&](auto *kernel) {
+    hipLaunchKernelGGL(kernel, grid, block, 0, s, c, a, rec, lse, scores, p.cut, inside);
+  };
+  if constexpr (HD == 256)
+    go(kv4_attention_kernel<HD, 1, 8, 2>);
+  else if (p.nsub == 2)
+    go(kv4_attention_kernel<HD, 2, 4, 2>);
+  else if (p.cut.W == 4)
+    go(kv4_attention_kernel<HD, 1, 4, 4>);
+  else
+    go(kv4_attention_kernel<HD, 1, 8, 4>);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (p.cut.S > 1) {
