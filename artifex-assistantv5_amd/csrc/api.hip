@@ -672,8 +672,9 @@ int gguf_hip_kv4_evict(void *kv, const float *weights, const int32_t *positions,
   if (!kv || !weights || !positions || !lengths || !pos || !weights_out || !positions_out ||
       !lengths_out || !work)
     return fail(GGUF_HIP_ERR_NULL, "[gguf-hip] null pointer");
-  if (!aligned(kv, 16) || !aligned(weights, 4) || !aligned(positions, 4) || !aligned(lengths, 8) ||
-      !aligned(pos, 8) || !aligned(weights_out, 4) || !aligned(positions_out, 4) ||
+  if (!aligned(kv, 16) || !aligned(weights, 16) || !aligned(positions, 16) ||
+      !aligned(lengths, 8) || !aligned(pos, 8) || !aligned(weights_out, 4) ||
+      !aligned(positions_out, 4) ||
       !aligned(lengths_out, 8) || !aligned(work, 16))
     return fail(GGUF_HIP_ERR_ALIGN, "[gguf-hip] kv4 buffers misaligned");
   if (work_bytes < need)

@@ -8,23 +8,30 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------------------
-// Storing rows: a wave per row and KV head (K and V), four neighbouring rows per workgroup, which
-// mostly share the four slots that V's words hold, so that their bytes meet in one L2.  (A wave
-// per row, KV head and K or V, its row found with vector loads: 29 us for 3700 packed rows of
-// 8 heads of 128, five sequences.)
+// Storing rows: a wave takes one row and N units (K or V of a KV head, 256 / HD of them side by
+// side); four neighbouring rows per workgroup, which mostly share the four slots that V's words
+// hold, so that their bytes meet in one L2.  Bound: vector instructions, then the chain of loads
+// that finds a row's place.  3716 packed rows of five sequences, 8 heads of 128: a channel per
+// lane 16.8 us (300 instructions for K and V of a head), four channels per lane: see DESIGN.
 // ---------------------------------------------------------------------------
-template <int HD>
+template <int HD, int N>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
                                                               const float *__restrict__ qkv,
                                                               int64_t ldq, uint32_t n_rows,
                                                               const int64_t *__restrict__ starts) {
-  const int lane = threadIdx.x & 63, h = blockIdx.y;
+  constexpr int LANES = Kv4Row<HD>::LANES, SIDE = 64 / LANES;
+  const int lane = threadIdx.x & 63, q = lane % LANES;
   const uint32_t r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   if (r >= n_rows) return;
-  const float *x = qkv + r * ldq + (int64_t)(c.nh + h) * HD;
-  Kv4Row<HD> k, v;
-  k.load(x, lane);
-  v.load(x + (int64_t)c.nkv * HD, lane);
+  // unit u: KV head u / 2, K or V; in qkv after the queries all of K, then all of V
+  const int u0 = blockIdx.y * N * SIDE + lane / LANES, units = 2 * c.nkv;
+  const float *x = qkv + r * ldq + (int64_t)c.nh * HD;
+  Kv4Row<HD> row[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {  // past the last unit: the last again, not stored
+    const int u = min(u0 + i * SIDE, units - 1);
+    row[i].load(x + (int64_t)((u & 1) * c.nkv + (u >> 1)) * HD, q);
+  }
   uint32_t s;
   int64_t i;
   if (starts) {
@@ -46,14 +53,19 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
   }
   const int64_t slot = c.lengths[s] + i, p = c.pos[s] + i;
   if (slot < 0 || slot >= c.slots || p < 0 || p >= c.rope_rows) return;
-  k.load_turn(c.cs + p * (HD / 2), c.sn + p * (HD / 2), lane);
-  const int64_t list = (int64_t)s * c.nkv + h;
-  uint8_t *base = kv4_list(c.kv, list, c.slots, Kv4<HD>::TB);
-  kv4_put_row<HD, false>(base, (int)slot, v, lane);
-  kv4_put_row<HD, true>(base, (int)slot, k, lane);
-  if (lane == 0) {
-    if (c.positions) c.positions[list * c.slots + slot] = (int32_t)p;
-    if (c.weights) c.weights[list * c.slots + slot] = 0.f;
+  row[0].load_turn(c.cs + p * (HD / 2), c.sn + p * (HD / 2), q);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int u = u0 + k * SIDE;
+    const int64_t list = (int64_t)s * c.nkv + (u >> 1);
+    row[k].c = row[0].c;
+    row[k].s = row[0].s;
+    kv4_put_row<HD>(kv4_list(c.kv, list, c.slots, Kv4<HD>::TB), (int)slot, row[k], q, !(u & 1),
+                    u < units);
+    if (u < units && (u & 1) && q == 0) {
+      if (c.positions) c.positions[list * c.slots + slot] = (int32_t)p;
+      if (c.weights) c.weights[list * c.slots + slot] = 0.f;
+    }
   }
 }
 
@@ -115,10 +127,10 @@ constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 
 // The order of the slots: larger is kept first.  NaN is 0, -0 equals +0.
 __device__ __forceinline__ uint32_t evict_key(float w, int32_t p, int32_t from, int32_t sinks) {
-  if (p >= from || p < sinks) w = INFINITY;
-  if (!(w == w)) return 0u;
-  const uint32_t u = __float_as_uint(w + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const bool first = (p >= from) | (p < sinks);  // selects, no branches
+  const uint32_t u = __float_as_uint(first ? INFINITY : w + 0.f);
+  const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (!first & !(w == w)) ? 0u : k;
 }
 
 // Work: per list the number of moves, then the slots given up below `keep` (holes) and the
@@ -156,21 +168,27 @@ __device__ __forceinline__ int again(int v) {
   return v;
 }
 
-// One workgroup per list; thread t holds the keys of slots t, t + 1024, ... (KPT of them; a
-// longer list is read again, segment by segment, for every pass).
+// One workgroup per list; a turn takes 4096 slots, four neighbouring ones per thread, and the
+// keys of T turns stay in registers (a longer list is read again, segment by segment, for every
+// pass).
 // - The keep-th largest key by digits of 11, 11 and 10 bits: a histogram in LDS (four copies
-//   for the first digit, where most keys share a few bins), then a scan from the top.
+//   for the first digit, where most keys share a few bins), then a scan from the top.  Where
+//   some of the keys equal to it go, their ranks decide (ranked).
 // - The ranks within a list need the counts of all waves' turns before one's own: every wave
 //   leaves the count of each turn, and one scan of the workgroup over them gives all ranks.
-// Bound: latency of these passes; 16000 slots are read in 3 us and take ten barriers.
-template <int KPT>
+// Bound: one CU's loads and vector instructions.  A slot per thread and turn, 11 bits a digit:
+// 29 us for 256 lists of 16000 slots, 72 for 48 lists of up to 61000 (in 30 of them the keys were
+// read and counted, in 29 the ranks made); four slots per thread, and ranks of equal keys only
+// where needed: see DESIGN.
+template <int T>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, Kv4Evict e, int half) {
-  constexpr int kBins = 2048, kSeg = KPT * kSelThreads;
-  __shared__ int hist[4][kBins], cnt[2][KPT * kSelWaves], part[kSelWaves], found[2];
+  constexpr int kBins = 2048, kTurn = 4 * kSelThreads, kSeg = T * kTurn, kCnt = T * kSelWaves;
+  __shared__ int hist[4][kBins], cnt[2][kCnt], part[kSelWaves], found[3];
   const int64_t list = blockIdx.x, lists = gridDim.x;
   const int64_t s = list / c.nkv % c.n_seq;
   const int64_t n64 = c.lengths[s];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint64_t below = (1ull << lane) - 1ull;
   int32_t *count = (int32_t *)e.work + list;
   const float *w = e.weights + list * c.slots;
@@ -191,22 +209,27 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
   const int64_t from64 = c.pos[s] - e.recent;
   const int32_t from = (int32_t)(from64 < -1 ? -1 : (from64 > INT32_MAX ? INT32_MAX : from64));
   const int32_t sinks = (int32_t)e.sinks;
-  uint32_t key[KPT];
+  uint32_t key[4 * T];
   int held = -1;  // the segment in `key`
   auto read = [&](int s0) {
     if (held == s0) return;
     held = s0;
-    const int tid = again(threadIdx.x);
+    const int at = 4 * again(threadIdx.x);
 #pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      const float *wk = w + s0 + k * kSelThreads;  // uniform
-      const int32_t *pk = p + s0 + k * kSelThreads;
-      key[k] = s0 + k * kSelThreads + tid < n ? evict_key(wk[tid], pk[tid], from, sinks) : 0u;
-      if (k % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // 16 loads in flight are enough
+    for (int t = 0; t < T; ++t) {
+      const int i = s0 + t * kTurn + at;
+      const int f = i < n ? i : 0;  // past the list: its first slots, not counted below
+      const float4 x = *(const float4 *)(w + f);
+      const int4 q = *(const int4 *)(p + f);
+      key[4 * t] = evict_key(x.x, q.x, from, sinks);
+      key[4 * t + 1] = evict_key(x.y, q.y, from, sinks);
+      key[4 * t + 2] = evict_key(x.z, q.z, from, sinks);
+      key[4 * t + 3] = evict_key(x.w, q.w, from, sinks);
+      if (t % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // 4 loads of a wave in flight at a time
     }
   };
   uint32_t prefix = 0;
-  int need = keep;  // of the keys that share the prefix, this many stay
+  int need = keep, alike = 0;  // of `alike` keys that share the prefix, `need` stay
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
@@ -217,14 +240,18 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
     __syncthreads();
     for (int s0 = 0; s0 < n; s0 += kSeg) {
       read(s0);
-      const int tid = again(threadIdx.x);
+      const int at = 4 * again(threadIdx.x);
+      int *h = hist[pass == 0 ? wave & 3 : 0];
 #pragma unroll
-      for (int k = 0; k < KPT; ++k) {
-        if (s0 + k * kSelThreads >= n) break;
-        const bool in = s0 + k * kSelThreads + tid < n &&
-                        (pass == 0 || (key[k] >> (shift + bits)) == (prefix >> (shift + bits)));
-        if (in) atomicAdd(&hist[pass == 0 ? wave & 3 : 0][(key[k] >> shift) & (kBins - 1) &
-                                                          ((1u << bits) - 1u)], 1);
+      for (int t = 0; t < T; ++t) {
+        if (s0 + t * kTurn >= n) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t k = key[4 * t + j];
+          if ((s0 + t * kTurn + at + j < n) &
+              (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))))
+            atomicAdd(&h[(k >> shift) & ((1u << bits) - 1u)], 1);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -241,79 +268,123 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
     if (before < need && before + h0 >= need) {
       found[0] = b0;
       found[1] = need - before;
+      found[2] = h0;
     } else if (before + h0 < need && before + h0 + h1 >= need) {
       found[0] = b0 - 1;
       found[1] = need - before - h0;
+      found[2] = h1;
     }
     __syncthreads();
     prefix |= (uint32_t)found[0] << shift;
     need = found[1];
+    alike = found[2];
   }
+  const bool ranked = need < alike;
   int32_t *holes = evict_holes(e.work, lists, list, half), *late = holes + half;
   int ties = 0, nh = 0, nl = 0;  // of the segments before
   for (int s0 = 0; s0 < n; s0 += kSeg) {
     read(s0);
-    uint64_t stays = 0;
-    int t = again(tid);
+    uint64_t stays = 0;  // bit k: the slot of key[k]
+    int at = 4 * again(tid), all;
+    if (!ranked) {
 #pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      const uint64_t m = __ballot(s0 + k * kSelThreads + t < n && key[k] == prefix);
-      if (lane == 0) cnt[0][k * kSelWaves + wave] = __popcll(m);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    __syncthreads();
-    int all;
-    {
-      const int v = tid < KPT * kSelWaves ? cnt[0][tid] : 0;
-      const int b = block_before(v, part, all);
-      if (tid < KPT * kSelWaves) cnt[0][tid] = ties + b;
+      for (int k = 0; k < 4 * T; ++k) {
+        stays |= (uint64_t)((s0 + (k >> 2) * kTurn + at + (k & 3) < n) & (key[k] >= prefix)) << k;
+        if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        int sum = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sum += __popcll(__ballot((s0 + t * kTurn + at + j < n) & (key[4 * t + j] == prefix)));
+        if (lane == 0) cnt[0][t * kSelWaves + wave] = sum;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __syncthreads();
+      const int v = tid < kCnt ? cnt[0][tid] : 0, b = block_before(v, part, all);
+      if (tid < kCnt) cnt[0][tid] = ties + b;
       ties += all;
-    }
-    __syncthreads();
-    t = again(tid);
+      __syncthreads();
+      at = 4 * again(tid);
 #pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      const bool in = s0 + k * kSelThreads + t < n, tie = in && key[k] == prefix;
-      const uint64_t m = __ballot(tie);
-      const bool st = in && (key[k] > prefix ||
-                             (tie && cnt[0][k * kSelWaves + wave] + __popcll(m & below) < need));
-      stays |= (uint64_t)st << k;
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    __syncthreads();
-    t = again(tid);
+      for (int t = 0; t < T; ++t) {
+        bool tie[4];
+        int rank = cnt[0][t * kSelWaves + wave];
 #pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      const int i = s0 + k * kSelThreads + t;
-      const bool st = (stays >> k) & 1u;
-      const uint64_t mh = __ballot(i < keep && !st), mm = __ballot(i >= keep && st);
+        for (int j = 0; j < 4; ++j) {
+          tie[j] = (s0 + t * kTurn + at + j < n) & (key[4 * t + j] == prefix);
+          rank += __popcll(__ballot(tie[j]) & below);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool st = (s0 + t * kTurn + at + j < n) &
+                          ((key[4 * t + j] > prefix) | (tie[j] & (rank < need)));
+          rank += tie[j];
+          stays |= (uint64_t)st << (4 * t + j);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __syncthreads();
+    }
+    // a hole: a slot below `keep` that goes; a move: one from `keep` on that stays
+    at = 4 * again(tid);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      int sh = 0, sm = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool low = s0 + t * kTurn + at + j < keep, st = (stays >> (4 * t + j)) & 1u;
+        const uint64_t m = __ballot(low != st), ml = __ballot(low);
+        sh += __popcll(m & ml);
+        sm += __popcll(m & ~ml);
+      }
       if (lane == 0) {
-        cnt[0][k * kSelWaves + wave] = __popcll(mh);
-        cnt[1][k * kSelWaves + wave] = __popcll(mm);
+        cnt[0][t * kSelWaves + wave] = sh;
+        cnt[1][t * kSelWaves + wave] = sm;
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int v = tid < KPT * kSelWaves ? cnt[j][tid] : 0;
-      const int b = block_before(v, part, all);
-      if (tid < KPT * kSelWaves) cnt[j][tid] = (j ? nl : nh) + b;
+      const int v = tid < kCnt ? cnt[j][tid] : 0, b = block_before(v, part, all);
+      if (tid < kCnt) cnt[j][tid] = (j ? nl : nh) + b;
       (j ? nl : nh) += all;
     }
     __syncthreads();
-    t = again(tid);
+    at = 4 * again(tid);
 #pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      if (s0 + k * kSelThreads >= n) break;
-      const int i = s0 + k * kSelThreads + t;  // keep < n: every hole is in use
-      const bool st = (stays >> k) & 1u, hole = i < keep && !st, moves = i >= keep && st;
-      const uint64_t mh = __ballot(hole), mm = __ballot(moves);
-      if (hole) holes[cnt[0][k * kSelWaves + wave] + __popcll(mh & below)] = i;
-      if (moves) late[cnt[1][k * kSelWaves + wave] + __popcll(mm & below)] = i;
-      if (i < keep && st) {
-        if (wo != w) wo[i] = w[i];
-        if (po != p) po[i] = p[i];
+    for (int t = 0; t < T; ++t) {
+      const int first = s0 + t * kTurn + wave * 256;  // of this wave's turn
+      if (first >= n) break;
+      const uint32_t mine = (uint32_t)(stays >> (4 * t)) & 15u;
+      auto put = [&](int32_t *to, int rank, bool hole) {
+        bool in[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool low = s0 + t * kTurn + at + j < keep, st = (mine >> j) & 1u;
+          in[j] = (low == hole) & (st != hole);
+          rank += __popcll(__ballot(in[j]) & below);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (in[j]) to[rank] = s0 + t * kTurn + at + j;
+          rank += in[j];
+        }
+      };
+      if (first < keep) put(holes, cnt[0][t * kSelWaves + wave], true);
+      if (first + 256 > keep) put(late, cnt[1][t * kSelWaves + wave], false);
+      if (first < keep && (wo != w || po != p)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = s0 + t * kTurn + at + j;
+          if (i < keep && (mine >> j) & 1u) {
+            if (wo != w) wo[i] = w[i];
+            if (po != p) po[i] = p[i];
+          }
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -415,9 +486,14 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(Kv4Cache c, Kv4Evi
 
 hipError_t launch_kv4_append(const Kv4Cache &c, const float *qkv, int64_t ldq, int64_t n_rows,
                              const int64_t *starts, hipStream_t s) {
-  const dim3 grid((unsigned)((n_rows + 3) / 4), (unsigned)c.nkv);
-  KV4_DISPATCH(c.hd, hipLaunchKernelGGL(kv4_append_kernel<HD>, grid, dim3(kThreads), 0, s, c, qkv,
-                                        ldq, (uint32_t)n_rows, starts));
+  // few rows: as many waves as there are units; many: fewer waves with more in flight
+  const int n = n_rows * c.nkv >= 8192 ? 4 : 1, per = n * (256 / c.hd);
+  const dim3 grid((unsigned)((n_rows + 3) / 4), (unsigned)((2 * c.nkv + per - 1) / per));
+  KV4_DISPATCH(c.hd, if (n == 4) hipLaunchKernelGGL((kv4_append_kernel<HD, 4>), grid,
+                                                    dim3(kThreads), 0, s, c, qkv, ldq,
+                                                    (uint32_t)n_rows, starts);
+               else hipLaunchKernelGGL((kv4_append_kernel<HD, 1>), grid, dim3(kThreads), 0, s, c,
+                                       qkv, ldq, (uint32_t)n_rows, starts));
   return hipGetLastError();
 }
 
@@ -440,11 +516,11 @@ hipError_t launch_kv4_evict(const Kv4Cache &c, const Kv4Evict &e, hipStream_t s)
   const int half = c.slots / 2;  // at most min(keep, slots - keep) slots move
   const dim3 sel((unsigned)lists), st(kSelThreads);
   if (c.slots <= 4 * kSelThreads)
-    hipLaunchKernelGGL(evict_select_kernel<4>, sel, st, 0, s, c, e, half);
+    hipLaunchKernelGGL(evict_select_kernel<1>, sel, st, 0, s, c, e, half);
   else if (c.slots <= 16 * kSelThreads)
-    hipLaunchKernelGGL(evict_select_kernel<16>, sel, st, 0, s, c, e, half);
+    hipLaunchKernelGGL(evict_select_kernel<4>, sel, st, 0, s, c, e, half);
   else
-    hipLaunchKernelGGL(evict_select_kernel<64>, sel, st, 0, s, c, e, half);
+    hipLaunchKernelGGL(evict_select_kernel<16>, sel, st, 0, s, c, e, half);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   const int64_t most = e.keep < c.slots - e.keep ? e.keep : c.slots - e.keep;

@@ -285,7 +285,10 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
   // What comes before the barrier is requested before the tile, since loads return in order:
   // behind a full chip's tiles the queries took 5.6 us (130000 slots).
   float4 xo[2], xp[2], cv[2], sv[2];  // wave < NSUB: the queries of group `wave`: lane (r, g)
-  Kv4Row<HD> row;                     // holds channels 32 b + 8 g + 0..7 of its row
+                                      // holds channels 32 b + 8 g + 0..7 of its row
+  constexpr int LANES = Kv4Row<HD>::LANES, STORERS = HD == 256 ? 2 : 1;
+  Kv4Row<HD> row;  // waves NSUB ..: the new row's K (unit 0) and V (1), HD / 4 lanes each
+  const int unit = (wave - NSUB) * (64 / LANES) + lane / LANES, rq = lane % LANES;
   if (wave < NSUB) {
     const int v = v0 + wave * HPS + h, i = v < V ? v / grp : 0;
     const float *x = row0 + i * a.ldq + (int64_t)(kvh * grp + (v < V ? v % grp : 0)) * HD;
@@ -298,11 +301,9 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
       cv[j] = *(const float4 *)(c.cs + p + 4 * j);
       sv[j] = *(const float4 *)(c.sn + p + 4 * j);
     }
-  } else if (stores && wave == NSUB) {
-    row.load(kx, lane);
-    row.load_turn(c.cs + pos0 * half, c.sn + pos0 * half, lane);
-  } else if (stores && wave == NSUB + 1) {
-    row.load(vx, lane);
+  } else if (stores && wave < NSUB + STORERS && unit < 2) {
+    row.load(unit ? vx : kx, rq);
+    row.load_turn(c.cs + pos0 * half, c.sn + pos0 * half, rq);
   }
   __builtin_amdgcn_sched_barrier(0);
   TileRegs<HD> d;
@@ -347,44 +348,33 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
       q_[wave][k][0][lane] = b == k ? hi : zero;
       q_[wave][k][1][lane] = b == k ? lo : zero;
     }
-  } else if (stores && wave < NSUB + 2) {
-    const bool writes = blockIdx.z == 0;
-    const int j = filled % kKv4Tile;
-    uint8_t byte[HD / 64];
-    half_t scale[HD / 64];
+  } else if (stores && wave < NSUB + STORERS) {
+    uint32_t word;
+    half_t scale;
+    kv4_quantize<HD>(row, rq, unit == 0, word, scale);
+    const int j = filled % kKv4Tile, blk = rq >> 3;
     uint8_t *to = base + (int64_t)(filled / kKv4Tile) * L::TB;
-    if (wave == NSUB) {
-      kv4_quantize<HD, true>(row, lane, byte, scale);
+    const bool writes = blockIdx.z == 0;
+    if (unit == 0 && !(rq & 1)) {
+      const int at = (((rq >> 1) & 3) * NB + blk) * 4;
+      *(uint32_t *)(fresh[0] + at) = word;
+      if (writes) *(uint32_t *)(to + j * half + at) = word;
+    } else if (unit == 1 && (rq & 7) < 4) {
 #pragma unroll
-      for (int k = 0; k < HD / 64; ++k) {
-        const int blk = 2 * k + (lane >> 5), at = (((lane >> 3) & 3) * NB + blk) * 4 + (lane & 3);
-        if ((lane & 7) < 4) {
-          fresh[0][at] = byte[k];
-          if (writes) to[j * half + at] = byte[k];
-        }
-        if ((lane & 31) == 0) {
-          fscale[0][blk] = scale[k];
-          if (writes) *(half_t *)(to + L::KS + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = scale[k];
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int at = (4 * (rq & 3) + i) * NB + blk;
+        fresh[1][at] = (uint8_t)(word >> (8 * i));
+        if (writes) to[L::VO + (j >> 2) * (2 * HD) + at * 4 + (j & 3)] = (uint8_t)(word >> (8 * i));
       }
-    } else {
-      kv4_quantize<HD, false>(row, lane, byte, scale);
-#pragma unroll
-      for (int k = 0; k < HD / 64; ++k) {
-        const int blk = 2 * k + (lane >> 5), at = (lane & 15) * NB + blk;
-        if ((lane & 31) < 16) {
-          fresh[1][at] = byte[k];
-          if (writes) to[L::VO + (j >> 2) * (2 * HD) + at * 4 + (j & 3)] = byte[k];
-        }
-        if ((lane & 31) == 0) {
-          fscale[1][blk] = scale[k];
-          if (writes) *(half_t *)(to + L::VS + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = scale[k];
-        }
-      }
-      if (lane == 0 && writes) {
-        if (c.positions) c.positions[list * c.slots + filled] = (int32_t)pos0;
-        if (c.weights) c.weights[list * c.slots + filled] = 0.f;
-      }
+    }
+    if (unit < 2 && !(rq & 7)) {
+      fscale[unit][blk] = scale;
+      if (writes)
+        *(half_t *)(to + (unit ? L::VS : L::KS) + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = scale;
+    }
+    if (writes && unit == 1 && rq == 0) {
+      if (c.positions) c.positions[list * c.slots + filled] = (int32_t)pos0;
+      if (c.weights) c.weights[list * c.slots + filled] = 0.f;
     }
   }
   __syncthreads();
