@@ -32,6 +32,13 @@ torch f32 ops instead, and ``fused=False`` does the same for decode steps.
 A decode step keeps
 the token and position in device tensors, so it can be captured once in a HIP
 graph and replayed for every generated token without host synchronization.
+
+``kv_bits=4`` holds the caches in 4 bits (``kv4``): a prompt's rows attend in f32 to what the
+cache holds (read back) and to each other, and are stored quantized; a decode step stores its
+row and attends over the codes.  With ``kv_keep`` the caches have a fixed number of slots,
+independent of ``max_seq``: each slot's attention weight is accumulated (the last rows of a
+prompt, then every step), and a full cache is cut back to the ``kv_keep`` slots of largest
+weight, the latest and the first positions always among them.
 """
 
 from __future__ import annotations
@@ -44,7 +51,7 @@ from typing import Optional, Union
 import numpy as np
 import torch
 
-from . import glue, quantize
+from . import glue, kv4, quantize
 from .ggml import FUSED_TYPES, Q4_K, Q6_K, TILE_ROWS, raw_row_bytes
 from .linear import (GGUFWeight, LayerWeights, QuantEmbedding, concat_rows, dispatch_matmul_gguf,
                      interleave_tiles, repack_gguf_for_gpu, split_interleaved)
@@ -219,19 +226,34 @@ def glue_shapes(cfg: DecoderConfig) -> bool:
 
 
 class QuantDecoder:
-    """Greedy decoder over ``DecoderWeights`` with an f32 KV cache in HBM."""
+    """Greedy decoder over ``DecoderWeights`` with an f32 or 4-bit KV cache in HBM.
+
+    ``kv_bits`` 4: ``kv_slots`` (default: enough for ``max_seq``) slots per KV head, rounded up
+    to a multiple of 32; ``kv_keep``: a full cache is cut back to that many slots, of which the
+    last ``kv_recent`` and the first ``kv_sinks`` positions are never given up.  ``max_seq``
+    then bounds the positions only."""
+
+    WINDOW = 32  # rows at a prompt's end whose attention weights are counted
 
     def __init__(self, cfg: DecoderConfig, weights: DecoderWeights, device="cuda",
-                 fused: bool = True, hip_glue: bool = True):
+                 fused: bool = True, hip_glue: bool = True, kv_bits: int = 32,
+                 kv_slots: Optional[int] = None, kv_keep: Optional[int] = None,
+                 kv_recent: int = 64, kv_sinks: int = 4):
         # a weight of a type without fused decode-step kernels runs the step unfused
         grid = any(w.ggml_type not in FUSED_TYPES for w in all_weights(weights))
         self.cfg, self.w, self.device = cfg, weights, torch.device(device)
         self.fused = fused and not grid
         self.hip_glue = hip_glue and glue_shapes(cfg)
         L, kv, T, hd = cfg.n_layers, cfg.n_kv_heads, cfg.max_seq, cfg.head_dim
-        self.k_cache = torch.zeros(L, kv, T, hd, device=self.device)
-        self.v_cache = torch.zeros(L, kv, T, hd, device=self.device)
-        self.cos, self.sin = rope_tables(cfg, self.device)
+        self.kv_bits, self.kv_keep = kv_bits, kv_keep
+        if kv_bits == 4:
+            self._init_kv4(kv_slots, kv_keep, kv_recent, kv_sinks)
+        elif kv_bits != 32 or kv_slots is not None or kv_keep is not None:
+            raise ValueError(f"kv_bits {kv_bits} not 32 or 4, or kv_slots / kv_keep without 4")
+        else:
+            self.k_cache = torch.zeros(L, kv, T, hd, device=self.device)
+            self.v_cache = torch.zeros(L, kv, T, hd, device=self.device)
+            self.cos, self.sin = rope_tables(cfg, self.device)
         self.t_idx = torch.arange(T, device=self.device)
         self._graph = None
         # static buffers of the fused decode step
@@ -241,8 +263,101 @@ class QuantDecoder:
         self.b_att, self.b_o = e(cfg.n_heads * hd), e(d)
         self.b_gu, self.b_a, self.b_d = e(2 * cfg.ffn), e(cfg.ffn), e(d)
         self.b_logits = e(cfg.vocab)
-        self.w_att = glue.attention_workspace(cfg.n_heads, cfg.n_kv_heads, hd, T, self.device)
+        if kv_bits == 32:
+            self.w_att = glue.attention_workspace(cfg.n_heads, cfg.n_kv_heads, hd, T, self.device)
         self.w_arg = glue.argmax_workspace(self.device)
+
+    # -- the 4-bit cache --
+    def _init_kv4(self, slots, keep, recent, sinks) -> None:
+        cfg, dev = self.cfg, self.device
+        if not (self.fused and self.hip_glue):
+            raise ValueError("kv_bits=4 needs the fused decode step and the HIP glue")
+        slots = -(-(cfg.max_seq if slots is None else slots) // kv4.TILE) * kv4.TILE
+        if keep is not None and not (0 <= recent and 0 <= sinks
+                                     and recent + sinks <= keep < slots):
+            raise ValueError(f"kv_keep {keep}: kv_recent {recent} + kv_sinks {sinks} must fit it, and "
+                             f"it must be below the {slots} slots")
+        L, nkv, hd = cfg.n_layers, cfg.n_kv_heads, cfg.head_dim
+        self.kv_slots, self.kv_recent, self.kv_sinks = slots, recent, sinks
+        self.kv4 = kv4.empty(1, nkv, hd, slots, dev, n_layers=L)
+        self.kv_lengths = torch.zeros(1, dtype=torch.long, device=dev)
+        # one layer's rows in f32, for the attention of a prompt
+        self.k_cache = torch.zeros(nkv, slots, hd, device=dev)
+        self.v_cache = torch.zeros(nkv, slots, hd, device=dev)
+        # a prompt's slot t stands at position t + an offset below max_seq
+        self.cos, self.sin = rope_tables(
+            dataclasses.replace(cfg, max_seq=cfg.max_seq + slots), dev)
+        self.kv_weights = self.kv_positions = None
+        if keep is not None:
+            self.kv_weights = torch.zeros(L, 1, nkv, slots, device=dev)
+            self.kv_positions = torch.zeros(L, 1, nkv, slots, dtype=torch.int32, device=dev)
+            self.w_evict = kv4.evict_workspace(self.kv4)
+        self.w_att = kv4.attention_workspace(self.kv4[0], cfg.n_heads, weights=keep is not None)
+        self.w_window = {}  # by rows: workspaces of a prompt's last rows
+
+    def _kv_slot(self, l: int):
+        """Layer l's positions and weights (None without eviction)."""
+        if self.kv_keep is None:
+            return dict(positions=None, weights=None)
+        return dict(positions=self.kv_positions[l], weights=self.kv_weights[l])
+
+    def _evict(self, pos: torch.Tensor) -> None:
+        """Cut the caches back if they are full (decided on the device)."""
+        kv4.evict(self.kv4, self.kv_weights, self.kv_positions, self.kv_lengths, pos, self.kv_keep,
+                  self.w_evict, recent=self.kv_recent, sinks=self.kv_sinks, trigger=self.kv_slots)
+
+    def _cache_state(self) -> list:
+        """The tensors that a step changes, besides token and position."""
+        if self.kv_bits == 32:
+            return [self.k_cache, self.v_cache]
+        return [t for t in (self.kv4, self.kv_lengths, self.kv_weights, self.kv_positions)
+                if t is not None]
+
+    def _attend_rows(self, l: int, qkv: torch.Tensor, pos: torch.Tensor, att: torch.Tensor,
+                     held: int) -> None:
+        """Attention of a prompt's rows in layer l; ``held`` slots are in use before them."""
+        cfg = self.cfg
+        if self.kv_bits == 32:
+            glue.attention_prefill(qkv, pos, self.cos, self.sin, self.k_cache[l], self.v_cache[l],
+                                   att, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim)
+            return
+        m, cache = qkv.shape[0], self.kv4[l]
+        first = pos[:1]
+        if held:
+            kv4.load(cache, self.kv_lengths, self.k_cache[None], self.v_cache[None])
+        off = self._prompt_pos - held
+        glue.attention_prefill(qkv, pos - off, self.cos.narrow(0, off, self.kv_slots),
+                               self.sin.narrow(0, off, self.kv_slots), self.k_cache, self.v_cache,
+                               att, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim)
+        kv4.append(qkv, self.kv_lengths, first, self.cos, self.sin, cache, cfg.n_heads,
+                   **self._kv_slot(l))
+        if self.kv_keep is not None:
+            w = min(m, self.WINDOW)
+            if w not in self.w_window:
+                self.w_window[w] = kv4.attention_workspace(cache, cfg.n_heads, rows=w, weights=True)
+            kv4.attention(qkv[m - w:], self.kv_lengths + (m - w), first + (m - w), self.cos,
+                          self.sin, cache, torch.empty_like(att[:w]), cfg.n_heads,
+                          self.w_window[w], store=False, weights=self.kv_weights[l],
+                          accumulate=True)
+
+    def _prefill_kv4(self, tokens: torch.Tensor, pos0: int) -> torch.Tensor:
+        if pos0 == 0:
+            self.kv_lengths.zero_()
+        held, done, h = int(self.kv_lengths.item()), 0, None
+        while done < tokens.numel():
+            m = min(tokens.numel() - done, self.kv_slots - held)
+            if m == 0:
+                raise ValueError(f"sequence exceeds the cache's {self.kv_slots} slots (kv_keep "
+                                 "bounds it)")
+            self._prompt_pos = pos0 + done
+            pos = torch.arange(pos0 + done, pos0 + done + m, device=self.device)
+            h = self._layers_glue(self._embed(tokens[done:done + m]), pos, held)
+            self.kv_lengths += m
+            held, done = held + m, done + m
+            if self.kv_keep is not None and held == self.kv_slots:
+                self._evict(pos[-1:] + 1)
+                held = self.kv_keep
+        return self._proj(h[-1:], self.w.lm_head_gg, "lm_head")
 
     # -- one pass of all layers over M tokens at positions ``pos`` (device [M]) --
     def _proj(self, x: torch.Tensor, w: GGUFWeight, label: str) -> torch.Tensor:
@@ -305,9 +420,10 @@ class QuantDecoder:
             x = x + self._proj(a, lw.down_gg, f"L{l}-down")
         return x
 
-    def _layers_glue(self, x: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
+    def _layers_glue(self, x: torch.Tensor, pos: torch.Tensor, held: int = 0) -> torch.Tensor:
         """All layers over the M rows of ``x`` (updated in place) with the glue as
-        libgguf_hip kernels; returns the rows after the final RMSNorm."""
+        libgguf_hip kernels; returns the rows after the final RMSNorm.  ``held``: the
+        slots of a 4-bit cache in use before the rows."""
         cfg, layers = self.cfg, self.w.layers
         M = x.shape[0]
         h = torch.empty_like(x)
@@ -316,9 +432,7 @@ class QuantDecoder:
         glue.rmsnorm(x, layers[0].attn_norm, cfg.eps, h)
         for l, lw in enumerate(layers):
             qkv = self._proj_slot(h, lw, "qkv", f"L{l}-qkv")
-            glue.attention_prefill(qkv, pos, self.cos, self.sin, self.k_cache[l],
-                                   self.v_cache[l], att, cfg.n_heads, cfg.n_kv_heads,
-                                   cfg.head_dim)
+            self._attend_rows(l, qkv, pos, att, held)
             glue.add_rmsnorm(x, self._proj(att, lw.o_gg, f"L{l}-o"), lw.ffn_norm, cfg.eps, h)
             w = lw.get("gateUpI_gg")
             if w is not None:  # tile-interleaved gate / up columns -> [gate | up] rows, one copy
@@ -339,10 +453,13 @@ class QuantDecoder:
     @torch.no_grad()
     def prefill(self, tokens: torch.Tensor, pos0: int = 0) -> torch.Tensor:
         """Run ``tokens`` (device int64 [M]) at positions pos0.. and return the
-        last position's logits [1, vocab]."""
+        last position's logits [1, vocab].  With a 4-bit cache ``pos0`` is 0 (a new
+        sequence) or the position after the last one."""
         M = tokens.numel()
         if pos0 + M > self.cfg.max_seq:
             raise ValueError(f"sequence of {pos0 + M} exceeds max_seq {self.cfg.max_seq}")
+        if self.kv_bits == 4:
+            return self._prefill_kv4(tokens, pos0)
         pos = torch.arange(pos0, pos0 + M, device=self.device)
         x = self._embed(tokens)
         if self.hip_glue:
@@ -362,16 +479,23 @@ class QuantDecoder:
         SwiGLU epilogue (interleaved gate / up tiles), down projection
         accumulated into the residual.  With concatenated or split gate / up
         weights, SwiGLU runs as the down projection's prologue instead; with
-        n_heads * head_dim above 8192 the attention merges its own records."""
+        n_heads * head_dim above 8192 the attention merges its own records.  A 4-bit
+        cache's attention writes its output (a second launch where the slots are
+        split), and eviction adds two launches per step."""
         cfg, W = self.cfg, self.w
         x = self.b_x
-        merge = cfg.n_heads * cfg.head_dim <= 8192
+        merge = cfg.n_heads * cfg.head_dim <= 8192 and self.kv_bits == 32
         self._embed(tok, x)
         for l, lw in enumerate(W.layers):
             self._fused_slot(x, lw, "qkv", self.b_qkv, lw.attn_norm)
-            glue.attention_decode(self.b_qkv, pos, self.cos, self.sin, self.k_cache[l],
-                                  self.v_cache[l], None if merge else self.b_att, cfg.n_heads,
-                                  cfg.n_kv_heads, cfg.head_dim, self.w_att)
+            if self.kv_bits == 4:
+                kv4.attention(self.b_qkv, self.kv_lengths, pos, self.cos, self.sin, self.kv4[l],
+                              self.b_att, cfg.n_heads, self.w_att, accumulate=True,
+                              **self._kv_slot(l))
+            else:
+                glue.attention_decode(self.b_qkv, pos, self.cos, self.sin, self.k_cache[l],
+                                      self.v_cache[l], None if merge else self.b_att, cfg.n_heads,
+                                      cfg.n_kv_heads, cfg.head_dim, self.w_att)
             if merge:
                 glue.matmul_attn_merge(self.w_att, pos, lw.o_gg, x, cfg.n_heads, cfg.n_kv_heads,
                                        cfg.head_dim, cfg.max_seq, accumulate=True)
@@ -390,6 +514,10 @@ class QuantDecoder:
                           cfg.eps)
         glue.argmax(self.b_logits, tok, self.w_arg)
         pos.add_(1)
+        if self.kv_bits == 4:
+            self.kv_lengths.add_(1)
+            if self.kv_keep is not None:
+                self._evict(pos)
         return self.b_logits
 
     def _fused_slot(self, x, lw, slot, y, norm_w) -> None:
@@ -421,22 +549,22 @@ class QuantDecoder:
         s = torch.cuda.Stream(device=self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
         t0, p0 = tok.clone(), pos.clone()
-        kc, vc = self.k_cache.clone(), self.v_cache.clone()
+        saved = [t.clone() for t in self._cache_state()]
+
+        def restore():
+            tok.copy_(t0)
+            pos.copy_(p0)
+            for t, before in zip(self._cache_state(), saved):
+                t.copy_(before)
+
         with torch.cuda.stream(s):
             self.step(tok, pos)                    # warm-up outside the graph
         torch.cuda.current_stream(self.device).wait_stream(s)
-        tok.copy_(t0)
-        pos.copy_(p0)
-        self.k_cache.copy_(kc)
-        self.v_cache.copy_(vc)
+        restore()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self._graph_logits = self.step(tok, pos)
-        tok.copy_(t0)
-        pos.copy_(p0)
-        self.k_cache.copy_(kc)
-        self.v_cache.copy_(vc)
-        del kc, vc
+        restore()
         self._graph = g
 
     @torch.no_grad()
@@ -447,8 +575,13 @@ class QuantDecoder:
         if prompt.numel() + n_new > self.cfg.max_seq:
             raise ValueError(f"prompt {prompt.numel()} + {n_new} new tokens exceed max_seq "
                              f"{self.cfg.max_seq}")
-        self.k_cache.zero_()
-        self.v_cache.zero_()
+        if (self.kv_bits == 4 and self.kv_keep is None
+                and prompt.numel() + n_new > self.kv_slots + 1):
+            raise ValueError(f"prompt {prompt.numel()} + {n_new} new tokens exceed the cache's "
+                             f"{self.kv_slots} slots (kv_keep bounds it)")
+        if self.kv_bits == 32:
+            self.k_cache.zero_()
+            self.v_cache.zero_()
         torch.cuda.synchronize(dev)
         t0 = time.perf_counter()
         logits = self.prefill(prompt, 0)

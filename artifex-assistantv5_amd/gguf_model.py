@@ -85,8 +85,9 @@ def unpermute_rows(n_heads: int, head_dim: int) -> np.ndarray:
 
 
 def load_decoder(path: str, device="cuda", max_seq: int = 2048, fused: bool = True,
-                 on_progress=None) -> Tuple[QuantDecoder, LoadedGGUFModel]:
-    """Load a llama-architecture GGUF file into a ``QuantDecoder`` on ``device``."""
+                 on_progress=None, **cache) -> Tuple[QuantDecoder, LoadedGGUFModel]:
+    """Load a llama-architecture GGUF file into a ``QuantDecoder`` on ``device``; ``cache``: the
+    decoder's ``kv_bits``, ``kv_slots``, ``kv_keep``, ``kv_recent`` and ``kv_sinks``."""
     file = parse_gguf_path(path)
     cfg = config_from_gguf(file, max_seq)
     _check_tensors(file, cfg)
@@ -169,4 +170,4 @@ def load_decoder(path: str, device="cuda", max_seq: int = 2048, fused: bool = Tr
         raise ValueError(f"[GGUF] token_embd.weight is [{embed.n}, {embed.k}], expected "
                          f"[{cfg.vocab}, {d}]")
     weights = DecoderWeights(layers, vec("output_norm.weight", d), lm, embed)
-    return QuantDecoder(cfg, weights, device=dev, fused=fused), loaded
+    return QuantDecoder(cfg, weights, device=dev, fused=fused, **cache), loaded

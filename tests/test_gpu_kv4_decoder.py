@@ -1,0 +1,152 @@
+"""QuantDecoder with a 4-bit KV cache: prompts, decode steps and eviction.
+
+The reference is the float64 decoder of test_gpu_decoder.py, whose attention takes the rows that
+the decoder's own cache holds (read back): what the codes are is tested bit for bit in
+test_gpu_kv4.py, so only the arithmetic around them remains, to the tolerance of that file's
+float64 comparisons (1e-4 of the logits).
+"""
+import importlib
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_decoder import TINY, Reference, _rel  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dec():
+    return importlib.import_module("artifex-assistantv5_amd.decoder")
+
+
+@pytest.fixture(scope="module")
+def kv4(pkg):
+    return importlib.import_module("artifex-assistantv5_amd.kv4")
+
+
+def _model(dec, **over):
+    cfg = dec.DecoderConfig(**{**TINY, **over})
+    return cfg, dec.synthetic_weights(cfg, seed=3, device="cuda", distinct_layers=True)
+
+
+class FromCache(Reference):
+    """A Reference whose attention takes the given rows of each layer, [T, n_kv, hd]."""
+
+    def token(self, tok, pos, rows):
+        c = self.cfg
+        x = self.embed[tok]
+        nh, nkv, hd = c.n_heads, c.n_kv_heads, c.head_dim
+        for (K, V), L in zip(rows, self.layers):
+            qkv = L["qkv"] @ self.norm(x, L["an"])
+            q = self.rope(qkv[:nh * hd].view(nh, hd), pos)
+            heads = []
+            for h in range(nh):
+                kv = h // (nh // nkv)
+                s = (K[:, kv] @ q[h]) / hd ** 0.5
+                p = torch.exp(s - s.max())
+                heads.append((p / p.sum()) @ V[:, kv])
+            x = x + L["o"] @ torch.cat(heads)
+            gu = L["gu"] @ self.norm(x, L["fn"])
+            g, u = gu[:c.ffn], gu[c.ffn:]
+            x = x + L["down"] @ (u * g / (1 + torch.exp(-g)))
+        return self.lm @ self.norm(x, self.fnorm)
+
+
+def _cached(kv4, m):
+    """The cached rows of every layer, float64 [T, n_kv, hd]."""
+    n = int(m.kv_lengths.item())
+    shape = (*m.kv4.shape[:3], n, m.cfg.head_dim)
+    k, v = (torch.zeros(shape, device="cuda") for _ in range(2))
+    kv4.load(m.kv4, m.kv_lengths, k, v)
+    return [(a[0].transpose(0, 1).double(), b[0].transpose(0, 1).double()) for a, b in zip(k, v)]
+
+
+def _tokens(cfg, n, seed):
+    return torch.from_numpy(np.random.default_rng(seed).integers(0, cfg.vocab, n)).cuda()
+
+
+@pytest.mark.parametrize("over", [{}, dict(n_heads=2, n_kv_heads=1, head_dim=128),
+                                  dict(n_heads=8, n_kv_heads=1, head_dim=256)])
+def test_prompt_and_steps(dec, kv4, over):
+    cfg, w = _model(dec, **over)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4)
+    exact = Reference(cfg, w)
+    ref = FromCache(cfg, w)
+    prompt = _tokens(cfg, 30, 5)
+    logits = m.prefill(prompt, 0)[0]
+    for p, t in enumerate(prompt.tolist()):
+        rl = exact.token(t, p)
+    assert _rel(logits, rl) < 1e-4           # one chunk: its rows attend in f32
+    tok, pos = torch.argmax(logits).view(1), torch.tensor([30], device="cuda")
+    for _ in range(4):
+        t, p = int(tok.item()), int(pos.item())
+        lg = m.step(tok, pos)[0]
+        assert int(m.kv_lengths.item()) == p + 1
+        assert _rel(lg, ref.token(t, p, _cached(kv4, m))) < 1e-4
+    # a second prompt behind the steps: the last row attends to the cache and, in f32, its chunk
+    more = _tokens(cfg, 7, 6)
+    held = _cached(kv4, m)
+    lg = m.prefill(more, 34)[0]
+    assert int(m.kv_lengths.item()) == 41
+    ref2 = Reference(cfg, w)
+    ref2.k, ref2.v = [list(k) for k, _ in held], [list(v) for _, v in held]
+    for i, t in enumerate(more.tolist()):
+        rl = ref2.token(t, 34 + i)
+    assert _rel(lg, rl) < 1e-4
+
+
+def test_graph_matches_eager_with_eviction(dec):
+    """Generation over a cache that fills up again and again; prompts longer than the cache."""
+    cfg, w = _model(dec, max_seq=400)
+    for prompt_len in (20, 150):
+        prompt = _tokens(cfg, prompt_len, 7)
+        outs = []
+        for graph in (False, True):
+            m = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=64, kv_keep=40, kv_recent=16)
+            outs.append(m.generate(prompt, 120, graph=graph)["tokens"])
+            n = int(m.kv_lengths.item())
+            assert 40 <= n < 64
+            at = m.kv_positions[:, 0, :, :n]
+            last = prompt_len + 119 - 1          # of the last token that was fed
+            for row in at.reshape(-1, n).tolist():
+                assert len(set(row)) == n and set(range(4)) <= set(row)
+                assert set(range(last - 15, last + 1)) <= set(row) and max(row) == last
+        assert torch.equal(*outs)
+
+
+def test_eviction_keeps_what_fits(dec):
+    """Until the cache is full nothing differs from a cache without eviction."""
+    cfg, w = _model(dec, max_seq=128)
+    prompt = _tokens(cfg, 30, 8)
+    a = dec.QuantDecoder(cfg, w, kv_bits=4).generate(prompt, 30)["tokens"]
+    b = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=96, kv_keep=48,
+                         kv_recent=10).generate(prompt, 30)["tokens"]
+    assert torch.equal(a, b)
+
+
+def test_weights_of_a_prompt(dec, kv4):
+    """After a prompt each slot holds the attention weight of the last rows: per layer and KV
+    head they add up to one per row and query head."""
+    cfg, w = _model(dec)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=64, kv_keep=40, kv_recent=8)
+    m.prefill(_tokens(cfg, 50, 9), 0)
+    s = m.kv_weights[:, 0, :, :50].double().sum(-1)
+    grp = cfg.n_heads // cfg.n_kv_heads
+    assert torch.allclose(s, torch.full_like(s, 32.0 * grp), rtol=1e-5)
+
+
+def test_refusals(dec):
+    cfg, w = _model(dec)
+    for bad in (dict(kv_bits=8), dict(kv_slots=64), dict(kv_keep=32), dict(kv_bits=4, fused=False),
+                dict(kv_bits=4, hip_glue=False), dict(kv_bits=4, kv_slots=64, kv_keep=64),
+                dict(kv_bits=4, kv_keep=20, kv_recent=17), dict(kv_bits=4, kv_slots=0)):
+        with pytest.raises(ValueError):
+            dec.QuantDecoder(cfg, w, **bad)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=32)
+    with pytest.raises(ValueError, match="slots"):
+        m.prefill(_tokens(cfg, 33, 1), 0)
+    with pytest.raises(ValueError, match="slots"):
+        m.generate(_tokens(cfg, 20, 1), 20)
