@@ -11,7 +11,14 @@ namespace gguf {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kLog2e = 1.4426950408889634f;
+
+// log2(e) / sqrt(head_dim) as two floats: one alone would be off by up to 2^-25, and that times
+// a score is the relative error of its probability.
+template <int HD>
+struct ScoreScale {
+  static constexpr double v = 1.4426950408889634074 / (HD == 64 ? 8.0 : (HD == 128 ? 11.313708498984760390 : 16.0));
+  static constexpr float hi = (float)v, lo = (float)(v - (double)hi);
+};
 
 // A record: sum of p v per channel, then per block of 32 channels the maximum m that its p
 // are relative to (in log2 units) and the sum of its p.
@@ -107,30 +114,29 @@ __host__ __device__ __forceinline__ int64_t score_stride(int slots) {
   return (int64_t)(((slots + 63) / 64) | 1) * 64;
 }
 
-// Eight 4-bit codes (element 0..3 in the low nibbles of bytes 0..3, 4..7 in the high ones) as
-// f16 integers 0..15: a byte below 16 read as E4M3 is code * 2^-9, exactly.
-__device__ __forceinline__ half8_t k_codes(uint32_t w) {
-  const uint32_t lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
-  const uint32_t r[4] = {
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true))};
-  return __builtin_bit_cast(half8_t, r);
-}
-// Codes of V as f16 integers: bits 0-3 and 16-19 of w give code - 8 (1024 + code, less 1032),
+// 4-bit codes as f16 integers: bits 0-3 and 16-19 of w give code - 8 (1024 + code, less 1032),
 // bits 4-7 and 20-23 give 16 (code - 8) (1024 + 16 code, less 1152) without a shift.  `magic`
-// holds 1024.0 twice in a vector register, so that mask and OR are one instruction.
+// holds 1024.0 twice in a vector register, so that mask and OR are one instruction.  The
+// offset goes before the matrix core: left to the sums (as -8 sum q, or -8 sum w at the end) it
+// costs them low bits (scores: 1.0e-6 in log2 units against 4e-7 of a plain f32 product).
 template <int SCALE>
-__device__ __forceinline__ half2_t v_codes(uint32_t w, uint32_t magic) {
+__device__ __forceinline__ half2_t codes2(uint32_t w, uint32_t magic) {
   const half2_t c = __builtin_bit_cast(half2_t, (w & (0x000F000Fu * SCALE)) | magic);
   return c - half2_t{(half_t)(1024.f + 8.f * SCALE), (half_t)(1024.f + 8.f * SCALE)};
 }
+// A word of K: elements 0, 2, 1, 3, then 16 times elements 4, 6, 5, 7.
+__device__ __forceinline__ half8_t k_frag(uint32_t w, uint32_t magic) {
+  const uint32_t h = w >> 8;
+  const half2_t r[4] = {codes2<1>(w, magic), codes2<1>(h, magic), codes2<16>(w, magic),
+                        codes2<16>(h, magic)};
+  return __builtin_bit_cast(half8_t, r);
+}
+// Two words of V (h: 8 bits on): slots 0, 2, 1, 3 of both.
 template <int SCALE>
 __device__ __forceinline__ half8_t v_frag(uint32_t w0, uint32_t h0, uint32_t w1, uint32_t h1,
                                           uint32_t magic) {
-  const half2_t r[4] = {v_codes<SCALE>(w0, magic), v_codes<SCALE>(h0, magic),
-                        v_codes<SCALE>(w1, magic), v_codes<SCALE>(h1, magic)};
+  const half2_t r[4] = {codes2<SCALE>(w0, magic), codes2<SCALE>(h0, magic),
+                        codes2<SCALE>(w1, magic), codes2<SCALE>(h1, magic)};
   return __builtin_bit_cast(half8_t, r);
 }
 __device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) {
@@ -142,14 +148,17 @@ __device__ __forceinline__ float mul_f16(float x, half_t h) { return fmaf(x, (fl
 
 // v plus that of the lane N to the left in its 16, cyclically.
 template <int N>
+__device__ __forceinline__ float ror16(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
+}
+template <int N>
 __device__ __forceinline__ float add_ror16(float v) {
-  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
+  return v + ror16<N>(v);
 }
 
 template <int N>
 __device__ __forceinline__ float max_ror16(float v) {
-  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF,
-                                                             true)));
+  return fmaxf(v, ror16<N>(v));
 }
 
 // What a wave reads of a tile.  Lane (r = lane % 16, g = lane / 16), halves t = 0, 1: K codes of
@@ -223,8 +232,8 @@ struct TileRegs {
 //   channels) and the queries as B.  A block's sum has to be multiplied by the slot's scale of
 //   that block before the blocks are added, so column HPS b + h of B holds query row h in block
 //   b's K step and zero in the others: one accumulator holds every block's sum of HPS rows.
-//   Its offset of 8 per code is the accumulator's initial value.  Each lane multiplies by its
-//   block's scales; rotations within 16 lanes add the blocks, leaving the score in each.
+//   Each lane multiplies by its block's scales; rotations within 16 lanes add the blocks,
+//   leaving the score in each.
 // - Queries are scaled by a power of two per row and enter as two f16 parts (22 bits), twice
 //   the MFMAs: the scores are f32-grade.  The operands, three quarters of them zeros at 128
 //   channels, are made once per workgroup and read from LDS each turn: in registers they would
@@ -233,8 +242,7 @@ struct TileRegs {
 //   of P . V when K index j of lane group g means slot 4 g + j % 4 of half j / 4; V is stored
 //   so that a lane's words hold these slots.  Row HPS b + h of A is p * (scale of V's block b)
 //   of query row h, so the scales need no pass of their own; only the channels of block b of
-//   that row's output are used.  p * scale enters as two f16 parts.  V's codes enter as
-//   code - 8, exactly: an offset taken off at the end would cost the sums their low bits.
+//   that row's output are used.  p * scale enters as two f16 parts.
 // - Each row's p is 2^(score - m) with a running m, so that p * scale is at most 2^10 when m is
 //   set and stays below 2^14 in f16, whatever V's range; where a tile passes that (or p 2^40:
 //   scales near zero), m is raised to the largest score + log2 |scale| (the float's bits read as
@@ -245,7 +253,7 @@ struct TileRegs {
 template <int HD, int NSUB, int W, int WPS>
 __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, Kv4Attn a,
                                                                float *__restrict__ rec,
-                                                               float *__restrict__ lse,
+                                                               float2 *__restrict__ lse,
                                                                float *__restrict__ scores, Cut cut,
                                                                bool store) {
   using L = Kv4<HD>;
@@ -254,7 +262,7 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
   __shared__ float lo_[W][NSUB][512];          // per wave and group: HPS rows of HD sums
   __shared__ float2 lm[W][NSUB][16];           // and the 16 rows' (m, sum of p)
   __shared__ half8_t q_[NSUB][NB][2][64];      // queries: per block, hi and lo part, a B operand
-  __shared__ float2 qc[NSUB][16];              // per row: initial value, log2 units per unit
+  __shared__ float qc[NSUB][16];               // per row: log2 units per unit of a score
   __shared__ __align__(16) uint8_t fresh[2][half];  // the stored row's K and V code bytes,
   __shared__ half_t fscale[2][NB];                  // and scales
   Item it;
@@ -321,7 +329,8 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float o = (&xo[j >> 2].x)[j & 3], t = (&xp[j >> 2].x)[j & 3];
-      y[j] = on ? o * (&cv[j >> 2].x)[j & 3] + sign * (t * (&sv[j >> 2].x)[j & 3]) : 0.f;
+      const float x = on ? o * (&cv[j >> 2].x)[j & 3] + sign * (t * (&sv[j >> 2].x)[j & 3]) : 0.f;
+      y[j] = fmaf(x, ScoreScale<HD>::hi, x * ScoreScale<HD>::lo);
     }
     float mx = 0.f;
 #pragma unroll
@@ -332,16 +341,14 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
     const int e = stage_exp(mx);
     const float up = pow2f(e);
     half8_t hi, lo;
-    float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float t = y[j] * up;
+    for (int j = 0; j < 8; ++j) {  // in the codes' order, and those that enter 16-fold over 16
+      const int k = (j & 4) | (j & 1) << 1 | (j & 2) >> 1;
+      const float t = y[k] * (j < 4 ? up : up * 0.0625f);
       hi[j] = (half_t)t;
       lo[j] = (half_t)(t - (float)hi[j]);
-      sum += (float)hi[j] + (float)lo[j];
     }
-    sum = sum_xor32(sum_xor16(sum));
-    if (g == 0) qc[wave][r] = make_float2(-8.f * sum, pow2f(-e) * (kLog2e / sqrtf((float)HD)));
+    if (g == 0) qc[wave][r] = pow2f(-e);
     const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
@@ -378,19 +385,18 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
     }
   }
   __syncthreads();
-  float q0[NSUB], f[NSUB];  // the accumulators' initial value; log2 units per accumulated unit
+  float f[NSUB];            // log2 units per accumulated unit
   int vis[NSUB];            // slots that the row sees
 #pragma unroll
   for (int u = 0; u < NSUB; ++u) {
-    q0[u] = qc[u][r].x;
-    f[u] = qc[u][r].y;
+    f[u] = qc[u][r];
     const int v = v0 + u * HPS + h;
     vis[u] = filled + (v < V ? v / grp : 0) + 1;
   }
   const int all_see = filled + v0 / grp + 1;  // slots that every row of the workgroup sees
 
   float4_t acc[NSUB][2 * NB];
-  float m[NSUB], l[NSUB];  // m: p = 2^(score - m)
+  float m[NSUB], l[NSUB];  // p = 2^(score - m)
 #pragma unroll
   for (int u = 0; u < NSUB; ++u) {
     m[u] = -INFINITY;
@@ -415,11 +421,11 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int u = 0; u < NSUB; ++u) sc[u][t] = float4_t{q0[u], q0[u], q0[u], q0[u]};
+        for (int u = 0; u < NSUB; ++u) sc[u][t] = float4_t{0.f, 0.f, 0.f, 0.f};
       }
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
-        const half8_t k0 = k_codes(d.k[0][k]), k1 = k_codes(d.k[1][k]);
+        const half8_t k0 = k_frag(d.k[0][k], magic), k1 = k_frag(d.k[1][k], magic);
 #pragma unroll
         for (int u = 0; u < NSUB; ++u) {
           const half8_t hi = q_[u][k][0][ql], lo = q_[u][k][1][ql];
@@ -435,7 +441,7 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 #pragma unroll
         for (int u = 0; u < NSUB; ++u) {
           float x = mul_f16(sc[u][i >> 2][i & 3], ks);
-          if constexpr (NB > 1) x = add_ror16<8>(x);
+          x = add_ror16<8>(x);
           if constexpr (NB > 2) x = add_ror16<4>(x);
           if constexpr (NB > 4) x = add_ror16<2>(x);
           y[u][i] = x;
@@ -446,13 +452,17 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
     d.load_k(next, r, g, b);
     if (scores) {
 #pragma unroll
-      for (int u = 0; u < NSUB; ++u)
+      for (int u = 0; u < NSUB; ++u) {
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = y[u][i] * f[u];
         if (r < HPS && v0 + u * HPS + r < V) {
           float *o = scores + (list * V + v0 + u * HPS + r) * score_stride(c.slots) + slot0;
-          *(float4 *)o = make_float4(y[u][0] * f[u], y[u][1] * f[u], y[u][2] * f[u], y[u][3] * f[u]);
+          *(float4 *)o = make_float4(z[0], z[1], z[2], z[3]);
           *(float4 *)(o + 16) =
-              make_float4(y[u][4] * f[u], y[u][5] * f[u], y[u][6] * f[u], y[u][7] * f[u]);
+              make_float4(z[4], z[5], z[6], z[7]);
         }
+      }
     }
     const bool masked = (tile + 1) * kKv4Tile > all_see;
     half8_t wh[NSUB], wl[NSUB];
@@ -508,10 +518,9 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 #pragma unroll
       for (int k = 0; k < 4; ++k) {  // V's pairs: slots (0, 2), (1, 3) of each half
         const int i = (k & 1) + (k >> 1) * 4;
-        hp[k] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(w[i], w[i + 2]));
-        lp[k] = __builtin_bit_cast(half2_t,
-                                   __builtin_amdgcn_cvt_pkrtz(fmaf((float)hp[k][0], minus1, w[i]),
-                                                              fmaf((float)hp[k][1], minus1, w[i + 2])));
+        hp[k] = half2_t{(half_t)w[i], (half_t)w[i + 2]};
+        lp[k] = half2_t{(half_t)fmaf((float)hp[k][0], minus1, w[i]),
+                        (half_t)fmaf((float)hp[k][1], minus1, w[i + 2])};
       }
       wh[u] = __builtin_bit_cast(half8_t, hp);
       wl[u] = __builtin_bit_cast(half8_t, lp);
@@ -564,7 +573,7 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
     }
     if (sp.n == 1) {  // nothing to join
       a.out[(s * a.rows + v / grp) * a.ldo + (kvh * grp + v % grp) * HD + ch] = o / ls;
-      if (lse && ch == 0) lse[list * V + v] = mx + log2f(ls);
+      if (lse && ch == 0) lse[list * V + v] = make_float2(mx, 1.f / ls);
     } else {
       out[v * RS + ch] = o;
       if ((ch & 31) == 0) *(float2 *)(out + v * RS + HD + 2 * (ch >> 5)) = make_float2(mx, ls);
@@ -577,7 +586,7 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 template <int HD>
 __global__ __launch_bounds__(kThreads) void kv4_merge_kernel(Kv4Cache c, Kv4Attn a,
                                                              const float *__restrict__ rec,
-                                                             float *__restrict__ lse, Cut cut) {
+                                                             float2 *__restrict__ lse, Cut cut) {
   constexpr int RS = record_floats<HD>(), Q = HD / 4, G = kThreads / Q;
   __shared__ float4 o_[G][Q];
   __shared__ float2 ml_[G][Q];
@@ -625,14 +634,15 @@ __global__ __launch_bounds__(kThreads) void kv4_merge_kernel(Kv4Cache c, Kv4Attn
   *(float4 *)(a.out + (s * a.rows + v / grp) * a.ldo +
               (int64_t)(list % c.nkv * grp + v % grp) * HD + 4 * q) =
       make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
-  if (lse && q == 0) lse[list * V + v] = m + log2f(l);
+  if (lse && q == 0) lse[list * V + v] = make_float2(m, 1.f / l);
 }
 
 // The attention weights of a list's slots: 64 threads of four slots each times four shares of
-// the query rows, whose scores are taken against the rows' log-sum-exp; shares joined in order.
+// the query rows, whose scores are taken against the rows' maximum and sum (apart: their
+// log-sum-exp in one float would lose the low bits); shares joined in order.
 constexpr int kWeightSlots = 256;
 __global__ __launch_bounds__(kThreads) void kv4_weights_kernel(Kv4Cache c, Kv4Attn a,
-                                                               const float *__restrict__ lse,
+                                                               const float2 *__restrict__ lse,
                                                                const float *__restrict__ scores) {
   __shared__ float4 part[3][64];
   const int64_t list = blockIdx.y, s = list / c.nkv;
@@ -642,28 +652,29 @@ __global__ __launch_bounds__(kThreads) void kv4_weights_kernel(Kv4Cache c, Kv4At
   const int t = blockIdx.x * kWeightSlots + 4 * x;
   if (filled < 0 || (int)(blockIdx.x * kWeightSlots) >= filled + a.rows) return;
   const int64_t step = score_stride(c.slots);
-  const float *e = lse + list * V, *sc = scores + list * V * step + t;
+  const float2 *e = lse + list * V;
+  const float *sc = scores + list * V * step + t;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   if (t < filled + a.rows) {
     if (t + 3 <= filled) {  // every row sees the four slots
 #pragma unroll 8
       for (int v = share; v < V; v += 4) {
         const float4 y = *(const float4 *)(sc + v * step);
-        const float z = e[v];
-        sum.x += __builtin_amdgcn_exp2f(y.x - z);
-        sum.y += __builtin_amdgcn_exp2f(y.y - z);
-        sum.z += __builtin_amdgcn_exp2f(y.z - z);
-        sum.w += __builtin_amdgcn_exp2f(y.w - z);
+        const float2 z = e[v];
+        sum.x = fmaf(__builtin_amdgcn_exp2f(y.x - z.x), z.y, sum.x);
+        sum.y = fmaf(__builtin_amdgcn_exp2f(y.y - z.x), z.y, sum.y);
+        sum.z = fmaf(__builtin_amdgcn_exp2f(y.z - z.x), z.y, sum.z);
+        sum.w = fmaf(__builtin_amdgcn_exp2f(y.w - z.x), z.y, sum.w);
       }
     } else {
       for (int v = share; v < V; v += 4) {
         const int last = filled + v / grp;  // the last slot that row v sees
         const float4 y = *(const float4 *)(sc + v * step);
-        const float z = e[v];
-        if (t <= last) sum.x += __builtin_amdgcn_exp2f(y.x - z);
-        if (t + 1 <= last) sum.y += __builtin_amdgcn_exp2f(y.y - z);
-        if (t + 2 <= last) sum.z += __builtin_amdgcn_exp2f(y.z - z);
-        if (t + 3 <= last) sum.w += __builtin_amdgcn_exp2f(y.w - z);
+        const float2 z = e[v];
+        if (t <= last) sum.x = fmaf(__builtin_amdgcn_exp2f(y.x - z.x), z.y, sum.x);
+        if (t + 1 <= last) sum.y = fmaf(__builtin_amdgcn_exp2f(y.y - z.x), z.y, sum.y);
+        if (t + 2 <= last) sum.z = fmaf(__builtin_amdgcn_exp2f(y.z - z.x), z.y, sum.z);
+        if (t + 3 <= last) sum.w = fmaf(__builtin_amdgcn_exp2f(y.w - z.x), z.y, sum.w);
       }
     }
   }
@@ -721,18 +732,19 @@ Plan plan(int rows, int n_seq, int nh, int nkv, int hd, int slots) {
   return p;
 }
 
-// Work: records (several splits), then per query row its log-sum-exp and its scores (weights).
+// Work: records (several splits), then per query row its (m, 1 / sum of p) and its scores (weights).
 int64_t record_bytes(const Plan &p, int hd) {
   return p.cut.S > 1 ? p.lists * p.cut.S * p.V * (int64_t)(hd + hd / 16) * 4 : 0;
 }
-int64_t lse_bytes(const Plan &p) { return (p.lists * p.V * 4 + 15) / 16 * 16; }
+int64_t lse_bytes(const Plan &p) { return (p.lists * p.V * 8 + 15) / 16 * 16; }
 
 template <int HD>
 hipError_t launch(const Kv4Cache &c, const Kv4Attn &a, hipStream_t s) {
   const Plan p = plan(a.rows, c.n_seq, c.nh, c.nkv, HD, c.slots);
-  float *rec = (float *)a.work, *lse = nullptr, *scores = nullptr;
+  float *rec = (float *)a.work, *scores = nullptr;
+  float2 *lse = nullptr;
   if (a.weights_mode) {
-    lse = (float *)((char *)a.work + record_bytes(p, HD));
+    lse = (float2 *)((char *)a.work + record_bytes(p, HD));
     scores = (float *)((char *)lse + lse_bytes(p));
   }
   const bool inside = a.store && a.rows == 1;  // the one row is stored by the workgroups
