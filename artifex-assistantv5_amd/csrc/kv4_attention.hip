@@ -146,6 +146,16 @@ __device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) {
 // that is added to something would be fused into that.
 __device__ __forceinline__ float mul_f16(float x, half_t h) { return fmaf(x, (float)h, 0.f); }
 
+// x and y in f16 parts hi + lo, both to nearest: what is left is under 2^-22 of them.  `minus1` is
+// -1 in a scalar register, which has the low parts made in one instruction each.
+__device__ __forceinline__ void split_f16(float x, float y, float minus1, half2_t &hi,
+                                          half2_t &lo) {
+  uint32_t h = __builtin_bit_cast(uint32_t, half2_t{(half_t)x, (half_t)y});
+  asm("" : "+v"(h));  // else x and y are each rounded once more for the low parts
+  hi = __builtin_bit_cast(half2_t, h);
+  lo = half2_t{(half_t)fmaf((float)hi[0], minus1, x), (half_t)fmaf((float)hi[1], minus1, y)};
+}
+
 // v plus that of the lane N to the left in its 16, cyclically.
 template <int N>
 __device__ __forceinline__ float ror16(float v) {
@@ -160,6 +170,55 @@ template <int N>
 __device__ __forceinline__ float max_ror16(float v) {
   return fmaxf(v, ror16<N>(v));
 }
+
+// The one new row of a decode step, in LDS: K and V code bytes and scales.
+template <int HD>
+struct FreshRow {
+  using L = Kv4<HD>;
+  static constexpr int NB = L::NB;
+  __align__(16) uint8_t code[2][HD / 2];
+  half_t scale[2][NB];
+  // Made by HD / 4 lanes each (rq) for K (unit 0) and V (unit 1); stored in the cache if `writes`.
+  __device__ __forceinline__ void make(const Kv4Cache &c, Kv4Row<HD> &row, int unit, int rq,
+                                       uint8_t *base, int64_t list, int slot, int32_t pos,
+                                       bool writes) {
+    uint32_t word;
+    half_t d;
+    kv4_quantize<HD>(row, rq, unit == 0, word, d);
+    const int j = slot % kKv4Tile, blk = rq >> 3;
+    uint8_t *to = base + (int64_t)(slot / kKv4Tile) * L::TB;
+    if (unit == 0 && !(rq & 1)) {
+      const int at = (((rq >> 1) & 3) * NB + blk) * 4;
+      *(uint32_t *)(code[0] + at) = word;
+      if (writes) *(uint32_t *)(to + j * (HD / 2) + at) = word;
+    } else if (unit == 1 && (rq & 7) < 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = (4 * (rq & 3) + i) * NB + blk;
+        code[1][at] = (uint8_t)(word >> (8 * i));
+        if (writes) to[L::VO + (j >> 2) * (2 * HD) + at * 4 + (j & 3)] = (uint8_t)(word >> (8 * i));
+      }
+    }
+    if (unit < 2 && !(rq & 7)) {
+      scale[unit][blk] = d;
+      if (writes) *(half_t *)(to + (unit ? L::VS : L::KS) + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = d;
+    }
+    if (writes && unit == 1 && rq == 0) {
+      if (c.positions) c.positions[list * c.slots + slot] = pos;
+      if (c.weights) c.weights[list * c.slots + slot] = 0.f;
+    }
+  }
+  // Scale of slot j in the four that w holds.  By value: a reference to one of the two words would
+  // put registers in memory.
+  __device__ __forceinline__ static void put(uint2 &w, int j, half_t d) {
+    const int sh = 16 * (j & 1);
+    const uint32_t keep = ~(0xFFFFu << sh), n = (uint32_t)__builtin_bit_cast(uint16_t, d) << sh;
+    if (j & 2)
+      w.y = (w.y & keep) | n;
+    else
+      w.x = (w.x & keep) | n;
+  }
+};
 
 // What a wave reads of a tile.  Lane (r = lane % 16, g = lane / 16), halves t = 0, 1: K codes of
 // slot 16 t + r, channels 32 b + 8 g + 0..7 of every block b; V codes of slots 16 t + 4 g + 0..3,
@@ -184,32 +243,28 @@ struct TileRegs {
       words(tile + (uint32_t)(Kv4<HD>::VO + (4 * t + g) * (2 * HD) + r * NB * 4), v[t]);
     }
   }
-  // Slot j of the tile from its bytes and scales.
-  __device__ __forceinline__ void patch(const uint8_t (&fresh)[2][HD / 2],
-                                        const half_t (&fscale)[2][NB], int j, int r, int g, int b) {
-    const int sh = 8 * (j & 3), ss = 16 * (j & 1);
-    const uint32_t kd = __builtin_bit_cast(uint16_t, fscale[0][b]);
-    const uint32_t vd = __builtin_bit_cast(uint16_t, fscale[1][b]);
+  // Slot j's codes from its bytes.
+  __device__ __forceinline__ void patch_codes(const FreshRow<HD> &f, int j, int r, int g) {
+    const int sh = 8 * (j & 3);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       if (j == 16 * t + r)
 #pragma unroll
-        for (int i = 0; i < NB; ++i) k[t][i] = *(const uint32_t *)(fresh[0] + (g * NB + i) * 4);
-      if (j >> 2 == 4 * t + g) {
+        for (int i = 0; i < NB; ++i) k[t][i] = *(const uint32_t *)(f.code[0] + (g * NB + i) * 4);
+      if (j >> 2 == 4 * t + g)
 #pragma unroll
         for (int i = 0; i < NB; ++i)
-          v[t][i] = (v[t][i] & ~(0xFFu << sh)) | ((uint32_t)fresh[1][r * NB + i] << sh);
-        // by value: a reference to one of two words would put the registers in memory
-        const uint32_t keep = ~(0xFFFFu << ss), kn = kd << ss, vn = vd << ss;
-        if (j & 2) {
-          ks[t].y = (ks[t].y & keep) | kn;
-          vs[t].y = (vs[t].y & keep) | vn;
-        } else {
-          ks[t].x = (ks[t].x & keep) | kn;
-          vs[t].x = (vs[t].x & keep) | vn;
-        }
-      }
+          v[t][i] = (v[t][i] & ~(0xFFu << sh)) | ((uint32_t)f.code[1][r * NB + i] << sh);
     }
+  }
+  __device__ __forceinline__ void patch(const FreshRow<HD> &f, int j, int r, int g, int b) {
+    patch_codes(f, j, r, g);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (j >> 2 == 4 * t + g) {
+        FreshRow<HD>::put(ks[t], j, f.scale[0][b]);
+        FreshRow<HD>::put(vs[t], j, f.scale[1][b]);
+      }
   }
   static __device__ __forceinline__ void words(const uint8_t *p, uint32_t (&w)[NB]) {
     if constexpr (NB == 2) {
@@ -225,9 +280,9 @@ struct TileRegs {
   }
 };
 
-// A workgroup takes one list, one range of its tiles and NSUB groups of HPS = 512 / HD query
-// rows; its waves take the range's tiles in turn and join at the end.  Nothing but registers
-// carries a tile through:
+// For few query rows.  A workgroup takes one list, one range of its tiles and HPS = 512 / HD
+// query rows; its waves take the range's tiles in turn and join at the end.  Nothing but
+// registers carries a tile through:
 // - Scores: v_mfma_f32_16x16x32_f16 with the slots' codes as A (one K step is one block of 32
 //   channels) and the queries as B.  A block's sum has to be multiplied by the slot's scale of
 //   that block before the blocks are added, so column HPS b + h of B holds query row h in block
@@ -250,7 +305,7 @@ struct TileRegs {
 // - K's registers take the next tile as soon as its scores are made, V's after its products:
 //   one tile in flight per wave, four waves per SIMD.
 // Bound: HBM, 9/8 head_dim bytes per slot and list.
-template <int HD, int NSUB, int W, int WPS>
+template <int HD, int W, int WPS>
 __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, Kv4Attn a,
                                                                float *__restrict__ rec,
                                                                float2 *__restrict__ lse,
@@ -259,12 +314,11 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
   using L = Kv4<HD>;
   constexpr int NB = L::NB, HPS = 16 / NB, half = HD / 2, RS = record_floats<HD>();
   constexpr float kLift = 10.f, kMostW = 16384.f, kMostP = 0x1p40f;
-  __shared__ float lo_[W][NSUB][512];          // per wave and group: HPS rows of HD sums
-  __shared__ float2 lm[W][NSUB][16];           // and the 16 rows' (m, sum of p)
-  __shared__ half8_t q_[NSUB][NB][2][64];      // queries: per block, hi and lo part, a B operand
-  __shared__ float qc[NSUB][16];               // per row: log2 units per unit of a score
-  __shared__ __align__(16) uint8_t fresh[2][half];  // the stored row's K and V code bytes,
-  __shared__ half_t fscale[2][NB];                  // and scales
+  __shared__ float lo_[W][512];      // per wave: HPS rows of HD sums
+  __shared__ float2 lm[W][16];       // and the 16 rows' (m, sum of p)
+  __shared__ half8_t q_[NB][2][64];  // queries: per block, hi and lo part, a B operand
+  __shared__ float qc[16];           // per row: log2 units per unit of a score
+  __shared__ FreshRow<HD> fresh;
   Item it;
   if (!kv4_item(c, a.rows, blockIdx.x, cut, it)) return;
   it.s = __builtin_amdgcn_readfirstlane(it.s);  // all known uniform from here on
@@ -281,7 +335,7 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
   const int b = r / HPS, h = r % HPS;
   const int tile0 = it.split * sp.per, tile1 = min(tile0 + sp.per, kv4_tiles(filled, a.rows));
   uint8_t *base = kv4_list(c.kv, list, c.slots, L::TB);
-  const int v0 = blockIdx.z * NSUB * HPS;
+  const int v0 = blockIdx.z * HPS;
   // the workgroups whose range has the one new row (a call of more rows stores them beforehand)
   // make its bytes in LDS, for the wave whose first tile lacks them; those of the first group of
   // query rows store them
@@ -292,13 +346,13 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 
   // What comes before the barrier is requested before the tile, since loads return in order:
   // behind a full chip's tiles the queries took 5.6 us (130000 slots).
-  float4 xo[2], xp[2], cv[2], sv[2];  // wave < NSUB: the queries of group `wave`: lane (r, g)
-                                      // holds channels 32 b + 8 g + 0..7 of its row
+  float4 xo[2], xp[2], cv[2], sv[2];  // wave 0: the queries, lane (r, g) channels
+                                      // 32 b + 8 g + 0..7 of its row
   constexpr int LANES = Kv4Row<HD>::LANES, STORERS = HD == 256 ? 2 : 1;
-  Kv4Row<HD> row;  // waves NSUB ..: the new row's K (unit 0) and V (1), HD / 4 lanes each
-  const int unit = (wave - NSUB) * (64 / LANES) + lane / LANES, rq = lane % LANES;
-  if (wave < NSUB) {
-    const int v = v0 + wave * HPS + h, i = v < V ? v / grp : 0;
+  Kv4Row<HD> row;  // waves 1 ..: the new row's K (unit 0) and V (1), HD / 4 lanes each
+  const int unit = (wave - 1) * (64 / LANES) + lane / LANES, rq = lane % LANES;
+  if (wave == 0) {
+    const int v = v0 + h, i = v < V ? v / grp : 0;
     const float *x = row0 + i * a.ldq + (int64_t)(kvh * grp + (v < V ? v % grp : 0)) * HD;
     const int e0 = 32 * b + 8 * g, ep = b < NB / 2 ? e0 + half : e0 - half;
     const int64_t p = (pos0 + i) * half + (b < NB / 2 ? e0 : ep);
@@ -309,7 +363,7 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
       cv[j] = *(const float4 *)(c.cs + p + 4 * j);
       sv[j] = *(const float4 *)(c.sn + p + 4 * j);
     }
-  } else if (stores && wave < NSUB + STORERS && unit < 2) {
+  } else if (stores && wave < 1 + STORERS && unit < 2) {
     row.load(unit ? vx : kx, rq);
     row.load_turn(c.cs + pos0 * half, c.sn + pos0 * half, rq);
   }
@@ -322,8 +376,8 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
     d.load_v(base + (int64_t)tile * L::TB, r, g);
   }
   __builtin_amdgcn_sched_barrier(0);
-  if (wave < NSUB) {
-    const bool on = v0 + wave * HPS + h < V;  // past the last query row: zeros
+  if (wave == 0) {
+    const bool on = v0 + h < V;  // past the last query row: zeros
     const float sign = b < NB / 2 ? -1.f : 1.f;
     float y[8];
 #pragma unroll
@@ -348,155 +402,434 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
       hi[j] = (half_t)t;
       lo[j] = (half_t)(t - (float)hi[j]);
     }
-    if (g == 0) qc[wave][r] = pow2f(-e);
+    if (g == 0) qc[r] = pow2f(-e);
     const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
-      q_[wave][k][0][lane] = b == k ? hi : zero;
-      q_[wave][k][1][lane] = b == k ? lo : zero;
+      q_[k][0][lane] = b == k ? hi : zero;
+      q_[k][1][lane] = b == k ? lo : zero;
     }
-  } else if (stores && wave < NSUB + STORERS) {
-    uint32_t word;
-    half_t scale;
-    kv4_quantize<HD>(row, rq, unit == 0, word, scale);
-    const int j = filled % kKv4Tile, blk = rq >> 3;
-    uint8_t *to = base + (int64_t)(filled / kKv4Tile) * L::TB;
-    const bool writes = blockIdx.z == 0;
-    if (unit == 0 && !(rq & 1)) {
-      const int at = (((rq >> 1) & 3) * NB + blk) * 4;
-      *(uint32_t *)(fresh[0] + at) = word;
-      if (writes) *(uint32_t *)(to + j * half + at) = word;
-    } else if (unit == 1 && (rq & 7) < 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = (4 * (rq & 3) + i) * NB + blk;
-        fresh[1][at] = (uint8_t)(word >> (8 * i));
-        if (writes) to[L::VO + (j >> 2) * (2 * HD) + at * 4 + (j & 3)] = (uint8_t)(word >> (8 * i));
-      }
-    }
-    if (unit < 2 && !(rq & 7)) {
-      fscale[unit][blk] = scale;
-      if (writes)
-        *(half_t *)(to + (unit ? L::VS : L::KS) + ((j >> 2) * NB + blk) * 8 + (j & 3) * 2) = scale;
-    }
-    if (writes && unit == 1 && rq == 0) {
-      if (c.positions) c.positions[list * c.slots + filled] = (int32_t)pos0;
-      if (c.weights) c.weights[list * c.slots + filled] = 0.f;
-    }
+  } else if (stores && wave < 1 + STORERS) {
+    fresh.make(c, row, unit, rq, base, list, filled, (int32_t)pos0, blockIdx.z == 0);
   }
   __syncthreads();
-  float f[NSUB];            // log2 units per accumulated unit
-  int vis[NSUB];            // slots that the row sees
-#pragma unroll
-  for (int u = 0; u < NSUB; ++u) {
-    f[u] = qc[u][r];
-    const int v = v0 + u * HPS + h;
-    vis[u] = filled + (v < V ? v / grp : 0) + 1;
-  }
+  const float f = qc[r];  // log2 units per accumulated unit
+  const int vis = filled + (v0 + h < V ? (v0 + h) / grp : 0) + 1;  // slots that the row sees
   const int all_see = filled + v0 / grp + 1;  // slots that every row of the workgroup sees
 
-  float4_t acc[NSUB][2 * NB];
-  float m[NSUB], l[NSUB];  // p = 2^(score - m)
+  float4_t acc[2 * NB];
+  float m = -INFINITY, l = 0.f;  // p = 2^(score - m)
 #pragma unroll
-  for (int u = 0; u < NSUB; ++u) {
-    m[u] = -INFINITY;
-    l[u] = 0.f;
-#pragma unroll
-    for (int t = 0; t < 2 * NB; ++t) acc[u][t] = float4_t{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int t = 0; t < 2 * NB; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
 
   uint32_t magic;
   asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(magic));
   float minus1 = -1.f;  // not known to be: x - (float)h stays one fused instruction
   asm volatile("" : "+s"(minus1));
-  if (stores && tile == filled / kKv4Tile) d.patch(fresh, fscale, filled % kKv4Tile, r, g, b);
+  if (stores && tile == filled / kKv4Tile) d.patch(fresh, filled % kKv4Tile, r, g, b);
   int ql = lane;  // made anew every turn: the queries are read from LDS there, not kept
   for (; tile >= tile0; tile -= W) {
     const uint8_t *next = base + (int64_t)max(tile - W, tile0) * L::TB;  // the last one: unused
     const int slot0 = tile * kKv4Tile + 4 * g;  // of half 0, i = 0
     asm volatile("" : "+v"(ql));
-    float y[NSUB][8];  // scores / f
+    float y[8];  // scores / f
     {
-      float4_t sc[NSUB][2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int u = 0; u < NSUB; ++u) sc[u][t] = float4_t{0.f, 0.f, 0.f, 0.f};
-      }
+      float4_t sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
         const half8_t k0 = k_frag(d.k[0][k], magic), k1 = k_frag(d.k[1][k], magic);
-#pragma unroll
-        for (int u = 0; u < NSUB; ++u) {
-          const half8_t hi = q_[u][k][0][ql], lo = q_[u][k][1][ql];
-          sc[u][0] = mfma(k0, hi, sc[u][0]);
-          sc[u][1] = mfma(k1, hi, sc[u][1]);
-          sc[u][0] = mfma(k0, lo, sc[u][0]);
-          sc[u][1] = mfma(k1, lo, sc[u][1]);
-        }
+        const half8_t hi = q_[k][0][ql], lo = q_[k][1][ql];
+        sc[0] = mfma(k0, hi, sc[0]);
+        sc[1] = mfma(k1, hi, sc[1]);
+        sc[0] = mfma(k0, lo, sc[0]);
+        sc[1] = mfma(k1, lo, sc[1]);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const half_t ks = __builtin_bit_cast(half4_t, d.ks[i >> 2])[i & 3];
-#pragma unroll
-        for (int u = 0; u < NSUB; ++u) {
-          float x = mul_f16(sc[u][i >> 2][i & 3], ks);
-          x = add_ror16<8>(x);
-          if constexpr (NB > 2) x = add_ror16<4>(x);
-          if constexpr (NB > 4) x = add_ror16<2>(x);
-          y[u][i] = x;
-        }
+        float x = mul_f16(sc[i >> 2][i & 3], ks);
+        x = add_ror16<8>(x);
+        if constexpr (NB > 2) x = add_ror16<4>(x);
+        if constexpr (NB > 4) x = add_ror16<2>(x);
+        y[i] = x;
       }
     }
     const half4_t dv[2] = {__builtin_bit_cast(half4_t, d.vs[0]), __builtin_bit_cast(half4_t, d.vs[1])};
     d.load_k(next, r, g, b);
     if (scores) {
+      float z[8];
 #pragma unroll
-      for (int u = 0; u < NSUB; ++u) {
-        float z[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = y[u][i] * f[u];
-        if (r < HPS && v0 + u * HPS + r < V) {
-          float *o = scores + (list * V + v0 + u * HPS + r) * score_stride(c.slots) + slot0;
-          *(float4 *)o = make_float4(z[0], z[1], z[2], z[3]);
-          *(float4 *)(o + 16) =
-              make_float4(z[4], z[5], z[6], z[7]);
-        }
+      for (int i = 0; i < 8; ++i) z[i] = y[i] * f;
+      if (r < HPS && v0 + r < V) {
+        float *o = scores + (list * V + v0 + r) * score_stride(c.slots) + slot0;
+        *(float4 *)o = make_float4(z[0], z[1], z[2], z[3]);
+        *(float4 *)(o + 16) = make_float4(z[4], z[5], z[6], z[7]);
       }
     }
     const bool masked = (tile + 1) * kKv4Tile > all_see;
-    half8_t wh[NSUB], wl[NSUB];
+    float p[8], w[8], sum, most;
+    auto hidden = [&](int i) { return slot0 + (i < 4 ? i : 12 + i) >= vis; };
+    auto weigh = [&]() {
 #pragma unroll
-    for (int u = 0; u < NSUB; ++u) {
-      float p[8], w[8], sum, most;
-      // the first slot past those that the row sees, from slot0: hides i from there on (unrolled
-      // turns share nothing of this but where a tile is masked)
+      for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(fmaf(y[i], f, -m));
+        w[i] = mul_f16(p[i], dv[i >> 2][i & 3]);
+      }
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (hidden(i)) p[i] = w[i] = 0.f;
+      }
+      sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      most = fabsf(w[0]);
+#pragma unroll
+      for (int i = 1; i < 7; i += 2) most = fmaxf(fmaxf(most, fabsf(w[i])), fabsf(w[i + 1]));
+      most = fmaxf(most, fabsf(w[7]));
+    };
+    weigh();
+    if (__any(most > kMostW || sum > kMostP)) {
+      float n = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t bits = __float_as_uint((float)dv[i >> 2][i & 3]) & 0x7FFFFFFFu;
+        const float lg =  // of at least 2^-24
+            fmaf((float)(int)(bits < 0x33800000u ? 0x33800000u : bits), 0x1p-23f, -127.f - kLift);
+        if (!masked || !hidden(i)) n = fmaxf(n, fmaf(y[i], f, lg));
+      }
+      n = max_xor16(n);
+      n = max_xor32(n);
+      const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - n);
+      m = n;
+      l *= al;
+      float ar[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ar[i] = __shfl(al, 4 * g + i);
+#pragma unroll
+      for (int t = 0; t < 2 * NB; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] *= ar[i];
+      weigh();
+    }
+    l += sum;
+    half2_t hp[4], lp[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // V's pairs: slots (0, 2), (1, 3) of each half
+      const int i = (k & 1) + (k >> 1) * 4;
+      split_f16(w[i], w[i + 2], minus1, hp[k], lp[k]);
+    }
+    const half8_t wh = __builtin_bit_cast(half8_t, hp), wl = __builtin_bit_cast(half8_t, lp);
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const uint32_t w0 = d.v[0][k], h0 = w0 >> 8, w1 = d.v[1][k], h1 = w1 >> 8;
+      const half8_t va = v_frag<1>(w0, h0, w1, h1, magic);
+      const half8_t vb = v_frag<16>(w0, h0, w1, h1, magic);  // channels 16..31 of the block
+      acc[2 * k] = mfma(wh, va, acc[2 * k]);
+      acc[2 * k + 1] = mfma(wh, vb, acc[2 * k + 1]);
+      acc[2 * k] = mfma(wl, va, acc[2 * k]);
+      acc[2 * k + 1] = mfma(wl, vb, acc[2 * k + 1]);
+    }
+    d.load_v(next, r, g);
+  }
+
+  __syncthreads();
+  // the waves' sums: lane (r, g), register i holds row 4 g + i, channel 16 t + r
+  float sum = sum_xor32(sum_xor16(l));
+  if (g == 0) lm[wave][r] = make_float2(m, sum);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 4 * g + i, rb = row / HPS;
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t)
+      if (rb == t / 2)
+        lo_[wave][row % HPS * HD + 16 * t + r] = acc[t][i] * (t & 1 ? 0.0625f : 1.f);
+  }
+  __syncthreads();
+  float *out = rec + (list * cut.S + it.split) * V * RS;
+  for (int e = tid; e < 512; e += 64 * W) {
+    const int hh = e / HD, ch = e & (HD - 1), row = (ch >> 5) * HPS + hh;
+    const int v = v0 + hh;
+    if (v >= V) continue;
+    float mx = lm[0][row].x, o = 0.f, ls = 0.f;
+#pragma unroll
+    for (int k = 1; k < W; ++k) mx = fmaxf(mx, lm[k][row].x);
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const float2 ml = lm[k][row];
+      const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
+      o = fmaf(w, lo_[k][e], o);
+      ls = fmaf(w, ml.y, ls);
+    }
+    if (sp.n == 1) {  // nothing to join
+      a.out[(s * a.rows + v / grp) * a.ldo + (kvh * grp + v % grp) * HD + ch] = o / ls;
+      if (lse && ch == 0) lse[list * V + v] = make_float2(mx, 1.f / ls);
+    } else {
+      out[v * RS + ch] = o;
+      if ((ch & 31) == 0) *(float2 *)(out + v * RS + HD + 2 * (ch >> 5)) = make_float2(mx, ls);
+    }
+  }
+}
+
+// The same for many query rows: NS groups of 16, a column each.  Every block's scores are a product
+// of their own, multiplied by the slots' scales as they are added, and P times V's scales is made
+// for every block.  So a lane holds all blocks' scales of its slots (32 registers at 128 channels
+// where the kernel above has 8), but every column is a row of its own: a quarter of the MFMAs and
+// exponentials per row at 128 channels, an eighth at 256.
+// The largest |p * scale| is bounded by the largest p times the largest |scale| of the lane's
+// slots; where m is raised for it, by each slot's own.
+// Bound: vector instructions, about 150 for a tile's codes and 190 for each group of rows (128
+// channels).
+template <int HD, int NS>
+__global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
+                                                          float *__restrict__ rec,
+                                                          float2 *__restrict__ lse,
+                                                          float *__restrict__ scores, Cut cut,
+                                                          bool store) {
+  using L = Kv4<HD>;
+  constexpr int W = 4, NB = L::NB, half = HD / 2, RS = record_floats<HD>();
+  constexpr float kLift = 10.f, kMostW = 16384.f, kMostP = 0x1p40f;
+  // Queries (per block, hi and lo part, a B operand) while tiles are read, then the waves' sums, 16
+  // rows of HD per group: 64 KB together, so two workgroups fit a CU's LDS, 82 apart.
+  __shared__ union {
+    half8_t q[NS][NB][2][64];
+    float o[W][NS][16 * HD];
+  } sh;
+  auto &q_ = sh.q;
+  auto &lo_ = sh.o;
+  __shared__ float2 lm[W][NS][16];             // the rows' (m, sum of p)
+  __shared__ float qc[NS][16];                 // per row: log2 units per unit of a score
+  __shared__ FreshRow<HD> fresh;
+  Item it;
+  if (!kv4_item(c, a.rows, blockIdx.x, cut, it)) return;
+  it.s = __builtin_amdgcn_readfirstlane(it.s);  // all known uniform from here on
+  it.kvh = __builtin_amdgcn_readfirstlane(it.kvh);
+  it.split = __builtin_amdgcn_readfirstlane(it.split);
+  it.filled = __builtin_amdgcn_readfirstlane(it.filled);
+  it.sp.per = __builtin_amdgcn_readfirstlane(it.sp.per);
+  it.sp.n = __builtin_amdgcn_readfirstlane(it.sp.n);
+  const int64_t s = it.s, list = s * c.nkv + it.kvh;
+  const int kvh = it.kvh, grp = c.nh / c.nkv, V = a.rows * grp, filled = it.filled;
+  const Splits sp = it.sp;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tile0 = it.split * sp.per, tile1 = min(tile0 + sp.per, kv4_tiles(filled, a.rows));
+  uint8_t *base = kv4_list(c.kv, list, c.slots, L::TB);
+  const int v0 = blockIdx.z * NS * 16;
+  const bool stores = store && filled / kKv4Tile >= tile0 && filled / kKv4Tile < tile1;
+  const float *row0 = a.qkv + s * a.rows * a.ldq;
+  const float *kx = row0 + (int64_t)(c.nh + kvh) * HD, *vx = kx + (int64_t)c.nkv * HD;
+  const int64_t pos0 = c.pos[s];
+  TileRegs<HD> d;               // codes; the scales of every block apart
+  uint2 ks[2][NB], vs[2][NB];   // of slots 16 t + 4 g + 0..3
+  auto load_scales = [&](const uint8_t *tile) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int k = 0; k < NB; k += 2) {
+        const uint8_t *p = tile + (uint32_t)(L::KS + ((4 * t + g) * NB + k) * 8);
+        const uint4 x = *(const uint4 *)p, y = *(const uint4 *)(p + 2 * HD);
+        ks[t][k] = make_uint2(x.x, x.y), ks[t][k + 1] = make_uint2(x.z, x.w);
+        vs[t][k] = make_uint2(y.x, y.y), vs[t][k + 1] = make_uint2(y.z, y.w);
+      }
+  };
+  auto load_k = [&](const uint8_t *tile) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      TileRegs<HD>::words(tile + (uint32_t)((16 * t + r) * half + g * NB * 4), d.k[t]);
+  };
+  // from the last tile down: the new row's is some wave's first
+  int tile = tile1 - 1 - wave;
+  if (wave < NS) {
+    // queries of group `wave`: lane (r, g) holds channels 32 k + 8 g + 0..7 of row r, every block k
+    const int v = v0 + wave * 16 + r, i = v < V ? v / grp : 0;
+    const float *x = row0 + i * a.ldq + (int64_t)(kvh * grp + (v < V ? v % grp : 0)) * HD + 8 * g;
+    const int64_t p = (pos0 + i) * half + 8 * g;
+    float y[NB][8], mx = 0.f;
+#pragma unroll
+    for (int k = 0; k < NB / 2; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const float4 x0 = *(const float4 *)(x + 32 * k + j), x1 = *(const float4 *)(x + half + 32 * k + j);
+        const float4 cv = *(const float4 *)(c.cs + p + 32 * k + j);
+        const float4 sv = *(const float4 *)(c.sn + p + 32 * k + j);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float e = (&x0.x)[n], o = (&x1.x)[n], cc = (&cv.x)[n], ss = (&sv.x)[n];
+          const float e1 = e * cc - o * ss, o1 = o * cc + e * ss;
+          y[k][j + n] = v < V ? fmaf(e1, ScoreScale<HD>::hi, e1 * ScoreScale<HD>::lo) : 0.f;
+          y[k + NB / 2][j + n] = v < V ? fmaf(o1, ScoreScale<HD>::hi, o1 * ScoreScale<HD>::lo) : 0.f;
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(y[k][j]));
+    const int e = stage_exp(max_xor32(max_xor16(mx)));
+    const float up = pow2f(e);
+    if (g == 0) qc[wave][r] = pow2f(-e);
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      half8_t hi, lo;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {  // in the codes' order, and those that enter 16-fold over 16
+        const float t = y[k][(j & 4) | (j & 1) << 1 | (j & 2) >> 1] * (j < 4 ? up : up * 0.0625f);
+        hi[j] = (half_t)t;
+        lo[j] = (half_t)(t - (float)hi[j]);
+      }
+      q_[wave][k][0][lane] = hi;
+      q_[wave][k][1][lane] = lo;
+    }
+  } else if (stores && wave == NS) {
+    constexpr int LANES = Kv4Row<HD>::LANES;
+#pragma unroll
+    for (int k = 0; k < (HD == 256 ? 2 : 1); ++k) {
+      const int unit = k + lane / LANES, rq = lane % LANES;
+      Kv4Row<HD> row;
+      if (unit < 2) {
+        row.load(unit ? vx : kx, rq);
+        row.load_turn(c.cs + pos0 * half, c.sn + pos0 * half, rq);
+      }
+      fresh.make(c, row, unit, rq, base, list, filled, (int32_t)pos0, blockIdx.z == 0);
+    }
+  }
+  if (tile >= tile0) {
+    const uint8_t *p = base + (int64_t)tile * L::TB;
+    load_k(p);
+    load_scales(p);
+    d.load_v(p, r, g);
+  }
+  __syncthreads();
+  if (stores && tile == filled / kKv4Tile) {
+    const int j = filled % kKv4Tile;
+    d.patch_codes(fresh, j, r, g);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (j >> 2 == 4 * t + g) {
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+          FreshRow<HD>::put(ks[t][k], j, fresh.scale[0][k]);
+          FreshRow<HD>::put(vs[t][k], j, fresh.scale[1][k]);
+        }
+      }
+  }
+  float f[NS];
+  int vis[NS];  // slots that row r of the group sees
+#pragma unroll
+  for (int u = 0; u < NS; ++u) {
+    f[u] = qc[u][r];
+    const int v = v0 + u * 16 + r;
+    vis[u] = filled + (v < V ? v / grp : 0) + 1;
+  }
+  const int all_see = filled + v0 / grp + 1, end = filled + a.rows;
+
+  float4_t acc[NS][2 * NB];
+  float m[NS], l[NS];  // p = 2^(score - m)
+#pragma unroll
+  for (int u = 0; u < NS; ++u) {
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t) acc[u][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  uint32_t magic;
+  asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(magic));
+  float minus1 = -1.f;
+  asm volatile("" : "+s"(minus1));
+  int ql = lane;
+  auto at = [](const uint2 &w, int i) { return __builtin_bit_cast(half4_t, w)[i]; };
+  for (; tile >= tile0; tile -= W) {
+    const uint8_t *next = base + (int64_t)max(tile - W, tile0) * L::TB;  // the last one: unused
+    const int slot0 = tile * kKv4Tile + 4 * g;
+    const bool masked = (tile + 1) * kKv4Tile > all_see;
+    asm volatile("" : "+v"(ql));
+    float y[NS][8];  // scores / f
+    float4_t sc[2][NS][2];
+#pragma unroll
+    for (int k = 0; k <= NB; ++k) {
+      if (k < NB) {
+        const half8_t k0 = k_frag(d.k[0][k], magic), k1 = k_frag(d.k[1][k], magic);
+#pragma unroll
+        for (int u = 0; u < NS; ++u) {
+          const half8_t hi = q_[u][k][0][ql], lo = q_[u][k][1][ql];
+          const float4_t z = {0.f, 0.f, 0.f, 0.f};
+          sc[k & 1][u][0] = mfma(k0, lo, mfma(k0, hi, z));
+          sc[k & 1][u][1] = mfma(k1, lo, mfma(k1, hi, z));
+        }
+      }
+      // a block's products are added while the next one's are made; no further ahead, which would
+      // take more registers than there are
+      if (k > 0)
+#pragma unroll
+        for (int u = 0; u < NS; ++u)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            y[u][i] = fmaf(sc[(k - 1) & 1][u][i >> 2][i & 3], (float)at(ks[i >> 2][k - 1], i & 3),
+                           k > 1 ? y[u][i] : 0.f);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    load_k(next);
+    if (scores) {
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+        if (v0 + u * 16 + r < V) {
+          float *o = scores + (list * V + v0 + u * 16 + r) * score_stride(c.slots) + slot0;
+          *(float4 *)o = make_float4(y[u][0] * f[u], y[u][1] * f[u], y[u][2] * f[u], y[u][3] * f[u]);
+          *(float4 *)(o + 16) =
+              make_float4(y[u][4] * f[u], y[u][5] * f[u], y[u][6] * f[u], y[u][7] * f[u]);
+        }
+    }
+    if (masked) {  // slots that no row sees hold anything: scales of zero for V
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int n = end - (slot0 + 16 * t);  // of the four, the first n
+        const uint32_t x = n > 1 ? ~0u : (n == 1 ? 0xFFFFu : 0u);
+        const uint32_t z = n > 3 ? ~0u : (n == 3 ? 0xFFFFu : 0u);
+#pragma unroll
+        for (int k = 0; k < NB; ++k) vs[t][k].x &= x, vs[t][k].y &= z;
+      }
+    }
+    // the largest |scale| of the lane's slots: f16 magnitudes compare as integers
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 top = {0, 0};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, vs[t][k].x & 0x7FFF7FFFu));
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, vs[t][k].y & 0x7FFF7FFFu));
+      }
+    const uint16_t tops = top[0] > top[1] ? top[0] : top[1];
+    const float dm = (float)__builtin_bit_cast(half_t, tops);
+    float p[NS][8];
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
       auto hidden = [&](int i) { return slot0 + (i < 4 ? i : 12 + i) >= vis[u]; };
+      float sum, most;
       auto weigh = [&]() {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(fmaf(y[u][i], f[u], -m[u]));
-          w[i] = mul_f16(p[i], dv[i >> 2][i & 3]);
-        }
+        for (int i = 0; i < 8; ++i) p[u][i] = __builtin_amdgcn_exp2f(fmaf(y[u][i], f[u], -m[u]));
         if (masked) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (hidden(i)) p[i] = w[i] = 0.f;
+            if (hidden(i)) p[u][i] = 0.f;
         }
-        sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        most = fabsf(w[0]);
+        sum = ((p[u][0] + p[u][1]) + (p[u][2] + p[u][3])) + ((p[u][4] + p[u][5]) + (p[u][6] + p[u][7]));
+        most = p[u][0];
 #pragma unroll
-        for (int i = 1; i < 7; i += 2) most = fmaxf(fmaxf(most, fabsf(w[i])), fabsf(w[i + 1]));
-        most = fmaxf(most, fabsf(w[7]));
+        for (int i = 1; i < 7; i += 2) most = fmaxf(fmaxf(most, p[u][i]), p[u][i + 1]);
+        most = fmaxf(most, p[u][7]) * dm;
       };
       weigh();
-      if (__any(most > kMostW || sum > kMostP)) {
+      if (__any(!(most <= kMostW) || sum > kMostP)) {
         float n = m[u];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint32_t bits = __float_as_uint((float)dv[i >> 2][i & 3]) & 0x7FFFFFFFu;
-          const float lg =  // of at least 2^-24
-              fmaf((float)(int)(bits < 0x33800000u ? 0x33800000u : bits), 0x1p-23f, -127.f - kLift);
+          uint32_t bits = 0x33800000u;  // at least 2^-24
+#pragma unroll
+          for (int k = 0; k < NB; ++k) {
+            const uint32_t x = __float_as_uint((float)at(vs[i >> 2][k], i & 3)) & 0x7FFFFFFFu;
+            bits = x > bits ? x : bits;
+          }
+          const float lg = fmaf((float)(int)bits, 0x1p-23f, -127.f - kLift);
           if (!masked || !hidden(i)) n = fmaxf(n, fmaf(y[u][i], f[u], lg));
         }
         n = max_xor16(n);
@@ -514,53 +847,52 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
         weigh();
       }
       l[u] += sum;
-      half2_t hp[4], lp[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {  // V's pairs: slots (0, 2), (1, 3) of each half
-        const int i = (k & 1) + (k >> 1) * 4;
-        hp[k] = half2_t{(half_t)w[i], (half_t)w[i + 2]};
-        lp[k] = half2_t{(half_t)fmaf((float)hp[k][0], minus1, w[i]),
-                        (half_t)fmaf((float)hp[k][1], minus1, w[i + 2])};
-      }
-      wh[u] = __builtin_bit_cast(half8_t, hp);
-      wl[u] = __builtin_bit_cast(half8_t, lp);
     }
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
       const uint32_t w0 = d.v[0][k], h0 = w0 >> 8, w1 = d.v[1][k], h1 = w1 >> 8;
       const half8_t va = v_frag<1>(w0, h0, w1, h1, magic);
-      const half8_t vb = v_frag<16>(w0, h0, w1, h1, magic);  // channels 16..31 of the block
+      const half8_t vb = v_frag<16>(w0, h0, w1, h1, magic);
 #pragma unroll
-      for (int u = 0; u < NSUB; ++u) {
-        acc[u][2 * k] = mfma(wh[u], va, acc[u][2 * k]);
-        acc[u][2 * k + 1] = mfma(wh[u], vb, acc[u][2 * k + 1]);
-        acc[u][2 * k] = mfma(wl[u], va, acc[u][2 * k]);
-        acc[u][2 * k + 1] = mfma(wl[u], vb, acc[u][2 * k + 1]);
+      for (int u = 0; u < NS; ++u) {
+        half2_t hp[4], lp[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {  // V's pairs: slots (0, 2), (1, 3) of each half
+          const int i = (n & 1) + (n >> 1) * 4, t = n >> 1;
+          float wa = mul_f16(p[u][i], at(vs[t][k], i & 3));
+          float wb = mul_f16(p[u][i + 2], at(vs[t][k], (i & 3) + 2));
+          asm("" : "+v"(wa), "+v"(wb));  // else each is made again as it is rounded
+          split_f16(wa, wb, minus1, hp[n], lp[n]);
+        }
+        const half8_t wh = __builtin_bit_cast(half8_t, hp), wl = __builtin_bit_cast(half8_t, lp);
+        acc[u][2 * k] = mfma(wh, va, acc[u][2 * k]);
+        acc[u][2 * k + 1] = mfma(wh, vb, acc[u][2 * k + 1]);
+        acc[u][2 * k] = mfma(wl, va, acc[u][2 * k]);
+        acc[u][2 * k + 1] = mfma(wl, vb, acc[u][2 * k + 1]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    load_scales(next);
     d.load_v(next, r, g);
   }
 
+  __syncthreads();
   // the waves' sums: lane (r, g), register i holds row 4 g + i, channel 16 t + r
 #pragma unroll
-  for (int u = 0; u < NSUB; ++u) {
-    float sum = sum_xor32(sum_xor16(l[u]));
+  for (int u = 0; u < NS; ++u) {
+    const float sum = sum_xor32(sum_xor16(l[u]));
     if (g == 0) lm[wave][u][r] = make_float2(m[u], sum);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 4 * g + i, rb = row / HPS;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int t = 0; t < 2 * NB; ++t)
-        if (rb == t / 2)
-          lo_[wave][u][row % HPS * HD + 16 * t + r] = acc[u][t][i] * (t & 1 ? 0.0625f : 1.f);
-    }
+        lo_[wave][u][(4 * g + i) * HD + 16 * t + r] = acc[u][t][i] * (t & 1 ? 0.0625f : 1.f);
   }
   __syncthreads();
   float *out = rec + (list * cut.S + it.split) * V * RS;
-  for (int e = tid; e < NSUB * 512; e += 64 * W) {
-    const int u = e >> 9, hh = (e & 511) / HD, ch = e & (HD - 1), row = (ch >> 5) * HPS + hh;
-    const int v = v0 + u * HPS + hh;
-    if (v >= V) continue;
+  for (int e = tid; e < NS * 16 * HD; e += 64 * W) {
+    const int u = e / (16 * HD), row = e / HD % 16, ch = e % HD, v = v0 + u * 16 + row;
+    if (v >= V) break;
     float mx = lm[0][u][row].x, o = 0.f, ls = 0.f;
 #pragma unroll
     for (int k = 1; k < W; ++k) mx = fmaxf(mx, lm[k][u][row].x);
@@ -568,7 +900,7 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
     for (int k = 0; k < W; ++k) {
       const float2 ml = lm[k][u][row];
       const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
-      o = fmaf(w, lo_[k][u][e & 511], o);
+      o = fmaf(w, lo_[k][u][row * HD + ch], o);
       ls = fmaf(w, ml.y, ls);
     }
     if (sp.n == 1) {  // nothing to join
@@ -693,10 +1025,12 @@ __global__ __launch_bounds__(kThreads) void kv4_weights_kernel(Kv4Cache c, Kv4At
     if (t + k < filled + a.rows) to[k] = a.weights_mode == 2 ? to[k] + w[k] : w[k];
 }
 
-// How a call is cut: NSUB groups of HPS query rows per workgroup of W waves, `wgs` workgroups
-// at a time on the GPU for each group of rows, a list in S of them at most.
+// How a call is cut: kv4_rows_kernel with nsub groups of 16 query rows per workgroup (dense), or
+// kv4_attention_kernel with HPS rows; W waves per workgroup, `wgs` workgroups at a time on the
+// GPU for each set of rows, a list in S of them at most.
 struct Plan {
   int V, nsub, nz;
+  bool dense;
   Cut cut;
   int64_t lists;
 };
@@ -704,19 +1038,24 @@ Plan plan(int rows, int n_seq, int nh, int nkv, int hd, int slots) {
   Plan p;
   const int hps = 512 / hd;
   p.V = rows * (nh / nkv);
-  p.nsub = hd < 256 && p.V > hps ? 2 : 1;
-  p.nz = (p.V + p.nsub * hps - 1) / (p.nsub * hps);
+  // The two kernels, V query rows per list (us; 4 sequences of 4095 slots, 8 KV heads, 4 of 256
+  // channels; kv4_attention_kernel in as many groups as it takes against kv4_rows_kernel):
+  //   channels 64:  V 8 16.4 / 16.5, 16 20.2 / 18.7, 64 36.0 / 28.9
+  //   channels 128: V 4 one group, 8 21.3 / 19.7, 16 26.5 / 22.9, 128 92.9 / 54.5
+  //   channels 256: V 4 18.2 / 20.3, 8 25.2 / 25.6, 12 45.0 / 28.1, 128 165 / 58.0
+  p.dense = p.V > (hd == 128 ? 4 : 8);
+  const int group = p.dense ? 16 : hps;
+  p.nsub = p.dense && p.V > 16 && hd < 256 ? 2 : 1;
+  p.nz = (p.V + p.nsub * group - 1) / (p.nsub * group);
   p.lists = (int64_t)n_seq * nkv;
-  // Waves per workgroup and workgroups at a time, measured (us; 32 / 8 heads of 128 unless said):
-  // many lists of different lengths balance better in small workgroups (16 sequences of up to
-  // 4095 slots: 8 x 512 24.8, 4 x 768 21.2); few lists leave fewer records with large ones (6000
-  // slots: 11.1 against 12.7; 130000: 40.2 against 40.8).  Two groups of rows take 182 registers:
-  // two workgroups of four waves (32 rows over 20000 slots: 4 x 512 133, 8 x 512 142, 8 x 256 218,
-  // where ten of the 256 CUs get two); 256 channels 160 (4 sequences of 9000 slots, 16 / 2 heads:
-  // 8 x 256 32.3, 4 x 768 34.2).
+  // Waves per workgroup and workgroups at a time (us; 32 / 8 heads of 128): many lists of
+  // different lengths balance better in small workgroups (16 sequences of up to 4095 slots:
+  // 8 x 512 24.8, 4 x 768 21.2); few lists leave fewer records with large ones (6000 slots: 11.1
+  // against 12.7; 130000: 40.2 against 40.8).  Of 256 channels and with many rows a kernel takes
+  // up to 256 registers: two waves per SIMD.
   const bool many = p.lists * p.nz >= 32;
   int resident;
-  if (p.nsub == 2) {
+  if (p.dense) {
     p.cut.W = 4, resident = 512;
   } else if (hd == 256) {
     p.cut.W = 8, resident = 256;
@@ -760,14 +1099,22 @@ hipError_t launch(const Kv4Cache &c, const Kv4Attn &a, hipStream_t s) {
   auto go = [&](auto *kernel) {
     hipLaunchKernelGGL(kernel, grid, block, 0, s, c, a, rec, lse, scores, p.cut, inside);
   };
-  if constexpr (HD == 256)
-    go(kv4_attention_kernel<HD, 1, 8, 2>);
-  else if (p.nsub == 2)
-    go(kv4_attention_kernel<HD, 2, 4, 2>);
-  else if (p.cut.W == 4)
-    go(kv4_attention_kernel<HD, 1, 4, 4>);
-  else
-    go(kv4_attention_kernel<HD, 1, 8, 4>);
+  if (p.dense) {
+    if constexpr (HD < 256) {
+      if (p.nsub == 2)
+        go(kv4_rows_kernel<HD, 2>);
+      else
+        go(kv4_rows_kernel<HD, 1>);
+    } else {
+      go(kv4_rows_kernel<HD, 1>);
+    }
+  } else if constexpr (HD == 256) {
+    go(kv4_attention_kernel<HD, 8, 2>);
+  } else if (p.cut.W == 4) {
+    go(kv4_attention_kernel<HD, 4, 4>);
+  } else {
+    go(kv4_attention_kernel<HD, 8, 4>);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (p.cut.S > 1) {
