@@ -578,7 +578,7 @@ int gguf_hip_kv4_append(const float *qkv, int64_t ldqkv, int64_t n_rows, const i
   if (!aligned(starts, 8)) return fail(GGUF_HIP_ERR_ALIGN, "[gguf-hip] kv4 buffers misaligned");
   const gguf::Kv4Cache c{(uint8_t *)kv, lengths,   pos,   cos_table, sin_table,  positions, weights,
                          rope_rows,     n_seq,     n_heads, n_kv_heads, head_dim, (int)slots};
-  return hip_status(gguf::launch_kv4_append(c, qkv, ldqkv, n_rows, starts, (hipStream_t)stream),
+  return hip_status(gguf::launch_kv4_append(c, qkv, ldqkv, n_rows, starts, false, (hipStream_t)stream),
                     "kv4_append launch");
 }
 

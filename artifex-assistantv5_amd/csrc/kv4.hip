@@ -18,7 +18,8 @@ template <int HD, int N>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
                                                               const float *__restrict__ qkv,
                                                               int64_t ldq, uint32_t n_rows,
-                                                              const int64_t *__restrict__ starts) {
+                                                              const int64_t *__restrict__ starts,
+                                                              bool whole) {
   constexpr int LANES = Kv4Row<HD>::LANES, SIDE = 64 / LANES;
   const int lane = threadIdx.x & 63, q = lane % LANES;
   const uint32_t r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -33,7 +34,7 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
     row[i].load(x + (int64_t)((u & 1) * c.nkv + (u >> 1)) * HD, q);
   }
   uint32_t s;
-  int64_t i;
+  int64_t i, more = 0;  // `whole`: the sequence's rows behind this one
   if (starts) {
     if (r < starts[0] || r >= starts[c.n_seq]) return;
     uint32_t lo = 0, hi = c.n_seq;  // starts[lo] <= r < starts[hi]
@@ -50,9 +51,10 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
     const uint32_t per = n_rows / (uint32_t)c.n_seq;
     s = r / per;
     i = r - s * per;
+    if (whole) more = per - 1 - i;
   }
-  const int64_t slot = c.lengths[s] + i, p = c.pos[s] + i;
-  if (slot < 0 || slot >= c.slots || p < 0 || p >= c.rope_rows) return;
+  const int64_t slot = c.lengths[s] + i, p = c.pos[s] + i, before = whole ? i : 0;
+  if (slot < before || slot >= c.slots - more || p < before || p >= c.rope_rows - more) return;
   row[0].load_turn(c.cs + p * (HD / 2), c.sn + p * (HD / 2), q);
 #pragma unroll
   for (int k = 0; k < N; ++k) {
@@ -485,15 +487,15 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(Kv4Cache c, Kv4Evi
   }
 
 hipError_t launch_kv4_append(const Kv4Cache &c, const float *qkv, int64_t ldq, int64_t n_rows,
-                             const int64_t *starts, hipStream_t s) {
+                             const int64_t *starts, bool whole, hipStream_t s) {
   // few rows: as many waves as there are units; many: fewer waves with more in flight
   const int n = n_rows * c.nkv >= 8192 ? 4 : 1, per = n * (256 / c.hd);
   const dim3 grid((unsigned)((n_rows + 3) / 4), (unsigned)((2 * c.nkv + per - 1) / per));
   KV4_DISPATCH(c.hd, if (n == 4) hipLaunchKernelGGL((kv4_append_kernel<HD, 4>), grid,
                                                     dim3(kThreads), 0, s, c, qkv, ldq,
-                                                    (uint32_t)n_rows, starts);
+                                                    (uint32_t)n_rows, starts, whole);
                else hipLaunchKernelGGL((kv4_append_kernel<HD, 1>), grid, dim3(kThreads), 0, s, c,
-                                       qkv, ldq, (uint32_t)n_rows, starts));
+                                       qkv, ldq, (uint32_t)n_rows, starts, whole));
   return hipGetLastError();
 }
 

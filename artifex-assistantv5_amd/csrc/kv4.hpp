@@ -149,8 +149,9 @@ __device__ __forceinline__ void kv4_put_row(uint8_t *list, int slot, Kv4Row<HD> 
     *(half_t *)(tile + (is_k ? L::KS : L::VS) + ((j >> 2) * L::NB + b) * 8 + (j & 3) * 2) = scale;
 }
 
+// whole (without starts): of a sequence whose rows do not all fit, none is stored.
 hipError_t launch_kv4_append(const Kv4Cache &c, const float *qkv, int64_t ldq, int64_t n_rows,
-                             const int64_t *starts, hipStream_t s);
+                             const int64_t *starts, bool whole, hipStream_t s);
 hipError_t launch_kv4_load(const uint8_t *kv, const int64_t *lengths, float *k, float *v,
                            int64_t out_slots, int n_layers, int n_seq, int nkv, int hd, int slots,
                            hipStream_t s);

@@ -30,7 +30,7 @@ constexpr int record_floats() {
 // The slots in use before the call, or -1 if the sequence takes no part.
 __device__ __forceinline__ int kv4_filled(const Kv4Cache &c, int64_t s, int rows) {
   const int64_t n = c.lengths[s], p = c.pos[s];
-  return n < 0 || n + rows > c.slots || p < 0 || p + rows > c.rope_rows ? -1 : (int)n;
+  return n < 0 || n > c.slots - rows || p < 0 || p > c.rope_rows - rows ? -1 : (int)n;
 }
 
 // How the tiles of a list are cut: `per` for each workgroup, `n` of them at most S.  Every
@@ -299,9 +299,11 @@ struct TileRegs {
 //   of query row h, so the scales need no pass of their own; only the channels of block b of
 //   that row's output are used.  p * scale enters as two f16 parts.
 // - Each row's p is 2^(score - m) with a running m, so that p * scale is at most 2^10 when m is
-//   set and stays below 2^14 in f16, whatever V's range; where a tile passes that (or p 2^40:
-//   scales near zero), m is raised to the largest score + log2 |scale| (the float's bits read as
-//   a number, within 0.09) and the sums are scaled down.  That is rare after the first tiles.
+//   set and stays below 2^14 in f16, whatever V's range; where a tile passes that (or p 2^100:
+//   scales of zero), m is raised to the largest score + log2 |scale| (the float's bits read as a
+//   number, within 0.09) and the sums are scaled down.  That is rare after the first tiles.  A
+//   scale of zero counts as 2^-84, so that a slot of zeros far above the others takes no bits
+//   from them and p's sum stays a float.
 // - K's registers take the next tile as soon as its scores are made, V's after its products:
 //   one tile in flight per wave, four waves per SIMD.
 // Bound: HBM, 9/8 head_dim bytes per slot and list.
@@ -313,7 +315,7 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
                                                                bool store) {
   using L = Kv4<HD>;
   constexpr int NB = L::NB, HPS = 16 / NB, half = HD / 2, RS = record_floats<HD>();
-  constexpr float kLift = 10.f, kMostW = 16384.f, kMostP = 0x1p40f;
+  constexpr float kLift = 10.f, kMostW = 16384.f, kMostP = 0x1p100f;
   __shared__ float lo_[W][512];      // per wave: HPS rows of HD sums
   __shared__ float2 lm[W][16];       // and the 16 rows' (m, sum of p)
   __shared__ half8_t q_[NB][2][64];  // queries: per block, hi and lo part, a B operand
@@ -492,8 +494,8 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t bits = __float_as_uint((float)dv[i >> 2][i & 3]) & 0x7FFFFFFFu;
-        const float lg =  // of at least 2^-24
-            fmaf((float)(int)(bits < 0x33800000u ? 0x33800000u : bits), 0x1p-23f, -127.f - kLift);
+        const float lg =  // zero: as 2^-84
+            fmaf((float)(int)(bits < 0x15800000u ? 0x15800000u : bits), 0x1p-23f, -127.f - kLift);
         if (!masked || !hidden(i)) n = fmaxf(n, fmaf(y[i], f, lg));
       }
       n = max_xor16(n);
@@ -575,7 +577,9 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 // where the kernel above has 8), but every column is a row of its own: a quarter of the MFMAs and
 // exponentials per row at 128 channels, an eighth at 256.
 // The largest |p * scale| is bounded by the largest p times the largest |scale| of the lane's
-// slots; where m is raised for it, by each slot's own.
+// slots; where m is raised for it, by each slot's own.  m is that of all blocks: p * scale of a
+// block whose scales are under 2^-13 of the others' falls below 2^-3, where two f16 parts hold
+// fewer bits (2^-25 absolute: 2^-35 of the row's largest).
 // Bound: vector instructions, about 150 for a tile's codes and 190 for each group of rows (128
 // channels).
 template <int HD, int NS>
@@ -586,7 +590,8 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
                                                           bool store) {
   using L = Kv4<HD>;
   constexpr int W = 4, NB = L::NB, half = HD / 2, RS = record_floats<HD>();
-  constexpr float kLift = 10.f, kMostW = 16384.f, kMostP = 0x1p40f;
+  constexpr float kLift = 10.f, kMostW = 16384.f, kMostP = 0x1p100f;
+  constexpr bool kStores = HD == 128;  // of the others no call of one new row has that many heads
   // Queries (per block, hi and lo part, a B operand) while tiles are read, then the waves' sums, 16
   // rows of HD per group: 64 KB together, so two workgroups fit a CU's LDS, 82 apart.
   __shared__ union {
@@ -678,18 +683,13 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
       q_[wave][k][0][lane] = hi;
       q_[wave][k][1][lane] = lo;
     }
-  } else if (stores && wave == NS) {
+  } else if (kStores && stores && wave == NS) {
     constexpr int LANES = Kv4Row<HD>::LANES;
-#pragma unroll
-    for (int k = 0; k < (HD == 256 ? 2 : 1); ++k) {
-      const int unit = k + lane / LANES, rq = lane % LANES;
-      Kv4Row<HD> row;
-      if (unit < 2) {
-        row.load(unit ? vx : kx, rq);
-        row.load_turn(c.cs + pos0 * half, c.sn + pos0 * half, rq);
-      }
-      fresh.make(c, row, unit, rq, base, list, filled, (int32_t)pos0, blockIdx.z == 0);
-    }
+    const int unit = lane / LANES, rq = lane % LANES;
+    Kv4Row<HD> row;
+    row.load(unit ? vx : kx, rq);
+    row.load_turn(c.cs + pos0 * half, c.sn + pos0 * half, rq);
+    fresh.make(c, row, unit, rq, base, list, filled, (int32_t)pos0, blockIdx.z == 0);
   }
   if (tile >= tile0) {
     const uint8_t *p = base + (int64_t)tile * L::TB;
@@ -698,7 +698,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
     d.load_v(p, r, g);
   }
   __syncthreads();
-  if (stores && tile == filled / kKv4Tile) {
+  if (kStores && stores && tile == filled / kKv4Tile) {
     const int j = filled % kKv4Tile;
     d.patch_codes(fresh, j, r, g);
 #pragma unroll
@@ -823,7 +823,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
         float n = m[u];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          uint32_t bits = 0x33800000u;  // at least 2^-24
+          uint32_t bits = 0x15800000u;  // zeros: 2^-84
 #pragma unroll
           for (int k = 0; k < NB; ++k) {
             const uint32_t x = __float_as_uint((float)at(vs[i >> 2][k], i & 3)) & 0x7FFFFFFFu;
@@ -1089,7 +1089,7 @@ hipError_t launch(const Kv4Cache &c, const Kv4Attn &a, hipStream_t s) {
   const bool inside = a.store && a.rows == 1;  // the one row is stored by the workgroups
   if (a.store && !inside) {
     const hipError_t e =
-        launch_kv4_append(c, a.qkv, a.ldq, (int64_t)c.n_seq * a.rows, nullptr, s);
+        launch_kv4_append(c, a.qkv, a.ldq, (int64_t)c.n_seq * a.rows, nullptr, true, s);
     if (e != hipSuccess) return e;
   }
   // No call has more items than wgs + lists (every list but for its last workgroup gets whole

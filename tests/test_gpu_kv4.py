@@ -150,7 +150,13 @@ def _reference(cache, qkv, lengths, pos, cos, sin, heads, kv, hd, rows):
                                                 n + 1 + np.arange(rows))
             out[at, h] = o
             err = 2 * EPS * 4 * size + EPS
-            bound[at, h] = mass * err[:, None]
+            # p * scale enters the products as two f16 parts: off by 2^-22 of it (within err) or by
+            # 2^-25, half a step of the smallest f16.  It is scaled so that a row's largest is at
+            # least 2^9.9 (zero scales counting as 2^-84), so 2^-25 is at most 2^-34.9 of that;
+            # times a code of at most 8 = (largest |v| of the block) / scale, for every slot.
+            most = np.abs(vals[s, h // grp, :n + rows]).max(1)
+            top = (pr[:, :n + rows] * np.maximum(most, 2.0 ** -81)).max(1)
+            bound[at, h] = mass * err[:, None] + (2.0 ** -34.9 * (n + rows) * top)[:, None]
             weights[s, h // grp] += pr.sum(0)
             wbound[s, h // grp] += (pr * err[:, None]).sum(0)
     return out, bound, weights, wbound
@@ -173,6 +179,13 @@ CASES = [
     (16, 2, 256, 64, [20, 31], 3),
     (8, 1, 128, 96, [31], 64),                    # the most rows
     (8, 2, 128, 2048, [2047, 1025], 1),
+    (8, 1, 64, 96, [50, 94, 62], 2),              # 16, 6, 24 and 72 query rows of a list
+    (12, 2, 128, 1024, [1000, -1, 0], 1),
+    (8, 1, 256, 160, [130, -1, 31], 3),
+    (16, 2, 256, 2048, [2000], 9),
+    (8, 1, 128, 4096, [4000, 900], 16),           # 128 over several workgroups
+    (16, 2, 64, 2048, [1990], 7),
+    (4, 2, 128, 64, [62, -2, 64, 61], 3),         # rows that fit in part: the sequence takes none
 ]
 
 
@@ -230,14 +243,15 @@ def test_attention(kv4, heads, kv, hd, slots, lengths, rows):
     assert np.array_equal(dev.cpu().numpy(), cache)
 
 
+@pytest.mark.parametrize("heads,rows", [(4, 1), (8, 2)])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("scale_q,scale_k,scale_v", [
     (1e-12, 1.0, 1.0), (1e4, 1e-3, 1e-4), (30.0, 1.0, 3e4), (1e-3, 1e4, 1e-2), (3.0, 1.0, 1e-5)])
-def test_attention_range(kv4, hd, scale_q, scale_k, scale_v):
+def test_attention_range(kv4, heads, rows, hd, scale_q, scale_k, scale_v):
     """Queries, keys and values far from one, slots with values a thousand times the others',
     scales that are f16 subnormals, and zero values."""
     rng = np.random.default_rng(7)
-    heads, kv, slots, n = 4, 1, 320, 301
+    kv, slots, n = 1, 320, 301
     cos, sin = _tables(400, hd)
     cache = np.zeros((1, kv, slots // 32, 36 * hd), np.uint8)
     for t in range(n):
@@ -245,17 +259,41 @@ def test_attention_range(kv4, hd, scale_q, scale_k, scale_v):
         v = v * (1000.0 if t % 37 == 5 and scale_v < 10 else 1.0) * (t % 5 != 0)
         model.put(cache, 0, 0, t, (k * scale_k).astype(np.float32),
                   (v * scale_v).astype(np.float32))
-    qkv = rng.standard_normal((1, (heads + 2) * hd)).astype(np.float32)
+    qkv = rng.standard_normal((rows, (heads + 2) * hd)).astype(np.float32)
     qkv[:, :heads * hd] *= scale_q
     qkv[:, heads * hd:(heads + 1) * hd] *= scale_k
     qkv[:, (heads + 1) * hd:] *= scale_v
-    dev, out = _cuda(cache), torch.empty(1, heads * hd, device="cuda")
+    dev, out = _cuda(cache), torch.empty(rows, heads * hd, device="cuda")
     kv4.attention(_cuda(qkv), _i64([n]), _i64([n]), _cuda(cos), _cuda(sin), dev, out, heads,
-                  kv4.attention_workspace(dev, heads))
+                  kv4.attention_workspace(dev, heads, rows=rows))
     cache = dev.cpu().numpy()
-    ref, bound, _, _ = _reference(cache, qkv, [n], [n], cos, sin, heads, kv, hd, 1)
+    ref, bound, _, _ = _reference(cache, qkv, [n], [n], cos, sin, heads, kv, hd, rows)
     got = out.cpu().numpy().reshape(ref.shape)
     assert (np.abs(got - ref) <= bound + 1e-38).all(), (np.abs(got - ref) / bound).max()
+
+
+@pytest.mark.parametrize("heads,rows", [(4, 1), (8, 2)])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_uneven_blocks(kv4, heads, rows, hd):
+    """Blocks of V's channels that differ 4096-fold, and single slots 4096 times the others: each
+    channel is as near as its own values allow."""
+    rng = np.random.default_rng(hd)
+    slots, n = 192, 170
+    cos, sin = _tables(200, hd)
+    cache = np.zeros((1, 1, slots // 32, 36 * hd), np.uint8)
+    size = np.repeat(np.resize([1.0, 4096.0], hd // 32), 32)
+    for t in range(n):
+        k, v = rng.standard_normal((2, hd))
+        v = v * size / 512 * (4096.0 if t == 160 else 1.0)   # scales below 65504
+        model.put(cache, 0, 0, t, k.astype(np.float32), v.astype(np.float32))
+    qkv = rng.standard_normal((rows, (heads + 2) * hd)).astype(np.float32)
+    dev, out = _cuda(cache), torch.empty(rows, heads * hd, device="cuda")
+    kv4.attention(_cuda(qkv), _i64([n]), _i64([n]), _cuda(cos), _cuda(sin), dev, out, heads,
+                  kv4.attention_workspace(dev, heads, rows=rows))
+    cache = dev.cpu().numpy()
+    ref, bound, _, _ = _reference(cache, qkv, [n], [n], cos, sin, heads, 1, hd, rows)
+    got = out.cpu().numpy().reshape(ref.shape)
+    assert (np.abs(got - ref) <= bound).all(), (np.abs(got - ref) / bound).max()
 
 
 def test_attention_far_lists(kv4):
