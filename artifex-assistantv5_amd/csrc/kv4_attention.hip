@@ -591,7 +591,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
   using L = Kv4<HD>;
   constexpr int W = 4, NB = L::NB, half = HD / 2, RS = record_floats<HD>();
   constexpr float kLift = 10.f, kMostW = 16384.f, kMostP = 0x1p100f;
-  constexpr bool kStores = HD == 128;  // of the others no call of one new row has that many heads
+  constexpr bool kStores = HD != 64;  // of 64 channels no call of one new row has that many heads
   // Queries (per block, hi and lo part, a B operand) while tiles are read, then the waves' sums, 16
   // rows of HD per group: 64 KB together, so two workgroups fit a CU's LDS, 82 apart.
   __shared__ union {
@@ -683,9 +683,9 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
       q_[wave][k][0][lane] = hi;
       q_[wave][k][1][lane] = lo;
     }
-  } else if (kStores && stores && wave == NS) {
-    constexpr int LANES = Kv4Row<HD>::LANES;
-    const int unit = lane / LANES, rq = lane % LANES;
+  } else if (kStores && stores && wave >= NS && wave < NS + (HD == 256 ? 2 : 1)) {
+    constexpr int LANES = Kv4Row<HD>::LANES;  // the new row's K (unit 0) and V (1)
+    const int unit = (wave - NS) * (64 / LANES) + lane / LANES, rq = lane % LANES;
     Kv4Row<HD> row;
     row.load(unit ? vx : kx, rq);
     row.load_turn(c.cs + pos0 * half, c.sn + pos0 * half, rq);
@@ -890,24 +890,30 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
   }
   __syncthreads();
   float *out = rec + (list * cut.S + it.split) * V * RS;
-  for (int e = tid; e < NS * 16 * HD; e += 64 * W) {
-    const int u = e / (16 * HD), row = e / HD % 16, ch = e % HD, v = v0 + u * 16 + row;
+  // four channels per thread: the rows' factors are most of the work
+  for (int e = tid; e < NS * 4 * HD; e += 64 * W) {
+    const int u = e / (4 * HD), row = e / (HD / 4) % 16, ch = e % (HD / 4) * 4, v = v0 + u * 16 + row;
     if (v >= V) break;
-    float mx = lm[0][u][row].x, o = 0.f, ls = 0.f;
+    float mx = lm[0][u][row].x, ls = 0.f;
+    float4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 1; k < W; ++k) mx = fmaxf(mx, lm[k][u][row].x);
 #pragma unroll
     for (int k = 0; k < W; ++k) {
       const float2 ml = lm[k][u][row];
       const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
-      o = fmaf(w, lo_[k][u][row * HD + ch], o);
+      const float4_t x = *(const float4_t *)&lo_[k][u][row * HD + ch];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) o[n] = fmaf(w, x[n], o[n]);
       ls = fmaf(w, ml.y, ls);
     }
     if (sp.n == 1) {  // nothing to join
-      a.out[(s * a.rows + v / grp) * a.ldo + (kvh * grp + v % grp) * HD + ch] = o / ls;
+      float *to = a.out + (s * a.rows + v / grp) * a.ldo + (kvh * grp + v % grp) * HD + ch;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) to[n] = o[n] / ls;
       if (lse && ch == 0) lse[list * V + v] = make_float2(mx, 1.f / ls);
     } else {
-      out[v * RS + ch] = o;
+      *(float4_t *)(out + v * RS + ch) = o;
       if ((ch & 31) == 0) *(float2 *)(out + v * RS + HD + 2 * (ch >> 5)) = make_float2(mx, ls);
     }
   }
@@ -1040,10 +1046,10 @@ Plan plan(int rows, int n_seq, int nh, int nkv, int hd, int slots) {
   p.V = rows * (nh / nkv);
   // The two kernels, V query rows per list (us; 4 sequences of 4095 slots, 8 KV heads, 4 of 256
   // channels; kv4_attention_kernel in as many groups as it takes against kv4_rows_kernel):
-  //   channels 64:  V 8 16.4 / 16.5, 16 20.2 / 18.7, 64 36.0 / 28.9
-  //   channels 128: V 4 one group, 8 21.3 / 19.7, 16 26.5 / 22.9, 128 92.9 / 54.5
-  //   channels 256: V 4 18.2 / 20.3, 8 25.2 / 25.6, 12 45.0 / 28.1, 128 165 / 58.0
-  p.dense = p.V > (hd == 128 ? 4 : 8);
+  //   channels 64:  V 8 16.3 / 16.1 (one sequence 13.4 / 14.1), 16 20.2 / 17.6, 64 36.0 / 27.2
+  //   channels 128: V 4 one group, 8 21.3 / 18.9, 16 26.5 / 21.0, 128 92.9 / 50.2
+  //   channels 256: V 4 18.0 / 19.6, 8 24.9 / 23.8, 12 45.0 / 25.6, 128 165 / 54.0
+  p.dense = p.V > (hd == 64 ? 8 : 4);
   const int group = p.dense ? 16 : hps;
   p.nsub = p.dense && p.V > 16 && hd < 256 ? 2 : 1;
   p.nz = (p.V + p.nsub * group - 1) / (p.nsub * group);
