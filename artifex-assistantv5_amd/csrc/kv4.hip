@@ -1,4 +1,6 @@
 // The 4-bit KV cache: storing rows, reading them back, eviction.
+#include <type_traits>
+
 #include "kv4.hpp"
 
 namespace gguf {
@@ -170,28 +172,44 @@ __device__ __forceinline__ int again(int v) {
   return v;
 }
 
+// x of the eight lanes (aligned) that this one is of, or-ed.
+__device__ __forceinline__ uint32_t or8(uint32_t x) {
+  x |= __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, true);   // lane ^ 1
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, true);   // lane ^ 2
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, true);  // 7 - lane: the other four
+  return x;
+}
+
 // One workgroup per list; a turn takes 4096 slots, four neighbouring ones per thread, and the
 // keys of T turns stay in registers (a longer list is read again, segment by segment, for every
 // pass).
 // - The keep-th largest key by digits of 11, 11 and 10 bits: a histogram in LDS (four copies
 //   for the first digit, where most keys share a few bins), then a scan from the top.  Where
 //   some of the keys equal to it go, their ranks decide (ranked).
-// - The ranks within a list need the counts of all waves' turns before one's own: every wave
-//   leaves the count of each turn, and one scan of the workgroup over them gives all ranks.
-// Bound: one CU's loads and vector instructions.  A slot per thread and turn, 11 bits a digit:
-// 29 us for 256 lists of 16000 slots, 72 for 48 lists of up to 61000 (in 30 of them the keys were
-// read and counted, in 29 the ranks made); four slots per thread, and ranks of equal keys only
-// where needed: see DESIGN.
+// - Ranks: the turns' four bits per thread (stays, equals) become a bitmap in LDS, of which each
+//   thread takes its segment's next 4 T slots: counts are bit counts, one scan of the workgroup
+//   gives all ranks.  The lists of slots are put together in LDS and written in order.
+// Bound: one CU's loads and vector instructions.  48 lists of up to 61000 slots: 11 us to read and
+// make the keys, 11 for the three digits, 13 for ranks and lists (35 where the ranks were counted
+// turn by turn with ballots).  An attend-and-evict step of 48 lists with its moves: 75.5 -> 53.1.
 template <int T>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, Kv4Evict e, int half) {
-  constexpr int kBins = 2048, kTurn = 4 * kSelThreads, kSeg = T * kTurn, kCnt = T * kSelWaves;
-  __shared__ int hist[4][kBins], cnt[2][kCnt], part[kSelWaves], found[3];
+  constexpr int kBins = 2048, kTurn = 4 * kSelThreads, kSeg = T * kTurn, kMine = 4 * T;
+  using Bits = std::conditional_t<T == 16, uint64_t, uint32_t>;  // of a thread's kMine slots
+  __shared__ __align__(16) union {
+    int hist[4][kBins];
+    struct {
+      uint32_t map[2][kSeg / 32];  // stays, equals: a bit per slot of the segment
+      uint16_t slot[kSeg];         // its holes, then its moves
+    };
+  } sh;
+  __shared__ int part[kSelWaves], found[3];
+  auto &hist = sh.hist;
   const int64_t list = blockIdx.x, lists = gridDim.x;
   const int64_t s = list / c.nkv % c.n_seq;
   const int64_t n64 = c.lengths[s];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint64_t below = (1ull << lane) - 1ull;
   int32_t *count = (int32_t *)e.work + list;
   const float *w = e.weights + list * c.slots;
   const int32_t *p = e.positions + list * c.slots;
@@ -227,7 +245,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
       key[4 * t + 1] = evict_key(x.y, q.y, from, sinks);
       key[4 * t + 2] = evict_key(x.z, q.z, from, sinks);
       key[4 * t + 3] = evict_key(x.w, q.w, from, sinks);
-      if (t % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // 4 loads of a wave in flight at a time
+      if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // 8 loads of a wave in flight at a time
     }
   };
   uint32_t prefix = 0;
@@ -277,121 +295,74 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
       found[2] = h1;
     }
     __syncthreads();
-    prefix |= (uint32_t)found[0] << shift;
-    need = found[1];
-    alike = found[2];
+    prefix |= (uint32_t)__builtin_amdgcn_readfirstlane(found[0]) << shift;
+    need = __builtin_amdgcn_readfirstlane(found[1]);
+    alike = __builtin_amdgcn_readfirstlane(found[2]);
   }
   const bool ranked = need < alike;
   int32_t *holes = evict_holes(e.work, lists, list, half), *late = holes + half;
+  const uint32_t lim = ranked ? prefix : prefix - 1;  // not ranked: all keys from `prefix` stay
+  auto take = [&](const uint32_t *map) -> Bits {
+    if constexpr (T == 16) return ((const uint64_t *)map)[tid];
+    if constexpr (T == 4) return ((const uint16_t *)map)[tid];
+    return map[tid >> 3] >> (4 * (tid & 7)) & 15u;
+  };
+  auto lowest = [](int k) -> Bits {  // k bits
+    return k <= 0 ? 0 : (k >= kMine ? (Bits)(~(Bits)0 >> (8 * sizeof(Bits) - kMine)) : ((Bits)1 << k) - 1);
+  };
+  auto bits = [](Bits x) { return (int)__popcll(x); };
   int ties = 0, nh = 0, nl = 0;  // of the segments before
   for (int s0 = 0; s0 < n; s0 += kSeg) {
     read(s0);
-    uint64_t stays = 0;  // bit k: the slot of key[k]
-    int at = 4 * again(tid), all;
-    if (!ranked) {
-#pragma unroll
-      for (int k = 0; k < 4 * T; ++k) {
-        stays |= (uint64_t)((s0 + (k >> 2) * kTurn + at + (k & 3) < n) & (key[k] >= prefix)) << k;
-        if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        int sum = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          sum += __popcll(__ballot((s0 + t * kTurn + at + j < n) & (key[4 * t + j] == prefix)));
-        if (lane == 0) cnt[0][t * kSelWaves + wave] = sum;
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      __syncthreads();
-      const int v = tid < kCnt ? cnt[0][tid] : 0, b = block_before(v, part, all);
-      if (tid < kCnt) cnt[0][tid] = ties + b;
-      ties += all;
-      __syncthreads();
-      at = 4 * again(tid);
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        bool tie[4];
-        int rank = cnt[0][t * kSelWaves + wave];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          tie[j] = (s0 + t * kTurn + at + j < n) & (key[4 * t + j] == prefix);
-          rank += __popcll(__ballot(tie[j]) & below);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool st = (s0 + t * kTurn + at + j < n) &
-                          ((key[4 * t + j] > prefix) | (tie[j] & (rank < need)));
-          rank += tie[j];
-          stays |= (uint64_t)st << (4 * t + j);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      __syncthreads();
-    }
-    // a hole: a slot below `keep` that goes; a move: one from `keep` on that stays
-    at = 4 * again(tid);
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      int sh = 0, sm = 0;
+      uint32_t over = 0, same = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const bool low = s0 + t * kTurn + at + j < keep, st = (stays >> (4 * t + j)) & 1u;
-        const uint64_t m = __ballot(low != st), ml = __ballot(low);
-        sh += __popcll(m & ml);
-        sm += __popcll(m & ~ml);
+        over |= key[4 * t + j] > lim ? 1u << j : 0u;
+        same |= key[4 * t + j] == prefix ? 1u << j : 0u;
       }
-      if (lane == 0) {
-        cnt[0][t * kSelWaves + wave] = sh;
-        cnt[1][t * kSelWaves + wave] = sm;
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int v = tid < kCnt ? cnt[j][tid] : 0, b = block_before(v, part, all);
-      if (tid < kCnt) cnt[j][tid] = (j ? nl : nh) + b;
-      (j ? nl : nh) += all;
-    }
-    __syncthreads();
-    at = 4 * again(tid);
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      const int first = s0 + t * kTurn + wave * 256;  // of this wave's turn
-      if (first >= n) break;
-      const uint32_t mine = (uint32_t)(stays >> (4 * t)) & 15u;
-      auto put = [&](int32_t *to, int rank, bool hole) {
-        bool in[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool low = s0 + t * kTurn + at + j < keep, st = (mine >> j) & 1u;
-          in[j] = (low == hole) & (st != hole);
-          rank += __popcll(__ballot(in[j]) & below);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (in[j]) to[rank] = s0 + t * kTurn + at + j;
-          rank += in[j];
-        }
-      };
-      if (first < keep) put(holes, cnt[0][t * kSelWaves + wave], true);
-      if (first + 256 > keep) put(late, cnt[1][t * kSelWaves + wave], false);
-      if (first < keep && (wo != w || po != p)) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = s0 + t * kTurn + at + j;
-          if (i < keep && (mine >> j) & 1u) {
-            if (wo != w) wo[i] = w[i];
-            if (po != p) po[i] = p[i];
-          }
-        }
+      over = or8(over << (4 * (lane & 7)));
+      if (ranked) same = or8(same << (4 * (lane & 7)));
+      if ((lane & 7) == 0) {
+        sh.map[0][t * (kTurn / 32) + (tid >> 3)] = over;
+        if (ranked) sh.map[1][t * (kTurn / 32) + (tid >> 3)] = same;
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
+    const int at = s0 + kMine * tid;
+    const Bits in = lowest(n - at), low = lowest(keep - at);
+    Bits stays = take(sh.map[0]) & in;
+    int all, moves;
+    if (ranked) {
+      Bits same = take(sh.map[1]) & in;
+      const int some = bits(same), k = need - ties - block_before(some, part, all);
+      ties += all;
+      if (k < some) {  // the first k of them
+        Bits rest = same;
+        for (int i = 0; i < k; ++i) rest &= rest - 1;
+        same ^= rest;
+      }
+      stays |= same;
+    }
+    // a hole: a slot below `keep` that goes; a move: one from `keep` on that stays
+    Bits hole = in & low & ~stays, move = stays & ~low;
+    int rh = block_before(bits(hole), part, all), rm = block_before(bits(move), part, moves) + all;
+    for (; hole; hole &= hole - 1) sh.slot[rh++] = (uint16_t)(kMine * tid + __builtin_ctzll(hole));
+    for (; move; move &= move - 1) sh.slot[rm++] = (uint16_t)(kMine * tid + __builtin_ctzll(move));
+    __syncthreads();
+    for (int i = tid; i < all; i += kSelThreads) holes[nh + i] = s0 + sh.slot[i];
+    for (int i = tid; i < moves; i += kSelThreads) late[nl + i] = s0 + sh.slot[all + i];
+    nh += all;
+    nl += moves;
   }
+  // what stays below `keep`; the holes among them are written by the moves
+  if (wo != w || po != p)
+    for (int i = tid; i < keep; i += kSelThreads) {
+      if (wo != w) wo[i] = w[i];
+      if (po != p) po[i] = p[i];
+    }
   if (tid == 0) *count = nl;
 }
 
