@@ -565,7 +565,7 @@ int gguf_hip_kv4_append(const float *qkv, int64_t ldqkv, int64_t n_rows, const i
                         int64_t slots, void *stream) {
   int rc = check_kv4_rows(n_seq, n_heads, n_kv_heads, head_dim, slots, ldqkv, rope_rows);
   if (rc) return rc;
-  if (n_rows < 0 || n_rows > ((int64_t)1 << 31) / n_kv_heads)
+  if (n_rows < 0 || n_rows > (int64_t)1 << 25)
     return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] kv4_append: %lld rows out of range",
                 (long long)n_rows);
   if (!starts && n_rows % n_seq)
@@ -674,8 +674,7 @@ int gguf_hip_kv4_evict(void *kv, const float *weights, const int32_t *positions,
     return fail(GGUF_HIP_ERR_NULL, "[gguf-hip] null pointer");
   if (!aligned(kv, 16) || !aligned(weights, 16) || !aligned(positions, 16) ||
       !aligned(lengths, 8) || !aligned(pos, 8) || !aligned(weights_out, 4) ||
-      !aligned(positions_out, 4) ||
-      !aligned(lengths_out, 8) || !aligned(work, 16))
+      !aligned(positions_out, 4) || !aligned(lengths_out, 8) || !aligned(work, 16))
     return fail(GGUF_HIP_ERR_ALIGN, "[gguf-hip] kv4 buffers misaligned");
   if (work_bytes < need)
     return fail(GGUF_HIP_ERR_BYTES, "[gguf-hip] kv4_evict: workspace of %lld bytes, needs %lld",

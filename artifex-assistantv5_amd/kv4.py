@@ -51,7 +51,7 @@ def _shape(kv: torch.Tensor, layers: bool = False):
     else:
         raise ValueError(f"kv4: cache of shape {tuple(kv.shape)}, need [{'layers, ' if layers else ''}"
                          "n_seq, n_kv_heads, slots / 32, 36 * head_dim]")
-    if s[3] % 36:
+    if 0 in s or s[3] % 36:
         raise ValueError(f"kv4: cache tiles of {s[3]} bytes are not 36 * head_dim")
     return n_layers, s[0], s[1], s[3] // 36, s[2] * TILE
 

@@ -58,7 +58,7 @@ int64_t gguf_hip_kv4_bytes(int n_seq, int n_kv_heads, int head_dim, int64_t slot
  * to slot lengths[s] + i with position pos[s] + i.  Rows past starts[n_seq], and rows
  * whose slot or position lies outside the cache or the tables, are not stored.  Neither
  * lengths nor pos is changed.  positions / weights (may be NULL): the stored slots get
- * their position and weight 0.  One launch; n_rows == 0 is a no-op. */
+ * their position and weight 0.  One launch; n_rows == 0 is a no-op, more than 2^25 are refused. */
 int gguf_hip_kv4_append(const float *qkv, int64_t ldqkv, int64_t n_rows, const int64_t *starts,
                         const int64_t *lengths, const int64_t *pos, const float *cos_table,
                         const float *sin_table, int64_t rope_rows, void *kv, int32_t *positions,
@@ -76,10 +76,11 @@ int gguf_hip_kv4_append(const float *qkv, int64_t ldqkv, int64_t n_rows, const i
  * written or added; other slots are left as they are.
  * A sequence with lengths[s] < 0, lengths[s] + rows > slots, pos[s] < 0 or
  * pos[s] + rows > rope_rows takes no part: nothing of it is written.  lengths and pos are
- * not changed.  work: gguf_hip_kv4_attention_workspace bytes, 16-byte aligned, no
- * initial value; calls that share it must not overlap.  Results do not depend on
- * timing.  f32-grade: codes enter the f16 matrix cores exactly, queries and
- * probabilities as two f16 parts each. */
+ * not changed.  out must not overlap qkv.  work: gguf_hip_kv4_attention_workspace bytes,
+ * 16-byte aligned, no initial value; calls that share it must not overlap.  Results do
+ * not depend on timing.  f32-grade: codes enter the f16 matrix cores exactly, queries and
+ * probabilities times V's scales as two f16 parts each, 22 bits of each product down to
+ * 2^-13 of a row's largest, below that 2^-35 of it. */
 int gguf_hip_kv4_attention(const float *qkv, int64_t ldqkv, int rows, const int64_t *lengths,
                            const int64_t *pos, const float *cos_table, const float *sin_table,
                            int64_t rope_rows, void *kv, int store, int32_t *positions,
@@ -108,8 +109,9 @@ int gguf_hip_kv4_load(const void *kv, const int64_t *lengths, float *k_out, floa
  * keep their bytes.  weights / positions [n_layers][n_seq][n_kv_heads][slots] of the
  * remaining slots go to weights_out / positions_out (the same arrays: in place), the
  * new lengths to lengths_out (may be lengths).  Sequences that are not cut keep their
- * caches, weights, positions and lengths.  Two launches.  work:
- * gguf_hip_kv4_evict_workspace bytes, 16-byte aligned, no initial value. */
+ * caches, weights, positions and lengths.  weights and positions are 16-byte aligned.
+ * Two launches.  work: gguf_hip_kv4_evict_workspace bytes, 16-byte aligned, no initial
+ * value; calls that share it must not overlap. */
 int gguf_hip_kv4_evict(void *kv, const float *weights, const int32_t *positions,
                        const int64_t *lengths, const int64_t *pos, int64_t keep, int64_t trigger,
                        int64_t recent, int64_t sinks, float *weights_out, int32_t *positions_out,
