@@ -4,6 +4,8 @@
 // the group; row v sees slots 0 .. lengths[s] + i.  The slots are split over workgroups;
 // each writes, per query row, a record of its partial softmax, and kv4_merge_kernel joins
 // them in split order (so the result does not depend on timing).
+#include <type_traits>
+
 #include "kv4.hpp"
 
 namespace gguf {
@@ -848,30 +850,39 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
       }
       l[u] += sum;
     }
+    auto products = [&](auto some_hidden) {
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const uint32_t w0 = d.v[0][k], h0 = w0 >> 8, w1 = d.v[1][k], h1 = w1 >> 8;
-      const half8_t va = v_frag<1>(w0, h0, w1, h1, magic);
-      const half8_t vb = v_frag<16>(w0, h0, w1, h1, magic);
+      for (int k = 0; k < NB; ++k) {
+        const uint32_t w0 = d.v[0][k], h0 = w0 >> 8, w1 = d.v[1][k], h1 = w1 >> 8;
+        const half8_t va = v_frag<1>(w0, h0, w1, h1, magic);
+        const half8_t vb = v_frag<16>(w0, h0, w1, h1, magic);
 #pragma unroll
-      for (int u = 0; u < NS; ++u) {
-        half2_t hp[4], lp[4];
+        for (int u = 0; u < NS; ++u) {
+          half2_t hp[4], lp[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {  // V's pairs: slots (0, 2), (1, 3) of each half
-          const int i = (n & 1) + (n >> 1) * 4, t = n >> 1;
-          float wa = mul_f16(p[u][i], at(vs[t][k], i & 3));
-          float wb = mul_f16(p[u][i + 2], at(vs[t][k], (i & 3) + 2));
-          asm("" : "+v"(wa), "+v"(wb));  // else each is made again as it is rounded
-          split_f16(wa, wb, minus1, hp[n], lp[n]);
+          for (int n = 0; n < 4; ++n) {  // V's pairs: slots (0, 2), (1, 3) of each half
+            const int i = (n & 1) + (n >> 1) * 4, t = n >> 1;
+            float wa = mul_f16(p[u][i], at(vs[t][k], i & 3));
+            float wb = mul_f16(p[u][i + 2], at(vs[t][k], (i & 3) + 2));
+            // a slot that this row does not see may hold any scale, infinite too
+            if (some_hidden.value && slot0 + 16 * t + (i & 3) >= vis[u]) wa = 0.f;
+            if (some_hidden.value && slot0 + 16 * t + (i & 3) + 2 >= vis[u]) wb = 0.f;
+            asm("" : "+v"(wa), "+v"(wb));  // else each is made again as it is rounded
+            split_f16(wa, wb, minus1, hp[n], lp[n]);
+          }
+          const half8_t wh = __builtin_bit_cast(half8_t, hp), wl = __builtin_bit_cast(half8_t, lp);
+          acc[u][2 * k] = mfma(wh, va, acc[u][2 * k]);
+          acc[u][2 * k + 1] = mfma(wh, vb, acc[u][2 * k + 1]);
+          acc[u][2 * k] = mfma(wl, va, acc[u][2 * k]);
+          acc[u][2 * k + 1] = mfma(wl, vb, acc[u][2 * k + 1]);
         }
-        const half8_t wh = __builtin_bit_cast(half8_t, hp), wl = __builtin_bit_cast(half8_t, lp);
-        acc[u][2 * k] = mfma(wh, va, acc[u][2 * k]);
-        acc[u][2 * k + 1] = mfma(wh, vb, acc[u][2 * k + 1]);
-        acc[u][2 * k] = mfma(wl, va, acc[u][2 * k]);
-        acc[u][2 * k + 1] = mfma(wl, vb, acc[u][2 * k + 1]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    };
+    if (masked)
+      products(std::true_type{});
+    else
+      products(std::false_type{});
     load_scales(next);
     d.load_v(next, r, g);
   }

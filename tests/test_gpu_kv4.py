@@ -296,6 +296,34 @@ def test_attention_uneven_blocks(kv4, heads, rows, hd):
     assert (np.abs(got - ref) <= bound).all(), (np.abs(got - ref) / bound).max()
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(2, 2, 128), (8, 2, 64), (8, 2, 128), (2, 2, 256),
+                                         (8, 1, 256)])
+@pytest.mark.parametrize("at", ["k", "v"])
+@pytest.mark.parametrize("what", [float("inf"), float("nan"), 2.0 ** 18])
+def test_attention_of_rows_before_a_bad_one(kv4, heads, kv, hd, at, what):
+    """What a later row of the call holds, infinite, NaN or huge, is nothing to the rows before."""
+    rng = np.random.default_rng(hd + heads)
+    slots, n, rows, bad = 192, 157, 8 if hd == 64 else 4, 2
+    cos, sin = _tables(200, hd)
+    cache = _filled(rng, 1, kv, hd, slots, [n])
+    qkv = rng.standard_normal((rows, (heads + 2 * kv) * hd)).astype(np.float32)
+    dev, clean = _cuda(cache), _cuda(cache)
+    outs = []
+    for c, put in ((clean, False), (dev, True)):
+        x = qkv.copy()
+        if put:
+            first = (heads + (kv if at == "v" else 0)) * hd
+            x[bad:, first:first + kv * hd:7] = what
+        out = torch.empty(rows, heads * hd, device="cuda")
+        kv4.attention(_cuda(x), _i64([n]), _i64([n]), _cuda(cos), _cuda(sin), c, out, heads,
+                      kv4.attention_workspace(c, heads, rows=rows))
+        outs.append(out.cpu().numpy())
+    ref, bound, _, _ = _reference(clean.cpu().numpy(), qkv, [n], [n], cos, sin, heads, kv, hd, rows)
+    for out in outs:
+        got = out.reshape(ref.shape)[:bad]
+        assert (np.abs(got - ref[:bad]) <= bound[:bad]).all()
+
+
 def test_attention_far_lists(kv4):
     """Lists and slots beyond 2^32 bytes: a cache of 5 GB whose last sequence is used."""
     heads, kv, hd, slots, seqs = 4, 2, 128, 131072, 132
