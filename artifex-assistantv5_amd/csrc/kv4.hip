@@ -143,26 +143,32 @@ __device__ __forceinline__ int32_t *evict_holes(void *work, int64_t lists, int64
   return (int32_t *)work + (lists + 3) / 4 * 4 + list * 2 * half;
 }
 
-// The sum of v over the threads below this one, and over all of them.
+// v plus those of the lanes below it: in rows of 16 by DPP shifts, then the rows' ends.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int row_sums(int v) {
+  v = dpp_add<0x111, 0xF>(v);
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  return dpp_add<0x118, 0xF>(v);
+}
+__device__ __forceinline__ int wave_sums(int v) {
+  v = dpp_add<0x142, 0xA>(row_sums(v));  // lane 15 to row 1, 47 to row 3
+  return dpp_add<0x143, 0xC>(v);         // lane 31 to rows 2 and 3
+}
+// The sum of v over the threads below this one, and over all of them.  Calls that follow each
+// other without a barrier between take different `part`s.
 __device__ __forceinline__ int block_before(int v, int *part, int &all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int run = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(run, o);
-    if (lane >= o) run += x;
-  }
-  __syncthreads();  // the last use of `part` is over
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int run = wave_sums(v);
   if (lane == 63) part[wave] = run;
   __syncthreads();
-  int x = part[lane & (kSelWaves - 1)];
-#pragma unroll
-  for (int o = 1; o < kSelWaves; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if ((lane & (kSelWaves - 1)) >= o) x += y;
-  }
-  all = __shfl(x, kSelWaves - 1);
-  return run - v + (wave ? __shfl(x, wave - 1) : 0);
+  static_assert(kSelWaves == 16);
+  const int x = row_sums(part[lane & 15]);
+  all = __builtin_amdgcn_readlane(x, 15);
+  return run - v + (wave ? __builtin_amdgcn_readlane(x, wave - 1) : 0);
 }
 
 // The same number, not known to be: what is computed from it is computed where it is used, and
@@ -189,21 +195,22 @@ __device__ __forceinline__ uint32_t or8(uint32_t x) {
 // - Ranks: the turns' four bits per thread (stays, equals) become a bitmap in LDS, of which each
 //   thread takes its segment's next 4 T slots: counts are bit counts, one scan of the workgroup
 //   gives all ranks.  The lists of slots are put together in LDS and written in order.
-// Bound: one CU's loads and vector instructions.  48 lists of up to 61000 slots: 11 us to read and
-// make the keys, 11 for the three digits, 13 for ranks and lists (35 where the ranks were counted
-// turn by turn with ballots).  An attend-and-evict step of 48 lists with its moves: 75.5 -> 53.1.
+// Bound: one CU's loads and vector instructions, and for short lists the chain of barriers.  48
+// lists of up to 61000 slots, with their moves: 75.5 us with ranks counted turn by turn by ballots,
+// 53.4 with bitmaps, 51.6 with scans by DPP instead of shuffles; 32 lists of 513 slots 15.0, 13.4,
+// 11.2.
 template <int T>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, Kv4Evict e, int half) {
   constexpr int kBins = 2048, kTurn = 4 * kSelThreads, kSeg = T * kTurn, kMine = 4 * T;
   using Bits = std::conditional_t<T == 16, uint64_t, uint32_t>;  // of a thread's kMine slots
   __shared__ __align__(16) union {
-    int hist[4][kBins];
+    int hist[6][kBins];  // the first digit in four copies, the others
     struct {
       uint32_t map[2][kSeg / 32];  // stays, equals: a bit per slot of the segment
       uint16_t slot[kSeg];         // its holes, then its moves
     };
   } sh;
-  __shared__ int part[kSelWaves], found[3];
+  __shared__ int part[2][kSelWaves], found[3];
   auto &hist = sh.hist;
   const int64_t list = blockIdx.x, lists = gridDim.x;
   const int64_t s = list / c.nkv % c.n_seq;
@@ -248,20 +255,18 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
       if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // 8 loads of a wave in flight at a time
     }
   };
+#pragma unroll
+  for (int i = 0; i < 6 * kBins / kSelThreads; ++i) ((int *)hist)[i * kSelThreads + tid] = 0;
+  __syncthreads();
   uint32_t prefix = 0;
   int need = keep, alike = 0;  // of `alike` keys that share the prefix, `need` stay
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < kBins; i += kSelThreads) {
-      hist[0][i] = 0;
-      if (pass == 0) hist[1][i] = hist[2][i] = hist[3][i] = 0;
-    }
-    __syncthreads();
     for (int s0 = 0; s0 < n; s0 += kSeg) {
       read(s0);
       const int at = 4 * again(threadIdx.x);
-      int *h = hist[pass == 0 ? wave & 3 : 0];
+      int *h = hist[pass == 0 ? wave & 3 : pass + 3];
 #pragma unroll
       for (int t = 0; t < T; ++t) {
         if (s0 + t * kTurn >= n) break;
@@ -278,13 +283,14 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
     __syncthreads();
     // bins from the top, two per thread: the first whose running count reaches `need`
     const int b0 = kBins - 1 - 2 * tid;
-    int h0 = hist[0][b0], h1 = hist[0][b0 - 1];
+    const int *h = hist[pass == 0 ? 0 : pass + 3];
+    int h0 = h[b0], h1 = h[b0 - 1];
     if (pass == 0) {
       h0 += hist[1][b0] + hist[2][b0] + hist[3][b0];
       h1 += hist[1][b0 - 1] + hist[2][b0 - 1] + hist[3][b0 - 1];
     }
     int all;
-    const int before = block_before(h0 + h1, part, all);
+    const int before = block_before(h0 + h1, part[pass & 1], all);
     if (before < need && before + h0 >= need) {
       found[0] = b0;
       found[1] = need - before;
@@ -337,7 +343,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
     int all, moves;
     if (ranked) {
       Bits same = take(sh.map[1]) & in;
-      const int some = bits(same), k = need - ties - block_before(some, part, all);
+      const int some = bits(same), k = need - ties - block_before(some, part[1], all);
       ties += all;
       if (k < some) {  // the first k of them
         Bits rest = same;
@@ -348,7 +354,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
     }
     // a hole: a slot below `keep` that goes; a move: one from `keep` on that stays
     Bits hole = in & low & ~stays, move = stays & ~low;
-    int rh = block_before(bits(hole), part, all), rm = block_before(bits(move), part, moves) + all;
+    int rh = block_before(bits(hole), part[0], all);
+    int rm = block_before(bits(move), part[1], moves) + all;
     for (; hole; hole &= hole - 1) sh.slot[rh++] = (uint16_t)(kMine * tid + __builtin_ctzll(hole));
     for (; move; move &= move - 1) sh.slot[rm++] = (uint16_t)(kMine * tid + __builtin_ctzll(move));
     __syncthreads();

@@ -1,7 +1,7 @@
 """The KV cache held in 4 bits: storing rows, attention over it, eviction (libgguf_hip).
 
-The reference keeps f32 caches here (attention.wgsl:60-234) and quantizes its cache in a
-separate pipeline (webgpu/src/engine, turboquant).  This cache holds Q4_0 blocks of 32
+The reference attends over f32 caches (attention.wgsl:60-234) and compresses its cache by
+other codes (webgpu/src/engine/turboquant-pipeline.ts).  This cache holds Q4_0 blocks of 32
 channels, the values of this package's own Q4_0 quantizer: 4.5 bits a value, so a token
 costs 9/64 of the bytes that it costs in f32.
 
