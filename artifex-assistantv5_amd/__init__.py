@@ -17,6 +17,7 @@ reference's WebGPU engine (``webgpu/src/engine/forward-pass.ts``):
 * ``parse_gguf``            — GGUF header / KV / tensor table (gguf.ts:241-299)
 * ``load_gguf_model``       — place a GGUF file's tensors in HBM (gguf-loader.ts:166-460)
 * ``load_decoder``          — a llama-architecture GGUF file as a ``QuantDecoder``
+* ``kv4`` (module)          — a KV cache held in 4 bits: attention over it, eviction
 
 Importing this package does not touch the GPU; the native library is loaded
 on first use and a missing or unbuilt library raises immediately.

@@ -197,7 +197,7 @@ __device__ __forceinline__ uint32_t or8(uint32_t x) {
 //   gives all ranks.  The lists of slots are put together in LDS and written in order.
 // Bound: one CU's loads and vector instructions, and for short lists the chain of barriers.  48
 // lists of up to 61000 slots, with their moves: 75.5 us with ranks counted turn by turn by ballots,
-// 53.4 with bitmaps, 51.6 with scans by DPP instead of shuffles; 32 lists of 513 slots 15.0, 13.4,
+// 53.4 with bitmaps, 51.6 with scans by DPP instead of shuffles; 32 lists of 2049 slots 15.0, 13.4,
 // 11.2.
 template <int T>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, Kv4Evict e, int half) {

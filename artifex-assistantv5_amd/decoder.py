@@ -344,6 +344,9 @@ class QuantDecoder:
         if pos0 == 0:
             self.kv_lengths.zero_()
         held, done, h = int(self.kv_lengths.item()), 0, None
+        if pos0 < held or (self.kv_keep is None and pos0 != held):
+            raise ValueError(f"position {pos0} does not follow the {held} slots that the 4-bit "
+                             "cache holds")
         while done < tokens.numel():
             m = min(tokens.numel() - done, self.kv_slots - held)
             if m == 0:

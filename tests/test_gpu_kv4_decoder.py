@@ -150,3 +150,22 @@ def test_refusals(dec):
         m.prefill(_tokens(cfg, 33, 1), 0)
     with pytest.raises(ValueError, match="slots"):
         m.generate(_tokens(cfg, 20, 1), 20)
+
+
+def test_a_prompt_follows_what_the_cache_holds(dec):
+    cfg, w = _model(dec)
+    tokens = _tokens(cfg, 12, 1)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4)
+    whole = m.prefill(tokens, 0)
+    m.prefill(tokens[:5], 0)
+    for pos0 in (3, 7):
+        with pytest.raises(ValueError, match="follow"):
+            m.prefill(tokens[5:], pos0)
+    # from position 5 on, over the first five rows as they are cached
+    rest = m.prefill(tokens[5:], 5)
+    assert int(m.kv_lengths.item()) == 12 and torch.isfinite(rest).all()
+    m = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=64, kv_keep=32, kv_recent=8)
+    m.prefill(tokens[:5], 0)
+    with pytest.raises(ValueError, match="follow"):
+        m.prefill(tokens[5:], 4)
+    assert whole.shape == rest.shape
