@@ -74,7 +74,8 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
 }
 
 // ---------------------------------------------------------------------------
-// Reading rows back: a workgroup per tile of 32 slots.
+// Reading rows back: a workgroup per tile of 32 slots.  Bound: the f32 rows written; 40 lists of
+// up to 2000 rows of 128 channels 12-16 us.
 // ---------------------------------------------------------------------------
 template <int HD>
 __global__ __launch_bounds__(kThreads) void kv4_load_kernel(const uint8_t *__restrict__ kv,
@@ -376,6 +377,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
 // A wave takes 16 moves at a time, slot late[i] to slot holes[i]: all their loads are issued
 // before the first store (a slot from `keep` on is never written, so the order of the waves
 // does not matter).  V's bytes are four apart, a lane takes one; K goes in 16 bytes a lane.
+// Bound: the lines that a slot's bytes lie in, 640 bytes read at 128 channels for its 144.  256
+// lists of 15999 slots cut to 2000, about 1750 moves each: 72 us, 400 MB, 5.5 TB/s.
 template <int HD>
 __global__ __launch_bounds__(kThreads) void evict_move_kernel(Kv4Cache c, Kv4Evict e, int half) {
   using L = Kv4<HD>;

@@ -306,7 +306,10 @@ struct TileRegs {
 //   from them and p's sum stays a float.
 // - K's registers take the next tile as soon as its scores are made, V's after its products:
 //   one tile in flight per wave, four waves per SIMD.
-// Bound: HBM, 9/8 head_dim bytes per slot and list.
+// Bound: HBM (9/8 head_dim bytes per slot and list) and, close behind, vector instructions, most
+// of them on the codes.  130000 slots of 8 lists, 128 channels, 150 MB: 33-36 us, 4.2-4.5 TB/s with
+// the vector unit busy 72 % of the time; short lists are bound by their start (6000 slots: 7.8 us,
+// of which 4.5 before the first tile is used).
 template <int HD, int W, int WPS>
 __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, Kv4Attn a,
                                                                float *__restrict__ rec,
@@ -580,8 +583,9 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 // slots; where m is raised for it, by each slot's own.  m is that of all blocks: p * scale of a
 // block whose scales are under 2^-13 of the others' falls below 2^-3, where two f16 parts hold
 // fewer bits (2^-25 absolute: 2^-35 of the row's largest).
-// Bound: vector instructions, about 150 for a tile's codes and 190 for each group of rows (128
-// channels).
+// Bound: vector instructions (70 % busy), about 150 for a tile's codes and 230 for each group of
+// rows (128 channels).  32 rows of 32 / 8 heads over 20000 slots: 50 us, 10.5 GFLOP of products in
+// four parts; the kernel for few rows took about 95.
 template <int HD, int NS>
 __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
                                                           float *__restrict__ rec,

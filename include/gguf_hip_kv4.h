@@ -94,7 +94,8 @@ int64_t gguf_hip_kv4_attention_workspace(int rows, int weights_mode, int n_seq, 
 
 /* Slots 0 .. lengths[s] - 1 as f32 rows: k_out / v_out [n_layers][n_seq][n_kv_heads]
  * [out_slots][head_dim] of caches [n_layers] (each gguf_hip_kv4_bytes long).  Slots from
- * out_slots on are not read, rows from lengths[s] on not written.  The layout is that of
+ * out_slots on are not read, rows from lengths[s] on not written, and nothing of a
+ * sequence with lengths[s] > slots.  The layout is that of
  * the f32 caches of gguf_hip_attention_prefill. */
 int gguf_hip_kv4_load(const void *kv, const int64_t *lengths, float *k_out, float *v_out,
                       int64_t out_slots, int n_layers, int n_seq, int n_kv_heads, int head_dim,

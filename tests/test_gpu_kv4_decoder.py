@@ -169,3 +169,21 @@ def test_a_prompt_follows_what_the_cache_holds(dec):
     with pytest.raises(ValueError, match="follow"):
         m.prefill(tokens[5:], 4)
     assert whole.shape == rest.shape
+
+
+def test_a_model_file_with_a_4_bit_cache(dec, tmp_path):
+    """load_decoder passes the cache's form on: the tokens are those of the same decoder built
+    directly, over an eviction, with RoPE frequency factors."""
+    import gguf_models as gm
+
+    gmodel = importlib.import_module("artifex-assistantv5_amd.gguf_model")
+    tensors = gm.make_model(seed=6, rope_freqs=True)
+    p = str(tmp_path / "m.gguf")
+    gm.write_model(p, tensors)
+    cache = dict(kv_bits=4, kv_slots=64, kv_keep=48, kv_recent=16)
+    model, _ = gmodel.load_decoder(p, "cuda", max_seq=128, **cache)
+    direct = dec.QuantDecoder(model.cfg, gm.direct_weights(tensors, gm.TINY), **cache)
+    prompt = torch.from_numpy(np.random.default_rng(7).integers(0, model.cfg.vocab, 56)).cuda()
+    a, b = model.generate(prompt, 30), direct.generate(prompt, 30, graph=False)
+    assert torch.equal(a["tokens"], b["tokens"])
+    assert int(model.kv_lengths.item()) == int(direct.kv_lengths.item()) < 64
