@@ -36,7 +36,7 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
     row[i].load(x + (int64_t)((u & 1) * c.nkv + (u >> 1)) * HD, q);
   }
   uint32_t s;
-  int64_t i, more = 0;  // `whole`: the sequence's rows behind this one
+  int64_t i, last;  // the row of s, and the one that has to fit for it to be stored
   if (starts) {
     if (r < starts[0] || r >= starts[c.n_seq]) return;
     uint32_t lo = 0, hi = c.n_seq;  // starts[lo] <= r < starts[hi]
@@ -48,15 +48,15 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
         hi = mid;
     }
     s = lo;
-    i = r - starts[lo];
+    last = i = r - starts[lo];
   } else {
     const uint32_t per = n_rows / (uint32_t)c.n_seq;
     s = r / per;
     i = r - s * per;
-    if (whole) more = per - 1 - i;
+    last = whole ? per - 1 : i;
   }
-  const int64_t slot = c.lengths[s] + i, p = c.pos[s] + i, before = whole ? i : 0;
-  if (slot < before || slot >= c.slots - more || p < before || p >= c.rope_rows - more) return;
+  const int64_t n = c.lengths[s], p0 = c.pos[s], slot = n + i, p = p0 + i;
+  if (n < 0 || n >= c.slots - last || p0 < 0 || p0 >= c.rope_rows - last) return;
   row[0].load_turn(c.cs + p * (HD / 2), c.sn + p * (HD / 2), q);
 #pragma unroll
   for (int k = 0; k < N; ++k) {

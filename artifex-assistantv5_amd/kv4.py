@@ -112,7 +112,8 @@ def append(qkv: torch.Tensor, lengths: torch.Tensor, pos: torch.Tensor, cos: tor
     Sequence ``s`` owns rows ``starts[s] .. starts[s + 1] - 1`` of ``qkv`` (device int64
     ``[n_seq + 1]``; without it every sequence has the same number of rows, in order).  Its
     row i goes to slot ``lengths[s] + i`` with position ``pos[s] + i``; rows outside every
-    sequence, the cache or the tables are not stored.  ``lengths`` and ``pos`` are the
+    sequence, the cache or the tables are not stored, nor those of a sequence of negative
+    length or position.  ``lengths`` and ``pos`` are the
     caller's to advance.  The stored slots' ``positions`` are set and their ``weights``
     cleared.  One launch."""
     n_seq, n_kv, hd, slots, ld, lp, pp, cp, sp, posp, wp = _common(

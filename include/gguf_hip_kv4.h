@@ -55,10 +55,11 @@ int64_t gguf_hip_kv4_bytes(int n_seq, int n_kv_heads, int head_dim, int64_t slot
  * (rope.wgsl:1-10; every product and sum rounded to f32) and v, quantized.
  * Sequence s owns rows starts[s] .. starts[s + 1] - 1 of qkv (device int64
  * [n_seq + 1], ascending; NULL: n_rows / n_seq rows each, in order).  Its row i goes
- * to slot lengths[s] + i with position pos[s] + i.  Rows past starts[n_seq], and rows
- * whose slot or position lies outside the cache or the tables, are not stored.  Neither
- * lengths nor pos is changed.  positions / weights (may be NULL): the stored slots get
- * their position and weight 0.  One launch; n_rows == 0 is a no-op, more than 2^25 are refused. */
+ * to slot lengths[s] + i with position pos[s] + i.  Rows past starts[n_seq], rows whose
+ * slot or position lies past the cache or the tables, and rows of a sequence with
+ * lengths[s] < 0 or pos[s] < 0, are not stored.  Neither lengths nor pos is changed.
+ * positions / weights (may be NULL): the stored slots get their position and weight 0.
+ * One launch; n_rows == 0 is a no-op, more than 2^25 are refused. */
 int gguf_hip_kv4_append(const float *qkv, int64_t ldqkv, int64_t n_rows, const int64_t *starts,
                         const int64_t *lengths, const int64_t *pos, const float *cos_table,
                         const float *sin_table, int64_t rope_rows, void *kv, int32_t *positions,

@@ -63,7 +63,7 @@ def _expect_append(cache, positions, weights, qkv, lengths, pos, cos, sin, heads
         for r in range(max(0, starts[s]), min(starts[s + 1], x.shape[0])):
             i = r - starts[s]
             slot, p = lengths[s] + i, pos[s] + i
-            if not (0 <= slot < slots and 0 <= p < cos.shape[0]):
+            if lengths[s] < 0 or pos[s] < 0 or slot >= slots or p >= cos.shape[0]:
                 continue
             for h in range(kv):
                 model.put(cache, s, h, slot, model.rope(x[r, heads + h], cos[p], sin[p]),
