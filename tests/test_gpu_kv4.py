@@ -570,7 +570,7 @@ def test_refusals_on_device_tensors(kv4):
     kv4.attention(**good)
     for over in (dict(qkv=qkv[:, :-1]), dict(qkv=qkv.half()), dict(qkv=qkv[:1]), dict(out=out[:1]),
                  dict(lengths=n.int()), dict(pos=_i64([0])), dict(cos=cos[:4]), dict(n_heads=5),
-                 dict(kv=kv[:, :1]), dict(kv=kv.float()), dict(work=work[:-1]), dict(n_heads=20),
+                 dict(kv=kv[:, :1]), dict(kv=kv.float()), dict(kv=kv[:0]), dict(work=work[:-1]), dict(n_heads=20),
                  dict(weights=torch.zeros(2, 2, 63, device="cuda")), dict(sin=sin.cpu()),
                  dict(positions=torch.zeros(2, 2, 64, device="cuda")), dict(out=out.t())):
         with pytest.raises(ValueError):
@@ -582,6 +582,9 @@ def test_refusals_on_device_tensors(kv4):
                  torch.zeros(2, 2, 11, 64, device="cuda"))
     w, p = torch.zeros(2, 2, 64, device="cuda"), torch.zeros(2, 2, 64, device="cuda").int()
     ew = kv4.evict_workspace(kv)
+    off = torch.zeros(2 * 2 * 64 + 1, device="cuda")[1:].view(2, 2, 64)    # 4 bytes off
+    with pytest.raises(ValueError):
+        kv4.evict(kv, off, p, n, n, keep=8, work=ew)
     for over in (dict(keep=0), dict(keep=65), dict(keep=8, recent=9), dict(keep=8, work=ew[:8])):
         with pytest.raises(ValueError):
             kv4.evict(kv, w, p, n, n, **{"work": ew, **over})
