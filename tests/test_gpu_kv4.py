@@ -392,6 +392,10 @@ def _evict_case(rng, layers, seqs, kv, hd, slots, lengths, ties):
     (1, 3, 1, 64, 96, [60, 70, 90], 50, 0, 0, 70, False),   # below the trigger
     (1, 1, 1, 64, 2080, [2079], 1000, 1000, 0, None, True), # nothing but the recent
     (2, 1, 3, 128, 4128, [4100], 1500, 200, 16, None, True),
+    (1, 2, 1, 64, 20480, [20000, 17001], 9000, 500, 16, None, True),
+    (1, 1, 2, 64, 20480, [20480], 20479, 0, 0, None, False),
+    (1, 1, 1, 64, 140000, [139990], 70001, 1000, 4, None, True),   # over three segments of 65536
+    (1, 2, 1, 64, 140000, [140000, 66000], 300, 100, 4, None, False),
     (1, 2, 1, 64, 32, [33, 32], 16, 3, 3, None, False),     # longer than its cache: not cut
 ])
 @pytest.mark.parametrize("inplace", [True, False])
