@@ -65,10 +65,15 @@ def _tensor(name: str, t: torch.Tensor, dtype, shape, device) -> int:
 
 def _row_matrix(name: str, t: torch.Tensor, width: int, device) -> int:
     """The row stride of f32 rows of at least ``width`` values (unit column stride)."""
-    if t.dtype != torch.float32 or t.device != device or t.dim() != 2 or t.shape[1] < width:
+    if t.dtype != torch.float32 or t.device != device or t.dim() != 2:
         raise ValueError(f"kv4: {name} must be float32 rows of at least {width} values on {device}")
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if t.stride(1) != 1 or ld < t.shape[1]:
+    n, columns = t.shape
+    if columns < width:
+        raise ValueError(f"kv4: {name} must be float32 rows of at least {width} values on {device}")
+    ld, step = t.stride()
+    if n <= 1:
+        ld = columns
+    if step != 1 or ld < columns:
         raise ValueError(f"kv4: {name} must be rows with unit column stride")
     return ld
 
@@ -94,7 +99,7 @@ def _common(qkv, lengths, pos, cos, sin, kv, n_heads, positions, weights):
 def _launch(fn, dev: torch.device, *args) -> None:
     """``fn`` on the current stream of ``dev``, which need not be the current device."""
     stream = _stream(dev)
-    if torch.cuda.current_device() == dev.index:
+    if torch._C._cuda_getDevice() == dev.index:  # current_device(), in less time
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
