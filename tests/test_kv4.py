@@ -159,3 +159,9 @@ def test_python_refuses_host_tensors(pkg):
         kv4.load(kv, torch.zeros(1, dtype=torch.int64), torch.zeros(1), torch.zeros(1))
     with pytest.raises(ValueError, match="slots"):
         kv4.empty(1, 2, 64, 33, device="cpu")
+
+
+def test_append_row_limit(lib, native):
+    """2^25 rows pass the check of their number (the next one, of the pointers, refuses)."""
+    assert _append(lib, rows=(1 << 25) + 2) == native.ERR_SHAPE
+    assert _append(lib, rows=1 << 25, qkv=None) == native.ERR_NULL
