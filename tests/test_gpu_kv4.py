@@ -592,3 +592,58 @@ def test_refusals_on_device_tensors(kv4):
     for over in (dict(keep=0), dict(keep=65), dict(keep=8, recent=9), dict(keep=8, work=ew[:8])):
         with pytest.raises(ValueError):
             kv4.evict(kv, w, p, n, n, **{"work": ew, **over})
+
+
+def test_graph_of_several_rows(kv4):
+    """Storing packed rows, attention of several rows with weights over several splits, and the
+    rows read back, in one graph: every replay equals the eager calls, two graphs share a
+    workspace."""
+    seqs, heads, kv, hd, slots, rows = 2, 8, 2, 128, 2048, 6
+    g = torch.Generator(device="cuda").manual_seed(11)
+    cos, sin = (_cuda(t) for t in _tables(2 * slots, hd))
+    cache = kv4.empty(seqs, kv, hd, slots)
+    weights = torch.zeros(seqs, kv, slots, device="cuda")
+    zero = _i64([0] * seqs)
+    prompt = torch.randn(3000, (heads + 2 * kv) * hd, device="cuda", generator=g)
+    starts, lengths = _i64([0, 1100, 3000]), _i64([1100, 1900])
+    qkv = torch.empty(seqs * rows, (heads + 2 * kv) * hd, device="cuda")
+    work = kv4.attention_workspace(cache, heads, rows=rows, weights=True)
+    outs = [torch.empty(seqs * rows, heads * hd, device="cuda") for _ in range(2)]
+    k, v = torch.zeros(2, seqs, kv, slots, hd, device="cuda")
+
+    def run(out):
+        kv4.append(prompt, zero, zero, cos, sin, cache, heads, starts=starts, weights=weights)
+        kv4.attention(qkv, lengths, lengths, cos, sin, cache, out, heads, work, weights=weights,
+                      accumulate=True)
+        kv4.load(cache, lengths + rows, k, v)
+
+    def state(out):
+        return [t.clone() for t in (out, cache, weights, k, v)]
+
+    graphs = []
+    for out in outs:
+        qkv.normal_(generator=g)
+        run(out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run(out)
+        graphs.append(graph)
+    for step in range(6):
+        qkv.normal_(generator=g)
+        run(outs[0])
+        want = state(outs[0])
+        for t in (outs[0], outs[1], k, v):
+            t.fill_(7.0)
+        weights.zero_()
+        graphs[step % 2].replay()
+        got = state(outs[step % 2])
+        torch.randn(1000, device="cuda").sum().item()
+        for a, b, name in zip(got, want, ("out", "cache", "weights", "k", "v")):
+            n = 1100 + rows
+            if name == "weights":
+                a, b = a[:, :, :n], b[:, :, :n]
+                assert (a[:, :, :1100] > 0).all()
+            if name in "kv":
+                a, b = a[:, :, :n], b[:, :, :n]
+            assert torch.equal(a, b), (step, name)
