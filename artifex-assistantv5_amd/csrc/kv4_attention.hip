@@ -536,7 +536,6 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
     d.load_v(next, r, g);
   }
 
-  __syncthreads();
   // the waves' sums: lane (r, g), register i holds row 4 g + i, channel 16 t + r
   float sum = sum_xor32(sum_xor16(l));
   if (g == 0) lm[wave][r] = make_float2(m, sum);
@@ -889,7 +888,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
     d.load_v(next, r, g);
   }
 
-  __syncthreads();
+  __syncthreads();  // the last use of the queries is over
   // the waves' sums: lane (r, g), register i holds row 4 g + i, channel 16 t + r
 #pragma unroll
   for (int u = 0; u < NS; ++u) {
