@@ -745,6 +745,9 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
     const bool masked = (tile + 1) * kKv4Tile > all_see;
     asm volatile("" : "+v"(ql));
     float y[NS][8];  // scores / f
+    // the wave that is at its matrix products goes first, the other fills the gaps (window of 32
+    // rows over 20000 slots, without weights: 53.3 us without, 51.2 so)
+    __builtin_amdgcn_s_setprio(1);
     float4_t sc[2][NS][2];
 #pragma unroll
     for (int k = 0; k <= NB; ++k) {
@@ -769,6 +772,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
                            k > 1 ? y[u][i] : 0.f);
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     load_k(next);
     if (scores) {
 #pragma unroll
@@ -880,10 +884,12 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
         __builtin_amdgcn_sched_barrier(0);
       }
     };
+    __builtin_amdgcn_s_setprio(1);
     if (masked)
       products(std::true_type{});
     else
       products(std::false_type{});
+    __builtin_amdgcn_s_setprio(0);
     load_scales(next);
     d.load_v(next, r, g);
   }
