@@ -35,9 +35,9 @@ __device__ __forceinline__ int kv4_filled(const Kv4Cache &c, int64_t s, int rows
 
 // How the tiles of a list are cut: `per` for each workgroup, `n` of them at most S.  Every
 // workgroup of the call gets about the same number, whatever the sequences' lengths: all lists'
-// tiles over `wgs` workgroups, in whole turns of a workgroup's W waves.
+// tiles over `wgs` workgroups, in whole turns of a workgroup's W waves, at least `least` tiles.
 struct Cut {
-  int S, wgs, W;
+  int S, wgs, W, least;
 };
 struct Splits {
   int per, n;
@@ -46,7 +46,7 @@ __device__ __forceinline__ int kv4_tiles(int filled, int rows) {
   return filled < 0 ? 0 : (filled + rows + kKv4Tile - 1) / kKv4Tile;
 }
 __device__ __forceinline__ Splits kv4_splits(int tiles, int fair, const Cut &k) {
-  const int per = (max(max(fair, 1), (tiles + k.S - 1) / k.S) + k.W - 1) / k.W * k.W;
+  const int per = (max(max(fair, k.least), (tiles + k.S - 1) / k.S) + k.W - 1) / k.W * k.W;
   return {per, (tiles + per - 1) / per};
 }
 // The fair share: a wave's lanes add the sequences.
@@ -1093,8 +1093,13 @@ Plan plan(int rows, int n_seq, int nh, int nkv, int hd, int slots) {
     p.cut.W = many ? 4 : 8, resident = many ? 768 : 512;
   }
   p.cut.wgs = (resident + p.nz - 1) / p.nz;
-  // a list is not cut below two turns of a workgroup's waves: one launch, and nothing to join
-  const int64_t tiles = slots / kKv4Tile, most = tiles <= 2 * p.cut.W ? 1 : (tiles + p.cut.W - 1) / p.cut.W;
+  // Turns at least: with many rows two, since the start and the end of a workgroup weigh more
+  // (8192 slots, 8 to 32 rows of 128 channels, us with one against two: 16.8 / 14.8, 23.6 / 20.2; 4
+  // x 9000 of 256 24.8 / 23.5; of 64, 20 rows 17.0 / 15.8), with few rows one (11.2 / 12.2).  A list
+  // of two turns is not cut: one launch, and nothing to join.
+  p.cut.least = (p.dense ? 2 : 1) * p.cut.W;
+  const int64_t tiles = slots / kKv4Tile;
+  const int64_t most = tiles <= 2 * p.cut.W ? 1 : (tiles + p.cut.least - 1) / p.cut.least;
   // sequences of different lengths: up to four times the workgroups that equal ones would take
   const int64_t want = (4 * p.cut.wgs + p.lists - 1) / p.lists;
   p.cut.S = (int)(want < most ? want : most);
