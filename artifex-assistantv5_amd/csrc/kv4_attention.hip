@@ -594,7 +594,6 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
   using L = Kv4<HD>;
   constexpr int W = 4, NB = L::NB, half = HD / 2, RS = record_floats<HD>();
   constexpr float kLift = 10.f, kMostW = 16384.f, kMostP = 0x1p100f;
-  constexpr bool kStores = HD != 64;  // of 64 channels no call of one new row has that many heads
   // Queries (per block, hi and lo part, a B operand) while tiles are read, then the waves' sums, 16
   // rows of HD per group: 64 KB together, so two workgroups fit a CU's LDS, 82 apart.
   __shared__ union {
@@ -686,7 +685,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
       q_[wave][k][0][lane] = hi;
       q_[wave][k][1][lane] = lo;
     }
-  } else if (kStores && stores && wave >= NS && wave < NS + (HD == 256 ? 2 : 1)) {
+  } else if (stores && wave >= NS && wave < NS + (HD == 256 ? 2 : 1)) {
     constexpr int LANES = Kv4Row<HD>::LANES;  // the new row's K (unit 0) and V (1)
     const int unit = (wave - NS) * (64 / LANES) + lane / LANES, rq = lane % LANES;
     Kv4Row<HD> row;
@@ -701,7 +700,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
     d.load_v(p, r, g);
   }
   __syncthreads();
-  if (kStores && stores && tile == filled / kKv4Tile) {
+  if (stores && tile == filled / kKv4Tile) {
     const int j = filled % kKv4Tile;
     d.patch_codes(fresh, j, r, g);
 #pragma unroll
@@ -1070,10 +1069,10 @@ Plan plan(int rows, int n_seq, int nh, int nkv, int hd, int slots) {
   p.V = rows * (nh / nkv);
   // The two kernels, V query rows per list (us; 4 sequences of 4095 slots, 8 KV heads, 4 of 256
   // channels; kv4_attention_kernel in as many groups as it takes against kv4_rows_kernel):
-  //   channels 64:  V 8 16.3 / 16.1 (one sequence 13.4 / 14.1), 16 20.2 / 17.6, 64 36.0 / 27.2
-  //   channels 128: V 4 one group, 8 21.3 / 18.9, 16 26.5 / 21.0, 128 92.9 / 50.2
-  //   channels 256: V 4 18.0 / 19.6, 8 24.9 / 23.8, 12 45.0 / 25.6, 128 165 / 54.0
-  p.dense = p.V > (hd == 64 ? 8 : 4);
+  //   channels 64:  V 8 16.2 / 16.1, 16 20.2 / 17.4, 64 36.0 / 26.6
+  //   channels 128: V 4 of 16 sequences 21.4 / 25.5, 8 21.3 / 19.2, 128 92.9 / 50.1
+  //   channels 256: V 4 18.0 / 19.6, 8 24.9 / 21.0, 128 165 / 56.4
+  p.dense = p.V > 4;
   const int group = p.dense ? 16 : hps;
   p.nsub = p.dense && p.V > 16 && hd < 256 ? 2 : 1;
   p.nz = (p.V + p.nsub * group - 1) / (p.nsub * group);
