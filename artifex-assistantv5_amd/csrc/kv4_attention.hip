@@ -35,9 +35,12 @@ __device__ __forceinline__ int kv4_filled(const Kv4Cache &c, int64_t s, int rows
 
 // How the tiles of a list are cut: `per` for each workgroup, `n` of them at most S.  Every
 // workgroup of the call gets about the same number, whatever the sequences' lengths: all lists'
-// tiles over `wgs` workgroups, in whole turns of a workgroup's W waves, at least `least` tiles.
+// tiles over `wgs` workgroups, in whole turns of a workgroup's W waves, and no fewer than eight:
+// they do not make up for a workgroup's start and end (4 x 9000 slots of 256 channels, 8 query
+// rows: four 24.8 us, eight 23.5).
+constexpr int kLeastTiles = 8;
 struct Cut {
-  int S, wgs, W, least;
+  int S, wgs, W;
 };
 struct Splits {
   int per, n;
@@ -46,7 +49,7 @@ __device__ __forceinline__ int kv4_tiles(int filled, int rows) {
   return filled < 0 ? 0 : (filled + rows + kKv4Tile - 1) / kKv4Tile;
 }
 __device__ __forceinline__ Splits kv4_splits(int tiles, int fair, const Cut &k) {
-  const int per = (max(max(fair, k.least), (tiles + k.S - 1) / k.S) + k.W - 1) / k.W * k.W;
+  const int per = (max(max(fair, kLeastTiles), (tiles + k.S - 1) / k.S) + k.W - 1) / k.W * k.W;
   return {per, (tiles + per - 1) / per};
 }
 // The fair share: a wave's lanes add the sequences.
@@ -583,19 +586,21 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 // block whose scales are under 2^-13 of the others' falls below 2^-3, where two f16 parts hold
 // fewer bits (2^-25 absolute: 2^-35 of the row's largest).
 // Bound: vector instructions (70 % busy), about 150 for a tile's codes and 230 for each group of
-// rows (128 channels).  32 rows of 32 / 8 heads over 20000 slots: 50 us, 10.5 GFLOP of products in
-// four parts; the kernel for few rows took about 95.
+// rows (128 channels).  32 rows of 32 / 8 heads over 20000 slots: 47 us, 10.5 GFLOP of products in
+// two parts each; the kernel for few rows took about 95.
+template <int HD>
+constexpr int kRowsWaves = HD == 256 ? 4 : 8;
 template <int HD, int NS>
-__global__ __launch_bounds__(256, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
+__global__ __launch_bounds__(64 * kRowsWaves<HD>, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
                                                           float *__restrict__ rec,
                                                           float2 *__restrict__ lse,
                                                           float *__restrict__ scores, Cut cut,
                                                           bool store) {
   using L = Kv4<HD>;
-  constexpr int W = 4, NB = L::NB, half = HD / 2, RS = record_floats<HD>();
+  constexpr int W = kRowsWaves<HD>, NB = L::NB, half = HD / 2, RS = record_floats<HD>();
   constexpr float kLift = 10.f, kMostW = 16384.f, kMostP = 0x1p100f;
   // Queries (per block, hi and lo part, a B operand) while tiles are read, then the waves' sums, 16
-  // rows of HD per group: 64 KB together, so two workgroups fit a CU's LDS, 82 apart.
+  // rows of HD per group: 64 KB for four waves, 128 for eight, so that eight waves fit a CU.
   __shared__ union {
     half8_t q[NS][NB][2][64];
     float o[W][NS][16 * HD];
@@ -1069,36 +1074,34 @@ Plan plan(int rows, int n_seq, int nh, int nkv, int hd, int slots) {
   p.V = rows * (nh / nkv);
   // The two kernels, V query rows per list (us; 4 sequences of 4095 slots, 8 KV heads, 4 of 256
   // channels; kv4_attention_kernel in as many groups as it takes against kv4_rows_kernel):
-  //   channels 64:  V 8 16.2 / 16.1, 16 20.2 / 17.4, 64 36.0 / 26.6
-  //   channels 128: V 4 of 16 sequences 21.4 / 25.5, 8 21.3 / 19.2, 128 92.9 / 50.1
+  //   channels 64:  V 8 16.2 / 15.6, 16 20.2 / 16.7, 64 36.0 / 26.5
+  //   channels 128: V 4 of 16 sequences 21.4 / 25.5, 8 21.3 / 18.9, 128 92.9 / 49.4
   //   channels 256: V 4 18.0 / 19.6, 8 24.9 / 21.0, 128 165 / 56.4
   p.dense = p.V > 4;
   const int group = p.dense ? 16 : hps;
   p.nsub = p.dense && p.V > 16 && hd < 256 ? 2 : 1;
   p.nz = (p.V + p.nsub * group - 1) / (p.nsub * group);
   p.lists = (int64_t)n_seq * nkv;
-  // Waves per workgroup and workgroups at a time (us; 32 / 8 heads of 128): many lists of
-  // different lengths balance better in small workgroups (16 sequences of up to 4095 slots:
-  // 8 x 512 24.8, 4 x 768 21.2); few lists leave fewer records with large ones (6000 slots: 11.1
-  // against 12.7; 130000: 40.2 against 40.8).  Of 256 channels and with many rows a kernel takes
-  // up to 256 registers: two waves per SIMD.
+  // Waves per workgroup and workgroups at a time (us; 32 / 8 heads of 128).  Few rows: many lists
+  // of different lengths balance better in small workgroups (16 sequences of up to 4095 slots:
+  // 8 x 512 25.6, 4 x 768 21.7); few lists leave fewer records with large ones (6000 slots: 11.1
+  // against 13.1; 130000: 42.2 against 42.7).  Of 256 channels and with many rows a kernel takes
+  // up to 256 registers: two waves per SIMD, with many rows as one workgroup per CU (32 rows of
+  // 20000 slots: 51.8 with two, 50.0 with one), but of 256 channels as two (4 x 9000 slots, 16 /
+  // 2 heads: 23.8 against 25.0).
   const bool many = p.lists * p.nz >= 32;
   int resident;
   if (p.dense) {
-    p.cut.W = 4, resident = 512;
+    p.cut.W = hd == 256 ? 4 : 8, resident = hd == 256 ? 512 : 256;
   } else if (hd == 256) {
     p.cut.W = 8, resident = 256;
   } else {
     p.cut.W = many ? 4 : 8, resident = many ? 768 : 512;
   }
   p.cut.wgs = (resident + p.nz - 1) / p.nz;
-  // Turns at least: with many rows two, since the start and the end of a workgroup weigh more
-  // (8192 slots, 8 to 32 rows of 128 channels, us with one against two: 16.8 / 14.8, 23.6 / 20.2; 4
-  // x 9000 of 256 24.8 / 23.5; of 64, 20 rows 17.0 / 15.8), with few rows one (11.2 / 12.2).  A list
-  // of two turns is not cut: one launch, and nothing to join.
-  p.cut.least = (p.dense ? 2 : 1) * p.cut.W;
+  // a list of two turns is not cut: one launch, and nothing to join
   const int64_t tiles = slots / kKv4Tile;
-  const int64_t most = tiles <= 2 * p.cut.W ? 1 : (tiles + p.cut.least - 1) / p.cut.least;
+  const int64_t most = tiles <= 2 * p.cut.W ? 1 : (tiles + kLeastTiles - 1) / kLeastTiles;
   // sequences of different lengths: up to four times the workgroups that equal ones would take
   const int64_t want = (4 * p.cut.wgs + p.lists - 1) / p.lists;
   p.cut.S = (int)(want < most ? want : most);
