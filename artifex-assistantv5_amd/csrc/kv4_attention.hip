@@ -585,7 +585,7 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 // slots; where m is raised for it, by each slot's own.  m is that of all blocks: p * scale of a
 // block whose scales are under 2^-13 of the others' falls below 2^-3, where two f16 parts hold
 // fewer bits (2^-25 absolute: 2^-35 of the row's largest).
-// Bound: vector instructions (70 % busy), about 150 for a tile's codes and 230 for each group of
+// Bound: vector instructions (76 % busy, and the matrix cores 21 %), about 150 for a tile's codes and 230 for each group of
 // rows (128 channels).  32 rows of 32 / 8 heads over 20000 slots: 47 us, 10.5 GFLOP of products in
 // two parts each; the kernel for few rows took about 95.
 template <int HD>
