@@ -576,6 +576,10 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
   }
 }
 
+// Waves of a workgroup of kv4_rows_kernel (measured at plan()).
+template <int HD>
+constexpr int kRowsWaves = HD == 256 ? 4 : 8;
+
 // The same for many query rows: NS groups of 16, a column each.  Every block's scores are a product
 // of their own, multiplied by the slots' scales as they are added, and P times V's scales is made
 // for every block.  So a lane holds all blocks' scales of its slots (32 registers at 128 channels
@@ -585,11 +589,9 @@ __global__ __launch_bounds__(64 * W, WPS) void kv4_attention_kernel(Kv4Cache c, 
 // slots; where m is raised for it, by each slot's own.  m is that of all blocks: p * scale of a
 // block whose scales are under 2^-13 of the others' falls below 2^-3, where two f16 parts hold
 // fewer bits (2^-25 absolute: 2^-35 of the row's largest).
-// Bound: vector instructions (76 % busy, and the matrix cores 21 %), about 150 for a tile's codes and 230 for each group of
-// rows (128 channels).  32 rows of 32 / 8 heads over 20000 slots: 47 us, 10.5 GFLOP of products in
-// two parts each; the kernel for few rows took about 95.
-template <int HD>
-constexpr int kRowsWaves = HD == 256 ? 4 : 8;
+// Bound: vector instructions (76 % busy, and the matrix cores 21 %), about 150 for a tile's codes
+// and 230 for each group of rows (128 channels).  32 rows of 32 / 8 heads over 20000 slots: 47 us,
+// 10.5 GFLOP of products in two parts each; the kernel for few rows took about 95.
 template <int HD, int NS>
 __global__ __launch_bounds__(64 * kRowsWaves<HD>, 2) void kv4_rows_kernel(Kv4Cache c, Kv4Attn a,
                                                           float *__restrict__ rec,
