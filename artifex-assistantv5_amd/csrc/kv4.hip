@@ -141,12 +141,13 @@ __global__ __launch_bounds__(kThreads) void kv4_load_kernel(const uint8_t *__res
 // ---------------------------------------------------------------------------
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 
-// The order of the slots: larger is kept first.  NaN is 0, -0 equals +0.
+// The order of the slots: larger is kept first.  NaN is 0, -0 equals +0, and a protected slot is
+// above every weight, infinite ones too.
 __device__ __forceinline__ uint32_t evict_key(float w, int32_t p, int32_t from, int32_t sinks) {
   const bool first = (p >= from) | (p < sinks);  // selects, no branches
-  const uint32_t u = __float_as_uint(first ? INFINITY : w + 0.f);
+  const uint32_t u = __float_as_uint(w + 0.f);
   const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
-  return (!first & !(w == w)) ? 0u : k;
+  return first ? ~0u : (w == w ? k : 0u);
 }
 
 // Work: per list the number of moves, then the slots given up below `keep` (holes) and the

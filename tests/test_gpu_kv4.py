@@ -647,3 +647,44 @@ def test_graph_of_several_rows(kv4):
             if name in "kv":
                 a, b = a[:, :, :n], b[:, :, :n]
             assert torch.equal(a, b), (step, name)
+
+
+def _kept(weights, positions, n, pos, keep, recent, sinks):
+    """The slots that an eviction keeps: protected ones first, then by weight, NaN last, of equal
+    ones the lower slot."""
+    w = weights[:n].astype(np.float64)
+
+    def place(t):
+        if positions[t] >= pos - recent or positions[t] < sinks:
+            return 0, 0.0, t
+        return (2, 0.0, t) if np.isnan(w[t]) else (1, -w[t], t)
+
+    order = sorted(range(n), key=place)
+    return set(order[:keep])
+
+
+@pytest.mark.parametrize("slots,n,keep,recent,sinks,pos", [
+    (96, 90, 40, 20, 4, 90),               # one, four and sixteen turns of a list
+    (5024, 5000, 1000, 300, 16, 5000),
+    (20480, 20001, 9000, 9000, 0, 20001),
+])
+def test_evict_protected_slots_come_first(kv4, slots, n, keep, recent, sinks, pos):
+    """More slots of infinite weight than `keep`, most of them before the protected ones."""
+    rng = np.random.default_rng(n)
+    weights = np.exp(rng.standard_normal((1, 2, slots))).astype(np.float32)
+    weights[..., 5:n - 30] = np.inf
+    weights[..., 7::10] = np.nan
+    weights[..., 8::10] = -np.inf
+    positions = np.broadcast_to(np.arange(slots, dtype=np.int32), (1, 2, slots)).copy()
+    cache = kv4.empty(1, 2, 64, slots)
+    dw, dp, length = _cuda(weights), _cuda(positions), _i64([n])
+    kv4.evict(cache, dw, dp, length, _i64([pos]), keep, kv4.evict_workspace(cache), recent=recent,
+              sinks=sinks)
+    assert length.tolist() == [keep]
+    for h in range(2):
+        want = _kept(weights[0, h], positions[0, h].tolist(), n, pos, keep, recent, sinks)
+        got = dp[0, h, :keep].tolist()
+        assert set(got) == want
+        assert [p for p in got if p < keep] == [p for i, p in enumerate(got) if p == i]
+        assert np.array_equal(dw[0, h, :keep].cpu().numpy().view(np.uint32),
+                              weights[0, h, got].view(np.uint32))
