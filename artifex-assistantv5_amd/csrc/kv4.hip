@@ -245,9 +245,10 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Kv4Cache c, K
     }
     return;
   }
-  // positions are below 2^31 - 1 (the tables' rows)
-  const int64_t from64 = c.pos[s] - e.recent;
-  const int32_t from = (int32_t)(from64 < -1 ? -1 : (from64 > INT32_MAX ? INT32_MAX : from64));
+  // positions are below 2^31 - 1 (the tables' rows); pos may be anything, so it is limited first
+  const int64_t pos = c.pos[s], most = (int64_t)INT32_MAX + e.recent;
+  const int64_t least = (int64_t)INT32_MIN + e.recent;
+  const int32_t from = (int32_t)((pos < least ? least : (pos > most ? most : pos)) - e.recent);
   const int32_t sinks = (int32_t)e.sinks;
   uint32_t key[4 * T];
   int held = -1;  // the segment in `key`

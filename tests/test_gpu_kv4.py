@@ -667,6 +667,9 @@ def _kept(weights, positions, n, pos, keep, recent, sinks):
     (96, 90, 40, 20, 4, 90),               # one, four and sixteen turns of a list
     (5024, 5000, 1000, 300, 16, 5000),
     (20480, 20001, 9000, 9000, 0, 20001),
+    (96, 90, 40, 8, 2, (1 << 63) - 1),     # nothing is recent
+    (96, 90, 40, 8, 2, -(1 << 63)),        # everything is: the lowest slots stay
+    (96, 90, 40, 40, 0, -(1 << 63) + 39),
 ])
 def test_evict_protected_slots_come_first(kv4, slots, n, keep, recent, sinks, pos):
     """More slots of infinite weight than `keep`, most of them before the protected ones."""
