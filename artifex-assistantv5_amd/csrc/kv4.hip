@@ -48,6 +48,7 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Cache c,
         hi = mid;
     }
     s = lo;
+    if (starts[lo] < -(int64_t)c.slots) return;  // r would be behind every slot, and i not fit 64 bits
     last = i = r - starts[lo];
   } else {
     const uint32_t per = n_rows / (uint32_t)c.n_seq;

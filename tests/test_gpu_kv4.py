@@ -691,3 +691,18 @@ def test_evict_protected_slots_come_first(kv4, slots, n, keep, recent, sinks, po
         assert [p for p in got if p < keep] == [p for i, p in enumerate(got) if p == i]
         assert np.array_equal(dw[0, h, :keep].cpu().numpy().view(np.uint32),
                               weights[0, h, got].view(np.uint32))
+
+
+@pytest.mark.parametrize("rows,slots,tables", [(40, 32, 16), (40, 64, 64), (2100, 32, 2400)])
+def test_append_of_starts_far_below(kv4, rows, slots, tables):
+    """Rows that stand 2^63 behind a sequence's first one have no slot: nothing is stored."""
+    kv, hd, least = 4, 64, -(1 << 63)
+    dev = torch.full((2, kv, slots // 32, 36 * hd), 0x5A, dtype=torch.uint8, device="cuda")
+    positions = torch.full((2, kv, slots), -7, dtype=torch.int32, device="cuda")
+    qkv = torch.ones(rows, 3 * kv * hd, device="cuda")
+    cos, sin = (_cuda(t) for t in _tables(tables, hd))
+    for starts in ([least, least + 3, rows], [least + 7, rows, rows], [-slots, -slots, rows],
+                   [least, -slots - 1, 0]):
+        kv4.append(qkv, _i64([0, 0]), _i64([0, 0]), cos, sin, dev, kv, starts=_i64(starts),
+                   positions=positions)
+        assert (dev == 0x5A).all() and (positions == -7).all(), starts
