@@ -341,17 +341,17 @@ class QuantDecoder:
                           accumulate=True)
 
     def _prefill_kv4(self, tokens: torch.Tensor, pos0: int) -> torch.Tensor:
-        if pos0 == 0:
-            self.kv_lengths.zero_()
-        held, done, h = int(self.kv_lengths.item()), 0, None
+        held, done, h = int(self.kv_lengths.item()) if pos0 else 0, 0, None
         if pos0 < held or (self.kv_keep is None and pos0 != held):
             raise ValueError(f"position {pos0} does not follow the {held} slots that the 4-bit "
                              "cache holds")
+        if self.kv_keep is None and held + tokens.numel() > self.kv_slots:
+            raise ValueError(f"sequence of {held + tokens.numel()} exceeds the cache's "
+                             f"{self.kv_slots} slots (kv_keep bounds it)")
+        if pos0 == 0:
+            self.kv_lengths.zero_()
         while done < tokens.numel():
             m = min(tokens.numel() - done, self.kv_slots - held)
-            if m == 0:
-                raise ValueError(f"sequence exceeds the cache's {self.kv_slots} slots (kv_keep "
-                                 "bounds it)")
             self._prompt_pos = pos0 + done
             pos = torch.arange(pos0 + done, pos0 + done + m, device=self.device)
             h = self._layers_glue(self._embed(tokens[done:done + m]), pos, held)

@@ -187,3 +187,26 @@ def test_a_model_file_with_a_4_bit_cache(dec, tmp_path):
     a, b = model.generate(prompt, 30), direct.generate(prompt, 30, graph=False)
     assert torch.equal(a["tokens"], b["tokens"])
     assert int(model.kv_lengths.item()) == int(direct.kv_lengths.item()) < 64
+
+
+def _state(m):
+    return [t.clone() for t in m._cache_state()]
+
+
+def _same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_a_prompt_that_does_not_fit_changes_nothing(dec):
+    """Refused before the first layer, as with an f32 cache: the sequence goes on behind it."""
+    cfg, w = _model(dec, max_seq=256)
+    tokens = _tokens(cfg, 120, 3)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=64)
+    m.prefill(tokens[:40], 0)
+    before = _state(m)
+    for n, pos0 in ((25, 40), (65, 0), (120, 0)):
+        with pytest.raises(ValueError, match="slots"):
+            m.prefill(tokens[:n], pos0)
+        assert _same(_state(m), before)
+    got = m.prefill(tokens[40:64], 40)
+    assert int(m.kv_lengths.item()) == 64 and torch.isfinite(got).all()
