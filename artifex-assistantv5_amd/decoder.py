@@ -341,6 +341,8 @@ class QuantDecoder:
                           accumulate=True)
 
     def _prefill_kv4(self, tokens: torch.Tensor, pos0: int) -> torch.Tensor:
+        if tokens.numel() == 0:
+            raise ValueError("an empty prompt has no logits")
         held, done, h = int(self.kv_lengths.item()) if pos0 else 0, 0, None
         if pos0 < held or (self.kv_keep is None and pos0 != held):
             raise ValueError(f"position {pos0} does not follow the {held} slots that the 4-bit "

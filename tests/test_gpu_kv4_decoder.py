@@ -210,3 +210,16 @@ def test_a_prompt_that_does_not_fit_changes_nothing(dec):
         assert _same(_state(m), before)
     got = m.prefill(tokens[40:64], 40)
     assert int(m.kv_lengths.item()) == 64 and torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("cache", [{}, dict(kv_slots=64, kv_keep=32, kv_recent=8)])
+def test_an_empty_prompt_is_refused(dec, cache):
+    cfg, w = _model(dec)
+    tokens = _tokens(cfg, 10, 3)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4, **cache)
+    m.prefill(tokens, 0)
+    before = _state(m)
+    for pos0 in (0, 10):
+        with pytest.raises(ValueError, match="empty"):
+            m.prefill(tokens[:0], pos0)
+        assert _same(_state(m), before)
