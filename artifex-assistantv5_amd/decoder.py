@@ -274,9 +274,9 @@ class QuantDecoder:
             raise ValueError("kv_bits=4 needs the fused decode step and the HIP glue")
         slots = -(-(cfg.max_seq if slots is None else slots) // kv4.TILE) * kv4.TILE
         if keep is not None and not (0 <= recent and 0 <= sinks
-                                     and recent + sinks <= keep < slots):
+                                     and max(1, recent + sinks) <= keep < slots):
             raise ValueError(f"kv_keep {keep}: kv_recent {recent} + kv_sinks {sinks} must fit it, and "
-                             f"it must be below the {slots} slots")
+                             f"it must be above 0 and below the {slots} slots")
         L, nkv, hd = cfg.n_layers, cfg.n_kv_heads, cfg.head_dim
         self.kv_slots, self.kv_recent, self.kv_sinks = slots, recent, sinks
         self.kv4 = kv4.empty(1, nkv, hd, slots, dev, n_layers=L)

@@ -223,3 +223,10 @@ def test_an_empty_prompt_is_refused(dec, cache):
         with pytest.raises(ValueError, match="empty"):
             m.prefill(tokens[:0], pos0)
         assert _same(_state(m), before)
+
+
+def test_nothing_kept_is_refused(dec):
+    cfg, w = _model(dec)
+    for keep in (0, -1):
+        with pytest.raises(ValueError, match="kv_keep"):
+            dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=64, kv_keep=keep, kv_recent=0, kv_sinks=0)
