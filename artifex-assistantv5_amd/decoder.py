@@ -491,6 +491,8 @@ class QuantDecoder:
         x = self.b_x
         merge = cfg.n_heads * cfg.head_dim <= 8192 and self.kv_bits == 32
         self._embed(tok, x)
+        if self.kv_bits == 4:
+            self.b_att.fill_(float("nan"))  # stays where the row has no slot or no position
         for l, lw in enumerate(W.layers):
             self._fused_slot(x, lw, "qkv", self.b_qkv, lw.attn_norm)
             if self.kv_bits == 4:
@@ -523,6 +525,8 @@ class QuantDecoder:
             self.kv_lengths.add_(1)
             if self.kv_keep is not None:
                 self._evict(pos)
+            else:
+                self.kv_lengths.clamp_(max=self.kv_slots)
         return self.b_logits
 
     def _fused_slot(self, x, lw, slot, y, norm_w) -> None:
@@ -537,7 +541,9 @@ class QuantDecoder:
     def step(self, tok: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         """One greedy decode step in place: reads token ``tok`` [1] at position
         ``pos`` [1], writes the next token into ``tok`` and advances ``pos``.
-        Touches no host state, so it can be captured in a graph."""
+        Touches no host state, so it can be captured in a graph.  With a 4-bit cache ``pos``
+        is the position after the last one; a step for which it has no slot left stores
+        nothing, and its logits are NaN."""
         if self.fused:
             return self._step_fused(tok, pos)
         x = self._embed(tok)

@@ -230,3 +230,48 @@ def test_nothing_kept_is_refused(dec):
     for keep in (0, -1):
         with pytest.raises(ValueError, match="kv_keep"):
             dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=64, kv_keep=keep, kv_recent=0, kv_sinks=0)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_step_past_the_last_slot_is_seen(dec, graph):
+    """Its logits are NaN, nothing is stored, and the cache still holds what it held."""
+    cfg, w = _model(dec, max_seq=256)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=32)
+    prompt = _tokens(cfg, 29, 4)
+    tok = torch.argmax(m.prefill(prompt, 0), dim=-1).view(1)
+    pos = torch.tensor([29], device="cuda")
+    if graph:
+        m.capture(tok, pos)
+
+    def step():
+        if not graph:
+            return m.step(tok, pos)
+        m._graph.replay()
+        return m._graph_logits
+
+    for _ in range(3):
+        assert torch.isfinite(step()).all()
+    before = _state(m)
+    for _ in range(3):
+        assert torch.isnan(step()).all()
+        assert _same(_state(m), before) and m.kv_lengths.tolist() == [32]
+    with pytest.raises(ValueError, match="slots"):
+        m.prefill(prompt[:1], 32)
+    again = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=32)
+    assert torch.equal(m.prefill(prompt, 0), again.prefill(prompt, 0))
+    tok.fill_(7)
+    pos.fill_(29)
+    got = step().clone()
+    tok.fill_(7)
+    pos.fill_(29)
+    assert torch.equal(got, again.step(tok, pos))
+
+
+def test_a_step_past_the_tables_is_seen(dec):
+    """With eviction the positions end with the RoPE tables."""
+    cfg, w = _model(dec)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=64, kv_keep=32, kv_recent=8)
+    m.prefill(_tokens(cfg, 20, 4), 0)
+    tok, pos = torch.tensor([1], device="cuda"), torch.tensor([m.cos.shape[0]], device="cuda")
+    m.step(tok.clone(), torch.tensor([20], device="cuda"))
+    assert torch.isnan(m.step(tok, pos)).all()
