@@ -280,7 +280,9 @@ class QuantDecoder:
         L, nkv, hd = cfg.n_layers, cfg.n_kv_heads, cfg.head_dim
         self.kv_slots, self.kv_recent, self.kv_sinks = slots, recent, sinks
         self.kv4 = kv4.empty(1, nkv, hd, slots, dev, n_layers=L)
-        self.kv_lengths = torch.zeros(1, dtype=torch.long, device=dev)
+        # the slots in use, and the position after the last one (with eviction further on)
+        self.kv_state = torch.zeros(2, dtype=torch.long, device=dev)
+        self.kv_lengths = self.kv_state[:1]
         # one layer's rows in f32, for the attention of a prompt
         self.k_cache = torch.zeros(nkv, slots, hd, device=dev)
         self.v_cache = torch.zeros(nkv, slots, hd, device=dev)
@@ -310,7 +312,7 @@ class QuantDecoder:
         """The tensors that a step changes, besides token and position."""
         if self.kv_bits == 32:
             return [self.k_cache, self.v_cache]
-        return [t for t in (self.kv4, self.kv_lengths, self.kv_weights, self.kv_positions)
+        return [t for t in (self.kv4, self.kv_state, self.kv_weights, self.kv_positions)
                 if t is not None]
 
     def _attend_rows(self, l: int, qkv: torch.Tensor, pos: torch.Tensor, att: torch.Tensor,
@@ -343,21 +345,22 @@ class QuantDecoder:
     def _prefill_kv4(self, tokens: torch.Tensor, pos0: int) -> torch.Tensor:
         if tokens.numel() == 0:
             raise ValueError("an empty prompt has no logits")
-        held, done, h = int(self.kv_lengths.item()) if pos0 else 0, 0, None
-        if pos0 < held or (self.kv_keep is None and pos0 != held):
-            raise ValueError(f"position {pos0} does not follow the {held} slots that the 4-bit "
-                             "cache holds")
+        held, follows = self.kv_state.tolist() if pos0 else (0, 0)
+        if pos0 != follows:
+            raise ValueError(f"position {pos0} does not follow what the 4-bit cache holds: "
+                             f"{held} slots, position {follows} is the next")
         if self.kv_keep is None and held + tokens.numel() > self.kv_slots:
             raise ValueError(f"sequence of {held + tokens.numel()} exceeds the cache's "
                              f"{self.kv_slots} slots (kv_keep bounds it)")
         if pos0 == 0:
-            self.kv_lengths.zero_()
+            self.kv_state.zero_()
+        done, h = 0, None
         while done < tokens.numel():
             m = min(tokens.numel() - done, self.kv_slots - held)
             self._prompt_pos = pos0 + done
             pos = torch.arange(pos0 + done, pos0 + done + m, device=self.device)
             h = self._layers_glue(self._embed(tokens[done:done + m]), pos, held)
-            self.kv_lengths += m
+            self.kv_state += m
             held, done = held + m, done + m
             if self.kv_keep is not None and held == self.kv_slots:
                 self._evict(pos[-1:] + 1)
@@ -520,13 +523,14 @@ class QuantDecoder:
         glue.matmul_fused(x, W.lm_head_gg, self.b_logits, glue.PROLOGUE_RMSNORM, W.final_norm,
                           cfg.eps)
         glue.argmax(self.b_logits, tok, self.w_arg)
-        pos.add_(1)
-        if self.kv_bits == 4:
-            self.kv_lengths.add_(1)
-            if self.kv_keep is not None:
-                self._evict(pos)
-            else:
-                self.kv_lengths.clamp_(max=self.kv_slots)
+        if self.kv_bits == 32:
+            pos.add_(1)
+            return self.b_logits
+        torch._foreach_add_([pos, self.kv_state], 1)  # one launch
+        if self.kv_keep is not None:
+            self._evict(pos)
+        else:
+            self.kv_state.clamp_(max=self.kv_slots)
         return self.b_logits
 
     def _fused_slot(self, x, lw, slot, y, norm_w) -> None:

@@ -275,3 +275,35 @@ def test_a_step_past_the_tables_is_seen(dec):
     tok, pos = torch.tensor([1], device="cuda"), torch.tensor([m.cos.shape[0]], device="cuda")
     m.step(tok.clone(), torch.tensor([20], device="cuda"))
     assert torch.isnan(m.step(tok, pos)).all()
+
+
+def test_a_prompt_follows_the_last_position(dec):
+    """With eviction the slots in use do not tell the next position: one too far or one that was
+    there already is refused, after prompts, steps and evictions, and what is held stays."""
+    cfg, w = _model(dec, max_seq=400)
+    tokens = _tokens(cfg, 200, 1)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=64, kv_keep=32, kv_recent=0, kv_sinks=0)
+
+    def refuses(*positions):
+        before = _state(m)
+        for p in positions:
+            with pytest.raises(ValueError, match="follow"):
+                m.prefill(tokens[:3], p)
+        assert _same(_state(m), before)
+
+    m.prefill(tokens[:5], 0)
+    refuses(4, 6, 64)
+    m.prefill(tokens[5:20], 5)
+    refuses(5, 19, 21)
+    m.prefill(tokens[20:150], 20)                     # over evictions
+    assert int(m.kv_lengths.item()) < 64
+    refuses(63, 149, 151, 200)
+    tok, pos = tokens[150:151].clone(), torch.tensor([150], device="cuda")
+    for _ in range(40):                               # and again
+        m.step(tok, pos)
+    refuses(150, 189, 191)
+    m.prefill(tokens[:1], 190)
+    out = m.generate(tokens[:50], 30)["tokens"]       # 79 tokens fed
+    assert out.numel() == 30
+    refuses(78, 80)
+    m.prefill(tokens[:2], 79)
