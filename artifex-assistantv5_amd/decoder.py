@@ -294,8 +294,10 @@ class QuantDecoder:
             self.kv_weights = torch.zeros(L, 1, nkv, slots, device=dev)
             self.kv_positions = torch.zeros(L, 1, nkv, slots, dtype=torch.int32, device=dev)
             self.w_evict = kv4.evict_workspace(self.kv4)
-        self.w_att = kv4.attention_workspace(self.kv4[0], cfg.n_heads, weights=keep is not None)
-        self.w_window = {}  # by rows: workspaces of a prompt's last rows
+        # of steps, and of a prompt's last rows
+        self.w_att = kv4.attention_workspace(self.kv4[0], cfg.n_heads,
+                                             rows=1 if keep is None else self.WINDOW,
+                                             weights=keep is not None)
 
     def _kv_slot(self, l: int):
         """Layer l's positions and weights (None without eviction)."""
@@ -335,11 +337,9 @@ class QuantDecoder:
                    **self._kv_slot(l))
         if self.kv_keep is not None:
             w = min(m, self.WINDOW)
-            if w not in self.w_window:
-                self.w_window[w] = kv4.attention_workspace(cache, cfg.n_heads, rows=w, weights=True)
             kv4.attention(qkv[m - w:], self.kv_lengths + (m - w), first + (m - w), self.cos,
                           self.sin, cache, torch.empty_like(att[:w]), cfg.n_heads,
-                          self.w_window[w], store=False, weights=self.kv_weights[l],
+                          self.w_att, store=False, weights=self.kv_weights[l],
                           accumulate=True)
 
     def _prefill_kv4(self, tokens: torch.Tensor, pos0: int) -> torch.Tensor:

@@ -132,11 +132,17 @@ def append(qkv: torch.Tensor, lengths: torch.Tensor, pos: torch.Tensor, cos: tor
 
 def attention_workspace(kv: torch.Tensor, n_heads: int, rows: int = 1,
                         weights: bool = False) -> torch.Tensor:
-    """Device workspace of ``attention`` calls of this shape (with ``weights`` if they have)."""
+    """Device workspace of ``attention`` calls of up to ``rows`` rows per sequence (with
+    ``weights`` if any of them has)."""
     _, n_seq, n_kv, hd, slots = _shape(kv)
     lib = _native.load_library()
-    n = _native.check(lib.gguf_hip_kv4_attention_workspace(rows, int(weights), n_seq, n_heads, n_kv,
-                                                           hd, slots), lib)
+
+    def size(m, mode):
+        return _native.check(lib.gguf_hip_kv4_attention_workspace(m, mode, n_seq, n_heads, n_kv, hd,
+                                                                  slots), lib)
+
+    # not always more for more rows: they are split over fewer workgroups
+    n = max([size(rows, int(weights))] + [size(m, int(weights)) for m in range(1, rows)])
     return torch.empty(n, dtype=torch.uint8, device=kv.device)
 
 

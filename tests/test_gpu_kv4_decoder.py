@@ -307,3 +307,20 @@ def test_a_prompt_follows_the_last_position(dec):
     assert out.numel() == 30
     refuses(78, 80)
     m.prefill(tokens[:2], 79)
+
+
+def test_prompts_of_any_length_share_a_workspace(dec):
+    """Prompts of 1 .. 40 rows leave no more memory in use than the first did."""
+    cfg, w = _model(dec, max_seq=2000)
+    tokens = _tokens(cfg, 40, 2)
+    warm = dec.QuantDecoder(cfg, w, kv_bits=4)        # what the projections keep is there
+    for n in range(1, 41):
+        warm.prefill(tokens[:n], 0)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=1024, kv_keep=512)
+    used, at = [], 0
+    for n in (1, 40, 2, 33, 7, 32, 31, 5):
+        m.prefill(tokens[:n], at)
+        at += n
+        torch.cuda.synchronize()
+        used.append(torch.cuda.memory_allocated())
+    assert used == used[:1] * len(used)
