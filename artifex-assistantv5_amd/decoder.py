@@ -225,6 +225,25 @@ def glue_shapes(cfg: DecoderConfig) -> bool:
             and cfg.ffn % 4 == 0)
 
 
+def kv_cache_slots(cfg: DecoderConfig, fused: bool, kv_bits: int, kv_slots: Optional[int],
+                   kv_keep: Optional[int], kv_recent: int, kv_sinks: int) -> int:
+    """The slots per KV head of a ``QuantDecoder``'s cache; ValueError for options that do not go
+    together.  ``fused``: the decoder has the fused decode step and the HIP glue."""
+    if kv_bits != 4:
+        if kv_bits != 32 or kv_slots is not None or kv_keep is not None:
+            raise ValueError(f"kv_bits {kv_bits} not 32 or 4, or kv_slots / kv_keep without 4")
+        return cfg.max_seq
+    if not fused:
+        raise ValueError("kv_bits=4 needs the fused decode step and the HIP glue")
+    slots = -(-(cfg.max_seq if kv_slots is None else kv_slots) // kv4.TILE) * kv4.TILE
+    kv4.cache_bytes(1, cfg.n_kv_heads, cfg.head_dim, slots)
+    if kv_keep is not None and not (0 <= kv_recent and 0 <= kv_sinks
+                                    and max(1, kv_recent + kv_sinks) <= kv_keep < slots):
+        raise ValueError(f"kv_keep {kv_keep}: kv_recent {kv_recent} + kv_sinks {kv_sinks} must fit "
+                         f"it, and it must be above 0 and below the {slots} slots")
+    return slots
+
+
 class QuantDecoder:
     """Greedy decoder over ``DecoderWeights`` with an f32 or 4-bit KV cache in HBM.
 
@@ -246,10 +265,10 @@ class QuantDecoder:
         self.hip_glue = hip_glue and glue_shapes(cfg)
         L, kv, T, hd = cfg.n_layers, cfg.n_kv_heads, cfg.max_seq, cfg.head_dim
         self.kv_bits, self.kv_keep = kv_bits, kv_keep
+        slots = kv_cache_slots(cfg, self.fused and self.hip_glue, kv_bits, kv_slots, kv_keep,
+                               kv_recent, kv_sinks)
         if kv_bits == 4:
-            self._init_kv4(kv_slots, kv_keep, kv_recent, kv_sinks)
-        elif kv_bits != 32 or kv_slots is not None or kv_keep is not None:
-            raise ValueError(f"kv_bits {kv_bits} not 32 or 4, or kv_slots / kv_keep without 4")
+            self._init_kv4(slots, kv_keep, kv_recent, kv_sinks)
         else:
             self.k_cache = torch.zeros(L, kv, T, hd, device=self.device)
             self.v_cache = torch.zeros(L, kv, T, hd, device=self.device)
@@ -270,13 +289,6 @@ class QuantDecoder:
     # -- the 4-bit cache --
     def _init_kv4(self, slots, keep, recent, sinks) -> None:
         cfg, dev = self.cfg, self.device
-        if not (self.fused and self.hip_glue):
-            raise ValueError("kv_bits=4 needs the fused decode step and the HIP glue")
-        slots = -(-(cfg.max_seq if slots is None else slots) // kv4.TILE) * kv4.TILE
-        if keep is not None and not (0 <= recent and 0 <= sinks
-                                     and max(1, recent + sinks) <= keep < slots):
-            raise ValueError(f"kv_keep {keep}: kv_recent {recent} + kv_sinks {sinks} must fit it, and "
-                             f"it must be above 0 and below the {slots} slots")
         L, nkv, hd = cfg.n_layers, cfg.n_kv_heads, cfg.head_dim
         self.kv_slots, self.kv_recent, self.kv_sinks = slots, recent, sinks
         self.kv4 = kv4.empty(1, nkv, hd, slots, dev, n_layers=L)

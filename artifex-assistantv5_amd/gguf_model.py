@@ -28,7 +28,7 @@ from typing import Optional, Tuple
 import numpy as np
 import torch
 
-from .decoder import DecoderConfig, DecoderWeights, QuantDecoder
+from .decoder import DecoderConfig, DecoderWeights, QuantDecoder, glue_shapes, kv_cache_slots
 from .ggml import GGML_TYPE_NAMES
 from .gguf_file import GGUFFile, GGUFTensorInfo, arch_kv, gguf_architecture, parse_gguf_path
 from .gguf_loader import LoadedGGUFModel, load_gguf_model
@@ -85,12 +85,17 @@ def unpermute_rows(n_heads: int, head_dim: int) -> np.ndarray:
 
 
 def load_decoder(path: str, device="cuda", max_seq: int = 2048, fused: bool = True,
-                 on_progress=None, **cache) -> Tuple[QuantDecoder, LoadedGGUFModel]:
-    """Load a llama-architecture GGUF file into a ``QuantDecoder`` on ``device``; ``cache``: the
-    decoder's ``kv_bits``, ``kv_slots``, ``kv_keep``, ``kv_recent`` and ``kv_sinks``."""
+                 on_progress=None, kv_bits: int = 32, kv_slots: Optional[int] = None,
+                 kv_keep: Optional[int] = None, kv_recent: int = 64,
+                 kv_sinks: int = 4) -> Tuple[QuantDecoder, LoadedGGUFModel]:
+    """Load a llama-architecture GGUF file into a ``QuantDecoder`` on ``device``, with the
+    decoder's KV cache options, which are checked before the tensors are placed."""
     file = parse_gguf_path(path)
     cfg = config_from_gguf(file, max_seq)
     _check_tensors(file, cfg)
+    cache = dict(kv_bits=kv_bits, kv_slots=kv_slots, kv_keep=kv_keep, kv_recent=kv_recent,
+                 kv_sinks=kv_sinks)
+    kv_cache_slots(cfg, fused and glue_shapes(cfg), **cache)
     dev = torch.device(device)
     perms = {}
     for l in range(cfg.n_layers):

@@ -29,11 +29,16 @@ TILE = _native.KV4_TILE
 MAX_ROWS = _native.KV4_MAX_ROWS
 
 
+def cache_bytes(n_seq: int, n_kv_heads: int, head_dim: int, slots: int) -> int:
+    """Bytes of one layer's cache; ValueError for a shape that there is no cache of."""
+    lib = _native.load_library()
+    return _native.check(lib.gguf_hip_kv4_bytes(n_seq, n_kv_heads, head_dim, slots), lib)
+
+
 def empty(n_seq: int, n_kv_heads: int, head_dim: int, slots: int, device="cuda",
           n_layers: Optional[int] = None) -> torch.Tensor:
     """A cache of one layer, or ``[n_layers, ...]`` of several, every value zero."""
-    lib = _native.load_library()
-    _native.check(lib.gguf_hip_kv4_bytes(n_seq, n_kv_heads, head_dim, slots), lib)
+    cache_bytes(n_seq, n_kv_heads, head_dim, slots)
     shape = (n_seq, n_kv_heads, slots // TILE, 36 * head_dim)
     return torch.zeros(shape if n_layers is None else (n_layers, *shape), dtype=torch.uint8,
                        device=device)

@@ -165,3 +165,44 @@ def test_append_row_limit(lib, native):
     """2^25 rows pass the check of their number (the next one, of the pointers, refuses)."""
     assert _append(lib, rows=(1 << 25) + 2) == native.ERR_SHAPE
     assert _append(lib, rows=1 << 25, qkv=None) == native.ERR_NULL
+
+
+@pytest.fixture
+def file_loader(pkg, tmp_path, monkeypatch):
+    """load_decoder on a small model file whose tensors are never placed: True if it got there."""
+    import gguf_models as gm
+
+    gmodel = importlib.import_module("artifex-assistantv5_amd.gguf_model")
+
+    class Placed(Exception):
+        pass
+
+    def place(*a, **k):
+        raise Placed
+
+    monkeypatch.setattr(gmodel, "load_gguf_model", place)
+
+    def load(**options):
+        p = str(tmp_path / "m.gguf")
+        gm.write_model(p, gm.make_model(seed=1))
+        try:
+            gmodel.load_decoder(p, "cuda", max_seq=128, **options)
+        except Placed:
+            return True
+
+    return load
+
+
+def test_cache_options_are_checked_before_a_file_is_loaded(file_loader):
+    """A cache that the decoder would refuse is refused before the tensors are placed."""
+    assert file_loader()
+    assert file_loader(kv_bits=4)
+    assert file_loader(kv_bits=4, kv_slots=64, kv_keep=40, kv_recent=16, kv_sinks=2)
+    with pytest.raises(TypeError):
+        file_loader(kv_bit=4)
+    for bad in (dict(kv_bits=8), dict(kv_slots=64), dict(kv_keep=32), dict(kv_bits=4, kv_slots=0),
+                dict(kv_bits=4, kv_slots=64, kv_keep=64), dict(kv_bits=4, kv_keep=20, kv_recent=17),
+                dict(kv_bits=4, kv_slots=64, kv_keep=0, kv_recent=0, kv_sinks=0),
+                dict(kv_bits=4, kv_slots=(1 << 20) + 1), dict(kv_bits=4, fused=False)):
+        with pytest.raises(ValueError):
+            file_loader(**bad)
