@@ -324,3 +324,34 @@ def test_prompts_of_any_length_share_a_workspace(dec):
         torch.cuda.synchronize()
         used.append(torch.cuda.memory_allocated())
     assert used == used[:1] * len(used)
+
+
+@pytest.mark.parametrize("over", [{}, dict(n_heads=8, n_kv_heads=1, head_dim=128)])
+def test_prompt_and_steps_behind_evictions(dec, kv4, over):
+    """Slots are out of order and behind the positions: a prompt's logits and those of steps are
+    float64's over the rows that the cache holds."""
+    cfg, w = _model(dec, max_seq=400, **over)
+    tokens = _tokens(cfg, 320, 2)
+    m = dec.QuantDecoder(cfg, w, kv_bits=4, kv_slots=64, kv_keep=40, kv_recent=16)
+    ref = FromCache(cfg, w)
+    m.prefill(tokens[:150], 0)
+    held, at = _cached(kv4, m), 150
+    assert m.kv_positions[0, 0, 0, :held[0][0].shape[0]].tolist() != list(range(held[0][0].shape[0]))
+    for turn in range(3):
+        n = min(9, 63 - held[0][0].shape[0])          # no eviction within
+        lg = m.prefill(tokens[at:at + n], at)[0]
+        exact = Reference(cfg, w)
+        exact.k, exact.v = [list(k) for k, _ in held], [list(v) for _, v in held]
+        for i in range(n):
+            rl = exact.token(int(tokens[at + i]), at + i)
+        assert _rel(lg, rl) < 1e-4
+        at += n
+        tok, pos = torch.argmax(lg).view(1), torch.tensor([at], device="cuda")
+        for _ in range(40):                           # through an eviction
+            t, p, before = int(tok.item()), int(pos.item()), int(m.kv_lengths.item())
+            lg = m.step(tok, pos)[0]
+            if before < 63:                           # else the rows attended to were cut
+                assert int(m.kv_lengths.item()) == before + 1
+                assert _rel(lg, ref.token(t, p, _cached(kv4, m))) < 1e-4
+            at += 1
+        held = _cached(kv4, m)
