@@ -1074,11 +1074,22 @@ Plan plan(int rows, int n_seq, int nh, int nkv, int hd, int slots) {
   Plan p;
   const int hps = 512 / hd;
   p.V = rows * (nh / nkv);
-  // The two kernels, V query rows per list (us; 4 sequences of 4095 slots, 8 KV heads, 4 of 256
-  // channels; kv4_attention_kernel in as many groups as it takes against kv4_rows_kernel):
-  //   channels 64:  V 8 16.2 / 15.6, 16 20.2 / 16.7, 64 36.0 / 26.5
-  //   channels 128: V 4 of 16 sequences 21.4 / 25.5, 8 21.3 / 18.9, 128 92.9 / 49.4
-  //   channels 256: V 4 18.0 / 19.6, 8 24.9 / 21.0, 128 165 / 56.4
+  // The two kernels, V query rows per list (us of a replayed call, caches warm, V of 8 and less one
+  // row per sequence; kv4_attention_kernel in as many groups as it takes / kv4_rows_kernel; 8 KV
+  // heads, 2 of 256 channels):
+  //                                    V 4          V 5          V 8          V 16         V 128
+  //   64,  one sequence,  300 slots    6.2 / 6.6    6.4 / 6.6    6.5 / 6.6    8.6 / 8.8   13.9 / 11.3
+  //        one sequence, 20000        13.8 / 12.5  13.9 / 12.7  14.2 / 12.8  18.5 / 15.6  56.3 / 31.6
+  //        16 sequences,  4095        20.3 / 21.1  20.4 / 20.8  21.1 / 21.0  36.2 / 26.6   142 / 91.8
+  //   128, one sequence,  300          7.4 / 8.4    7.4 / 8.5    7.5 / 8.5   12.6 / 11.0  16.0 / 15.1
+  //        one sequence, 20000        16.2 / 15.5  18.1 / 15.5  18.4 / 15.8  30.9 / 18.8   139 / 46.2
+  //        16 sequences,  4095        24.4 / 27.6  39.1 / 27.8  39.8 / 28.1  71.1 / 34.0   333 / 135
+  //   256, one sequence,  300          9.5 / 14.6   9.5 / 14.9   9.6 / 15.0  11.9 / 18.1  21.4 / 18.5
+  //        one sequence, 20000        15.6 / 17.5  16.2 / 17.7  18.3 / 18.1  26.7 / 21.9   194 / 39.1
+  //        16 sequences,  4095        22.9 / 22.1  40.0 / 22.4  32.6 / 22.7  53.5 / 28.1   330 / 89.7
+  // The rule follows the batches, where there is most to win.  It costs a lone sequence of few slots
+  // up to 1 us at 128 channels and 6 at 256 from V = 5 on, and one of 20000 slots of 64 channels 1.3
+  // at V = 4.
   p.dense = p.V > 4;
   const int group = p.dense ? 16 : hps;
   p.nsub = p.dense && p.V > 16 && hd < 256 ? 2 : 1;

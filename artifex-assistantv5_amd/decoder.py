@@ -250,7 +250,9 @@ class QuantDecoder:
     ``kv_bits`` 4: ``kv_slots`` (default: enough for ``max_seq``) slots per KV head, rounded up
     to a multiple of 32; ``kv_keep``: a full cache is cut back to that many slots, of which the
     last ``kv_recent`` and the first ``kv_sinks`` positions are never given up.  ``max_seq``
-    then bounds the positions only."""
+    then bounds the positions only.  A prompt longer than the cache goes on, after the first
+    cut, in chunks of ``kv_slots - kv_keep`` tokens, each a pass of the model that reads the
+    kept rows back: a ``kv_keep`` near ``kv_slots`` suits short prompts only."""
 
     WINDOW = 32  # rows at a prompt's end whose attention weights are counted
 
@@ -501,7 +503,8 @@ class QuantDecoder:
         weights, SwiGLU runs as the down projection's prologue instead; with
         n_heads * head_dim above 8192 the attention merges its own records.  A 4-bit
         cache's attention writes its output (a second launch where the slots are
-        split), and eviction adds two launches per step."""
+        split), is NaN beforehand, and adds the length's limit or an eviction's two
+        launches to the step."""
         cfg, W = self.cfg, self.w
         x = self.b_x
         merge = cfg.n_heads * cfg.head_dim <= 8192 and self.kv_bits == 32

@@ -105,8 +105,8 @@ int gguf_hip_kv4_load(const void *kv, const int64_t *lengths, float *k_out, floa
 /* Eviction.  Every list (layer, sequence, KV head) of a sequence with
  * lengths[s] > keep and lengths[s] >= trigger is cut back to `keep` slots: those of
  * largest weight (of equal ones the lower slot; NaN counts least), where slots with
- * positions >= pos[s] - recent or < sinks come before all others (recent + sinks <=
- * keep).  A kept slot below `keep` stays where it is; the kept slots from `keep` on
+ * positions >= pos[s] - recent or < sinks come before all others, whatever their weights
+ * (recent + sinks <= keep).  A kept slot below `keep` stays where it is; the kept slots from `keep` on
  * move, in order, into the slots below it that were given up.  Slots from `keep` on
  * keep their bytes.  weights / positions [n_layers][n_seq][n_kv_heads][slots] of the
  * remaining slots go to weights_out / positions_out (the same arrays: in place), the
