@@ -106,10 +106,10 @@ int gguf_hip_kv4_load(const void *kv, const int64_t *lengths, float *k_out, floa
  * lengths[s] > keep and lengths[s] >= trigger is cut back to `keep` slots: those of
  * largest weight (of equal ones the lower slot; NaN counts least), where slots with
  * positions >= pos[s] - recent or < sinks come before all others, whatever their weights
- * (recent + sinks <= keep).  A kept slot below `keep` stays where it is; the kept slots from `keep` on
- * move, in order, into the slots below it that were given up.  Slots from `keep` on
- * keep their bytes.  weights / positions [n_layers][n_seq][n_kv_heads][slots] of the
- * remaining slots go to weights_out / positions_out (the same arrays: in place), the
+ * (recent + sinks <= keep).  A kept slot below `keep` stays where it is; the kept slots
+ * from `keep` on move, in order, into the slots below it that were given up.  Slots from
+ * `keep` on keep their bytes.  weights / positions [n_layers][n_seq][n_kv_heads][slots] of
+ * the remaining slots go to weights_out / positions_out (the same arrays: in place), the
  * new lengths to lengths_out (may be lengths).  Sequences that are not cut keep their
  * caches, weights, positions and lengths.  weights and positions are 16-byte aligned.
  * Two launches.  work: gguf_hip_kv4_evict_workspace bytes, 16-byte aligned, no initial
