@@ -228,3 +228,30 @@ def test_append_of_many_rows(kv4, heads, kv, hd, slots, lengths, starts, rows):
     assert np.array_equal(dev.cpu().numpy(), cache)
     assert np.array_equal(dp.cpu().numpy(), positions)
     assert np.array_equal(dw.cpu().numpy(), weights)
+
+
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+@pytest.mark.parametrize("heads,kv,hd,lengths,rows", [
+    (4, 1, 64, [700], 1), (8, 2, 128, [700, 31], 1), (4, 1, 256, [700], 1),
+    (8, 1, 64, [700], 3), (8, 1, 128, [0, 700], 4), (16, 2, 256, [700], 2)])
+def test_a_bad_query_is_its_own(kv4, heads, kv, hd, lengths, rows, what):
+    """A query of NaN or infinities leaves the other heads' and rows' outputs as near as they
+    were: only the order in which their maximum is raised may change."""
+    g = torch.Generator(device="cuda").manual_seed(hd + rows)
+    slots, seqs = 1024, len(lengths)
+    cache = _cache(g, lengths, kv, hd, slots)
+    cos, sin = (_cuda(t) for t in _tables(slots, hd))
+    qkv = torch.randn(seqs * rows, (heads + 2 * kv) * hd, device="cuda", generator=g)
+    bad = qkv.clone()
+    bad[rows - 1, hd:2 * hd] = what                  # head 1 of the first sequence's last row
+    outs = []
+    for x in (qkv, bad):
+        out = torch.empty(seqs * rows, heads * hd, device="cuda")
+        kv4.attention(x, _i64(lengths), _i64(lengths), cos, sin, cache, out, heads,
+                      kv4.attention_workspace(cache, heads, rows=rows))
+        outs.append(out.view(seqs * rows, heads, hd))
+    assert torch.isnan(outs[1][rows - 1, 1]).all()
+    for out in outs:
+        out[rows - 1, 1] = 0
+    assert torch.isfinite(outs[1]).all()
+    assert (outs[1] - outs[0]).norm() <= 2 * NORM * outs[0].norm()   # each within NORM of exact
