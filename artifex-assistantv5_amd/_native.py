@@ -80,6 +80,36 @@ KV4_SIGNATURES = {
     "gguf_hip_kv4_evict_workspace": (_i64, [_i32, _i32, _i32, _i32, _i64]),
 }
 
+# Every symbol include/gguf_hip_paged.h declares (the KV cache in pages)
+PAGED_F16, PAGED_BF16 = 1, 2
+PAGED_MAX_SEQS, PAGED_MAX_SLOTS, PAGED_MAX_PAGES = 4096, 1 << 22, 1 << 24
+PAGED_SIGNATURES = {
+    "gguf_hip_paged_bytes": (_i64, [_i64, _i32, _i32, _i32]),
+    "gguf_hip_paged_append": (_i32, [_fp, _i64, _i64, _vp, _vp, _vp, _vp, _fp, _fp, _i64, _vp, _i32,
+                                     _i64, _i32, _i64, _i32, _i32, _i32, _i32, _vp]),
+    "gguf_hip_paged_attention": (_i32, [_fp, _i64, _vp, _vp, _vp, _fp, _fp, _i64, _vp, _i32, _fp,
+                                        _i64, _i64, _i32, _i64, _i32, _i32, _i32, _i32, _vp, _i64,
+                                        _vp]),
+    "gguf_hip_paged_attention_workspace": (_i64, [_i32, _i64, _i32, _i32, _i32, _i32]),
+    "gguf_hip_paged_load": (_i32, [_vp, _i32, _vp, _vp, _fp, _fp, _i64, _i64, _i32, _i64, _i32,
+                                   _i32, _i32, _vp]),
+    "gguf_hip_paged_fork": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "gguf_hip_paged_grow": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i64, _i32, _i32,
+                                   _i32, _vp, _i64, _vp]),
+    "gguf_hip_paged_grow_workspace": (_i64, [_i64, _i32, _i64, _i32]),
+    "gguf_hip_paged_compact": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i64, _i32,
+                                      _i32, _i32, _vp, _i64, _vp]),
+    "gguf_hip_paged_compact_workspace": (_i64, [_i64, _i64, _i32]),
+}
+
+# Every symbol include/gguf_hip_sample.h declares
+SAMPLE_MAX_VOCAB, SAMPLE_MAX_ROWS = 1 << 20, 65535
+SAMPLE_SIGNATURES = {
+    "gguf_hip_sample": (_i32, [_fp, _i64, _i64, _i64, _fp, _fp, ctypes.c_float, _vp, ctypes.c_int32,
+                               _fp, ctypes.c_float, _fp, ctypes.c_float, _vp, _fp, _vp, _i64, _vp]),
+    "gguf_hip_sample_workspace": (_i64, [_i64, _i64]),
+}
+
 
 class GGUFHipError(RuntimeError):
     """A HIP runtime or launch failure reported by the library."""
@@ -118,7 +148,8 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
             f"{p} is not built; run `python artifex-assistantv5_amd/build.py` "
             "(the GGUF HIP path has no CPU fallback)")
     lib = ctypes.CDLL(p, mode=ctypes.RTLD_GLOBAL)
-    for name, (res, args) in {**SIGNATURES, **KV4_SIGNATURES}.items():
+    for name, (res, args) in {**SIGNATURES, **KV4_SIGNATURES, **PAGED_SIGNATURES,
+                                **SAMPLE_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -10,7 +10,10 @@
 
 #include "common.hpp"
 #include "gguf_hip_kv4.h"
+#include "gguf_hip_paged.h"
+#include "gguf_hip_sample.h"
 #include "kv4.hpp"
+#include "paged.hpp"
 
 namespace {
 
@@ -684,6 +687,317 @@ int gguf_hip_kv4_evict(void *kv, const float *weights, const int32_t *positions,
   const gguf::Kv4Evict e{keep,        trigger,       recent,      sinks, weights, positions,
                          weights_out, positions_out, lengths_out, work,  n_layers};
   return hip_status(gguf::launch_kv4_evict(c, e, (hipStream_t)stream), "kv4_evict launch");
+}
+
+// ---------------------------------------------------------------------------
+// The KV cache in pages (gguf_hip_paged.h).
+// ---------------------------------------------------------------------------
+namespace {
+
+int check_page(int page) {
+  if (page != 16 && page != 32 && page != 64 && page != 128 && page != 256)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: pages of %d slots, not 16, 32, 64, 128 or 256",
+                page);
+  return GGUF_HIP_OK;
+}
+int page_shift(int page) { return __builtin_ctz((unsigned)page); }
+
+int check_paged_pool(int64_t n_pages, int page, int n_kv_heads, int head_dim) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: head_dim %d not 64, 128 or 256", head_dim);
+  if (n_kv_heads <= 0 || n_kv_heads > 1024)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: %d KV heads not in 1..1024", n_kv_heads);
+  if (n_pages <= 0 || n_pages > GGUF_HIP_PAGED_MAX_PAGES)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: %lld pages not in 1..%d", (long long)n_pages,
+                GGUF_HIP_PAGED_MAX_PAGES);
+  return check_page(page);
+}
+
+int check_paged_tables(int64_t columns, int n_seq) {
+  if (n_seq <= 0 || n_seq > GGUF_HIP_PAGED_MAX_SEQS)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: %d sequences not in 1..%d", n_seq,
+                GGUF_HIP_PAGED_MAX_SEQS);
+  if (columns <= 0 || columns > GGUF_HIP_PAGED_MAX_SLOTS / 16)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: tables of %lld columns", (long long)columns);
+  return GGUF_HIP_OK;
+}
+
+int check_paged_slots(int page, int64_t columns, int n_seq, int n_kv_heads) {
+  const int rc = check_paged_tables(columns, n_seq);
+  if (rc) return rc;
+  if (columns > GGUF_HIP_PAGED_MAX_SLOTS / page)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: tables of %lld pages of %d slots (at most %d)",
+                (long long)columns, page, GGUF_HIP_PAGED_MAX_SLOTS);
+  if (n_seq > 65535 / n_kv_heads)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: %d sequences of %d KV heads (1..65535 lists)",
+                n_seq, n_kv_heads);
+  return GGUF_HIP_OK;
+}
+
+int check_paged_dtype(int dtype) {
+  if (dtype != GGUF_HIP_PAGED_F16 && dtype != GGUF_HIP_PAGED_BF16)
+    return fail(GGUF_HIP_ERR_DTYPE, "[gguf-hip] paged: pages must be f16 (1) or bf16 (2), got %d",
+                dtype);
+  return GGUF_HIP_OK;
+}
+
+int check_paged_rows(int n_heads, int n_kv_heads, int head_dim, int64_t ldqkv, int64_t rope_rows) {
+  if (n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 8)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: n_heads %d must be 1..8 times n_kv_heads %d",
+                n_heads, n_kv_heads);
+  const int64_t row = (int64_t)(n_heads + 2 * n_kv_heads) * head_dim;
+  if (ldqkv < row || ldqkv % 4)
+    return fail(GGUF_HIP_ERR_SHAPE,
+                "[gguf-hip] paged: ldqkv %lld must hold a row of %lld and be a multiple of 4",
+                (long long)ldqkv, (long long)row);
+  if (rope_rows <= 0 || rope_rows > ((int64_t)1 << 31) - 1)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: rope_rows %lld out of range",
+                (long long)rope_rows);
+  return GGUF_HIP_OK;
+}
+
+int misaligned_pages() { return fail(GGUF_HIP_ERR_ALIGN, "[gguf-hip] paged buffers misaligned"); }
+int null_pointer() { return fail(GGUF_HIP_ERR_NULL, "[gguf-hip] null pointer"); }
+
+// Whether an output that is not its input overlaps it.
+bool partly(const void *in, const void *out, int64_t bytes) {
+  const intptr_t d = (intptr_t)out - (intptr_t)in;
+  return d && d < bytes && d > -bytes;
+}
+int overlapping(const char *what) {
+  return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] %s: an output overlaps its input and is not the same", what);
+}
+
+int check_paged_work(const char *what, const void *work, int64_t work_bytes, int64_t need) {
+  if (!work) return null_pointer();
+  if (!aligned(work, 16)) return misaligned_pages();
+  if (work_bytes < need)
+    return fail(GGUF_HIP_ERR_BYTES, "[gguf-hip] %s: workspace of %lld bytes, needs %lld", what,
+                (long long)work_bytes, (long long)need);
+  return GGUF_HIP_OK;
+}
+
+}  // namespace
+
+int64_t gguf_hip_paged_bytes(int64_t n_pages, int page, int n_kv_heads, int head_dim) {
+  const int rc = check_paged_pool(n_pages, page, n_kv_heads, head_dim);
+  if (rc) return rc;
+  ok();
+  return n_pages * 4 * n_kv_heads * page * head_dim;
+}
+
+int gguf_hip_paged_append(const float *qkv, int64_t ldqkv, int64_t n_rows, const int64_t *starts,
+                          const int64_t *lengths, const int64_t *room, const int32_t *tables,
+                          const float *cos_table, const float *sin_table, int64_t rope_rows,
+                          void *kv, int dtype, int64_t n_pages, int page, int64_t columns,
+                          int n_seq, int n_heads, int n_kv_heads, int head_dim, void *stream) {
+  int rc = check_paged_pool(n_pages, page, n_kv_heads, head_dim);
+  if (!rc) rc = check_paged_slots(page, columns, n_seq, n_kv_heads);
+  if (!rc) rc = check_paged_dtype(dtype);
+  if (!rc) rc = check_paged_rows(n_heads, n_kv_heads, head_dim, ldqkv, rope_rows);
+  if (rc) return rc;
+  if (n_rows < 0 || n_rows > (int64_t)1 << 25)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged_append: %lld rows out of range",
+                (long long)n_rows);
+  if (!starts && n_rows % n_seq)
+    return fail(GGUF_HIP_ERR_SHAPE,
+                "[gguf-hip] paged_append: %lld rows are not the same number for each of %d sequences",
+                (long long)n_rows, n_seq);
+  if (n_rows == 0) return ok();
+  if (!qkv || !lengths || !tables || !cos_table || !sin_table || !kv) return null_pointer();
+  if (!aligned(qkv, 16) || !aligned(starts, 8) || !aligned(lengths, 8) || !aligned(room, 8) ||
+      !aligned(tables, 4) || !aligned(cos_table, 16) || !aligned(sin_table, 16) || !aligned(kv, 16))
+    return misaligned_pages();
+  const gguf::PagedCache c{(uint16_t *)kv, tables, lengths, room, cos_table, sin_table, rope_rows,
+                           (int)n_pages, page, page_shift(page), (int)columns, n_seq, n_heads,
+                           n_kv_heads, head_dim, dtype == GGUF_HIP_PAGED_BF16};
+  return hip_status(gguf::launch_paged_append(c, qkv, ldqkv, n_rows, starts, (hipStream_t)stream),
+                    "paged_append launch");
+}
+
+int64_t gguf_hip_paged_attention_workspace(int page, int64_t columns, int n_seq, int n_heads,
+                                           int n_kv_heads, int head_dim) {
+  int rc = check_paged_pool(1, page, n_kv_heads, head_dim);
+  if (!rc) rc = check_paged_slots(page, columns, n_seq, n_kv_heads);
+  if (!rc)
+    rc = check_paged_rows(n_heads, n_kv_heads, head_dim,
+                          (int64_t)(n_heads + 2 * (int64_t)n_kv_heads) * head_dim, 1);
+  if (rc) return rc;
+  ok();
+  return gguf::paged_attention_work_bytes(page, columns, n_seq, n_heads, n_kv_heads, head_dim);
+}
+
+int gguf_hip_paged_attention(const float *qkv, int64_t ldqkv, const int64_t *lengths,
+                             const int64_t *room, const int32_t *tables, const float *cos_table,
+                             const float *sin_table, int64_t rope_rows, void *kv, int dtype,
+                             float *out, int64_t ldo, int64_t n_pages, int page, int64_t columns,
+                             int n_seq, int n_heads, int n_kv_heads, int head_dim, void *work,
+                             int64_t work_bytes, void *stream) {
+  const int64_t need =
+      gguf_hip_paged_attention_workspace(page, columns, n_seq, n_heads, n_kv_heads, head_dim);
+  if (need < 0) return (int)need;
+  int rc = check_paged_pool(n_pages, page, n_kv_heads, head_dim);
+  if (!rc) rc = check_paged_dtype(dtype);
+  if (!rc) rc = check_paged_rows(n_heads, n_kv_heads, head_dim, ldqkv, rope_rows);
+  if (rc) return rc;
+  if (ldo < (int64_t)n_heads * head_dim || ldo % 4)
+    return fail(GGUF_HIP_ERR_SHAPE,
+                "[gguf-hip] paged_attention: ldo %lld must hold a row of %lld and be a multiple of 4",
+                (long long)ldo, (long long)n_heads * head_dim);
+  if (!qkv || !lengths || !tables || !cos_table || !sin_table || !kv || !out) return null_pointer();
+  if (!aligned(qkv, 16) || !aligned(lengths, 8) || !aligned(room, 8) || !aligned(tables, 4) ||
+      !aligned(cos_table, 16) || !aligned(sin_table, 16) || !aligned(kv, 16) || !aligned(out, 16))
+    return misaligned_pages();
+  if ((rc = check_paged_work("paged_attention", work, work_bytes, need))) return rc;
+  const gguf::PagedCache c{(uint16_t *)kv, tables, lengths, room, cos_table, sin_table, rope_rows,
+                           (int)n_pages, page, page_shift(page), (int)columns, n_seq, n_heads,
+                           n_kv_heads, head_dim, dtype == GGUF_HIP_PAGED_BF16};
+  const gguf::PagedAttn a{qkv, ldqkv, out, ldo, work};
+  return hip_status(gguf::launch_paged_attention(c, a, (hipStream_t)stream),
+                    "paged_attention launch");
+}
+
+int gguf_hip_paged_load(const void *kv, int dtype, const int32_t *tables, const int64_t *lengths,
+                        float *k_out, float *v_out, int64_t out_slots, int64_t n_pages, int page,
+                        int64_t columns, int n_seq, int n_kv_heads, int head_dim, void *stream) {
+  int rc = check_paged_pool(n_pages, page, n_kv_heads, head_dim);
+  if (!rc) rc = check_paged_slots(page, columns, n_seq, n_kv_heads);
+  if (!rc) rc = check_paged_dtype(dtype);
+  if (rc) return rc;
+  if (out_slots < 0)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged_load: out_slots %lld", (long long)out_slots);
+  if (out_slots == 0) return ok();
+  if (!kv || !tables || !lengths || !k_out || !v_out) return null_pointer();
+  if (!aligned(kv, 16) || !aligned(tables, 4) || !aligned(lengths, 8) || !aligned(k_out, 16) ||
+      !aligned(v_out, 16))
+    return misaligned_pages();
+  const gguf::PagedCache c{(uint16_t *)kv, tables, lengths, nullptr, nullptr, nullptr, 0,
+                           (int)n_pages, page, page_shift(page), (int)columns, n_seq, 0,
+                           n_kv_heads, head_dim, dtype == GGUF_HIP_PAGED_BF16};
+  return hip_status(gguf::launch_paged_load(c, k_out, v_out, out_slots, (hipStream_t)stream),
+                    "paged_load launch");
+}
+
+int gguf_hip_paged_fork(const int32_t *tables, const int64_t *lengths, const int32_t *refs,
+                        const int64_t *parents, int32_t *tables_out, int64_t *lengths_out,
+                        int32_t *refs_out, int64_t n_pages, int64_t columns, int n_seq,
+                        void *stream) {
+  int rc = check_paged_pool(n_pages, 16, 1, 64);
+  if (!rc) rc = check_paged_tables(columns, n_seq);
+  if (rc) return rc;
+  if (!tables || !lengths || !refs || !parents || !tables_out || !lengths_out || !refs_out)
+    return null_pointer();
+  if (!aligned(tables, 4) || !aligned(lengths, 8) || !aligned(refs, 4) || !aligned(parents, 8) ||
+      !aligned(tables_out, 4) || !aligned(lengths_out, 8) || !aligned(refs_out, 4))
+    return misaligned_pages();
+  if (partly(tables, tables_out, 4 * columns * n_seq) || partly(lengths, lengths_out, 8 * n_seq) ||
+      partly(refs, refs_out, 4 * n_pages))
+    return overlapping("paged_fork");
+  return hip_status(gguf::launch_paged_fork(tables, lengths, refs, parents, tables_out, lengths_out,
+                                            refs_out, (int)n_pages, (int)columns, n_seq,
+                                            (hipStream_t)stream),
+                    "paged_fork launch");
+}
+
+int64_t gguf_hip_paged_grow_workspace(int64_t n_pages, int page, int64_t columns, int n_seq) {
+  int rc = check_paged_pool(n_pages, page, 1, 64);
+  if (!rc) rc = check_paged_slots(page, columns, n_seq, 1);
+  if (rc) return rc;
+  ok();
+  return gguf::paged_grow_work_bytes(n_seq);
+}
+
+int gguf_hip_paged_grow(void *kv, int32_t *tables, const int64_t *lengths, int32_t *refs,
+                        const int64_t *rows, int64_t *room, int n_layers, int64_t n_pages,
+                        int page, int64_t columns, int n_seq, int n_kv_heads, int head_dim,
+                        void *work, int64_t work_bytes, void *stream) {
+  const int64_t need = gguf_hip_paged_grow_workspace(n_pages, page, columns, n_seq);
+  if (need < 0) return (int)need;
+  int rc = check_paged_pool(n_pages, page, n_kv_heads, head_dim);
+  if (rc) return rc;
+  if (n_layers <= 0 || n_layers > 65535)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: %d layers not in 1..65535", n_layers);
+  if (!kv || !tables || !lengths || !refs || !rows || !room) return null_pointer();
+  if (!aligned(kv, 16) || !aligned(tables, 4) || !aligned(lengths, 8) || !aligned(refs, 4) ||
+      !aligned(rows, 8) || !aligned(room, 8))
+    return misaligned_pages();
+  if ((rc = check_paged_work("paged_grow", work, work_bytes, need))) return rc;
+  const int64_t head = (int64_t)page * head_dim;
+  const gguf::PagedPool c{(uint16_t *)kv, n_layers, (int)n_pages, page, page_shift(page),
+                          (int)columns, n_seq, 2 * n_kv_heads * head, head};
+  return hip_status(gguf::launch_paged_grow(c, tables, lengths, refs, rows, room, work,
+                                            (hipStream_t)stream),
+                    "paged_grow launch");
+}
+
+int64_t gguf_hip_paged_compact_workspace(int64_t n_pages, int64_t columns, int n_seq) {
+  int rc = check_paged_pool(n_pages, 16, 1, 64);
+  if (!rc) rc = check_paged_tables(columns, n_seq);
+  if (rc) return rc;
+  ok();
+  return gguf::paged_compact_work_bytes(n_pages);
+}
+
+int gguf_hip_paged_compact(void *kv, const int32_t *tables, const int32_t *refs,
+                           int32_t *tables_out, int32_t *refs_out, int64_t *live, int n_layers,
+                           int64_t n_pages, int page, int64_t columns, int n_seq, int n_kv_heads,
+                           int head_dim, void *work, int64_t work_bytes, void *stream) {
+  const int64_t need = gguf_hip_paged_compact_workspace(n_pages, columns, n_seq);
+  if (need < 0) return (int)need;
+  int rc = check_paged_pool(n_pages, page, n_kv_heads, head_dim);
+  if (!rc) rc = check_paged_slots(page, columns, n_seq, 1);
+  if (rc) return rc;
+  if (n_layers <= 0 || n_layers > 65535)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: %d layers not in 1..65535", n_layers);
+  if (!kv || !tables || !refs || !tables_out || !refs_out || !live) return null_pointer();
+  if (!aligned(kv, 16) || !aligned(tables, 4) || !aligned(refs, 4) || !aligned(tables_out, 4) ||
+      !aligned(refs_out, 4) || !aligned(live, 8))
+    return misaligned_pages();
+  if (partly(tables, tables_out, 4 * columns * n_seq) || partly(refs, refs_out, 4 * n_pages))
+    return overlapping("paged_compact");
+  if ((rc = check_paged_work("paged_compact", work, work_bytes, need))) return rc;
+  const int64_t head = (int64_t)page * head_dim;
+  const gguf::PagedPool c{(uint16_t *)kv, n_layers, (int)n_pages, page, page_shift(page),
+                          (int)columns, n_seq, 2 * n_kv_heads * head, head};
+  return hip_status(gguf::launch_paged_compact(c, tables, refs, tables_out, refs_out, live, work,
+                                               (hipStream_t)stream),
+                    "paged_compact launch");
+}
+
+// ---------------------------------------------------------------------------
+// Sampling (gguf_hip_sample.h).
+// ---------------------------------------------------------------------------
+int64_t gguf_hip_sample_workspace(int64_t rows, int64_t vocab) {
+  if (rows < 0 || rows > GGUF_HIP_SAMPLE_MAX_ROWS)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] sample: %lld rows not in 0..%d", (long long)rows,
+                GGUF_HIP_SAMPLE_MAX_ROWS);
+  if (vocab <= 0 || vocab > GGUF_HIP_SAMPLE_MAX_VOCAB)
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] sample: vocabulary of %lld not in 1..%d",
+                (long long)vocab, GGUF_HIP_SAMPLE_MAX_VOCAB);
+  ok();
+  return gguf::sample_work_bytes(rows, vocab);
+}
+
+int gguf_hip_sample(const float *logits, int64_t ld, int64_t rows, int64_t vocab, const float *u,
+                    const float *temperature, float temperature_all, const int32_t *top_k,
+                    int32_t top_k_all, const float *top_p, float top_p_all, const float *min_p,
+                    float min_p_all, int64_t *out, float *probs, void *work, int64_t work_bytes,
+                    void *stream) {
+  const int64_t need = gguf_hip_sample_workspace(rows, vocab);
+  if (need < 0) return (int)need;
+  if (rows > 1 && ld < vocab) return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] sample: ld < vocab");
+  if (rows == 0) return ok();
+  if (!logits || !u || !out || !work) return null_pointer();
+  if (!aligned(logits, 4) || !aligned(u, 4) || !aligned(temperature, 4) || !aligned(top_k, 4) ||
+      !aligned(top_p, 4) || !aligned(min_p, 4) || !aligned(out, 8) || !aligned(probs, 4) ||
+      !aligned(work, 16))
+    return fail(GGUF_HIP_ERR_ALIGN, "[gguf-hip] sample buffers misaligned");
+  if (work_bytes < need)
+    return fail(GGUF_HIP_ERR_BYTES, "[gguf-hip] sample: workspace of %lld bytes, needs %lld",
+                (long long)work_bytes, (long long)need);
+  const gguf::SampleArgs a{logits, ld, (int)rows, (int)vocab, u, temperature, top_k, top_p, min_p,
+                           temperature_all, top_k_all, top_p_all, min_p_all, out, probs, work};
+  return hip_status(gguf::launch_sample(a, (hipStream_t)stream), "sample launch");
 }
 
 }  // extern "C"

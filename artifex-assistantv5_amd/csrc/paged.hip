@@ -1,0 +1,514 @@
+// The KV cache in pages: storing rows, reading them back, and the pages themselves (forks, room
+// for new rows, compaction).
+#include <type_traits>
+
+#include "paged.hpp"
+
+namespace gguf {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// ---------------------------------------------------------------------------
+// Storing rows: a wave takes one row and N units (K or V of a KV head, 256 / HD of them side by
+// side).
+// ---------------------------------------------------------------------------
+template <int HD, bool BF, int N>
+__global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c,
+                                                                const float *__restrict__ qkv,
+                                                                int64_t ldq, uint32_t n_rows,
+                                                                const int64_t *__restrict__ starts) {
+  constexpr int LANES = Kv4Row<HD>::LANES, SIDE = 64 / LANES;
+  const int lane = threadIdx.x & 63, q = lane % LANES;
+  const uint32_t r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  if (r >= n_rows) return;
+  // unit u: KV head u / 2, K or V; in qkv after the queries all of K, then all of V
+  const int u0 = blockIdx.y * N * SIDE + lane / LANES, units = 2 * c.nkv;
+  const float *x = qkv + r * ldq + (int64_t)c.nh * HD;
+  Kv4Row<HD> row[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {  // past the last unit: the last again, not stored
+    const int u = min(u0 + i * SIDE, units - 1);
+    row[i].load(x + (int64_t)((u & 1) * c.nkv + (u >> 1)) * HD, q);
+  }
+  uint32_t s;
+  int64_t i;  // the row of s
+  if (starts) {
+    if (r < starts[0] || r >= starts[c.n_seq]) return;
+    uint32_t lo = 0, hi = c.n_seq;  // starts[lo] <= r < starts[hi]
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if (starts[mid] <= r)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    s = lo;
+    // so far back that r lies behind every slot: and i need not fit 64 bits
+    if (starts[lo] < -((int64_t)c.columns << c.shift)) return;
+    i = r - starts[lo];
+  } else {
+    const uint32_t per = n_rows / (uint32_t)c.n_seq;
+    s = r / per;
+    i = r - s * per;
+  }
+  const int64_t n = c.lengths[s], end = paged_end(c, s);
+  if (n < 0 || n >= end - i) return;
+  const int slot = (int)(n + i);
+  const int32_t page = c.tables[(int64_t)s * c.columns + (slot >> c.shift)];
+  if ((uint32_t)page >= (uint32_t)c.n_pages) return;
+  row[0].load_turn(c.cs + (int64_t)slot * (HD / 2), c.sn + (int64_t)slot * (HD / 2), q);
+  const int j = slot & (c.page - 1);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int u = u0 + k * SIDE;
+    row[k].c = row[0].c;
+    row[k].s = row[0].s;
+    float y[4];
+    paged_turn<HD>(row[k], q, !(u & 1), y);
+    if (u >= units) continue;
+    const uint2 w = paged_round<BF>(y);
+    if (!(u & 1)) {
+      *(uint2 *)(c.kv + paged_k_at(c, page, u >> 1, j) + 4 * q) = w;
+    } else {
+      uint16_t *v = c.kv + paged_v_at(c, page, u >> 1, j) + 64 * q;
+      v[0] = (uint16_t)w.x;
+      v[16] = (uint16_t)(w.x >> 16);
+      v[32] = (uint16_t)w.y;
+      v[48] = (uint16_t)(w.y >> 16);
+    }
+  }
+}
+
+template <bool BF>
+__device__ __forceinline__ float paged_value(uint32_t bits16) {
+  if (BF) return __uint_as_float(bits16 << 16);
+  return (float)__builtin_bit_cast(half_t, (uint16_t)bits16);
+}
+
+// ---------------------------------------------------------------------------
+// Reading rows back: a workgroup per block of 16 slots of a KV head.
+// ---------------------------------------------------------------------------
+template <int HD, bool BF>
+__global__ __launch_bounds__(HD) void paged_load_kernel(PagedCache c, float *__restrict__ ko,
+                                                        float *__restrict__ vo, int64_t out_slots) {
+  const int64_t list = blockIdx.y, s = list / c.nkv;
+  const int h = (int)(list % c.nkv), t0 = blockIdx.x * kPageBlock, tid = threadIdx.x;
+  const int64_t n64 = c.lengths[s], n = n64 < out_slots ? n64 : out_slots;
+  if (t0 >= n) return;
+  const int32_t page = c.tables[s * c.columns + (t0 >> c.shift)];
+  if ((uint32_t)page >= (uint32_t)c.n_pages) return;
+  const int tn = (int)(n - t0 < kPageBlock ? n - t0 : kPageBlock), j0 = t0 & (c.page - 1);
+  const uint16_t *kr = c.kv + paged_k_at(c, page, h, j0);
+  float *ro = ko + (list * out_slots + t0) * HD;
+  for (int w = tid; w < 2 * HD; w += HD) {  // eight channels of a slot
+    if (w / (HD / 8) >= tn) break;
+    const uint4 x = *(const uint4 *)(kr + 8 * w);
+    float *o = ro + 8 * w;
+    const uint32_t q[4] = {x.x, x.y, x.z, x.w};
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = paged_value<BF>(q[i >> 1] >> (16 * (i & 1)) & 0xFFFFu);
+    __builtin_nontemporal_store(float4_t{y[0], y[1], y[2], y[3]}, (float4_t *)o);
+    __builtin_nontemporal_store(float4_t{y[4], y[5], y[6], y[7]}, (float4_t *)(o + 4));
+  }
+  // a channel's 16 slots per thread: what a wave writes of a slot is one run
+  const uint16_t *vr = c.kv + paged_v_at(c, page, h, j0) + 16 * tid;
+  const uint4 a = *(const uint4 *)vr, b = *(const uint4 *)(vr + 8);
+  const uint32_t q[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  float *o = vo + (list * out_slots + t0) * HD + tid;
+#pragma unroll
+  for (int j = 0; j < kPageBlock; ++j)
+    if (j < tn)
+      __builtin_nontemporal_store(paged_value<BF>(q[j >> 1] >> (16 * (j & 1)) & 0xFFFFu), o + j * HD);
+}
+
+// ---------------------------------------------------------------------------
+// Forks.  A workgroup takes `stripe` columns of every table: it reads all of them before it writes
+// any, so that the tables may be their own output.
+// ---------------------------------------------------------------------------
+constexpr int kForkThreads = 1024, kForkWords = 16384;
+
+__global__ __launch_bounds__(kForkThreads) void paged_copy_refs_kernel(
+    const int32_t *__restrict__ refs, int32_t *__restrict__ refs_out, int n_pages) {
+  const int i = blockIdx.x * kForkThreads + threadIdx.x;
+  if (i < n_pages) refs_out[i] = refs[i];
+}
+
+__global__ __launch_bounds__(kForkThreads) void paged_fork_kernel(
+    const int32_t *tables, const int64_t *lengths, const int32_t *refs, const int64_t *parents,
+    int32_t *tables_out, int64_t *lengths_out, int32_t *refs_out, int n_pages, int columns,
+    int n_seq, int stripe, bool copy_refs) {
+  __shared__ union {
+    int32_t old[kForkWords];
+    int64_t len[kForkWords / 2];
+  } sh;
+  const int tid = threadIdx.x;
+  if (copy_refs)  // one workgroup does all
+    for (int i = tid; i < n_pages; i += kForkThreads) refs_out[i] = refs[i];
+  for (int c0 = blockIdx.x * stripe; c0 < columns; c0 += gridDim.x * stripe) {
+    const int w = min(stripe, columns - c0), all = w * n_seq;
+    __syncthreads();
+    for (int i = tid; i < all; i += kForkThreads)
+      sh.old[i] = tables[(int64_t)(i / w) * columns + c0 + i % w];
+    __syncthreads();
+    for (int i = tid; i < all; i += kForkThreads) {
+      const int s = i / w, x = i % w;
+      const int64_t parent = parents[s];
+      const int32_t was = sh.old[i];
+      const int32_t now = parent >= 0 && parent < n_seq ? sh.old[(int)parent * w + x] : -1;
+      tables_out[(int64_t)s * columns + c0 + x] = now;
+      if (now == was) continue;
+      if ((uint32_t)was < (uint32_t)n_pages) atomicSub(&refs_out[was], 1);
+      if ((uint32_t)now < (uint32_t)n_pages) atomicAdd(&refs_out[now], 1);
+    }
+  }
+  if (blockIdx.x) return;
+  __syncthreads();
+  for (int s = tid; s < n_seq; s += kForkThreads) sh.len[s] = lengths[s];
+  __syncthreads();
+  for (int s = tid; s < n_seq; s += kForkThreads) {
+    const int64_t parent = parents[s];
+    lengths_out[s] = parent >= 0 && parent < n_seq ? sh.len[parent] : 0;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Room for new rows.  One workgroup walks the entries (sequence, column) in order, 1024 at a
+// time: what an entry needs follows from refs, which the entries before it have brought up to
+// date, and from the entries of its own turn that hold the same page.  The n-th need takes the
+// n-th free page.  A second launch copies the pages.
+// ---------------------------------------------------------------------------
+constexpr int kGrowThreads = 1024, kGrowWaves = kGrowThreads / 64;
+constexpr int kGrowSeqs = 4096;
+
+struct GrowJob {
+  int32_t src, dst, blocks, pad;
+};
+
+// The sum of v over the threads below this one, and over all of them.
+__device__ __forceinline__ int sum_before(int v, int *part, int &all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int run = lanes_before(v);
+  __syncthreads();
+  if (lane == 63) part[wave] = run;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kGrowWaves; ++w) {
+    before += w < wave ? part[w] : 0;
+    all += part[w];
+  }
+  return before + run - v;
+}
+
+// refs as the atomics of earlier turns left it (they act behind the first cache).
+__device__ __forceinline__ int32_t current(const int32_t *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__global__ __launch_bounds__(kGrowThreads) void paged_grow_kernel(PagedPool c, int32_t *tables,
+                                                                  const int64_t *lengths,
+                                                                  int32_t *refs,
+                                                                  const int64_t *rows,
+                                                                  int64_t *room, GrowJob *jobs) {
+  __shared__ int ends[kGrowSeqs];        // entries of the sequences up to this one
+  __shared__ int32_t held[kGrowThreads];  // the turn's pages that others hold too, -1: none
+  __shared__ int32_t free_[2 * kGrowThreads];
+  __shared__ int part[kGrowWaves];
+  const int tid = threadIdx.x;
+  const int64_t slots = (int64_t)c.columns << c.shift;
+  int total = 0;
+  for (int s0 = 0; s0 < c.n_seq; s0 += kGrowThreads) {
+    const int s = s0 + tid;
+    int count = 0;
+    if (s < c.n_seq) {
+      const int64_t n = lengths[s], m = rows[s];
+      int64_t to = n < 0 ? 0 : n;
+      if (n >= 0 && n < slots && m > 0) {
+        const int64_t last = m > slots - n ? slots - 1 : n + m - 1;
+        count = (int)((last >> c.shift) - (n >> c.shift)) + 1;
+        to = ((last >> c.shift) + 1) << c.shift;
+      }
+      room[s] = to;
+      jobs[s].blocks = 0;
+    }
+    int all;
+    const int before = sum_before(count, part, all);
+    if (s < c.n_seq) ends[s] = total + before + count;
+    total += all;
+  }
+  __syncthreads();
+  int at = 0, have = 0, used = 0;  // refs read up to `at`; free_[used .. have) are free
+  for (int e0 = 0; e0 < total; e0 += kGrowThreads) {
+    const int e = e0 + tid;
+    int s = 0, column = 0, refcount = 0;
+    int32_t p = -1;
+    bool first = false;
+    if (e < total) {
+      int lo = 0, hi = c.n_seq - 1;  // the first sequence with e < ends[s]
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (e < ends[mid])
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      s = lo;
+      const int k = e - (s ? ends[s - 1] : 0);
+      first = k == 0;
+      column = (int)(lengths[s] >> c.shift) + k;
+      p = tables[(int64_t)s * c.columns + column];
+      if ((uint32_t)p >= (uint32_t)c.n_pages)
+        p = -1;
+      else
+        refcount = current(&refs[p]);
+    }
+    __syncthreads();
+    held[tid] = refcount > 1 ? p : -1;
+    __syncthreads();
+    int earlier = 0;  // entries of this turn that leave the same page first
+    if (refcount > 1)
+      for (int j = 0; j < tid; ++j) earlier += held[j] == p;
+    const bool copies = refcount - earlier > 1;
+    const bool needs = e < total && (p < 0 || copies);
+    int wanted;
+    const int k = sum_before(needs, part, wanted);
+    // free pages for this turn, in order
+    if (have - used < wanted) {
+      __syncthreads();
+      int32_t keep = 0;
+      if (tid < have - used) keep = free_[used + tid];
+      __syncthreads();
+      if (tid < have - used) free_[tid] = keep;
+      have -= used;
+      used = 0;
+      while (have < wanted && at < c.n_pages) {
+        const int i = at + tid;
+        const bool is_free = i < c.n_pages && current(&refs[i]) <= 0;
+        int found;
+        const int rank = sum_before(is_free, part, found);
+        if (is_free) free_[have + rank] = i;
+        have += found;
+        at += kGrowThreads;
+      }
+      __syncthreads();
+    }
+    const int got = min(wanted, have - used);
+    // an entry that keeps its page since the others leave it: if they all could
+    const bool fails = (needs && k >= got) || (refcount > 1 && !copies && k > got);
+    if (fails) {
+      const int64_t n = lengths[s], start = (int64_t)column << c.shift;
+      atomicMin((long long *)&room[s], (long long)(start < n ? n : start));
+    } else if (needs) {
+      const int32_t f = free_[used + k];
+      tables[(int64_t)s * c.columns + column] = f;
+      refs[f] = 1;
+      if (copies) {
+        atomicSub(&refs[p], 1);
+        const int filled = (int)(lengths[s] & (c.page - 1));
+        if (first && filled) {
+          jobs[s].src = p;
+          jobs[s].dst = f;
+          jobs[s].blocks = (filled + kPageBlock - 1) / kPageBlock;
+        }
+      }
+    }
+    used += got;
+    __syncthreads();
+  }
+}
+
+// Block y of sequence x's copy, or all of them in turn, of layer z.
+__global__ __launch_bounds__(kThreads) void paged_grow_copy_kernel(PagedPool c,
+                                                                   const GrowJob *__restrict__ jobs,
+                                                                   int64_t head_values) {
+  const GrowJob j = jobs[blockIdx.x];
+  const int64_t layer = (int64_t)blockIdx.z * c.n_pages;
+  const uint4 *src = (const uint4 *)(c.kv + (layer + j.src) * c.page_values);
+  uint4 *dst = (uint4 *)(c.kv + (layer + j.dst) * c.page_values);
+  // of each KV head's K and V the first blocks: 16-byte units
+  const int per = (int)(head_values / 8), n = per / (c.page / kPageBlock) * j.blocks;
+  const int heads = (int)(c.page_values / head_values);
+  if (!n) return;
+  for (int h = blockIdx.y; h < heads; h += gridDim.y)
+    for (int i = threadIdx.x; i < n; i += kThreads) dst[h * per + i] = src[h * per + i];
+}
+
+// ---------------------------------------------------------------------------
+// Compaction: a workgroup finds the moves, the second launch makes them.
+// ---------------------------------------------------------------------------
+struct CompactWork {
+  int32_t *count, *to, *src, *dst;  // moves; where each page goes; the moves
+};
+__host__ __device__ __forceinline__ CompactWork compact_work(void *work, int n_pages) {
+  int32_t *w = (int32_t *)work;
+  const int64_t half = n_pages / 2 + 1;
+  return {w, w + 4, w + 4 + n_pages, w + 4 + n_pages + half};
+}
+
+__global__ __launch_bounds__(kGrowThreads) void paged_compact_plan_kernel(
+    PagedPool c, const int32_t *refs, int32_t *refs_out, int64_t *live, CompactWork w) {
+  __shared__ int part[kGrowWaves];
+  const int tid = threadIdx.x;
+  int mine = 0, n;
+  for (int i = tid; i < c.n_pages; i += kGrowThreads) mine += refs[i] > 0;
+  sum_before(mine, part, n);
+  int holes = 0, moves = 0;
+  for (int i0 = 0; i0 < c.n_pages; i0 += kGrowThreads) {
+    const int i = i0 + tid;
+    const int32_t r = i < c.n_pages ? refs[i] : 0;
+    const bool hole = i < n && r <= 0, move = i >= n && i < c.n_pages && r > 0;
+    int all;
+    const int k = sum_before(hole | move << 16, part, all);
+    if (hole) w.dst[holes + (k & 0xFFFF)] = i;
+    if (move) w.src[moves + (k >> 16)] = i;
+    holes += all & 0xFFFF;
+    moves += all >> 16;
+    if (i < c.n_pages) {
+      w.to[i] = i;
+      if (refs_out != refs) refs_out[i] = r;
+    }
+  }
+  __syncthreads();
+  for (int k = tid; k < moves; k += kGrowThreads) {
+    const int32_t from = w.src[k], to = w.dst[k], r = refs[from];
+    w.to[from] = to;
+    refs_out[to] = r;
+    refs_out[from] = 0;
+  }
+  if (tid == 0) {
+    *w.count = moves;
+    *live = n;
+  }
+}
+
+// The moves of layer y in 16 KB pieces, and the tables.
+__global__ __launch_bounds__(kThreads) void paged_compact_move_kernel(
+    PagedPool c, const int32_t *tables, int32_t *tables_out, CompactWork w) {
+  const int64_t entries = (int64_t)c.n_seq * c.columns;
+  const int64_t wgs = (int64_t)gridDim.x * gridDim.y, wg = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  for (int64_t i = wg * kThreads + threadIdx.x; i < entries; i += wgs * kThreads) {
+    const int32_t p = tables[i];
+    tables_out[i] = (uint32_t)p < (uint32_t)c.n_pages ? w.to[p] : p;
+  }
+  const int moves = *w.count;
+  const int64_t units = c.page_values / 8, layer = (int64_t)blockIdx.y * c.n_pages;
+  constexpr int U = 4, kPiece = U * kThreads;
+  const int pieces = (int)((units + kPiece - 1) / kPiece);
+  const uint4 *kv = (const uint4 *)c.kv;
+  for (int64_t x = blockIdx.x; x < (int64_t)moves * pieces; x += gridDim.x) {
+    const int m = (int)(x / pieces), at = (int)(x % pieces) * kPiece + threadIdx.x;
+    const uint4 *src = kv + (layer + w.src[m]) * units;
+    uint4 *dst = (uint4 *)kv + (layer + w.dst[m]) * units;
+    uint4 v[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (at + i * kThreads < units) v[i] = src[at + i * kThreads];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (at + i * kThreads < units) dst[at + i * kThreads] = v[i];
+  }
+}
+
+}  // namespace
+
+#define PAGED_DISPATCH(c, call)                     \
+  do {                                              \
+    auto with_type = [&](auto bf) {                 \
+      constexpr bool BF = decltype(bf)::value;      \
+      if (c.hd == 64) {                             \
+        constexpr int HD = 64;                      \
+        call;                                       \
+      } else if (c.hd == 128) {                     \
+        constexpr int HD = 128;                     \
+        call;                                       \
+      } else {                                      \
+        constexpr int HD = 256;                     \
+        call;                                       \
+      }                                             \
+    };                                              \
+    if (c.bf16)                                     \
+      with_type(std::true_type{});                  \
+    else                                            \
+      with_type(std::false_type{});                 \
+  } while (0)
+
+hipError_t launch_paged_append(const PagedCache &c, const float *qkv, int64_t ldq, int64_t n_rows,
+                               const int64_t *starts, hipStream_t s) {
+  // few rows: as many waves as there are units; many: fewer waves with more in flight
+  const int n = n_rows * c.nkv >= 8192 ? 4 : 1, per = n * (256 / c.hd);
+  const dim3 grid((unsigned)((n_rows + 3) / 4), (unsigned)((2 * c.nkv + per - 1) / per));
+  PAGED_DISPATCH(c, if (n == 4) hipLaunchKernelGGL((paged_append_kernel<HD, BF, 4>), grid,
+                                                   dim3(kThreads), 0, s, c, qkv, ldq,
+                                                   (uint32_t)n_rows, starts);
+                 else hipLaunchKernelGGL((paged_append_kernel<HD, BF, 1>), grid, dim3(kThreads), 0,
+                                         s, c, qkv, ldq, (uint32_t)n_rows, starts));
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_load(const PagedCache &c, float *k, float *v, int64_t out_slots,
+                             hipStream_t s) {
+  const int64_t slots = (int64_t)c.columns << c.shift, most = out_slots < slots ? out_slots : slots;
+  const dim3 grid((unsigned)((most + kPageBlock - 1) / kPageBlock), (unsigned)(c.n_seq * c.nkv));
+  PAGED_DISPATCH(c, hipLaunchKernelGGL((paged_load_kernel<HD, BF>), grid, dim3(HD), 0, s, c, k, v,
+                                       out_slots));
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_fork(const int32_t *tables, const int64_t *lengths, const int32_t *refs,
+                             const int64_t *parents, int32_t *tables_out, int64_t *lengths_out,
+                             int32_t *refs_out, int n_pages, int columns, int n_seq, hipStream_t s) {
+  const int most = kForkWords / n_seq;
+  const bool other = refs_out != refs;
+  const bool one = other && n_pages <= 8 * kForkThreads && columns <= 4 * most;
+  if (other && !one) {
+    hipLaunchKernelGGL(paged_copy_refs_kernel, dim3((n_pages + kForkThreads - 1) / kForkThreads),
+                       dim3(kForkThreads), 0, s, refs, refs_out, n_pages);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  int stripe = one ? most : (columns + 255) / 256;
+  stripe = stripe < 1 ? 1 : (stripe > most ? most : stripe);
+  const int wgs = one ? 1 : (columns + stripe - 1) / stripe;
+  hipLaunchKernelGGL(paged_fork_kernel, dim3(wgs < 4096 ? wgs : 4096), dim3(kForkThreads), 0, s,
+                     tables, lengths, refs, parents, tables_out, lengths_out, refs_out, n_pages,
+                     columns, n_seq, stripe, one);
+  return hipGetLastError();
+}
+
+int64_t paged_grow_work_bytes(int n_seq) { return (int64_t)n_seq * sizeof(GrowJob); }
+
+hipError_t launch_paged_grow(const PagedPool &c, int32_t *tables, const int64_t *lengths,
+                             int32_t *refs, const int64_t *rows, int64_t *room, void *work,
+                             hipStream_t s) {
+  GrowJob *jobs = (GrowJob *)work;
+  hipLaunchKernelGGL(paged_grow_kernel, dim3(1), dim3(kGrowThreads), 0, s, c, tables, lengths, refs,
+                     rows, room, jobs);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(paged_grow_copy_kernel, dim3(c.n_seq, 4, c.n_layers), dim3(kThreads), 0, s, c,
+                     jobs, c.head_values);
+  return hipGetLastError();
+}
+
+int64_t paged_compact_work_bytes(int64_t n_pages) { return 4 * (4 + n_pages + 2 * (n_pages / 2 + 1)); }
+
+hipError_t launch_paged_compact(const PagedPool &c, const int32_t *tables, const int32_t *refs,
+                                int32_t *tables_out, int32_t *refs_out, int64_t *live, void *work,
+                                hipStream_t s) {
+  const CompactWork w = compact_work(work, c.n_pages);
+  hipLaunchKernelGGL(paged_compact_plan_kernel, dim3(1), dim3(kGrowThreads), 0, s, c, refs, refs_out,
+                     live, w);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  int x = 2048 / c.n_layers;
+  x = x < 1 ? 1 : x;
+  hipLaunchKernelGGL(paged_compact_move_kernel, dim3(x, c.n_layers), dim3(kThreads), 0, s, c, tables,
+                     tables_out, w);
+  return hipGetLastError();
+}
+
+}  // namespace gguf

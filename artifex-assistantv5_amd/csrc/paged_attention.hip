@@ -1,0 +1,540 @@
+// Attention of one new row per sequence over the KV cache in pages.
+//
+// The slots of a (sequence, KV head) are split over workgroups; each writes, per query head, a
+// record of its partial softmax, and paged_merge_kernel joins them in split order (so the result
+// does not depend on timing).
+#include <type_traits>
+
+#include "paged.hpp"
+
+namespace gguf {
+
+namespace {
+
+constexpr int kUnit = 32;  // slots that a wave takes at a time
+
+// log2(e) / sqrt(head_dim) as two floats: one alone would be off by up to 2^-25, and that times
+// a score is the relative error of its probability.
+template <int HD>
+struct ScoreScale {
+  static constexpr double v = 1.4426950408889634074 / (HD == 64 ? 8.0 : (HD == 128 ? 11.313708498984760390 : 16.0));
+  static constexpr float hi = (float)v, lo = (float)(v - (double)hi);
+};
+
+// A record: sum of p v per channel, then the maximum m that its p are relative to (in log2 units)
+// and the sum of its p.
+template <int HD>
+constexpr int record_floats() {
+  return HD + 4;
+}
+
+// The slots in use before the call, or -1 if the sequence takes no part (or 0 .. if only the page
+// of its new row can tell).
+__device__ __forceinline__ int filled_of(const PagedCache &c, int64_t s) {
+  const int64_t n = steady(c.lengths + s);
+  return n < 0 || n >= paged_end(c, s) ? -1 : (int)n;
+}
+// The page of the new row, or -1.
+__device__ __forceinline__ int32_t page_of(const PagedCache &c, int64_t s, int slot) {
+  const int32_t p = steady(c.tables + s * c.columns + (slot >> c.shift));
+  return (uint32_t)p < (uint32_t)c.n_pages ? p : -1;
+}
+
+// How the units of a list are cut: `per` for each workgroup, `n` of them at most S.  Every workgroup
+// of the call gets about the same number, whatever the sequences' lengths: all lists' units over
+// `wgs` workgroups, in whole turns of a workgroup's W waves, and no fewer than eight.
+constexpr int kLeastUnits = 8;
+struct Cut {
+  int S, wgs, W;
+};
+struct Splits {
+  int per, n;
+};
+__device__ __forceinline__ int units_of(int filled) {
+  return filled < 0 ? 0 : filled / kUnit + 1;
+}
+__device__ __forceinline__ Splits splits_of(int units, int fair, const Cut &k) {
+  const int per = (max(max(fair, kLeastUnits), (units + k.S - 1) / k.S) + k.W - 1) / k.W * k.W;
+  return {per, (units + per - 1) / per};
+}
+// The fair share: a wave's lanes add the sequences.
+__device__ __forceinline__ int fair_share(const PagedCache &c, const Cut &k) {
+  int sum = 0;
+  if (c.n_seq == 1) {
+    sum = units_of(filled_of(c, 0));
+  } else {
+    for (int s = threadIdx.x & 63; s < c.n_seq; s += 64) sum += units_of(filled_of(c, s));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    sum = __builtin_amdgcn_readfirstlane(sum);
+  }
+  return (int)(((int64_t)sum * c.nkv + k.wgs - 1) / k.wgs);
+}
+// Workgroup `item` of the call: sequences in order, within one the splits in order, each for
+// every KV head.
+struct Item {
+  int s, kvh, split, filled;
+  Splits sp;
+};
+__device__ __forceinline__ bool item_of(const PagedCache &c, int item, const Cut &k, Item &it) {
+  const int fair = fair_share(c, k);
+  if (c.n_seq == 1) {
+    it.s = 0;
+    it.filled = filled_of(c, 0);
+    it.sp = splits_of(units_of(it.filled), fair, k);
+    it.split = item / c.nkv;
+    it.kvh = item - it.split * c.nkv;
+    return it.filled >= 0 && it.split < it.sp.n;
+  }
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
+    const int filled = s0 + lane < c.n_seq ? filled_of(c, s0 + lane) : -1;
+    const Splits sp = splits_of(units_of(filled), fair, k);
+    const int run = lanes_before(sp.n);
+    const uint64_t hit = __ballot(item < (before + run) * c.nkv);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      it.s = s0 + at;
+      it.filled = __builtin_amdgcn_readlane(filled, at);
+      it.sp.per = __builtin_amdgcn_readlane(sp.per, at);
+      it.sp.n = __builtin_amdgcn_readlane(sp.n, at);
+      const int first = before + __builtin_amdgcn_readlane(run, at) - it.sp.n;
+      it.split = (item - first * c.nkv) / c.nkv;
+      it.kvh = item - first * c.nkv - it.split * c.nkv;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(run, 63);
+  }
+  return false;
+}
+
+__device__ __forceinline__ float4_t mfma(uint4 a, uint4 b, float4_t c, std::false_type) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a),
+                                                __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float4_t mfma(uint4 a, uint4 b, float4_t c, std::true_type) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8_t, a),
+                                                 __builtin_bit_cast(bhalf8_t, b), c, 0, 0, 0);
+}
+
+// v plus that of the lane 8 to the left in its 16, cyclically.
+__device__ __forceinline__ float ror8(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, true));
+}
+
+// Eight values as a matrix operand's lane.  Column r of the matrix cores' 16 holds query head r % 8:
+// in columns 0 .. 7 the high parts, in 8 .. 15 the next ones.  f16: hi + lo in one operand, 22 bits;
+// bf16: hi + mid in the first, lo + nothing in the second, 24 bits.
+template <bool BF>
+struct Parts {
+  uint4 w[BF ? 2 : 1];
+  __device__ __forceinline__ void make(const float (&x)[8], bool low) {
+    if constexpr (!BF) {
+      half8_t h;
+      const float sel = low ? -1.f : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const half_t hi = (half_t)x[i];
+        h[i] = (half_t)fmaf((float)hi, sel, x[i]);
+      }
+      w[0] = __builtin_bit_cast(uint4, h);
+    } else {
+      bhalf8_t a, b;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bhalf_t hi = (bhalf_t)x[i];
+        const float rest = x[i] - (float)hi;
+        const bhalf_t mid = (bhalf_t)rest;
+        a[i] = low ? mid : hi;
+        b[i] = (bhalf_t)(low ? 0.f : rest - (float)mid);
+      }
+      w[0] = __builtin_bit_cast(uint4, a);
+      w[BF ? 1 : 0] = __builtin_bit_cast(uint4, b);
+    }
+  }
+};
+
+// A workgroup takes one list and one range of its units of 32 slots; its waves take the range's
+// units in turn and join at the end.  Nothing but registers carries a unit through:
+// - Scores: v_mfma_f32_16x16x32 with the slots' K rows as A and the queries as B, each head's parts
+//   in two columns (Parts), which a rotation within 16 lanes adds.  Row m of A's half t holds
+//   slot 8 (m / 4) + 4 t + m % 4, so that lane (r, g) = (lane % 16, lane / 16) of the accumulators
+//   has the scores of slots 8 g .. 8 g + 7.
+// - Output: that is the B layout of V . P^T, with V's channels as A, 16 bytes of a block's channel
+//   a lane; a lane's accumulators are of one head, and its p's scale is its own.
+// - p = 2^(score - m) with a running m, raised where a p would pass 2^15: to the largest score
+//   less 10, so that p's f16 parts keep 22 bits down to 2^-13 of the largest.
+// - K's registers take the next unit as soon as its scores are made, V's after its products.
+template <int HD, bool BF, int W, int WPS>
+__global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache c, PagedAttn a,
+                                                                      float *__restrict__ rec,
+                                                                      Cut cut) {
+  constexpr int NB = HD / 32, CT = HD / 16, RS = record_floats<HD>(), half = HD / 2;
+  constexpr int NP = BF ? 2 : 1;
+  constexpr std::bool_constant<BF> bf{};
+  constexpr float kLift = 10.f, kMost = 15.f;
+  __shared__ __align__(16) float o_[W][8][HD];  // per wave and head its sums
+  __shared__ float2 ml_[W][8];
+  __shared__ __align__(16) uint16_t fresh[2][HD];  // the new row's K and V
+  Item it;
+  if (!item_of(c, blockIdx.x, cut, it)) return;
+  it.s = __builtin_amdgcn_readfirstlane(it.s);  // all known uniform from here on
+  it.kvh = __builtin_amdgcn_readfirstlane(it.kvh);
+  it.split = __builtin_amdgcn_readfirstlane(it.split);
+  it.filled = __builtin_amdgcn_readfirstlane(it.filled);
+  it.sp.per = __builtin_amdgcn_readfirstlane(it.sp.per);
+  it.sp.n = __builtin_amdgcn_readfirstlane(it.sp.n);
+  const int64_t s = it.s;
+  const int kvh = it.kvh, grp = c.nh / c.nkv, filled = it.filled;
+  const Splits sp = it.sp;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t *table = c.tables + s * c.columns;
+  const int32_t own_page = page_of(c, s, filled);
+  if (own_page < 0) return;
+  const int unit0 = it.split * sp.per, unit1 = min(unit0 + sp.per, units_of(filled));
+  const bool stores = filled / kUnit < unit1;  // the last range has the new row
+  const float *row = a.qkv + s * a.ldq;
+
+  // the two pages of a unit's blocks, and where their lists begin
+  const int to_block = c.shift - 4, in_page = (c.page >> 4) - 1;
+  auto ids = [&](int unit, int &p0, int &p1) {
+    const int b0 = 2 * unit, b1 = b0 + 1;
+    p0 = steady(table + min(b0 >> to_block, c.columns - 1));
+    p1 = steady(table + min(b1 >> to_block, c.columns - 1));
+  };
+  auto known = [&](int p) { return (uint32_t)p < (uint32_t)c.n_pages; };
+  const int64_t page_values = (int64_t)2 * c.nkv * c.page * HD;
+  const int row_in = 8 * ((r >> 2) & 1) + (r & 3);  // of K's half t: + 4 t
+  const int list_k = kvh * c.page * HD, list_v = (c.nkv + kvh) * c.page * HD;
+  uint4 kf[2][NB], vf[CT];
+  auto load_k = [&](int unit, int p0, int p1) {
+    const int b = 2 * unit + (r >> 3);
+    const int64_t p = r >> 3 ? (known(p1) ? p1 : 0) : (known(p0) ? p0 : 0);
+    const uint16_t *k = c.kv + p * page_values + (list_k + ((b & in_page) * 16 + row_in) * HD + 8 * g);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < NB; ++i) kf[t][i] = *(const uint4 *)(k + 4 * t * HD + 32 * i);
+  };
+  auto load_v = [&](int unit, int p0, int p1) {
+    const int b = 2 * unit + (g >> 1);
+    const int64_t p = g >> 1 ? (known(p1) ? p1 : 0) : (known(p0) ? p0 : 0);
+    const uint16_t *v =
+        c.kv + p * page_values + (list_v + (b & in_page) * 16 * HD + 16 * r + 8 * (g & 1));
+#pragma unroll
+    for (int i = 0; i < CT; ++i) vf[i] = *(const uint4 *)(v + 256 * i);
+  };
+
+  // the queries: lane (r, g) channels 32 i + 8 g + 0 .. 7 of head r % 8, whose RoPE partners are the
+  // same lane's of block i +- NB / 2
+  Parts<BF> qf[NB];
+  float f;  // log2 units per unit of an accumulated score
+  {
+    const int h = r & 7;
+    const float *x = row + (int64_t)(kvh * grp + (h < grp ? h : 0)) * HD + 8 * g;
+    const float *cr = c.cs + (int64_t)filled * half + 8 * g, *sr = c.sn + (int64_t)filled * half + 8 * g;
+    float y[NB][8], mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < NB / 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x1 = x[32 * i + j], x2 = x[32 * i + half + j], cv = cr[32 * i + j], sv = sr[32 * i + j];
+        const float a1 = h < grp ? x1 * cv - x2 * sv : 0.f, a2 = h < grp ? x2 * cv + x1 * sv : 0.f;
+        y[i][j] = fmaf(a1, ScoreScale<HD>::hi, a1 * ScoreScale<HD>::lo);
+        y[i + NB / 2][j] = fmaf(a2, ScoreScale<HD>::hi, a2 * ScoreScale<HD>::lo);
+        mx = fmaxf(mx, fmaxf(fabsf(y[i][j]), fabsf(y[i + NB / 2][j])));
+      }
+    mx = max_xor32(max_xor16(mx));
+    const int e = BF ? 0 : stage_exp(mx);
+    const float up = pow2f(e);
+    f = pow2f(-e);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[i][j] *= up;
+      qf[i].make(y[i], r >= 8);
+    }
+  }
+  // the new row, by the first wave: to its page, and to the workgroup
+  if (stores && wave == 0) {
+    constexpr int LANES = Kv4Row<HD>::LANES, SIDE = 64 / LANES, N = (2 + SIDE - 1) / SIDE;
+    const int q = lane % LANES, j = filled & (c.page - 1);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int u = min(n * SIDE + lane / LANES, 1);
+      Kv4Row<HD> x;
+      x.load(row + (int64_t)(c.nh + u * c.nkv + kvh) * HD, q);
+      x.load_turn(c.cs + (int64_t)filled * half, c.sn + (int64_t)filled * half, q);
+      float y[4];
+      paged_turn<HD>(x, q, u == 0, y);
+      const uint2 w = paged_round<BF>(y);
+      if (n * SIDE + lane / LANES < 2) {
+        *(uint2 *)(fresh[u] + 4 * q) = w;
+        if (u == 0) {
+          *(uint2 *)(c.kv + paged_k_at(c, own_page, kvh, j) + 4 * q) = w;
+        } else {
+          uint16_t *v = c.kv + paged_v_at(c, own_page, kvh, j) + 64 * q;
+          v[0] = (uint16_t)w.x;
+          v[16] = (uint16_t)(w.x >> 16);
+          v[32] = (uint16_t)w.y;
+          v[48] = (uint16_t)(w.y >> 16);
+        }
+      }
+    }
+  }
+  // from the last unit down: the new row's is some wave's first
+  int unit = unit1 - 1 - wave, p0 = 0, p1 = 0, n0 = 0, n1 = 0;
+  if (unit >= unit0) {
+    ids(unit, p0, p1);
+    load_k(unit, p0, p1);
+    load_v(unit, p0, p1);
+    ids(max(unit - W, unit0), n0, n1);
+  }
+  __syncthreads();
+  if (stores && unit == filled / kUnit) {
+    const int j = filled % kUnit, in = j & 15;
+    if (j >> 4 == r >> 3) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (in == row_in + 4 * t)
+#pragma unroll
+          for (int i = 0; i < NB; ++i) kf[t][i] = *(const uint4 *)(fresh[0] + 32 * i + 8 * g);
+    }
+    if (j >> 3 == g) {
+      const int e = j & 7, sh = 16 * (e & 1);
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        const uint32_t x = (uint32_t)fresh[1][16 * i + r] << sh, keep = ~(0xFFFFu << sh);
+        if (e < 2) vf[i].x = (vf[i].x & keep) | x;
+        else if (e < 4) vf[i].y = (vf[i].y & keep) | x;
+        else if (e < 6) vf[i].z = (vf[i].z & keep) | x;
+        else vf[i].w = (vf[i].w & keep) | x;
+      }
+    }
+  }
+
+  float4_t acc[CT];
+  float m = -INFINITY, l = 0.f;  // p = 2^(score - m)
+#pragma unroll
+  for (int i = 0; i < CT; ++i) acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+  for (; unit >= unit0; unit -= W) {
+    float y[8];
+    {
+      float4_t sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int k = NP - 1; k >= 0; --k) {
+          sc[0] = mfma(kf[0][i], qf[i].w[k], sc[0], bf);
+          sc[1] = mfma(kf[1][i], qf[i].w[k], sc[1], bf);
+        }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = sc[j >> 2][j & 3];
+        y[j] = x + ror8(x);
+      }
+    }
+    const int next = max(unit - W, unit0);  // the last one: unused
+    load_k(next, n0, n1);
+    // slots that are not seen: past the new row, or without a page
+    const bool masked = (unit + 1) * kUnit > filled + 1 || !known(p0) || !known(p1);
+    const int seen = known(g >> 1 ? p1 : p0) ? filled + 1 - (unit * kUnit + 8 * g) : 0;  // of the lane's
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {  // whatever they hold must not meet a p of zero
+        uint32_t x[4] = {vf[i].x, vf[i].y, vf[i].z, vf[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          x[k] = seen >= 2 * k + 2 ? x[k] : (seen == 2 * k + 1 ? x[k] & 0xFFFFu : 0u);
+        vf[i] = make_uint4(x[0], x[1], x[2], x[3]);
+      }
+    }
+    float p[8], sum;
+    auto weigh = [&]() {
+      bool over = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float t = fmaf(y[j], f, -m);
+        if (masked && j >= seen) t = -INFINITY;
+        over |= !(t <= kMost);
+        p[j] = __builtin_amdgcn_exp2f(t);
+      }
+      sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      return over;
+    };
+    if (__any(weigh())) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (!masked || j < seen) top = fmaxf(top, y[j] * f);
+      top = max_xor32(max_xor16(top)) - kLift;
+      const float n = fmaxf(m, top);
+      const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - n);
+      if (n != -INFINITY) {  // else nothing has been seen yet
+        m = n;
+        l *= al;
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[i][k] *= al;
+      }
+      weigh();
+    }
+    l += sum;
+    Parts<BF> pf;
+    pf.make(p, r >= 8);
+#pragma unroll
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+      for (int k = NP - 1; k >= 0; --k) acc[i] = mfma(vf[i], pf.w[k], acc[i], bf);
+    load_v(next, n0, n1);
+    p0 = n0;
+    p1 = n1;
+    ids(max(next - W, unit0), n0, n1);
+  }
+
+  // the waves' sums: lane (r, g), register k of i: channel 16 i + 4 g + k, head r % 8
+  const float ls = sum_xor32(sum_xor16(l));
+  if (g == 0 && r < 8) ml_[wave][r] = make_float2(m, ls);
+#pragma unroll
+  for (int i = 0; i < CT; ++i) {
+    float4_t x = acc[i];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] += ror8(x[k]);
+    if (r < grp) *(float4_t *)&o_[wave][r][16 * i + 4 * g] = x;
+  }
+  __syncthreads();
+  for (int e = tid; e < grp * (HD / 4); e += 64 * W) {
+    const int h = e / (HD / 4), ch = e % (HD / 4) * 4;
+    float mx = ml_[0][h].x, sum = 0.f;
+    float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 1; k < W; ++k) mx = fmaxf(mx, ml_[k][h].x);
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const float2 ml = ml_[k][h];
+      const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
+      const float4_t x = *(const float4_t *)&o_[k][h][ch];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) o[n] = fmaf(w, x[n], o[n]);
+      sum = fmaf(w, ml.y, sum);
+    }
+    if (sp.n == 1) {  // nothing to join
+      float *to = a.out + s * a.ldo + (int64_t)(kvh * grp + h) * HD + ch;
+      *(float4 *)to = make_float4(o[0] / sum, o[1] / sum, o[2] / sum, o[3] / sum);
+    } else {
+      float *to = rec + (((s * c.nkv + kvh) * cut.S + it.split) * grp + h) * RS;
+      *(float4_t *)(to + ch) = o;
+      if (ch == 0) *(float2 *)(to + HD) = make_float2(mx, sum);
+    }
+  }
+}
+
+// One workgroup per query head of a list with several splits: their records joined, G groups of
+// HD / 4 threads taking every G-th record, then the groups in order.
+template <int HD>
+constexpr int kMergeThreads = HD < 128 ? 256 : 2 * HD;
+template <int HD>
+__global__ __launch_bounds__(kMergeThreads<HD>) void paged_merge_kernel(PagedCache c, PagedAttn a,
+                                                                        const float *__restrict__ rec,
+                                                                        Cut cut) {
+  constexpr int RS = record_floats<HD>(), Q = HD / 4, G = kMergeThreads<HD> / Q;
+  __shared__ float4 o_[G][Q];
+  __shared__ float2 ml_[G][Q];
+  const int64_t list = blockIdx.y, s = list / c.nkv;
+  const int h = blockIdx.x, grp = c.nh / c.nkv;
+  const int q = threadIdx.x % Q, gi = threadIdx.x / Q;
+  const int filled = filled_of(c, s);
+  if (filled < 0 || page_of(c, s, filled) < 0) return;
+  const Splits sp = splits_of(units_of(filled), fair_share(c, cut), cut);
+  if (sp.n == 1) return;
+  const float *r = rec + (list * cut.S * grp + h) * RS;
+  const int64_t step = (int64_t)grp * RS;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto join = [&](float2 ml, float4 x) {
+    const float n = fmaxf(m, ml.x);
+    const float wo = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - n);
+    const float wn = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - n);
+    m = n;
+    l = l * wo + ml.y * wn;
+    o.x = o.x * wo + x.x * wn;
+    o.y = o.y * wo + x.y * wn;
+    o.z = o.z * wo + x.z * wn;
+    o.w = o.w * wo + x.w * wn;
+  };
+  for (int k0 = gi; k0 < sp.n; k0 += 4 * G) {
+    float2 ml[4];
+    float4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // past the last: the last again, unused
+      const float *rk = r + (int64_t)min(k0 + j * G, sp.n - 1) * step;
+      ml[j] = *(const float2 *)(rk + HD);
+      x[j] = *(const float4 *)(rk + 4 * q);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (k0 + j * G < sp.n) join(ml[j], x[j]);
+  }
+  o_[gi][q] = o;
+  ml_[gi][q] = make_float2(m, l);
+  __syncthreads();
+  if (gi > 0) return;
+  for (int k = 1; k < G; ++k) join(ml_[k][q], o_[k][q]);
+  *(float4 *)(a.out + s * a.ldo + (int64_t)(list % c.nkv * grp + h) * HD + 4 * q) =
+      make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
+}
+
+// How a call is cut: W waves per workgroup, `wgs` workgroups at a time on the GPU, a list in S of
+// them at most.
+struct Plan {
+  Cut cut;
+  int64_t lists;
+};
+Plan plan(int page, int64_t columns, int n_seq, int nkv, int hd) {
+  Plan p;
+  p.lists = (int64_t)n_seq * nkv;
+  p.cut.W = 4;
+  p.cut.wgs = hd == 256 ? 512 : 768;
+  // a list of two turns is not cut: one launch, and nothing to join
+  const int64_t units = (columns * page + kUnit - 1) / kUnit;
+  const int64_t most = units <= 2 * p.cut.W ? 1 : (units + kLeastUnits - 1) / kLeastUnits;
+  // sequences of different lengths: up to four times the workgroups that equal ones would take
+  const int64_t want = (4 * p.cut.wgs + p.lists - 1) / p.lists;
+  p.cut.S = (int)(want < most ? want : most);
+  return p;
+}
+
+template <int HD, bool BF>
+hipError_t launch(const PagedCache &c, const PagedAttn &a, hipStream_t s) {
+  const Plan p = plan(c.page, c.columns, c.n_seq, c.nkv, HD);
+  float *rec = (float *)a.work;
+  // No call has more items than wgs + lists (every list but for its last workgroup gets whole
+  // shares).
+  const int64_t most = p.lists * p.cut.S, items = most < p.cut.wgs + p.lists ? most : p.cut.wgs + p.lists;
+  const dim3 grid((unsigned)items), block(64 * p.cut.W);
+  hipLaunchKernelGGL((paged_attention_kernel<HD, BF, 4, HD == 256 ? 2 : 3>), grid, block, 0, s, c, a,
+                     rec, p.cut);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.cut.S == 1) return e;
+  hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3((unsigned)(c.nh / c.nkv), (unsigned)p.lists),
+                     dim3(kMergeThreads<HD>), 0, s, c, a, rec, p.cut);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t paged_attention_work_bytes(int page, int64_t columns, int n_seq, int nh, int nkv, int hd) {
+  const Plan p = plan(page, columns, n_seq, nkv, hd);
+  return (p.cut.S > 1 ? p.lists * p.cut.S * (nh / nkv) * (int64_t)(hd + 4) * 4 : 0) + 16;
+}
+
+hipError_t launch_paged_attention(const PagedCache &c, const PagedAttn &a, hipStream_t s) {
+  if (c.hd == 64) return c.bf16 ? launch<64, true>(c, a, s) : launch<64, false>(c, a, s);
+  if (c.hd == 128) return c.bf16 ? launch<128, true>(c, a, s) : launch<128, false>(c, a, s);
+  return c.bf16 ? launch<256, true>(c, a, s) : launch<256, false>(c, a, s);
+}
+
+}  // namespace gguf
