@@ -39,10 +39,10 @@ __device__ __forceinline__ int64_t paged_end(const PagedCache &c, int64_t s) {
 // 16-bit values from the start of page p to those of KV head h, slot j: its K row, and its V (channel
 // e at + e * 16).
 __device__ __forceinline__ int64_t paged_k_at(const PagedCache &c, int64_t p, int h, int j) {
-  return ((p * 2 * c.nkv + h << c.shift) + j) * c.hd;
+  return (((p * 2 * c.nkv + h) << c.shift) + j) * c.hd;
 }
 __device__ __forceinline__ int64_t paged_v_at(const PagedCache &c, int64_t p, int h, int j) {
-  return ((p * 2 + 1) * c.nkv + h << c.shift) * c.hd + (int64_t)(j >> 4) * (16 * c.hd) + (j & 15);
+  return (((p * 2 + 1) * c.nkv + h) << c.shift) * c.hd + (int64_t)(j >> 4) * (16 * c.hd) + (j & 15);
 }
 
 // Four channels rounded to a page's type, to nearest.
