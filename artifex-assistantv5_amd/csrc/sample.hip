@@ -14,11 +14,13 @@ namespace gguf {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kBins = 512;    // the last one holds the tokens of weight 0
+constexpr int kBins = 512;     // the last one holds the tokens of weight 0
 constexpr int kSorted = 4096;  // tokens that a workgroup puts in order
+constexpr int kRanked = 256;   // up to so many by counting, for each, those before it
+constexpr int kFewest = 512;   // a top_k of up to so many needs no bins' masses
 constexpr int kChunks = 64;
-constexpr double kOne = 0x1p43;  // a weight of 1
-constexpr double kNothing = 44.5;  // 2^-kNothing of it rounds to 0
+constexpr double kOne = 0x1p43;     // a weight of 1
+constexpr double kNothing = -44.0;  // the exponent from which on a weight is 0
 
 // Larger is drawn earlier; -0 is +0, NaN and -inf are 0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -72,45 +74,81 @@ __device__ __forceinline__ uint64_t mass_of(const Row &r, uint32_t key) {
   return fixed(weight(exponent(r, key)));
 }
 
+// Sums and maxima over lanes by DPP shifts within rows of 16, then the rows' ends.  A lane without a
+// source gets zero, which neither adds nor is larger.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T shifted(T v) {
+  if constexpr (sizeof(T) == 8) {
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
+    return (T)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+  } else {
+    return (T)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+  }
+}
+template <typename T>
+__device__ __forceinline__ T of_lane(T v, int lane) {
+  if constexpr (sizeof(T) == 8) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (T)((uint64_t)hi << 32 | lo);
+  } else {
+    return (T)__builtin_amdgcn_readlane((int)v, lane);
+  }
+}
+template <typename T>
+__device__ __forceinline__ T row_sums(T v) {
+  v += shifted<0x111, 0xF>(v);
+  v += shifted<0x112, 0xF>(v);
+  v += shifted<0x114, 0xF>(v);
+  return v + shifted<0x118, 0xF>(v);
+}
+// v and those of the lanes below
+template <typename T>
+__device__ __forceinline__ T wave_sums(T v) {
+  v = row_sums(v);
+  v += shifted<0x142, 0xA>(v);  // lane 15 to row 1, 47 to row 3
+  return v + shifted<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
+}
 template <typename T>
 __device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+  return of_lane(wave_sums(v), 63);
 }
 template <typename T>
 __device__ __forceinline__ T wave_max(T v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const T w = __shfl_xor(v, o);
-    v = w > v ? w : v;
-  }
-  return v;
+  auto larger = [](T x, T y) { return x > y ? x : y; };
+  v = larger(v, shifted<0x111, 0xF>(v));
+  v = larger(v, shifted<0x112, 0xF>(v));
+  v = larger(v, shifted<0x114, 0xF>(v));
+  v = larger(v, shifted<0x118, 0xF>(v));
+  v = larger(v, shifted<0x142, 0xA>(v));
+  v = larger(v, shifted<0x143, 0xC>(v));
+  return of_lane(v, 63);
 }
 // v and those of the threads below; `part` holds a value per wave.
 template <typename T>
 __device__ __forceinline__ T block_scan(T v, T *part) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T w = __shfl_up(v, o);
-    if (lane >= o) v += w;
-  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  v = wave_sums(v);
   __syncthreads();
   if (lane == 63) part[wave] = v;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves - 1; ++w) v += w < wave ? part[w] : 0;
-  return v;
+  static_assert(kWaves == 16);
+  const T before = row_sums(part[lane & 15]);
+  return wave ? v + of_lane(before, wave - 1) : v;
 }
 
 // The workspace: per row and chunk the place of its first token and the inverse of its smallest
-// key; the ends of its bins; their masses; the mass that min_p keeps; its tokens in the order of
-// the bins (indices within the chunk).
+// key; the mass that min_p keeps; its bins; its tokens in their order (indices within the chunk).
+struct Bin {
+  uint64_t mass;
+  uint32_t count, end;  // of the chunk's tokens in the order of the bins
+};
 struct Work {
-  uint64_t *first, *mass, *large;
+  uint64_t *first, *large;
+  Bin *bin;
   uint32_t *least;
-  uint16_t *ends, *order;
+  uint16_t *order;
 };
 struct Cut {
   int chunk, chunks;  // tokens of a chunk, chunks of a row
@@ -134,9 +172,8 @@ int64_t place_work(char *base, int64_t rows, const Cut &c, Work &w) {
   };
   w.first = (uint64_t *)take(lists * 8);
   w.large = (uint64_t *)take(lists * 8);
-  w.mass = (uint64_t *)take(lists * kBins * 8);
+  w.bin = (Bin *)take(lists * kBins * sizeof(Bin));
   w.least = (uint32_t *)take(lists * 4);
-  w.ends = (uint16_t *)take(lists * kBins * 2);
   w.order = (uint16_t *)take(lists * c.chunk * 2);
   return p - base;
 }
@@ -180,36 +217,49 @@ struct Bins {
 };
 __device__ __forceinline__ Bins bins_of(const SampleArgs &a, const Work &w, int row, int chunks) {
   const int lane = threadIdx.x & 63;
-  const int64_t list = (int64_t)row * chunks + lane;
+  const int64_t list = (int64_t)row * chunks + min(lane, chunks - 1);
   Bins b;
-  b.first = wave_max(lane < chunks ? w.first[list] : (uint64_t)0);
-  const uint32_t least = wave_max(lane < chunks ? w.least[list] : 0u);
-  b.t = a.temperature ? a.temperature[row] : a.temperature_all;
+  b.t = a.temperature ? steady(a.temperature + row) : a.temperature_all;
+  b.first = wave_max(w.first[list]);
+  const uint32_t least = wave_max(w.least[list]);
   b.r.scale = 1.4426950408889634074 / (double)b.t;
   b.r.top = key_value((uint32_t)(b.first >> 32));
-  double range = -exponent(b.r, ~least);
-  range = range < kNothing ? range : kNothing;
+  const double range = fmin(-exponent(b.r, ~least), -kNothing);
   b.per = range > 0.0 ? (kBins - 1) / range : 0.0;
   return b;
 }
-__device__ __forceinline__ int bin_of(const Bins &b, double e, uint64_t mass) {
-  if (!mass) return kBins - 1;
+__device__ __forceinline__ int bin_of(const Bins &b, double e) {
+  if (!(e > kNothing)) return kBins - 1;
   const int k = (int)(-e * b.per);
   return k < kBins - 2 ? k : kBins - 2;
 }
+// Where the first top_k tokens are all that counts, their masses are taken from them alone.
+__device__ __forceinline__ bool few(int32_t top_k) { return top_k > 0 && top_k <= kFewest; }
 
 template <int T>
-__global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Work w, int chunks) {
+__global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a, Work w, int chunks) {
   __shared__ uint32_t count[kBins];
   __shared__ unsigned long long mass[kBins];
   __shared__ uint32_t part[kWaves];
   __shared__ uint64_t partm[kWaves];
+  __shared__ __align__(16) uint16_t order[T * kThreads];
+  __shared__ uint32_t wanted, fewest;
   const int row = blockIdx.y, tid = threadIdx.x, i0 = blockIdx.x * T * kThreads;
+  const float *x = a.logits + row * a.ld;
+  constexpr int L = T < 8 ? T : 8;  // tokens of a thread in flight
+  float y[L];
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int j = 0; j < L; ++j) y[j] = x[min(i0 + (j0 + j) * kThreads + tid, a.vocab - 1)];
+  };
+  load(0);
+  const float min_p = a.min_p ? steady(a.min_p + row) : a.min_p_all;
+  const int32_t top_k = a.top_k ? steady(a.top_k + row) : a.top_k_all;
+  const bool counts_only = few(top_k);
+  for (int k = tid; k < kBins; k += kThreads) count[k] = 0, mass[k] = 0;
+  if (tid == 0) fewest = ~0u;
   const Bins b = bins_of(a, w, row, chunks);
   if (!b.first || !(b.t > 0.f)) return;  // nothing to draw, or no draw
-  const float *x = a.logits + row * a.ld;
-  const float min_p = a.min_p ? a.min_p[row] : a.min_p_all;
-  for (int k = tid; k < kBins; k += kThreads) count[k] = 0, mass[k] = 0;
   __syncthreads();
   uint32_t rank[T];  // bin and place in it
   uint64_t large = 0;
@@ -217,20 +267,25 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Wor
   for (int j = 0; j < T; ++j) {
     const int i = i0 + j * kThreads + tid;
     if (i >= a.vocab) break;
-    const double e = exponent(b.r, order_key(x[i])), v = weight(e);
-    const uint64_t m = fixed(v);
-    const int k = bin_of(b, e, m);
+    if (j && j % L == 0) load(j);
+    const double e = exponent(b.r, order_key(y[j % L]));
+    const int k = bin_of(b, e);
     rank[j] = atomicAdd(&count[k], 1u) | (uint32_t)k << 16;
+    if (counts_only) continue;
+    const double v = weight(e);
+    const uint64_t m = fixed(v);
     if (m) atomicAdd(&mass[k], (unsigned long long)m);
     if (v >= (double)min_p) large += m;
   }
   __syncthreads();
   const int64_t list = (int64_t)row * chunks + blockIdx.x;
   const uint32_t n = tid < kBins ? count[tid] : 0u, end = block_scan(n, part);
+  // those that may be asked for: not the tokens of weight zero, of the first top_k the chunk's own
+  if (tid == kBins - 2) wanted = end;
+  if (counts_only && tid < kBins - 1 && end >= top_k && end - n < top_k) fewest = end;
   if (tid < kBins) {
     count[tid] = end - n;
-    w.ends[list * kBins + tid] = (uint16_t)end;
-    w.mass[list * kBins + tid] = mass[tid];
+    w.bin[list * kBins + tid] = {mass[tid], n, end};
   }
   large = wave_sum(large);
   if ((tid & 63) == 0) partm[tid >> 6] = large;
@@ -239,25 +294,36 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Wor
     for (int v = 1; v < kWaves; ++v) large += partm[v];
     w.large[list] = large;
   }
-  uint16_t *order = w.order + list * (T * kThreads);
+  // put together here: written one by one, the indices took most of the kernel's time
 #pragma unroll
   for (int j = 0; j < T; ++j) {
     if (i0 + j * kThreads + tid >= a.vocab) break;
     order[count[rank[j] >> 16] + (rank[j] & 0xFFFFu)] = (uint16_t)(j * kThreads + tid);
   }
+  __syncthreads();
+  const uint32_t last = min(wanted, fewest);
+  uint4 *to = (uint4 *)(w.order + list * (T * kThreads));
+  for (uint32_t q = tid; 8 * q < last; q += kThreads) to[q] = ((const uint4 *)order)[q];
 }
 
 // A row's tokens by digits of their places, one workgroup reading the whole row again for each:
 // where more tokens share a bin than a workgroup sorts (many equal logits).  The place of the first
-// token, in order, at which the running count reaches `want` (by_count) or its running mass is
-// `enough`, and the running mass with it.
+// token, in order, at which it is enough, and the running mass with it.
 struct Found {
   uint64_t place, mass;
 };
-template <typename F>
-__device__ Found find_by_digits(const SampleArgs &a, int row, const Row &r, bool by_count,
-                                uint32_t want, F enough, uint32_t *count, unsigned long long *mass,
-                                uint32_t *part, uint64_t *partm, Found *found) {
+// When it is enough: `count` tokens, or (count 0) a mass of `mass`, or of more than that.
+struct Goal {
+  uint32_t count;
+  bool more;
+  double mass;
+  __device__ __forceinline__ bool operator()(uint32_t c, uint64_t m) const {
+    return count ? c >= count : (more ? (double)m > mass : (double)m >= mass);
+  }
+};
+__device__ Found find_by_digits(const SampleArgs &a, int row, const Row &r, const Goal &enough,
+                                uint32_t *count, unsigned long long *mass, uint32_t *part,
+                                uint64_t *partm, Found *found) {
   const float *x = a.logits + row * a.ld;
   const int tid = threadIdx.x;
   uint64_t prefix = 0, above_m = 0;
@@ -284,8 +350,7 @@ __device__ Found find_by_digits(const SampleArgs &a, int row, const Row &r, bool
     const uint64_t m = k >= 0 ? mass[k] : 0;
     const uint32_t ce = above + block_scan(c, part);
     const uint64_t me = above_m + block_scan(m, partm);
-    const bool now = by_count ? ce >= want : enough(me), before = by_count ? ce - c >= want : enough(me - m);
-    if (k >= 0 && c && now && !before) {
+    if (k >= 0 && c && enough(ce, me) && !enough(ce - c, me - m)) {
       found->place = prefix | (uint64_t)k << sh;
       found->mass = me - m;
       s_above = ce - c;
@@ -299,111 +364,120 @@ __device__ Found find_by_digits(const SampleArgs &a, int row, const Row &r, bool
   return {prefix, above_m + mass_of(r, (uint32_t)(prefix >> 32))};
 }
 
+// Tokens in order: those of a run of bins, or of a part of one.
+struct Sorted {
+  uint32_t before;      // tokens of the row before them
+  uint64_t mass_before;
+  int n;
+};
+
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Work w, Cut cut) {
   __shared__ uint32_t count[kBins];              // tokens up to the end of a bin
   __shared__ unsigned long long mass[kBins];     // and their mass
-  __shared__ __align__(16) uint64_t list[kSorted];
+  __shared__ __align__(16) uint64_t list[kSorted], next[kSorted];
   __shared__ uint32_t counts[kBins], part[kWaves], begin[kChunks], base[kChunks + 1];
   __shared__ unsigned long long masses[kBins];
   __shared__ uint64_t partm[kWaves];
   __shared__ Found found;
   __shared__ int found_bin;
+  __shared__ uint32_t appended;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, chunks = cut.chunks;
   const float *x = a.logits + row * a.ld;
+  const int64_t lists = (int64_t)row * chunks;
+  const int32_t top_k = a.top_k ? steady(a.top_k + row) : a.top_k_all;
+  const float top_p = a.top_p ? steady(a.top_p + row) : a.top_p_all;
+  const float min_p = a.min_p ? steady(a.min_p + row) : a.min_p_all;
+  float u = steady(a.u + row);
+  u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
+  // the row's bins: half of the threads take every other chunk
+  uint32_t c = 0;
+  uint64_t m = 0;
+  {
+    const Bin *bin = w.bin + lists * kBins + tid % kBins;
+#pragma unroll 20
+    for (int l = tid / kBins; l < chunks; l += 2) {
+      const Bin v = bin[l * kBins];
+      c += v.count;
+      m += v.mass;
+    }
+  }
+  uint64_t large = w.large[lists + min(lane, chunks - 1)];
   const Bins b = bins_of(a, w, row, chunks);
-  if (!b.first || !(b.t > 0.f)) {
+  if (!b.first || !(b.t > 0.f)) {  // the bins have not been made
     if (tid == 0) {
       a.out[row] = b.first ? (uint32_t)~(uint32_t)b.first : 0;
       if (a.probs) a.probs[row] = b.first ? 1.f : 0.f;
     }
     return;
   }
-  const int32_t top_k = a.top_k ? a.top_k[row] : a.top_k_all;
-  const float top_p = a.top_p ? a.top_p[row] : a.top_p_all;
-  const float min_p = a.min_p ? a.min_p[row] : a.min_p_all;
-  float u = a.u[row];
-  u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
-  const int64_t lists = (int64_t)row * chunks;
+  if (tid >= kBins) counts[tid - kBins] = c, masses[tid - kBins] = m;
+  __syncthreads();
+  c = tid < kBins ? c + counts[tid] : 0;
+  m = tid < kBins ? m + masses[tid] : 0;
+  const uint32_t ce = block_scan(c, part);
+  const uint64_t me = block_scan(m, partm);
+  if (tid < kBins) count[tid] = ce, mass[tid] = me;
+  large = wave_sum(lane < chunks ? large : (uint64_t)0);
+  __syncthreads();
 
-  // the row's bins: half of the threads take every other chunk
-  {
-    const int k = tid % kBins, half = tid / kBins;
-    uint32_t c = 0;
-    uint64_t m = 0;
-#pragma unroll 4
-    for (int l = half; l < chunks; l += 2) {
-      const uint16_t *e = w.ends + (lists + l) * kBins + k;
-      c += k ? e[0] - e[-1] : e[0];
-      m += w.mass[(lists + l) * kBins + k];
-    }
-    if (half) counts[k] = c, masses[k] = m;
-    __syncthreads();
-    if (!half) c += counts[k], m += masses[k];
-    else c = 0, m = 0;
-    const uint32_t ce = block_scan(c, part);
-    const uint64_t me = block_scan(m, partm);
-    if (!half) count[k] = ce, mass[k] = me;
-    __syncthreads();
-  }
-  uint64_t large = wave_sum(lane < chunks ? w.large[lists + lane] : (uint64_t)0);
-
-  // the first bin at whose end it is enough; of none, the last
-  auto bin_where = [&](auto enough) {
+  // the first of the bins (sums up to their ends) at which it is enough; of none, the last
+  auto bin_where = [&](const uint32_t *cs, const unsigned long long *ms, uint32_t c0, uint64_t m0,
+                       const Goal &enough) {
     if (tid == 0) found_bin = kBins - 1;
     __syncthreads();
-    if (tid < kBins && enough(count[tid], (uint64_t)mass[tid]) &&
-        !(tid && enough(count[tid - 1], (uint64_t)mass[tid - 1])))
+    if (tid < kBins && enough(c0 + cs[tid], m0 + ms[tid]) &&
+        !(tid && enough(c0 + cs[tid - 1], m0 + ms[tid - 1])))
       found_bin = tid;
     __syncthreads();
-    const int k = found_bin;
-    __syncthreads();
-    return k;
+    return found_bin;
   };
-  // The tokens of bins k0 .. k1 in order, each thread with four neighbours' places and the running
-  // masses at their ends.  False: more than fit.
-  int sorted = 0;
-  uint64_t run[kSorted / kThreads];
-  uint64_t run0;
-  auto sort_bins = [&](int k0, int k1) {
-    const uint32_t before = k0 ? count[k0 - 1] : 0, n = count[k1] - before;
-    if (n > kSorted) return false;
+  // The n tokens of bins k0 .. k1 (n <= kSorted) into `list`, in no order.
+  auto gather = [&](int k0, int k1, uint32_t n) {
     if (tid < 64) {
       uint32_t from = 0, len = 0;
       if (lane < chunks) {
-        const uint16_t *e = w.ends + (lists + lane) * kBins;
-        from = k0 ? e[k0 - 1] : 0;
-        len = e[k1] - from;
+        const Bin *bin = w.bin + (lists + lane) * kBins;
+        const Bin v = bin[k1], v0 = bin[k0];
+        from = v0.end - v0.count;
+        len = v.end - from;
       }
-      uint32_t end = len;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t v = __shfl_up(end, o);
-        if (lane >= o) end += v;
-      }
+      const uint32_t end = wave_sums(len);
       begin[lane] = from;
       base[lane] = end - len;
-      if (lane == 63) base[64] = end;
     }
-    int size = 64;
-    while (size < (int)n) size <<= 1;
     __syncthreads();
-    for (int j = tid; j < size; j += kThreads) {
-      uint64_t p = 0;
-      if (j < (int)n) {
-        int lo = 0, hi = chunks - 1;  // the last chunk with base <= j
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if ((int)base[mid] <= j)
-            lo = mid;
-          else
-            hi = mid - 1;
-        }
-        const uint32_t i =
-            lo * cut.chunk + w.order[(lists + lo) * cut.chunk + begin[lo] + j - base[lo]];
-        p = place(order_key(x[i]), i);
+    for (uint32_t j = tid; j < n; j += kThreads) {
+      int lo = 0, hi = chunks - 1;  // the last chunk with base <= j
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (base[mid] <= j)
+          lo = mid;
+        else
+          hi = mid - 1;
       }
-      list[j] = p;
+      const uint32_t i = lo * cut.chunk + w.order[(lists + lo) * cut.chunk + begin[lo] + j - base[lo]];
+      list[j] = place(order_key(x[i]), i);
     }
+    __syncthreads();
+  };
+  // the first n tokens of `list` put in order
+  auto sort = [&](int n) {
+    if (n <= kRanked) {
+      uint64_t p = 0;
+      int rank = 0;
+      if (tid < n) {
+        p = list[tid];
+#pragma unroll 16
+        for (int j = 0; j < n; ++j) rank += list[j] > p;
+      }
+      __syncthreads();
+      if (tid < n) list[rank] = p;
+      __syncthreads();
+      return;
+    }
+    int size = 2 * kRanked;
+    while (size < n) size <<= 1;
+    for (int j = n + tid; j < size; j += kThreads) list[j] = 0;
     for (int k = 2; k <= size; k <<= 1)
       for (int s = k >> 1; s > 0; s >>= 1) {
         __syncthreads();
@@ -414,25 +488,35 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
         }
       }
     __syncthreads();
-    sorted = (int)n;
+  };
+  // each thread's four neighbours of the sorted tokens: the running masses at their ends
+  constexpr int kEach = kSorted / kThreads;
+  Sorted in{0, 0, 0};
+  uint64_t run[kEach], run0 = 0;
+  auto masses_of = [&](const Sorted &of) {
+    in = of;
     uint64_t sum = 0;
 #pragma unroll
-    for (int j = 0; j < kSorted / kThreads; ++j) {
-      const int i = tid * (kSorted / kThreads) + j;
-      sum += i < sorted ? mass_of(b.r, (uint32_t)(list[i] >> 32)) : 0;
+    for (int j = 0; j < kEach; ++j) {
+      const int i = tid + j * kThreads;
+      if (i < in.n) next[i] = mass_of(b.r, (uint32_t)(list[i] >> 32));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = tid * kEach + j;
+      sum += i < in.n ? next[i] : 0;
       run[j] = sum;
     }
-    const uint64_t end = block_scan(sum, partm) + (k0 ? mass[k0 - 1] : 0);
-    run0 = end - sum;
-    return true;
+    run0 = block_scan(sum, partm) + in.mass_before - sum;
   };
   // the first sorted token at which it is enough
-  auto token_where = [&](uint32_t before, auto enough) {
+  auto token_where = [&](const Goal &enough) {
 #pragma unroll
-    for (int j = 0; j < kSorted / kThreads; ++j) {
-      const int i = tid * (kSorted / kThreads) + j;
-      if (i < sorted && enough(before + i + 1, run0 + run[j]) &&
-          !enough(before + i, run0 + (j ? run[j - 1] : 0))) {
+    for (int j = 0; j < kEach; ++j) {
+      const int i = tid * kEach + j;
+      if (i < in.n && enough(in.before + i + 1, run0 + run[j]) &&
+          !enough(in.before + i, run0 + (j ? run[j - 1] : 0))) {
         found.place = list[i];
         found.mass = run0 + run[j];
       }
@@ -442,38 +526,112 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
     __syncthreads();
     return f;
   };
-  // The first token of the row at which it is enough, of bin k.  `all`: the sorted tokens are the
-  // first of the row, this one among them.
-  bool all = false;
-  auto find = [&](bool by_count, uint32_t want, auto enough_mass) {
-    auto enough = [&](uint32_t c, uint64_t m) { return by_count ? c >= want : enough_mass(m); };
-    if (all) return token_where(0, enough);
-    const int k = bin_where(enough);
-    if (count[k] <= kSorted / 4 && sort_bins(0, k)) {
-      all = true;
-      return token_where(0, enough);
+  // Of the n tokens in `list`, from (c0, m0) on, more than are sorted by counting: those that share
+  // the bin, by their logits' bits, in which it is enough.
+  auto narrow = [&](const Sorted &of, const Goal &enough) {
+    uint32_t lo = ~0u, hi = 0;
+    for (int j = tid; j < of.n; j += kThreads) {
+      const uint32_t k = (uint32_t)(list[j] >> 32);
+      lo = k < lo ? k : lo;
+      hi = k > hi ? k : hi;
     }
-    if (sort_bins(k, k)) return token_where(k ? count[k - 1] : 0, enough);
-    const Found f = find_by_digits(a, row, b.r, by_count, want, enough_mass, counts, masses, part,
-                                   partm, &found);
-    return f;
+    lo = ~wave_max(~lo);
+    hi = wave_max(hi);
+    if (lane == 0) part[tid >> 6] = lo, partm[tid >> 6] = hi;
+    if (tid < kBins) counts[tid] = 0, masses[tid] = 0;
+    if (tid == 0) appended = 0;
+    __syncthreads();
+    for (int v = 0; v < kWaves; ++v) {
+      lo = part[v] < lo ? part[v] : lo;
+      hi = (uint32_t)partm[v] > hi ? (uint32_t)partm[v] : hi;
+    }
+    const uint32_t per = (hi - lo) / kBins + 1;  // keys of a bin
+    for (int j = tid; j < of.n; j += kThreads) {
+      const uint32_t key = (uint32_t)(list[j] >> 32), k = (hi - key) / per;
+      atomicAdd(&counts[k], 1u);
+      atomicAdd(&masses[k], (unsigned long long)mass_of(b.r, key));
+    }
+    __syncthreads();
+    const uint32_t cs = tid < kBins ? counts[tid] : 0;
+    const uint64_t ms = tid < kBins ? masses[tid] : 0;
+    const uint32_t ce = block_scan(cs, part);
+    const uint64_t me = block_scan(ms, partm);
+    if (tid < kBins) counts[tid] = ce, masses[tid] = me;
+    __syncthreads();
+    const int k = bin_where(counts, masses, of.before, of.mass_before, enough);
+    const int n = (int)(counts[k] - (k ? counts[k - 1] : 0));
+    const Sorted to{of.before + (k ? counts[k - 1] : 0), of.mass_before + (k ? masses[k - 1] : 0), n};
+    for (int j = tid; j < of.n; j += kThreads) {
+      const uint64_t p = list[j];
+      if ((int)((hi - (uint32_t)(p >> 32)) / per) == k) next[atomicAdd(&appended, 1u)] = p;
+    }
+    __syncthreads();
+    for (int j = tid; j < n; j += kThreads) list[j] = next[j];
+    __syncthreads();
+    return to;
+  };
+  // The first token of the row at which it is enough.  `all`: the sorted tokens are the first of the
+  // row, this one among them.
+  bool all = false, by_digits = false;
+  auto find = [&](const Goal &enough) {
+    if (!all) {
+      const int k = by_digits ? 0 : bin_where(count, mass, 0, 0, enough);
+      const uint32_t before = k ? count[k - 1] : 0;
+      all = !by_digits && (count[k] <= kRanked || (few(top_k) && count[k] <= kSorted));
+      Sorted of{before, k ? (uint64_t)mass[k - 1] : 0, (int)(count[k] - before)};
+      if (all) of = {0, 0, (int)count[k]};
+      if (by_digits || of.n > kSorted)
+        return find_by_digits(a, row, b.r, enough, counts, masses, part, partm, &found);
+      gather(all ? 0 : k, k, of.n);
+      if (!all && of.n > kRanked) of = narrow(of, enough);
+      sort(of.n);
+      masses_of(of);
+    }
+    return token_where(enough);
   };
 
-  const uint64_t whole = mass[kBins - 1];
-  uint64_t total = whole;
-  if (!(min_p > 0.f)) large = whole;
-  auto never = [](uint64_t) { return false; };
-  // (a first run down to tokens of weight zero keeps all mass)
-  if (top_k > 0 && (uint32_t)top_k < count[kBins - 2]) total = find(true, (uint32_t)top_k, never).mass;
-  if (top_p < 1.f) {
-    const double want = fmax((double)top_p * (double)total, 1.0);  // the first token has 2^43
-    const uint64_t kept = find(false, 0, [&](uint64_t m) { return (double)m >= want; }).mass;
-    total = kept < total ? kept : total;
+  uint64_t total = mass[kBins - 1];
+  const uint32_t most = count[kBins - 2];  // tokens of a weight above zero: a run of them keeps all mass
+  Found f{0, 0};
+#pragma unroll 1
+  for (int goal = 0; goal < 3; ++goal) {  // top_k, top_p, the draw
+    Goal enough{0, false, 0.0};
+    if (goal == 0) {
+      if (!few(top_k) && (top_k <= 0 || (uint32_t)top_k >= most)) continue;
+      enough.count = min((uint32_t)top_k, most);
+    } else if (goal == 1) {
+      if (!(top_p < 1.f)) continue;
+      enough.mass = fmax((double)top_p * (double)total, 1.0);  // the first token has 2^43
+    } else {
+      if (min_p > 0.f) {
+        if (few(top_k)) {  // not known yet: of the kept ones, or of all
+          large = 0;
+          const int n = all ? in.n : a.vocab;
+          for (int i = tid; i < n; i += kThreads) {
+            const double v = weight(exponent(b.r, all ? (uint32_t)(list[i] >> 32) : order_key(x[i])));
+            if (v >= (double)min_p) large += fixed(v);
+          }
+          large = wave_sum(large);
+          __syncthreads();
+          if (lane == 0) partm[tid >> 6] = large;
+          __syncthreads();
+          large = 0;
+          for (int v = 0; v < kWaves; ++v) large += partm[v];
+        }
+        total = large < total ? large : total;
+        total = total < (uint64_t)kOne ? (uint64_t)kOne : total;
+      }
+      enough.more = true;
+      enough.mass = (double)u * (double)total;
+    }
+    f = find(enough);
+    if (goal == 0) {
+      total = f.mass;
+      by_digits = few(top_k) && !all;  // the bins' masses have not been made
+    } else if (goal == 1) {
+      total = f.mass < total ? f.mass : total;
+    }
   }
-  total = large < total ? large : total;
-  total = total < (uint64_t)kOne ? (uint64_t)kOne : total;
-  const double want = (double)u * (double)total;
-  const Found f = find(false, 0, [&](uint64_t m) { return (double)m > want; });
   if (tid == 0) {
     a.out[row] = (uint32_t)~(uint32_t)f.place;
     if (a.probs) a.probs[row] = (float)((double)mass_of(b.r, (uint32_t)(f.place >> 32)) / (double)total);
