@@ -141,11 +141,10 @@ __device__ __forceinline__ T block_scan(T v, T *part) {
 // The workspace: per row and chunk the place of its first token and the inverse of its smallest
 // key; the mass that min_p keeps; its bins; its tokens in their order (indices within the chunk).
 struct Bin {
-  uint64_t mass;
-  uint32_t count, end;  // of the chunk's tokens in the order of the bins
+  uint16_t count, end;  // of the chunk's tokens in the order of the bins
 };
 struct Work {
-  uint64_t *first, *large;
+  uint64_t *first, *large, *mass;
   Bin *bin;
   uint32_t *least;
   uint16_t *order;
@@ -172,6 +171,7 @@ int64_t place_work(char *base, int64_t rows, const Cut &c, Work &w) {
   };
   w.first = (uint64_t *)take(lists * 8);
   w.large = (uint64_t *)take(lists * 8);
+  w.mass = (uint64_t *)take(lists * kBins * 8);
   w.bin = (Bin *)take(lists * kBins * sizeof(Bin));
   w.least = (uint32_t *)take(lists * 4);
   w.order = (uint16_t *)take(lists * c.chunk * 2);
@@ -215,13 +215,19 @@ struct Bins {
   uint64_t first;  // the row's first token
   float t;
 };
-__device__ __forceinline__ Bins bins_of(const SampleArgs &a, const Work &w, int row, int chunks) {
-  const int lane = threadIdx.x & 63;
-  const int64_t list = (int64_t)row * chunks + min(lane, chunks - 1);
+struct Chunk {  // what the first launch left of a lane's chunk
+  uint64_t first;
+  uint32_t least;
+};
+__device__ __forceinline__ Chunk chunk_of(const Work &w, int row, int chunks) {
+  const int64_t list = (int64_t)row * chunks + min((int)(threadIdx.x & 63), chunks - 1);
+  return {w.first[list], w.least[list]};
+}
+__device__ __forceinline__ Bins bins_of(const SampleArgs &a, int row, const Chunk &c) {
   Bins b;
   b.t = a.temperature ? steady(a.temperature + row) : a.temperature_all;
-  b.first = wave_max(w.first[list]);
-  const uint32_t least = wave_max(w.least[list]);
+  b.first = wave_max(c.first);
+  const uint32_t least = wave_max(c.least);
   b.r.scale = 1.4426950408889634074 / (double)b.t;
   b.r.top = key_value((uint32_t)(b.first >> 32));
   const double range = fmin(-exponent(b.r, ~least), -kNothing);
@@ -252,13 +258,14 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a, 
 #pragma unroll
     for (int j = 0; j < L; ++j) y[j] = x[min(i0 + (j0 + j) * kThreads + tid, a.vocab - 1)];
   };
+  const Chunk own = chunk_of(w, row, chunks);
   load(0);
   const float min_p = a.min_p ? steady(a.min_p + row) : a.min_p_all;
   const int32_t top_k = a.top_k ? steady(a.top_k + row) : a.top_k_all;
   const bool counts_only = few(top_k);
   for (int k = tid; k < kBins; k += kThreads) count[k] = 0, mass[k] = 0;
   if (tid == 0) fewest = ~0u;
-  const Bins b = bins_of(a, w, row, chunks);
+  const Bins b = bins_of(a, row, own);
   if (!b.first || !(b.t > 0.f)) return;  // nothing to draw, or no draw
   __syncthreads();
   uint32_t rank[T];  // bin and place in it
@@ -285,7 +292,8 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a, 
   if (counts_only && tid < kBins - 1 && end >= top_k && end - n < top_k) fewest = end;
   if (tid < kBins) {
     count[tid] = end - n;
-    w.bin[list * kBins + tid] = {mass[tid], n, end};
+    w.bin[list * kBins + tid] = {(uint16_t)n, (uint16_t)end};
+    if (!counts_only) w.mass[list * kBins + tid] = mass[tid];
   }
   large = wave_sum(large);
   if ((tid & 63) == 0) partm[tid >> 6] = large;
@@ -390,19 +398,22 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
   float u = steady(a.u + row);
   u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
   // the row's bins: half of the threads take every other chunk
+  const Chunk own = chunk_of(w, row, chunks);
+  uint64_t large = w.large[lists + min(lane, chunks - 1)];
   uint32_t c = 0;
   uint64_t m = 0;
   {
-    const Bin *bin = w.bin + lists * kBins + tid % kBins;
-#pragma unroll 20
-    for (int l = tid / kBins; l < chunks; l += 2) {
-      const Bin v = bin[l * kBins];
-      c += v.count;
-      m += v.mass;
-    }
+    const int64_t at = lists * kBins + tid % kBins;
+    const uint32_t *bin = (const uint32_t *)w.bin + at;
+    const uint64_t *mass = w.mass + at;
+    const int half = tid / kBins;
+#pragma unroll 16
+    for (int l = half; l < chunks; l += 2) c += bin[l * kBins] & 0xFFFFu;
+    if (!few(top_k))
+#pragma unroll 16
+      for (int l = half; l < chunks; l += 2) m += mass[l * kBins];
   }
-  uint64_t large = w.large[lists + min(lane, chunks - 1)];
-  const Bins b = bins_of(a, w, row, chunks);
+  const Bins b = bins_of(a, row, own);
   if (!b.first || !(b.t > 0.f)) {  // the bins have not been made
     if (tid == 0) {
       a.out[row] = b.first ? (uint32_t)~(uint32_t)b.first : 0;
