@@ -54,7 +54,10 @@ __device__ __forceinline__ int units_of(int filled) {
   return filled < 0 ? 0 : filled / kUnit + 1;
 }
 __device__ __forceinline__ Splits splits_of(int units, int fair, const Cut &k) {
-  const int per = (max(max(fair, kLeastUnits), (units + k.S - 1) / k.S) + k.W - 1) / k.W * k.W;
+  const int most = (max(max(fair, kLeastUnits), (units + k.S - 1) / k.S) + k.W - 1) / k.W * k.W;
+  const int n = (units + most - 1) / most;
+  // alike, in whole turns: the last one is not left with a few units
+  const int per = n > 1 ? ((units + n - 1) / n + k.W - 1) / k.W * k.W : most;
   return {per, (units + per - 1) / per};
 }
 // The fair share: a wave's lanes add the sequences.
@@ -118,21 +121,23 @@ __device__ __forceinline__ float4_t mfma(uint4 a, uint4 b, float4_t c, std::true
                                                  __builtin_bit_cast(bhalf8_t, b), c, 0, 0, 0);
 }
 
-// v plus that of the lane 8 to the left in its 16, cyclically.
-__device__ __forceinline__ float ror8(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, true));
+// That of the lane N to the left in its 16, cyclically.
+template <int N>
+__device__ __forceinline__ float ror16(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
 }
 
-// Eight values as a matrix operand's lane.  Column r of the matrix cores' 16 holds query head r % 8:
-// in columns 0 .. 7 the high parts, in 8 .. 15 the next ones.  f16: hi + lo in one operand, 22 bits;
-// bf16: hi + mid in the first, lo + nothing in the second, 24 bits.
-template <bool BF>
+// Eight values as a matrix operand's lane.  Column r of the matrix cores' 16 holds query head r % C,
+// part r / C of its values: f16 parts hi + lo, 22 bits; bf16 parts hi + mid + lo, 24 bits, where C = 8
+// leaves lo for a second operand.
+template <bool BF, int C>
 struct Parts {
-  uint4 w[BF ? 2 : 1];
-  __device__ __forceinline__ void make(const float (&x)[8], bool low) {
+  static constexpr int N = BF && C == 8 ? 2 : 1;  // operands
+  uint4 w[N];
+  __device__ __forceinline__ void make(const float (&x)[8], int part) {
     if constexpr (!BF) {
       half8_t h;
-      const float sel = low ? -1.f : 0.f;
+      const float sel = part ? -1.f : 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const half_t hi = (half_t)x[i];
@@ -146,19 +151,31 @@ struct Parts {
         const bhalf_t hi = (bhalf_t)x[i];
         const float rest = x[i] - (float)hi;
         const bhalf_t mid = (bhalf_t)rest;
-        a[i] = low ? mid : hi;
-        b[i] = (bhalf_t)(low ? 0.f : rest - (float)mid);
+        const float last = rest - (float)mid;
+        if constexpr (C == 8) {
+          a[i] = part ? mid : hi;
+          b[i] = (bhalf_t)(part ? 0.f : last);
+        } else {
+          a[i] = (bhalf_t)(part == 0 ? x[i] : (part == 1 ? rest : (part == 2 ? last : 0.f)));
+        }
       }
       w[0] = __builtin_bit_cast(uint4, a);
-      w[BF ? 1 : 0] = __builtin_bit_cast(uint4, b);
+      if constexpr (C == 8) w[N - 1] = __builtin_bit_cast(uint4, b);
     }
   }
 };
+// The sum of a head's parts, in each of its columns.
+template <bool BF, int C>
+__device__ __forceinline__ float all_parts(float v) {
+  v += ror16<8>(v);
+  if constexpr (BF && C == 4) v += ror16<4>(v);
+  return v;
+}
 
 // A workgroup takes one list and one range of its units of 32 slots; its waves take the range's
 // units in turn and join at the end.  Nothing but registers carries a unit through:
 // - Scores: v_mfma_f32_16x16x32 with the slots' K rows as A and the queries as B, each head's parts
-//   in two columns (Parts), which a rotation within 16 lanes adds.  Row m of A's half t holds
+//   in columns of their own (Parts), which rotations within 16 lanes add.  Row m of A's half t holds
 //   slot 8 (m / 4) + 4 t + m % 4, so that lane (r, g) = (lane % 16, lane / 16) of the accumulators
 //   has the scores of slots 8 g .. 8 g + 7.
 // - Output: that is the B layout of V . P^T, with V's channels as A, 16 bytes of a block's channel
@@ -166,16 +183,18 @@ struct Parts {
 // - p = 2^(score - m) with a running m, raised where a p would pass 2^15: to the largest score
 //   less 10, so that p's f16 parts keep 22 bits down to 2^-13 of the largest.
 // - K's registers take the next unit as soon as its scores are made, V's after its products.
-template <int HD, bool BF, int W, int WPS>
+template <int HD, bool BF, int C, int W, int WPS>
 __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache c, PagedAttn a,
                                                                       float *__restrict__ rec,
                                                                       Cut cut) {
   constexpr int NB = HD / 32, CT = HD / 16, RS = record_floats<HD>(), half = HD / 2;
-  constexpr int NP = BF ? 2 : 1;
+  constexpr int NP = Parts<BF, C>::N;
+  constexpr bool kInLds = HD == 256;  // the queries: in registers there would be too few
   constexpr std::bool_constant<BF> bf{};
   constexpr float kLift = 10.f, kMost = 15.f;
   __shared__ __align__(16) float o_[W][8][HD];  // per wave and head its sums
   __shared__ float2 ml_[W][8];
+  __shared__ uint4 q_[kInLds ? NB : 1][NP][64];
   __shared__ __align__(16) uint16_t fresh[2][HD];  // the new row's K and V
   Item it;
   if (!item_of(c, blockIdx.x, cut, it)) return;
@@ -227,12 +246,12 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
     for (int i = 0; i < CT; ++i) vf[i] = *(const uint4 *)(v + 256 * i);
   };
 
-  // the queries: lane (r, g) channels 32 i + 8 g + 0 .. 7 of head r % 8, whose RoPE partners are the
+  // the queries: lane (r, g) channels 32 i + 8 g + 0 .. 7 of head r % C, whose RoPE partners are the
   // same lane's of block i +- NB / 2
-  Parts<BF> qf[NB];
+  Parts<BF, C> qf[NB];
   float f;  // log2 units per unit of an accumulated score
   {
-    const int h = r & 7;
+    const int h = r % C;
     const float *x = row + (int64_t)(kvh * grp + (h < grp ? h : 0)) * HD + 8 * g;
     const float *cr = c.cs + (int64_t)filled * half + 8 * g, *sr = c.sn + (int64_t)filled * half + 8 * g;
     float y[NB][8], mx = 0.f;
@@ -254,7 +273,10 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
     for (int i = 0; i < NB; ++i) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[i][j] *= up;
-      qf[i].make(y[i], r >= 8);
+      qf[i].make(y[i], r / C);
+      if (kInLds && wave == 0)
+#pragma unroll
+        for (int k = 0; k < NP; ++k) q_[i][k][lane] = qf[i].w[k];
     }
   }
   // the new row, by the first wave: to its page, and to the workgroup
@@ -315,11 +337,13 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
     }
   }
 
+  int ql = lane;  // made anew every turn: the queries are read from LDS there, not kept
   float4_t acc[CT];
   float m = -INFINITY, l = 0.f;  // p = 2^(score - m)
 #pragma unroll
   for (int i = 0; i < CT; ++i) acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
   for (; unit >= unit0; unit -= W) {
+    if (kInLds) asm volatile("" : "+v"(ql));
     float y[8];
     {
       float4_t sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -327,14 +351,12 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
       for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int k = NP - 1; k >= 0; --k) {
-          sc[0] = mfma(kf[0][i], qf[i].w[k], sc[0], bf);
-          sc[1] = mfma(kf[1][i], qf[i].w[k], sc[1], bf);
+          const uint4 q = kInLds ? q_[i][k][ql] : qf[i].w[k];
+          sc[0] = mfma(kf[0][i], q, sc[0], bf);
+          sc[1] = mfma(kf[1][i], q, sc[1], bf);
         }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = sc[j >> 2][j & 3];
-        y[j] = x + ror8(x);
-      }
+      for (int j = 0; j < 8; ++j) y[j] = all_parts<BF, C>(sc[j >> 2][j & 3]);
     }
     const int next = max(unit - W, unit0);  // the last one: unused
     load_k(next, n0, n1);
@@ -383,8 +405,8 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
       weigh();
     }
     l += sum;
-    Parts<BF> pf;
-    pf.make(p, r >= 8);
+    Parts<BF, C> pf;
+    pf.make(p, r / C);
 #pragma unroll
     for (int i = 0; i < CT; ++i)
 #pragma unroll
@@ -395,14 +417,14 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
     ids(max(next - W, unit0), n0, n1);
   }
 
-  // the waves' sums: lane (r, g), register k of i: channel 16 i + 4 g + k, head r % 8
+  // the waves' sums: lane (r, g), register k of i: channel 16 i + 4 g + k, head r % C
   const float ls = sum_xor32(sum_xor16(l));
-  if (g == 0 && r < 8) ml_[wave][r] = make_float2(m, ls);
+  if (g == 0 && r < C) ml_[wave][r] = make_float2(m, ls);
 #pragma unroll
   for (int i = 0; i < CT; ++i) {
     float4_t x = acc[i];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] += ror8(x[k]);
+    for (int k = 0; k < 4; ++k) x[k] = all_parts<BF, C>(x[k]);
     if (r < grp) *(float4_t *)&o_[wave][r][16 * i + 4 * g] = x;
   }
   __syncthreads();
@@ -496,18 +518,19 @@ struct Plan {
 Plan plan(int page, int64_t columns, int n_seq, int nkv, int hd) {
   Plan p;
   p.lists = (int64_t)n_seq * nkv;
-  p.cut.W = 4;
-  p.cut.wgs = hd == 256 ? 512 : 768;
-  // a list of two turns is not cut: one launch, and nothing to join
   const int64_t units = (columns * page + kUnit - 1) / kUnit;
-  const int64_t most = units <= 2 * p.cut.W ? 1 : (units + kLeastUnits - 1) / kLeastUnits;
+  // a list of two turns is not cut: one launch, and nothing to join
+  const bool whole = units <= 16;
+  p.cut.W = whole && units > 8 ? 8 : 4;
+  p.cut.wgs = hd == 256 ? 512 : 768;
+  const int64_t most = whole ? 1 : (units + kLeastUnits - 1) / kLeastUnits;
   // sequences of different lengths: up to four times the workgroups that equal ones would take
   const int64_t want = (4 * p.cut.wgs + p.lists - 1) / p.lists;
   p.cut.S = (int)(want < most ? want : most);
   return p;
 }
 
-template <int HD, bool BF>
+template <int HD, bool BF, int C>
 hipError_t launch(const PagedCache &c, const PagedAttn &a, hipStream_t s) {
   const Plan p = plan(c.page, c.columns, c.n_seq, c.nkv, HD);
   float *rec = (float *)a.work;
@@ -515,13 +538,21 @@ hipError_t launch(const PagedCache &c, const PagedAttn &a, hipStream_t s) {
   // shares).
   const int64_t most = p.lists * p.cut.S, items = most < p.cut.wgs + p.lists ? most : p.cut.wgs + p.lists;
   const dim3 grid((unsigned)items), block(64 * p.cut.W);
-  hipLaunchKernelGGL((paged_attention_kernel<HD, BF, 4, HD == 256 ? 2 : 3>), grid, block, 0, s, c, a,
-                     rec, p.cut);
+  if (p.cut.W == 8)
+    hipLaunchKernelGGL((paged_attention_kernel<HD, BF, C, 8, 2>), grid, block, 0, s, c, a, rec, p.cut);
+  else
+    hipLaunchKernelGGL((paged_attention_kernel<HD, BF, C, 4, HD == 256 ? 2 : 3>), grid, block, 0, s, c,
+                       a, rec, p.cut);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.cut.S == 1) return e;
   hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3((unsigned)(c.nh / c.nkv), (unsigned)p.lists),
                      dim3(kMergeThreads<HD>), 0, s, c, a, rec, p.cut);
   return hipGetLastError();
+}
+template <int HD>
+hipError_t launch(const PagedCache &c, const PagedAttn &a, hipStream_t s) {
+  if (!c.bf16) return launch<HD, false, 8>(c, a, s);
+  return c.nh / c.nkv <= 4 ? launch<HD, true, 4>(c, a, s) : launch<HD, true, 8>(c, a, s);
 }
 
 }  // namespace
@@ -532,9 +563,9 @@ int64_t paged_attention_work_bytes(int page, int64_t columns, int n_seq, int nh,
 }
 
 hipError_t launch_paged_attention(const PagedCache &c, const PagedAttn &a, hipStream_t s) {
-  if (c.hd == 64) return c.bf16 ? launch<64, true>(c, a, s) : launch<64, false>(c, a, s);
-  if (c.hd == 128) return c.bf16 ? launch<128, true>(c, a, s) : launch<128, false>(c, a, s);
-  return c.bf16 ? launch<256, true>(c, a, s) : launch<256, false>(c, a, s);
+  if (c.hd == 64) return launch<64>(c, a, s);
+  if (c.hd == 128) return launch<128>(c, a, s);
+  return launch<256>(c, a, s);
 }
 
 }  // namespace gguf
