@@ -121,6 +121,14 @@ __device__ __forceinline__ float4_t mfma(uint4 a, uint4 b, float4_t c, std::true
                                                  __builtin_bit_cast(bhalf8_t, b), c, 0, 0, 0);
 }
 
+// 16 bytes; STREAM: past the caches, since no other wave reads them.
+template <bool STREAM>
+__device__ __forceinline__ uint4 load16(const uint16_t *p) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  if (STREAM) return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const u32x4 *)p));
+  return *(const uint4 *)p;
+}
+
 // That of the lane N to the left in its 16, cyclically.
 template <int N>
 __device__ __forceinline__ float ror16(float v) {
@@ -183,7 +191,7 @@ __device__ __forceinline__ float all_parts(float v) {
 // - p = 2^(score - m) with a running m, raised where a p would pass 2^15: to the largest score
 //   less 10, so that p's f16 parts keep 22 bits down to 2^-13 of the largest.
 // - K's registers take the next unit as soon as its scores are made, V's after its products.
-template <int HD, bool BF, int C, int W, int WPS>
+template <int HD, bool BF, int C, int W, int WPS, bool STREAM>
 __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache c, PagedAttn a,
                                                                       float *__restrict__ rec,
                                                                       Cut cut) {
@@ -235,7 +243,7 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < NB; ++i) kf[t][i] = *(const uint4 *)(k + 4 * t * HD + 32 * i);
+      for (int i = 0; i < NB; ++i) kf[t][i] = load16<STREAM>(k + 4 * t * HD + 32 * i);
   };
   auto load_v = [&](int unit, int p0, int p1) {
     const int b = 2 * unit + (g >> 1);
@@ -243,7 +251,7 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
     const uint16_t *v =
         c.kv + p * page_values + (list_v + (b & in_page) * 16 * HD + 16 * r + 8 * (g & 1));
 #pragma unroll
-    for (int i = 0; i < CT; ++i) vf[i] = *(const uint4 *)(v + 256 * i);
+    for (int i = 0; i < CT; ++i) vf[i] = load16<STREAM>(v + 256 * i);
   };
 
   // the queries: lane (r, g) channels 32 i + 8 g + 0 .. 7 of head r % C, whose RoPE partners are the
@@ -514,6 +522,7 @@ __global__ __launch_bounds__(kMergeThreads<HD>) void paged_merge_kernel(PagedCac
 struct Plan {
   Cut cut;
   int64_t lists;
+  bool stream;
 };
 Plan plan(int page, int64_t columns, int n_seq, int nkv, int hd) {
   Plan p;
@@ -527,6 +536,10 @@ Plan plan(int page, int64_t columns, int n_seq, int nkv, int hd) {
   // sequences of different lengths: up to four times the workgroups that equal ones would take
   const int64_t want = (4 * p.cut.wgs + p.lists - 1) / p.lists;
   p.cut.S = (int)(want < most ? want : most);
+  // Tables of more than the last cache holds (256 MB) are read past the caches: 130000 slots of 8
+  // lists 110 us, so 101, 32 sequences of 4000 112 and 102, a list of 6000 slots, whose pages the
+  // caches still hold from the call before, 11.6 and 13.9.
+  p.stream = p.lists * columns * page * hd * 4 > (int64_t)256 << 20;
   return p;
 }
 
@@ -538,11 +551,14 @@ hipError_t launch(const PagedCache &c, const PagedAttn &a, hipStream_t s) {
   // shares).
   const int64_t most = p.lists * p.cut.S, items = most < p.cut.wgs + p.lists ? most : p.cut.wgs + p.lists;
   const dim3 grid((unsigned)items), block(64 * p.cut.W);
+  constexpr int WPS = HD == 256 ? 2 : 3;
+  auto go = [&](auto *kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, c, a, rec, p.cut); };
   if (p.cut.W == 8)
-    hipLaunchKernelGGL((paged_attention_kernel<HD, BF, C, 8, 2>), grid, block, 0, s, c, a, rec, p.cut);
+    go(paged_attention_kernel<HD, BF, C, 8, 2, false>);
+  else if (p.stream)
+    go(paged_attention_kernel<HD, BF, C, 4, WPS, true>);
   else
-    hipLaunchKernelGGL((paged_attention_kernel<HD, BF, C, 4, HD == 256 ? 2 : 3>), grid, block, 0, s, c,
-                       a, rec, p.cut);
+    go(paged_attention_kernel<HD, BF, C, 4, WPS, false>);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.cut.S == 1) return e;
   hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3((unsigned)(c.nh / c.nkv), (unsigned)p.lists),
