@@ -11,10 +11,9 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------------------
-// Storing rows: a wave takes one row and N units (K or V of a KV head, 256 / HD of them side by
-// side).
+// Storing rows: a wave takes one row and 256 / HD units (K or V of a KV head) side by side.
 // ---------------------------------------------------------------------------
-template <int HD, bool BF, int N>
+template <int HD, bool BF>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c,
                                                                 const float *__restrict__ qkv,
                                                                 int64_t ldq, uint32_t n_rows,
@@ -24,14 +23,10 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c,
   const uint32_t r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   if (r >= n_rows) return;
   // unit u: KV head u / 2, K or V; in qkv after the queries all of K, then all of V
-  const int u0 = blockIdx.y * N * SIDE + lane / LANES, units = 2 * c.nkv;
-  const float *x = qkv + r * ldq + (int64_t)c.nh * HD;
-  Kv4Row<HD> row[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {  // past the last unit: the last again, not stored
-    const int u = min(u0 + i * SIDE, units - 1);
-    row[i].load(x + (int64_t)((u & 1) * c.nkv + (u >> 1)) * HD, q);
-  }
+  const int u = blockIdx.y * SIDE + lane / LANES, units = 2 * c.nkv;
+  const int ul = min(u, units - 1);  // past the last unit: the last again, not stored
+  Kv4Row<HD> row;
+  row.load(qkv + r * ldq + (int64_t)(c.nh + (ul & 1) * c.nkv + (ul >> 1)) * HD, q);
   uint32_t s;
   int64_t i;  // the row of s
   if (starts) {
@@ -55,28 +50,130 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c,
   }
   const int64_t n = c.lengths[s], end = paged_end(c, s);
   if (n < 0 || n >= end - i) return;
-  const int slot = (int)(n + i);
+  const int slot = (int)(n + i), j = slot & (c.page - 1);
   const int32_t page = c.tables[(int64_t)s * c.columns + (slot >> c.shift)];
   if ((uint32_t)page >= (uint32_t)c.n_pages) return;
-  row[0].load_turn(c.cs + (int64_t)slot * (HD / 2), c.sn + (int64_t)slot * (HD / 2), q);
-  const int j = slot & (c.page - 1);
+  row.load_turn(c.cs + (int64_t)slot * (HD / 2), c.sn + (int64_t)slot * (HD / 2), q);
+  float y[4];
+  paged_turn<HD>(row, q, !(u & 1), y);
+  if (u >= units) return;
+  const uint2 w = paged_round<BF>(y);
+  if (!(u & 1)) {
+    *(uint2 *)(c.kv + paged_k_at(c, page, u >> 1, j) + 4 * q) = w;
+  } else {
+    uint16_t *v = c.kv + paged_v_at(c, page, u >> 1, j) + 64 * q;
+    v[0] = (uint16_t)w.x;
+    v[16] = (uint16_t)(w.x >> 16);
+    v[32] = (uint16_t)w.y;
+    v[48] = (uint16_t)(w.y >> 16);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Storing prompts: a wave takes the rows of one block of 16 slots, K and V of one KV head.  V's 16
+// slots of a channel are 32 bytes, which a lane has from its loads of the 16 rows; K's rows go as
+// they come.
+// ---------------------------------------------------------------------------
+// The rows of sequence s that are stored: rows first .. first + n - 1 of qkv in slots from `slot` on.
+struct Stretch {
+  int first, n, slot;
+  __device__ __forceinline__ int blocks() const {
+    return n > 0 ? ((slot + n - 1) >> 4) - (slot >> 4) + 1 : 0;
+  }
+};
+__device__ __forceinline__ Stretch stretch_of(const PagedCache &c, int s, int64_t n_rows,
+                                              const int64_t *starts) {
+  const int64_t per = starts ? 0 : n_rows / c.n_seq;
+  const int64_t from = starts ? starts[s] : s * per, to = starts ? starts[s + 1] : from + per;
+  const int64_t held = c.lengths[s], end = paged_end(c, s);
+  // so far back that all its rows lie behind every slot: and differences need not fit 64 bits
+  if (held < 0 || held >= end || from >= n_rows || from < -((int64_t)c.columns << c.shift))
+    return {0, 0, 0};
+  const int64_t first = from < 0 ? 0 : from, last = to < n_rows ? (to < 0 ? 0 : to) : n_rows;
+  const int64_t slot = held + (first - from), room = end - slot;
+  const int64_t n = last - first < room ? last - first : room;
+  return {(int)first, n > 0 ? (int)n : 0, (int)slot};
+}
+
+template <int HD, bool BF>
+__global__ __launch_bounds__(kThreads) void paged_append_blocks_kernel(
+    PagedCache c, const float *__restrict__ qkv, int64_t ldq, int64_t n_rows,
+    const int64_t *__restrict__ starts) {
+  constexpr int LANES = Kv4Row<HD>::LANES, SIDE = 64 / LANES, CH = HD / 64;
+  const int lane = threadIdx.x & 63, q = lane % LANES;
+  const int h = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6));
+  if (h >= c.nkv) return;
+  // block blockIdx.x of the call: sequences in order
+  int s = -1, block = 0;
+  Stretch x{0, 0, 0};
+  for (int s0 = 0, before = 0; s0 < c.n_seq; s0 += 64) {
+    const Stretch mine = s0 + lane < c.n_seq ? stretch_of(c, s0 + lane, n_rows, starts) : Stretch{0, 0, 0};
+    const int n = mine.blocks(), run = before + lanes_before(n);
+    const uint64_t hit = __ballot((int)blockIdx.x < run);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      s = s0 + at;
+      block = blockIdx.x - (__builtin_amdgcn_readlane(run, at) - __builtin_amdgcn_readlane(n, at));
+      x = {__builtin_amdgcn_readlane(mine.first, at), __builtin_amdgcn_readlane(mine.n, at),
+           __builtin_amdgcn_readlane(mine.slot, at)};
+      break;
+    }
+    before = __builtin_amdgcn_readlane(run, 63);
+  }
+  if (s < 0) return;
+  const int slot0 = (x.slot & ~15) + 16 * block;     // of the block
+  const int j0 = max(x.slot - slot0, 0), j1 = min(x.slot + x.n - slot0, 16);  // its slots
+  const int32_t page = c.tables[(int64_t)s * c.columns + (slot0 >> c.shift)];
+  if ((uint32_t)page >= (uint32_t)c.n_pages) return;
+  const float *rows = qkv + (int64_t)(x.first + (slot0 - x.slot)) * ldq + (int64_t)c.nh * HD;  // of slot0
+  const int j_in = slot0 & (c.page - 1);
+  // V: lane's channels CH lane .. of the 16 rows (past the ends: the nearest, not stored)
+  const float *v = rows + (int64_t)(c.nkv + h) * HD + CH * lane;
+  float y[16][CH];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int u = u0 + k * SIDE;
-    row[k].c = row[0].c;
-    row[k].s = row[0].s;
-    float y[4];
-    paged_turn<HD>(row[k], q, !(u & 1), y);
-    if (u >= units) continue;
-    const uint2 w = paged_round<BF>(y);
-    if (!(u & 1)) {
-      *(uint2 *)(c.kv + paged_k_at(c, page, u >> 1, j) + 4 * q) = w;
+  for (int j = 0; j < 16; ++j) {
+    const float *src = v + (int64_t)min(max(j, j0), j1 - 1) * ldq;
+    if constexpr (CH == 1) {
+      y[j][0] = *src;
+    } else if constexpr (CH == 2) {
+      const float2 w = *(const float2 *)src;
+      y[j][0] = w.x, y[j][1] = w.y;
     } else {
-      uint16_t *v = c.kv + paged_v_at(c, page, u >> 1, j) + 64 * q;
-      v[0] = (uint16_t)w.x;
-      v[16] = (uint16_t)(w.x >> 16);
-      v[32] = (uint16_t)w.y;
-      v[48] = (uint16_t)(w.y >> 16);
+      const float4 w = *(const float4 *)src;
+      y[j][0] = w.x, y[j][1] = w.y, y[j][2] = w.z, y[j][3] = w.w;
+    }
+  }
+  // K: 64 / LANES rows at a time
+  const float *k = rows + (int64_t)h * HD;
+  uint16_t *ko = c.kv + paged_k_at(c, page, h, j_in);
+#pragma unroll 8
+  for (int i = 0; i < 16; i += SIDE) {
+    const int j = i + lane / LANES, at = min(max(j, j0), j1 - 1);
+    Kv4Row<HD> row;
+    row.load(k + at * ldq, q);
+    row.load_turn(c.cs + (int64_t)(slot0 + at) * (HD / 2), c.sn + (int64_t)(slot0 + at) * (HD / 2), q);
+    float t[4];
+    paged_turn<HD>(row, q, true, t);
+    const uint2 w = paged_round<BF>(t);
+    if (j >= j0 && j < j1) *(uint2 *)(ko + j * HD + 4 * q) = w;
+  }
+  uint16_t *vo = c.kv + paged_v_at(c, page, h, j_in) + 16 * CH * lane;
+#pragma unroll
+  for (int e = 0; e < CH; ++e) {
+    uint2 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float four[4] = {y[4 * i][e], y[4 * i + 1][e], y[4 * i + 2][e], y[4 * i + 3][e]};
+      w[i] = paged_round<BF>(four);
+    }
+    if (j0 == 0 && j1 == 16) {
+      *(uint4 *)(vo + 16 * e) = make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
+      *(uint4 *)(vo + 16 * e + 8) = make_uint4(w[2].x, w[2].y, w[3].x, w[3].y);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j >= j0 && j < j1)
+          vo[16 * e + j] = (uint16_t)((j & 2 ? w[j >> 2].y : w[j >> 2].x) >> (16 * (j & 1)));
     }
   }
 }
@@ -438,14 +535,18 @@ __global__ __launch_bounds__(kThreads) void paged_compact_move_kernel(
 
 hipError_t launch_paged_append(const PagedCache &c, const float *qkv, int64_t ldq, int64_t n_rows,
                                const int64_t *starts, hipStream_t s) {
-  // few rows: as many waves as there are units; many: fewer waves with more in flight
-  const int n = n_rows * c.nkv >= 8192 ? 4 : 1, per = n * (256 / c.hd);
+  // By blocks where the sequences' rows fill some: 3281 rows of five sequences, 8 heads of 128,
+  // 26 us a row at a time.
+  if (n_rows >= 16 * (int64_t)c.n_seq) {
+    const dim3 blocks((unsigned)(n_rows / 16 + 2 * c.n_seq), (unsigned)((c.nkv + 3) / 4));
+    PAGED_DISPATCH(c, hipLaunchKernelGGL((paged_append_blocks_kernel<HD, BF>), blocks, dim3(kThreads),
+                                         0, s, c, qkv, ldq, n_rows, starts));
+    return hipGetLastError();
+  }
+  const int per = 256 / c.hd;
   const dim3 grid((unsigned)((n_rows + 3) / 4), (unsigned)((2 * c.nkv + per - 1) / per));
-  PAGED_DISPATCH(c, if (n == 4) hipLaunchKernelGGL((paged_append_kernel<HD, BF, 4>), grid,
-                                                   dim3(kThreads), 0, s, c, qkv, ldq,
-                                                   (uint32_t)n_rows, starts);
-                 else hipLaunchKernelGGL((paged_append_kernel<HD, BF, 1>), grid, dim3(kThreads), 0,
-                                         s, c, qkv, ldq, (uint32_t)n_rows, starts));
+  PAGED_DISPATCH(c, hipLaunchKernelGGL((paged_append_kernel<HD, BF>), grid, dim3(kThreads), 0, s, c,
+                                       qkv, ldq, (uint32_t)n_rows, starts));
   return hipGetLastError();
 }
 

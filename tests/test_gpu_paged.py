@@ -92,6 +92,12 @@ def _stored(table, slot, columns, page, n_pages, rope_rows, room=None):
     (8, 1, 256, 64, [30, 9], [2, 9, 12], 14, 33, None),                # RoPE tables end first
     (6, 2, 128, 16, [-1, 3, 20], None, 9, 150, [100, 5, -7]),          # the same number each; room
     (2, 2, 64, 16, [1, 1], [-(1 << 62), 3, 5], 6, 150, None),          # starts far before the rows
+    # by whole blocks: aligned and not, empty ones, padding rows, what ends first, many heads
+    (2, 2, 64, 16, [0, 16, 3, 9], [0, 32, 64, 64, 67], 70, 150, None),
+    (9, 9, 128, 32, [7, -1, 60], [-5, 20, 30, 61], 60, 70, None),
+    (8, 1, 256, 64, [30, 9], [2, 40, 102], 110, 230, [55, 1 << 40]),
+    (4, 4, 64, 16, [70, 2, 11], None, 90, 150, [80, -(1 << 62), 30]),
+    (2, 2, 64, 16, [1, 1, 5], [-(1 << 62), -3, 5, 1 << 62], 48, 150, None),
 ])
 def test_append_is_exact(paged, dtype, heads, kv, hd, page, lengths, starts, rows, rope, room):
     rng = np.random.default_rng(hd + rows)
