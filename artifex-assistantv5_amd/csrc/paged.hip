@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c,
 }
 
 // ---------------------------------------------------------------------------
-// Storing prompts: a wave takes the rows of one block of 16 slots, K and V of one KV head.  V's 16
+// Storing prompts: a wave takes the rows of one block of 16 slots, K or V of one KV head.  V's 16
 // slots of a channel are 32 bytes, which a lane has from its loads of the 16 rows; K's rows go as
 // they come.
 // ---------------------------------------------------------------------------
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_blocks_kernel(
     const int64_t *__restrict__ starts) {
   constexpr int LANES = Kv4Row<HD>::LANES, SIDE = 64 / LANES, CH = HD / 64;
   const int lane = threadIdx.x & 63, q = lane % LANES;
-  const int h = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6));
+  const int u = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6)), h = u >> 1;
   if (h >= c.nkv) return;
   // block blockIdx.x of the call: sequences in order
   int s = -1, block = 0;
@@ -127,6 +127,22 @@ __global__ __launch_bounds__(kThreads) void paged_append_blocks_kernel(
   if ((uint32_t)page >= (uint32_t)c.n_pages) return;
   const float *rows = qkv + (int64_t)(x.first + (slot0 - x.slot)) * ldq + (int64_t)c.nh * HD;  // of slot0
   const int j_in = slot0 & (c.page - 1);
+  if (!(u & 1)) {  // K: 64 / LANES rows at a time
+    const float *k = rows + (int64_t)h * HD;
+    uint16_t *ko = c.kv + paged_k_at(c, page, h, j_in);
+#pragma unroll 8
+    for (int i = 0; i < 16; i += SIDE) {
+      const int j = i + lane / LANES, at = min(max(j, j0), j1 - 1);
+      Kv4Row<HD> row;
+      row.load(k + at * ldq, q);
+      row.load_turn(c.cs + (int64_t)(slot0 + at) * (HD / 2), c.sn + (int64_t)(slot0 + at) * (HD / 2), q);
+      float t[4];
+      paged_turn<HD>(row, q, true, t);
+      const uint2 w = paged_round<BF>(t);
+      if (j >= j0 && j < j1) *(uint2 *)(ko + j * HD + 4 * q) = w;
+    }
+    return;
+  }
   // V: lane's channels CH lane .. of the 16 rows (past the ends: the nearest, not stored)
   const float *v = rows + (int64_t)(c.nkv + h) * HD + CH * lane;
   float y[16][CH];
@@ -142,20 +158,6 @@ __global__ __launch_bounds__(kThreads) void paged_append_blocks_kernel(
       const float4 w = *(const float4 *)src;
       y[j][0] = w.x, y[j][1] = w.y, y[j][2] = w.z, y[j][3] = w.w;
     }
-  }
-  // K: 64 / LANES rows at a time
-  const float *k = rows + (int64_t)h * HD;
-  uint16_t *ko = c.kv + paged_k_at(c, page, h, j_in);
-#pragma unroll 8
-  for (int i = 0; i < 16; i += SIDE) {
-    const int j = i + lane / LANES, at = min(max(j, j0), j1 - 1);
-    Kv4Row<HD> row;
-    row.load(k + at * ldq, q);
-    row.load_turn(c.cs + (int64_t)(slot0 + at) * (HD / 2), c.sn + (int64_t)(slot0 + at) * (HD / 2), q);
-    float t[4];
-    paged_turn<HD>(row, q, true, t);
-    const uint2 w = paged_round<BF>(t);
-    if (j >= j0 && j < j1) *(uint2 *)(ko + j * HD + 4 * q) = w;
   }
   uint16_t *vo = c.kv + paged_v_at(c, page, h, j_in) + 16 * CH * lane;
 #pragma unroll
@@ -538,7 +540,7 @@ hipError_t launch_paged_append(const PagedCache &c, const float *qkv, int64_t ld
   // By blocks where the sequences' rows fill some: 3281 rows of five sequences, 8 heads of 128,
   // 26 us a row at a time.
   if (n_rows >= 16 * (int64_t)c.n_seq) {
-    const dim3 blocks((unsigned)(n_rows / 16 + 2 * c.n_seq), (unsigned)((c.nkv + 3) / 4));
+    const dim3 blocks((unsigned)(n_rows / 16 + 2 * c.n_seq), (unsigned)((2 * c.nkv + 3) / 4));
     PAGED_DISPATCH(c, hipLaunchKernelGGL((paged_append_blocks_kernel<HD, BF>), blocks, dim3(kThreads),
                                          0, s, c, qkv, ldq, n_rows, starts));
     return hipGetLastError();

@@ -197,12 +197,13 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
                                                                       Cut cut) {
   constexpr int NB = HD / 32, CT = HD / 16, RS = record_floats<HD>(), half = HD / 2;
   constexpr int NP = Parts<BF, C>::N;
-  constexpr bool kInLds = HD == 256;  // the queries: in registers there would be too few
+  constexpr bool kInLds = HD == 256;  // the queries are read again each turn
   constexpr std::bool_constant<BF> bf{};
   constexpr float kLift = 10.f, kMost = 15.f;
   __shared__ __align__(16) float o_[W][8][HD];  // per wave and head its sums
   __shared__ float2 ml_[W][8];
-  __shared__ uint4 q_[kInLds ? NB : 1][NP][64];
+  __shared__ uint4 q_[NB][NP][64];  // queries: per block and operand
+  __shared__ float qc[16];
   __shared__ __align__(16) uint16_t fresh[2][HD];  // the new row's K and V
   Item it;
   if (!item_of(c, blockIdx.x, cut, it)) return;
@@ -254,20 +255,57 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
     for (int i = 0; i < CT; ++i) vf[i] = load16<STREAM>(v + 256 * i);
   };
 
-  // the queries: lane (r, g) channels 32 i + 8 g + 0 .. 7 of head r % C, whose RoPE partners are the
-  // same lane's of block i +- NB / 2
-  Parts<BF, C> qf[NB];
-  float f;  // log2 units per unit of an accumulated score
-  {
-    const int h = r % C;
+  // What comes before the barrier is requested before the unit, since loads return in order.  The
+  // first wave makes the queries: lane (r, g) channels 32 i + 8 g + 0 .. 7 of head r % C, whose RoPE
+  // partners are the same lane's of block i +- NB / 2.  The second one makes the new row, for its
+  // page and for the workgroup.
+  constexpr int LANES = Kv4Row<HD>::LANES, SIDE = 64 / LANES, N = (2 + SIDE - 1) / SIDE;
+  const int h = r % C, rq = lane % LANES;
+  const float *cr = c.cs + (int64_t)filled * half, *sr = c.sn + (int64_t)filled * half;
+  float4 xq[2 * NB], cq[NB], sq[NB];
+  Kv4Row<HD> own[N];
+  auto request = [&]() {
     const float *x = row + (int64_t)(kvh * grp + (h < grp ? h : 0)) * HD + 8 * g;
-    const float *cr = c.cs + (int64_t)filled * half + 8 * g, *sr = c.sn + (int64_t)filled * half + 8 * g;
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) xq[i] = *(const float4 *)(x + 32 * (i >> 1) + 4 * (i & 1));
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      cq[i] = *(const float4 *)(cr + 8 * g + 32 * (i >> 1) + 4 * (i & 1));
+      sq[i] = *(const float4 *)(sr + 8 * g + 32 * (i >> 1) + 4 * (i & 1));
+    }
+  };
+  constexpr bool kFirst = HD < 256;  // of 256 channels there are no registers for both
+  if (kFirst && wave == 0) request();
+  if (stores && wave == 1) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int u = min(n * SIDE + lane / LANES, 1);
+      own[n].load(row + (int64_t)(c.nh + u * c.nkv + kvh) * HD, rq);
+      own[n].load_turn(cr, sr, rq);
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  // from the last unit down: the new row's is some wave's first
+  int unit = unit1 - 1 - wave, p0 = 0, p1 = 0, n0 = 0, n1 = 0;
+  auto begin = [&]() {
+    if (unit < unit0) return;
+    ids(unit, p0, p1);
+    load_k(unit, p0, p1);
+    load_v(unit, p0, p1);
+    ids(max(unit - W, unit0), n0, n1);
+  };
+  if (kFirst) begin();
+  __builtin_amdgcn_sched_barrier(0);
+  if (wave == 0) {
+    if (!kFirst) request();
+    auto at = [](const float4 *w, int i) { return (&w[i >> 2].x)[i & 3]; };
     float y[NB][8], mx = 0.f;
 #pragma unroll
     for (int i = 0; i < NB / 2; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x1 = x[32 * i + j], x2 = x[32 * i + half + j], cv = cr[32 * i + j], sv = sr[32 * i + j];
+        const float x1 = at(xq, 8 * i + j), x2 = at(xq, 8 * (i + NB / 2) + j);
+        const float cv = at(cq, 8 * i + j), sv = at(sq, 8 * i + j);
         const float a1 = h < grp ? x1 * cv - x2 * sv : 0.f, a2 = h < grp ? x2 * cv + x1 * sv : 0.f;
         y[i][j] = fmaf(a1, ScoreScale<HD>::hi, a1 * ScoreScale<HD>::lo);
         y[i + NB / 2][j] = fmaf(a2, ScoreScale<HD>::hi, a2 * ScoreScale<HD>::lo);
@@ -276,53 +314,46 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
     mx = max_xor32(max_xor16(mx));
     const int e = BF ? 0 : stage_exp(mx);
     const float up = pow2f(e);
-    f = pow2f(-e);
+    if (g == 0) qc[r] = pow2f(-e);
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[i][j] *= up;
-      qf[i].make(y[i], r / C);
-      if (kInLds && wave == 0)
+      Parts<BF, C> w;
+      w.make(y[i], r / C);
 #pragma unroll
-        for (int k = 0; k < NP; ++k) q_[i][k][lane] = qf[i].w[k];
+      for (int k = 0; k < NP; ++k) q_[i][k][lane] = w.w[k];
     }
-  }
-  // the new row, by the first wave: to its page, and to the workgroup
-  if (stores && wave == 0) {
-    constexpr int LANES = Kv4Row<HD>::LANES, SIDE = 64 / LANES, N = (2 + SIDE - 1) / SIDE;
-    const int q = lane % LANES, j = filled & (c.page - 1);
+  } else if (stores && wave == 1) {
+    const int j = filled & (c.page - 1);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int u = min(n * SIDE + lane / LANES, 1);
-      Kv4Row<HD> x;
-      x.load(row + (int64_t)(c.nh + u * c.nkv + kvh) * HD, q);
-      x.load_turn(c.cs + (int64_t)filled * half, c.sn + (int64_t)filled * half, q);
+      const int u = n * SIDE + lane / LANES;
       float y[4];
-      paged_turn<HD>(x, q, u == 0, y);
+      paged_turn<HD>(own[n], rq, u == 0, y);
       const uint2 w = paged_round<BF>(y);
-      if (n * SIDE + lane / LANES < 2) {
-        *(uint2 *)(fresh[u] + 4 * q) = w;
-        if (u == 0) {
-          *(uint2 *)(c.kv + paged_k_at(c, own_page, kvh, j) + 4 * q) = w;
-        } else {
-          uint16_t *v = c.kv + paged_v_at(c, own_page, kvh, j) + 64 * q;
-          v[0] = (uint16_t)w.x;
-          v[16] = (uint16_t)(w.x >> 16);
-          v[32] = (uint16_t)w.y;
-          v[48] = (uint16_t)(w.y >> 16);
-        }
+      if (u == 0) {
+        *(uint2 *)(fresh[0] + 4 * rq) = w;
+        *(uint2 *)(c.kv + paged_k_at(c, own_page, kvh, j) + 4 * rq) = w;
+      } else if (u == 1) {
+        *(uint2 *)(fresh[1] + 4 * rq) = w;
+        uint16_t *v = c.kv + paged_v_at(c, own_page, kvh, j) + 64 * rq;
+        v[0] = (uint16_t)w.x;
+        v[16] = (uint16_t)(w.x >> 16);
+        v[32] = (uint16_t)w.y;
+        v[48] = (uint16_t)(w.y >> 16);
       }
     }
   }
-  // from the last unit down: the new row's is some wave's first
-  int unit = unit1 - 1 - wave, p0 = 0, p1 = 0, n0 = 0, n1 = 0;
-  if (unit >= unit0) {
-    ids(unit, p0, p1);
-    load_k(unit, p0, p1);
-    load_v(unit, p0, p1);
-    ids(max(unit - W, unit0), n0, n1);
-  }
+  if (!kFirst) begin();
   __syncthreads();
+  uint4 qf[kInLds ? 1 : NB][NP];
+  if (!kInLds)
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int k = 0; k < NP; ++k) qf[i][k] = q_[i][k][lane];
+  const float f = qc[r];  // log2 units per unit of an accumulated score
   if (stores && unit == filled / kUnit) {
     const int j = filled % kUnit, in = j & 15;
     if (j >> 4 == r >> 3) {
@@ -359,7 +390,7 @@ __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache
       for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int k = NP - 1; k >= 0; --k) {
-          const uint4 q = kInLds ? q_[i][k][ql] : qf[i].w[k];
+          const uint4 q = kInLds ? q_[i][k][ql] : qf[kInLds ? 0 : i][k];
           sc[0] = mfma(kf[0][i], q, sc[0], bf);
           sc[1] = mfma(kf[1][i], q, sc[1], bf);
         }
