@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 from .ggml import GGMLTypeError
 
@@ -110,6 +111,22 @@ SAMPLE_SIGNATURES = {
     "gguf_hip_sample_workspace": (_i64, [_i64, _i64]),
 }
 
+# Every symbol include/gguf_hip_packed.h declares, and the entry points it reaches: their number
+# there and the struct format of their arguments, the stream's handle last.
+PACKED_SIGNATURES = {"gguf_hip_packed_call": (_i32, [_i32, ctypes.c_char_p, _i64])}
+
+
+def _format(signature):
+    return struct.Struct("".join("f4x" if t is ctypes.c_float else ("Q" if t is _vp else "q")
+                                 for t in signature[1]))
+
+
+PACKED = ["gguf_hip_paged_append", "gguf_hip_paged_attention", "gguf_hip_paged_load",
+          "gguf_hip_paged_fork", "gguf_hip_paged_grow", "gguf_hip_paged_compact", "gguf_hip_sample"]
+(PAGED_APPEND, PAGED_ATTENTION, PAGED_LOAD, PAGED_FORK, PAGED_GROW, PAGED_COMPACT,
+ SAMPLE) = range(len(PACKED))
+_PACK = [_format({**PAGED_SIGNATURES, **SAMPLE_SIGNATURES}[name]).pack for name in PACKED]
+
 
 class GGUFHipError(RuntimeError):
     """A HIP runtime or launch failure reported by the library."""
@@ -149,7 +166,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
             "(the GGUF HIP path has no CPU fallback)")
     lib = ctypes.CDLL(p, mode=ctypes.RTLD_GLOBAL)
     for name, (res, args) in {**SIGNATURES, **KV4_SIGNATURES, **PAGED_SIGNATURES,
-                                **SAMPLE_SIGNATURES}.items():
+                                **SAMPLE_SIGNATURES, **PACKED_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
@@ -179,3 +196,20 @@ def check(rc: int, lib=None) -> int:
     if rc in (ERR_SHAPE, ERR_NULL, ERR_ALIGN, ERR_DTYPE, ERR_BYTES):
         raise ValueError(msg)
     raise GGUFHipError(rc, msg)
+
+
+def call(op: int, device: int, *args) -> None:
+    """Entry point ``PACKED[op]`` with ``args`` (addresses, 0 for none, and numbers) on the current
+    stream of ``device``, which need not be the current one.  The arguments go as one array of words:
+    passed one by one, they cost more than the call's checks and launches together."""
+    import torch  # loaded before the library anyway
+
+    packed = _PACK[op](*args, torch._C._cuda_getCurrentRawStream(device))
+    lib = _lib or load_library()
+    if torch._C._cuda_getDevice() == device:
+        rc = lib.gguf_hip_packed_call(op, packed, len(packed))
+    else:
+        with torch.cuda.device(device):
+            rc = lib.gguf_hip_packed_call(op, packed, len(packed))
+    if rc:
+        check(rc, lib)

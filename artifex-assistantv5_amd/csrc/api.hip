@@ -7,9 +7,15 @@
 // gguf-dequant.ts:678-680,837, forward-pass.ts:1486-1489,1524.
 #include <stdarg.h>
 #include <stdio.h>
+#include <string.h>
+
+#include <tuple>
+#include <type_traits>
+#include <utility>
 
 #include "common.hpp"
 #include "gguf_hip_kv4.h"
+#include "gguf_hip_packed.h"
 #include "gguf_hip_paged.h"
 #include "gguf_hip_sample.h"
 #include "kv4.hpp"
@@ -998,6 +1004,65 @@ int gguf_hip_sample(const float *logits, int64_t ld, int64_t rows, int64_t vocab
   const gguf::SampleArgs a{logits, ld, (int)rows, (int)vocab, u, temperature, top_k, top_p, min_p,
                            temperature_all, top_k_all, top_p_all, min_p_all, out, probs, work};
   return hip_status(gguf::launch_sample(a, (hipStream_t)stream), "sample launch");
+}
+
+// ---------------------------------------------------------------------------
+// Calls with their arguments as an array (gguf_hip_packed.h).
+// ---------------------------------------------------------------------------
+}  // extern "C"
+
+namespace {
+
+// A word as a parameter; `fits` is cleared where the parameter cannot hold it.
+template <typename T>
+T unpacked(const char *word, bool &fits) {
+  if constexpr (std::is_pointer_v<T>) {
+    T p;
+    memcpy(&p, word, sizeof p);
+    return p;
+  } else if constexpr (std::is_floating_point_v<T>) {
+    T v;
+    memcpy(&v, word, sizeof v);
+    return v;
+  } else {
+    int64_t v;
+    memcpy(&v, word, sizeof v);
+    fits = fits && (int64_t)(T)v == v;
+    return (T)v;
+  }
+}
+
+template <typename... T, size_t... I>
+int call_packed(int (*entry)(T...), const void *args, int64_t bytes, std::index_sequence<I...>) {
+  if (bytes != (int64_t)sizeof...(T) * 8)
+    return fail(GGUF_HIP_ERR_BYTES, "[gguf-hip] packed call: %lld bytes for %d arguments",
+                (long long)bytes, (int)sizeof...(T));
+  if (!args) return null_pointer();
+  bool fits = true;
+  const std::tuple<T...> t{unpacked<T>((const char *)args + 8 * I, fits)...};
+  if (!fits) return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] packed call: a number out of range");
+  return entry(std::get<I>(t)...);
+}
+template <typename... T>
+int call_packed(int (*entry)(T...), const void *args, int64_t bytes) {
+  return call_packed(entry, args, bytes, std::index_sequence_for<T...>{});
+}
+
+}  // namespace
+
+extern "C" {
+
+int gguf_hip_packed_call(int op, const void *args, int64_t bytes) {
+  switch (op) {
+    case GGUF_HIP_PACKED_PAGED_APPEND: return call_packed(gguf_hip_paged_append, args, bytes);
+    case GGUF_HIP_PACKED_PAGED_ATTENTION: return call_packed(gguf_hip_paged_attention, args, bytes);
+    case GGUF_HIP_PACKED_PAGED_LOAD: return call_packed(gguf_hip_paged_load, args, bytes);
+    case GGUF_HIP_PACKED_PAGED_FORK: return call_packed(gguf_hip_paged_fork, args, bytes);
+    case GGUF_HIP_PACKED_PAGED_GROW: return call_packed(gguf_hip_paged_grow, args, bytes);
+    case GGUF_HIP_PACKED_PAGED_COMPACT: return call_packed(gguf_hip_paged_compact, args, bytes);
+    case GGUF_HIP_PACKED_SAMPLE: return call_packed(gguf_hip_sample, args, bytes);
+    default: return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] packed call: unknown entry point %d", op);
+  }
 }
 
 }  // extern "C"

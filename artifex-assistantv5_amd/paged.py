@@ -29,11 +29,11 @@ from typing import Optional
 import torch
 
 from . import _native
-from .kv4 import _launch
 
 BLOCK = 16
 PAGES = (16, 32, 64, 128, 256)
 _DTYPES = {torch.float16: _native.PAGED_F16, torch.bfloat16: _native.PAGED_BF16}
+_call = _native.call
 
 
 def pool_bytes(n_pages: int, n_kv_heads: int, head_dim: int, page: int = 16) -> int:
@@ -59,64 +59,65 @@ def empty_tables(n_seq: int, columns: int, n_pages: int, device="cuda"):
             torch.zeros(n_pages, dtype=torch.int32, device=device))
 
 
-def _shape(kv: torch.Tensor, layers: bool = False):
-    """(layers, pages, KV heads, page, head_dim) of a pool."""
-    if kv.dtype not in _DTYPES or not kv.is_cuda or not kv.is_contiguous():
-        raise ValueError("paged: the pool must be a contiguous float16 or bfloat16 device tensor")
-    s = kv.shape
-    if len(s) == 6 and layers:
-        n_layers, s = s[0], s[1:]
-    elif len(s) == 5:
-        n_layers = 1
-    else:
-        raise ValueError(f"paged: pool of shape {tuple(kv.shape)}, need [{'layers, ' if layers else ''}"
-                         "n_pages, 2, n_kv_heads, page, head_dim]")
-    if s[1] != 2 or 0 in kv.shape:
+def _pool(kv: torch.Tensor, layers: bool = False):
+    """(device index, layers, pages, KV heads, page, head_dim) of a pool."""
+    shape = kv.shape
+    n_layers = 1
+    if layers and len(shape) == 6:
+        n_layers, *shape = shape
+    device = kv.get_device()
+    if len(shape) != 5 or device < 0 or kv.dtype not in _DTYPES or not kv.is_contiguous():
+        raise ValueError(f"paged: pool {kv.dtype} {tuple(kv.shape)} on {kv.device}, need a contiguous "
+                         f"float16 or bfloat16 device tensor [{'layers, ' if layers else ''}n_pages, "
+                         "2, n_kv_heads, page, head_dim]")
+    n_pages, two, n_kv, page, hd = shape
+    if two != 2 or not (n_layers and n_pages and n_kv and page and hd):
         raise ValueError(f"paged: pool of shape {tuple(kv.shape)} is not [.., n_pages, 2, ..]")
-    return n_layers, s[0], s[2], s[3], s[4]
+    return device, n_layers, n_pages, n_kv, page, hd
 
 
-def _tensor(name: str, t: torch.Tensor, dtype, shape, device) -> int:
-    if t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"paged: {name} must be a contiguous {dtype} tensor {tuple(shape)} on "
-                         f"{device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+# Checks in as few steps as they need: a call of several of them costs more than its launches.
+def _array(name: str, t: torch.Tensor, dtype, shape, device: int) -> int:
+    if (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == device):
+        return t.data_ptr()
+    raise ValueError(f"paged: {name} must be a contiguous {dtype} tensor {tuple(shape)} on device "
+                     f"{device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _tables(tables: torch.Tensor, device):
+def _tables(tables: torch.Tensor, device: int):
     if tables.dim() != 2:
         raise ValueError("paged: tables must be [n_seq, columns]")
-    n_seq, columns = tables.shape
-    return n_seq, columns, _tensor("tables", tables, torch.int32, (n_seq, columns), device)
+    shape = tables.shape
+    return *shape, _array("tables", tables, torch.int32, shape, device)
 
 
-def _row_matrix(name: str, t: torch.Tensor, width: int, device) -> int:
-    """The row stride of f32 rows of at least ``width`` values (unit column stride)."""
-    if t.dtype != torch.float32 or t.device != device or t.dim() != 2 or t.shape[1] < width:
-        raise ValueError(f"paged: {name} must be float32 rows of at least {width} values on {device}")
-    n, columns = t.shape
-    ld, step = t.stride()
-    if n <= 1:
-        ld = columns
-    if step != 1 or ld < columns:
-        raise ValueError(f"paged: {name} must be rows with unit column stride")
-    return ld
+def _row_matrix(name: str, t: torch.Tensor, rows: int, width: int, device: int):
+    """The address and row stride of ``rows`` f32 rows of at least ``width`` values (any number of
+    them: -1)."""
+    if t.dtype is torch.float32 and t.dim() == 2 and t.get_device() == device:
+        n, columns = t.shape
+        ld, step = t.stride()
+        if n <= 1:
+            ld = columns
+        if columns >= width and step == 1 and ld >= columns and (n == rows or rows < 0):
+            return t.data_ptr(), ld
+    raise ValueError(f"paged: {name} must be {rows if rows >= 0 else ''} float32 rows of at least "
+                     f"{width} values with unit column stride on device {device}, got {t.dtype} "
+                     f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
 
-def _rows(qkv, lengths, tables, cos, sin, kv, n_heads, room):
-    """The checks that append and attention share, and their arguments."""
-    _, n_pages, n_kv, page, hd = _shape(kv)
-    dev = kv.device
-    ld = _row_matrix("qkv", qkv, (n_heads + 2 * n_kv) * hd, dev)
-    n_seq, columns, tp = _tables(tables, dev)
+def _rope(cos: torch.Tensor, sin: torch.Tensor, hd: int, device: int):
     if cos.dim() != 2:
         raise ValueError("paged: cos and sin must be [positions, head_dim / 2]")
-    rope = (cos.shape[0], hd // 2)
-    return (n_seq, columns, n_pages, n_kv, page, hd, ld, tp,
-            _tensor("lengths", lengths, torch.int64, (n_seq,), dev),
-            None if room is None else _tensor("room", room, torch.int64, (n_seq,), dev),
-            _tensor("cos", cos, torch.float32, rope, dev),
-            _tensor("sin", sin, torch.float32, rope, dev))
+    shape = (len(cos), hd // 2)
+    return (_array("cos", cos, torch.float32, shape, device),
+            _array("sin", sin, torch.float32, shape, device), shape[0])
+
+
+def _work(work: torch.Tensor, device: int):
+    if work.get_device() != device or not work.is_contiguous():
+        raise ValueError("paged: the workspace must be a contiguous tensor on the pool's device")
+    return work.data_ptr(), work.nbytes
 
 
 def append(qkv: torch.Tensor, lengths: torch.Tensor, tables: torch.Tensor, cos: torch.Tensor,
@@ -130,29 +131,25 @@ def append(qkv: torch.Tensor, lengths: torch.Tensor, tables: torch.Tensor, cos: 
     goes to slot ``lengths[s] + i``; rows outside every sequence, without a page, past the tables
     or ``room[s]`` (``grow``) are not stored, nor those of a sequence of negative length.
     ``lengths`` is the caller's to advance.  One launch."""
-    n_seq, columns, n_pages, n_kv, page, hd, ld, tp, lp, mp, cp, sp = _rows(
-        qkv, lengths, tables, cos, sin, kv, n_heads, room)
-    st = None if starts is None else _tensor("starts", starts, torch.int64, (n_seq + 1,), kv.device)
-    _launch(_native.load_library().gguf_hip_paged_append, kv.device, qkv.data_ptr(), ld,
-            qkv.shape[0], st, lp, mp, tp, cp, sp, cos.shape[0], kv.data_ptr(), _DTYPES[kv.dtype],
-            n_pages, page, columns, n_seq, n_heads, n_kv, hd)
+    dev, _, n_pages, n_kv, page, hd = _pool(kv)
+    qp, ld = _row_matrix("qkv", qkv, -1, (n_heads + 2 * n_kv) * hd, dev)
+    n_seq, columns, tp = _tables(tables, dev)
+    lp = _array("lengths", lengths, torch.int64, (n_seq,), dev)
+    mp = 0 if room is None else _array("room", room, torch.int64, (n_seq,), dev)
+    st = 0 if starts is None else _array("starts", starts, torch.int64, (n_seq + 1,), dev)
+    _call(_native.PAGED_APPEND, dev, qp, ld, len(qkv), st, lp, mp, tp, *_rope(cos, sin, hd, dev),
+          kv.data_ptr(), _DTYPES[kv.dtype], n_pages, page, columns, n_seq, n_heads, n_kv, hd)
     return kv
 
 
 def attention_workspace(kv: torch.Tensor, tables: torch.Tensor, n_heads: int) -> torch.Tensor:
     """Device workspace of ``attention`` calls over such tables."""
-    _, _, n_kv, page, hd = _shape(kv)
-    n_seq, columns, _ = _tables(tables, kv.device)
+    dev, _, _, n_kv, page, hd = _pool(kv)
+    n_seq, columns, _ = _tables(tables, dev)
     lib = _native.load_library()
     n = _native.check(lib.gguf_hip_paged_attention_workspace(page, columns, n_seq, n_heads, n_kv, hd),
                       lib)
     return torch.empty(n, dtype=torch.uint8, device=kv.device)
-
-
-def _work(work: torch.Tensor, device):
-    if work.device != device or not work.is_contiguous():
-        raise ValueError("paged: the workspace must be a contiguous tensor on the pool's device")
-    return work.data_ptr(), work.numel() * work.element_size()
 
 
 def attention(qkv: torch.Tensor, lengths: torch.Tensor, tables: torch.Tensor, cos: torch.Tensor,
@@ -163,16 +160,15 @@ def attention(qkv: torch.Tensor, lengths: torch.Tensor, tables: torch.Tensor, co
     Row s is stored in slot ``lengths[s]`` and attends to slots ``0 .. lengths[s]``, of which those
     without a page are not seen.  A sequence whose row cannot be stored (negative length, no page,
     past the tables or ``room[s]``) takes no part: nothing of it is written."""
-    n_seq, columns, n_pages, n_kv, page, hd, ld, tp, lp, mp, cp, sp = _rows(
-        qkv, lengths, tables, cos, sin, kv, n_heads, room)
-    ldo = _row_matrix("out", out, n_heads * hd, kv.device)
-    if qkv.shape[0] != n_seq or out.shape[0] != n_seq:
-        raise ValueError(f"paged: qkv has {qkv.shape[0]} rows and out {out.shape[0]} for {n_seq} "
-                         "sequences")
-    wp, wb = _work(work, kv.device)
-    _launch(_native.load_library().gguf_hip_paged_attention, kv.device, qkv.data_ptr(), ld, lp, mp,
-            tp, cp, sp, cos.shape[0], kv.data_ptr(), _DTYPES[kv.dtype], out.data_ptr(), ldo, n_pages,
-            page, columns, n_seq, n_heads, n_kv, hd, wp, wb)
+    dev, _, n_pages, n_kv, page, hd = _pool(kv)
+    n_seq, columns, tp = _tables(tables, dev)
+    qp, ld = _row_matrix("qkv", qkv, n_seq, (n_heads + 2 * n_kv) * hd, dev)
+    op, ldo = _row_matrix("out", out, n_seq, n_heads * hd, dev)
+    lp = _array("lengths", lengths, torch.int64, (n_seq,), dev)
+    mp = 0 if room is None else _array("room", room, torch.int64, (n_seq,), dev)
+    _call(_native.PAGED_ATTENTION, dev, qp, ld, lp, mp, tp, *_rope(cos, sin, hd, dev), kv.data_ptr(),
+          _DTYPES[kv.dtype], op, ldo, n_pages, page, columns, n_seq, n_heads, n_kv, hd,
+          *_work(work, dev))
     return out
 
 
@@ -182,20 +178,14 @@ def load(kv: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, k_out: t
     ``k_out`` / ``v_out`` ``[n_seq, n_kv_heads, out_slots, head_dim]``.  Rows from ``lengths[s]`` on,
     and of slots without a page, are not written.  For one sequence this is the layout of
     ``glue.attention_prefill``'s caches.  One launch."""
-    _, n_pages, n_kv, page, hd = _shape(kv)
-    n_seq, columns, tp = _tables(tables, kv.device)
+    dev, _, n_pages, n_kv, page, hd = _pool(kv)
+    n_seq, columns, tp = _tables(tables, dev)
     shape = (n_seq, n_kv, k_out.shape[-2] if k_out.dim() > 1 else 0, hd)
-    kp = _tensor("k_out", k_out, torch.float32, shape, kv.device)
-    vp = _tensor("v_out", v_out, torch.float32, shape, kv.device)
-    lp = _tensor("lengths", lengths, torch.int64, (n_seq,), kv.device)
-    _launch(_native.load_library().gguf_hip_paged_load, kv.device, kv.data_ptr(), _DTYPES[kv.dtype],
-            tp, lp, kp, vp, shape[2], n_pages, page, columns, n_seq, n_kv, hd)
-
-
-def _refs(refs: torch.Tensor, device) -> int:
-    if refs.dim() != 1:
-        raise ValueError("paged: refs must be [n_pages]")
-    return _tensor("refs", refs, torch.int32, refs.shape, device)
+    kp = _array("k_out", k_out, torch.float32, shape, dev)
+    vp = _array("v_out", v_out, torch.float32, shape, dev)
+    lp = _array("lengths", lengths, torch.int64, (n_seq,), dev)
+    _call(_native.PAGED_LOAD, dev, kv.data_ptr(), _DTYPES[kv.dtype], tp, lp, kp, vp, shape[2],
+          n_pages, page, columns, n_seq, n_kv, hd)
 
 
 def fork(tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor,
@@ -206,27 +196,24 @@ def fork(tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, parent
     it is, a parent outside the sequences (-1) frees it.  In place, or into the ``*_out`` tensors,
     which must not overlap the inputs.  No page is copied: ``grow`` does that before a shared one
     is written.  One launch, or two where ``refs_out`` is another tensor and large."""
-    dev = tables.device
-    tables_out = tables if tables_out is None else tables_out
-    lengths_out = lengths if lengths_out is None else lengths_out
-    refs_out = refs if refs_out is None else refs_out
-    if not tables.is_cuda:
-        raise ValueError("paged: tables must be a device tensor")
+    dev = tables.get_device()
+    if dev < 0 or refs.dim() != 1:
+        raise ValueError("paged: tables must be a device tensor, refs [n_pages]")
     n_seq, columns, tp = _tables(tables, dev)
-    lp = _tensor("lengths", lengths, torch.int64, (n_seq,), dev)
-    rp = _refs(refs, dev)
-    pp = _tensor("parents", parents, torch.int64, (n_seq,), dev)
-    to = _tensor("tables_out", tables_out, torch.int32, tables.shape, dev)
-    lo = _tensor("lengths_out", lengths_out, torch.int64, (n_seq,), dev)
-    ro = _tensor("refs_out", refs_out, torch.int32, refs.shape, dev)
-    _launch(_native.load_library().gguf_hip_paged_fork, dev, tp, lp, rp, pp, to, lo, ro,
-            refs.shape[0], columns, n_seq)
+    n, pages = (n_seq,), refs.shape
+    lp = _array("lengths", lengths, torch.int64, n, dev)
+    rp = _array("refs", refs, torch.int32, pages, dev)
+    pp = _array("parents", parents, torch.int64, n, dev)
+    to = tp if tables_out is None else _array("tables_out", tables_out, torch.int32, tables.shape, dev)
+    lo = lp if lengths_out is None else _array("lengths_out", lengths_out, torch.int64, n, dev)
+    ro = rp if refs_out is None else _array("refs_out", refs_out, torch.int32, pages, dev)
+    _call(_native.PAGED_FORK, dev, tp, lp, rp, pp, to, lo, ro, pages[0], columns, n_seq)
 
 
 def grow_workspace(kv: torch.Tensor, tables: torch.Tensor) -> torch.Tensor:
     """Device workspace of ``grow`` calls over such a pool and tables."""
-    _, n_pages, _, page, _ = _shape(kv, layers=True)
-    n_seq, columns, _ = _tables(tables, kv.device)
+    dev, _, n_pages, _, page, _ = _pool(kv, layers=True)
+    n_seq, columns, _ = _tables(tables, dev)
     lib = _native.load_library()
     n = _native.check(lib.gguf_hip_paged_grow_workspace(n_pages, page, columns, n_seq), lib)
     return torch.empty(n, dtype=torch.uint8, device=kv.device)
@@ -241,22 +228,21 @@ def grow(kv: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, refs: to
     entries hold too, into whose new page the blocks of 16 slots in use are copied.  ``room[s]``
     becomes the end of the slots that the sequence may write, ``lengths[s]`` at least: less than
     was asked for where the pool has no free page left.  Two launches."""
-    n_layers, n_pages, n_kv, page, hd = _shape(kv, layers=True)
-    dev = kv.device
+    dev, n_layers, n_pages, n_kv, page, hd = _pool(kv, layers=True)
     n_seq, columns, tp = _tables(tables, dev)
-    lp = _tensor("lengths", lengths, torch.int64, (n_seq,), dev)
-    rp = _tensor("refs", refs, torch.int32, (n_pages,), dev)
-    np_ = _tensor("rows", rows, torch.int64, (n_seq,), dev)
-    mp = _tensor("room", room, torch.int64, (n_seq,), dev)
-    wp, wb = _work(work, dev)
-    _launch(_native.load_library().gguf_hip_paged_grow, dev, kv.data_ptr(), tp, lp, rp, np_, mp,
-            n_layers, n_pages, page, columns, n_seq, n_kv, hd, wp, wb)
+    n = (n_seq,)
+    lp = _array("lengths", lengths, torch.int64, n, dev)
+    rp = _array("refs", refs, torch.int32, (n_pages,), dev)
+    np_ = _array("rows", rows, torch.int64, n, dev)
+    mp = _array("room", room, torch.int64, n, dev)
+    _call(_native.PAGED_GROW, dev, kv.data_ptr(), tp, lp, rp, np_, mp, n_layers, n_pages, page,
+          columns, n_seq, n_kv, hd, *_work(work, dev))
 
 
 def compact_workspace(kv: torch.Tensor, tables: torch.Tensor) -> torch.Tensor:
     """Device workspace of ``compact`` calls over such a pool and tables."""
-    _, n_pages, _, _, _ = _shape(kv, layers=True)
-    n_seq, columns, _ = _tables(tables, kv.device)
+    dev, _, n_pages, _, _, _ = _pool(kv, layers=True)
+    n_seq, columns, _ = _tables(tables, dev)
     lib = _native.load_library()
     n = _native.check(lib.gguf_hip_paged_compact_workspace(n_pages, columns, n_seq), lib)
     return torch.empty(n, dtype=torch.uint8, device=kv.device)
@@ -269,15 +255,12 @@ def compact(kv: torch.Tensor, tables: torch.Tensor, refs: torch.Tensor, live: to
     here) of the pool: those behind them, in order, into the free ones among them, in order.
     ``tables`` and ``refs`` follow, in place or into the ``*_out`` tensors, which must not overlap
     the inputs.  Two launches."""
-    n_layers, n_pages, n_kv, page, hd = _shape(kv, layers=True)
-    dev = kv.device
-    tables_out = tables if tables_out is None else tables_out
-    refs_out = refs if refs_out is None else refs_out
+    dev, n_layers, n_pages, n_kv, page, hd = _pool(kv, layers=True)
     n_seq, columns, tp = _tables(tables, dev)
-    rp = _tensor("refs", refs, torch.int32, (n_pages,), dev)
-    lp = _tensor("live", live, torch.int64, (1,), dev)
-    to = _tensor("tables_out", tables_out, torch.int32, tables.shape, dev)
-    ro = _tensor("refs_out", refs_out, torch.int32, refs.shape, dev)
-    wp, wb = _work(work, dev)
-    _launch(_native.load_library().gguf_hip_paged_compact, dev, kv.data_ptr(), tp, rp, to, ro, lp,
-            n_layers, n_pages, page, columns, n_seq, n_kv, hd, wp, wb)
+    pages = (n_pages,)
+    rp = _array("refs", refs, torch.int32, pages, dev)
+    lp = _array("live", live, torch.int64, (1,), dev)
+    to = tp if tables_out is None else _array("tables_out", tables_out, torch.int32, tables.shape, dev)
+    ro = rp if refs_out is None else _array("refs_out", refs_out, torch.int32, pages, dev)
+    _call(_native.PAGED_COMPACT, dev, kv.data_ptr(), tp, rp, to, ro, lp, n_layers, n_pages, page,
+          columns, n_seq, n_kv, hd, *_work(work, dev))

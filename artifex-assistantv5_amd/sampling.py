@@ -15,7 +15,6 @@ from typing import Optional, Union
 import torch
 
 from . import _native
-from .kv4 import _launch
 
 
 def workspace(rows: int, vocab: int, device="cuda") -> torch.Tensor:
@@ -25,18 +24,18 @@ def workspace(rows: int, vocab: int, device="cuda") -> torch.Tensor:
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-def _array(name: str, t: torch.Tensor, dtype, rows: int, device) -> int:
-    if t.dtype != dtype or t.device != device or t.shape != (rows,) or not t.is_contiguous():
-        raise ValueError(f"sample: {name} must be a contiguous {dtype} tensor of {rows} values on "
-                         f"{device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+def _array(name: str, t: torch.Tensor, dtype, shape, device: int) -> int:
+    if (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == device):
+        return t.data_ptr()
+    raise ValueError(f"sample: {name} must be a contiguous {dtype} tensor {tuple(shape)} on device "
+                     f"{device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _setting(name: str, v, dtype, rows: int, device):
-    """(pointer or None, value for every row) of a setting."""
+def _setting(name: str, v, dtype, shape, device: int):
+    """The address of a setting (0: the same for every row), and its value."""
     if isinstance(v, torch.Tensor):
-        return _array(name, v, dtype, rows, device), 0
-    return None, v
+        return _array(name, v, dtype, shape, device), 0
+    return 0, v
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, out: torch.Tensor, work: torch.Tensor,
@@ -51,7 +50,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, out: torch.Tensor, work: torch
     the first of the largest.  ``probs`` (f32 ``[rows]``): the drawn tokens' probabilities among
     the kept ones.  ``work``: from ``workspace``, for calls that do not overlap.  Allocates and
     synchronises nothing."""
-    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda:
+    dev = logits.get_device()
+    if logits.dim() != 2 or logits.dtype is not torch.float32 or dev < 0:
         raise ValueError("sample: logits must be float32 device rows [rows, vocab]")
     rows, vocab = logits.shape
     ld, step = logits.stride()
@@ -59,18 +59,16 @@ def sample(logits: torch.Tensor, u: torch.Tensor, out: torch.Tensor, work: torch
         ld = max(vocab, 1)
     if (vocab > 1 and step != 1) or ld < vocab:
         raise ValueError("sample: logits must be rows with unit column stride")
-    dev = logits.device
-    up = _array("u", u, torch.float32, rows, dev)
-    op = _array("out", out, torch.int64, rows, dev)
-    tp, tv = _setting("temperature", temperature, torch.float32, rows, dev)
-    kp, kv = _setting("top_k", top_k, torch.int32, rows, dev)
-    pp, pv = _setting("top_p", top_p, torch.float32, rows, dev)
-    mp, mv = _setting("min_p", min_p, torch.float32, rows, dev)
-    qp = None if probs is None else _array("probs", probs, torch.float32, rows, dev)
-    if work.device != dev or not work.is_contiguous():
+    n = (rows,)
+    up = _array("u", u, torch.float32, n, dev)
+    op = _array("out", out, torch.int64, n, dev)
+    tp, tv = _setting("temperature", temperature, torch.float32, n, dev)
+    kp, kv = _setting("top_k", top_k, torch.int32, n, dev)
+    pp, pv = _setting("top_p", top_p, torch.float32, n, dev)
+    mp, mv = _setting("min_p", min_p, torch.float32, n, dev)
+    qp = 0 if probs is None else _array("probs", probs, torch.float32, n, dev)
+    if work.get_device() != dev or not work.is_contiguous():
         raise ValueError("sample: the workspace must be a contiguous tensor on the logits' device")
-    kv = max(0, min(int(kv), 2 ** 31 - 1))
-    _launch(_native.load_library().gguf_hip_sample, dev, logits.data_ptr(), ld, rows, vocab, up, tp,
-            tv, kp, kv, pp, pv, mp, mv, op, qp, work.data_ptr(),
-            work.numel() * work.element_size())
+    _native.call(_native.SAMPLE, dev, logits.data_ptr(), ld, rows, vocab, up, tp, tv, kp,
+                 max(0, min(int(kv), 2 ** 31 - 1)), pp, pv, mp, mv, op, qp, work.data_ptr(), work.nbytes)
     return out

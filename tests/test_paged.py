@@ -196,3 +196,39 @@ def test_python_refusals_without_device_tensors(pkg):
         paged.grow_workspace(kv, t)
     with pytest.raises(ValueError, match="device tensor"):
         paged.fork(t, n, r, n)
+
+
+def _words(native, op, *args):
+    return native._PACK[op](*args)
+
+
+def test_packed_calls(lib, native):
+    """The entry points by number: their own refusals, and those of the array."""
+    with open(os.path.join(ROOT, "include", "gguf_hip_packed.h"), encoding="utf-8") as f:
+        text = f.read()
+    assert re.findall(r"^int\s+(gguf_hip_\w+)\(", text, re.M) == list(native.PACKED_SIGNATURES)
+    d = {m[0].lower(): int(m[1]) for m in re.findall(r"#define\s+GGUF_HIP_PACKED_(\w+)\s+(\d+)", text)}
+    assert d == {n[len("gguf_hip_"):]: i for i, n in enumerate(native.PACKED)}
+    call = lib.gguf_hip_packed_call
+    fork = [A, B, C, D, A, B, C, 10, 4, 2, 0]
+    for change, want in (({7: 0}, native.ERR_SHAPE), ({9: 0}, native.ERR_SHAPE),
+                         ({0: 0}, native.ERR_NULL), ({1: B + 4}, native.ERR_ALIGN),
+                         ({9: 1 << 32}, native.ERR_SHAPE), ({9: -(1 << 31) - 1}, native.ERR_SHAPE)):
+        words = _words(native, native.PAGED_FORK, *[change.get(i, v) for i, v in enumerate(fork)])
+        assert call(native.PAGED_FORK, words, len(words)) == want, change
+    assert "out of range" in native.last_error(lib)
+    words = _words(native, native.PAGED_FORK, *fork)
+    assert call(native.PAGED_FORK, words, len(words) - 8) == native.ERR_BYTES
+    assert call(native.PAGED_FORK, None, len(words)) == native.ERR_NULL
+    for op in (-1, len(native.PACKED)):
+        assert call(op, words, len(words)) == native.ERR_SHAPE
+    # every entry point takes as many words as it has arguments
+    for op, name in enumerate(native.PACKED):
+        signature = {**native.PAGED_SIGNATURES, **native.SAMPLE_SIGNATURES}[name][1]
+        zeros = bytes(8 * len(signature))
+        assert call(op, zeros, len(zeros)) in (native.ERR_SHAPE, 0), name
+        assert call(op, zeros, len(zeros) + 8) == native.ERR_BYTES, name
+    # floats and integers arrive as they are: the settings come after the counts that are refused
+    sample = [A, 10, 2, 10, A, 0, 0.7, 0, 3, 0, 0.5, 0, 0.25, A, 0, W, 0, 0]
+    words = _words(native, native.SAMPLE, *sample)
+    assert call(native.SAMPLE, words, len(words)) == native.ERR_BYTES     # its workspace of 0 bytes
