@@ -17,7 +17,10 @@ reference's WebGPU engine (``webgpu/src/engine/forward-pass.ts``):
 * ``parse_gguf``            — GGUF header / KV / tensor table (gguf.ts:241-299)
 * ``load_gguf_model``       — place a GGUF file's tensors in HBM (gguf-loader.ts:166-460)
 * ``load_decoder``          — a llama-architecture GGUF file as a ``QuantDecoder``
+* ``load_batch_decoder``    — such a file as a ``BatchDecoder`` of several sequences
 * ``kv4`` (module)          — a KV cache held in 4 bits: attention over it, eviction
+* ``paged`` (module)        — a KV cache in pages that sequences share: attention, forks, compaction
+* ``sampling`` (module)     — a token per row of logits by temperature, top-k, top-p and min-p
 
 Importing this package does not touch the GPU; the native library is loaded
 on first use and a missing or unbuilt library raises immediately.
@@ -31,12 +34,12 @@ from .linear import (GGUFWeight, LayerWeights, QuantEmbedding, concat_rows,  # n
                      interleave_tiles, qlinear, repack_gguf_for_gpu, split_interleaved)
 from .gguf_file import parse_gguf, parse_gguf_path, write_gguf  # noqa: F401
 from .gguf_loader import load_gguf_model  # noqa: F401
-from .gguf_model import load_decoder  # noqa: F401
+from .gguf_model import load_batch_decoder, load_decoder  # noqa: F401
 from ._native import GGUFHipError, load_library  # noqa: F401
 
 __all__ = [
     "GGML_TYPES", "GGMLTypeError", "GGUFHipError", "GGUFWeight", "LayerWeights",
-    "QuantEmbedding", "load_decoder", "load_gguf_model", "parse_gguf", "parse_gguf_path",
+    "QuantEmbedding", "load_batch_decoder", "load_decoder", "load_gguf_model", "parse_gguf", "parse_gguf_path",
     "write_gguf",
     "concat_rows", "interleave_tiles", "split_interleaved", "dequant_ggml", "dequant_raw", "dispatch_matmul_gguf",
     "dispatch_projection", "ggml_tensor_bytes", "ggml_type_traits", "load_library",

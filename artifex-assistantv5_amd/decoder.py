@@ -5,7 +5,7 @@ per-layer loop of webgpu/src/engine/forward-pass.ts:2925-3297 (input RMSNorm,
 Q/K/V projections, rotate_half RoPE, GQA causal attention over a KV cache,
 output projection and residual, FFN RMSNorm, gate+up projection, gate_silu,
 down projection and residual), the final norm and LM head
-(forward-pass.ts:3642-3644), and greedy argmax sampling.
+(forward-pass.ts:3642-3644), and greedy argmax or drawn tokens (``sampling``).
 
 Glue semantics follow the reference's shaders:
 * RMSNorm  ``x * 1/sqrt(mean(x^2) + eps) * w``           rmsnorm.wgsl:1-9,58-67
@@ -51,7 +51,7 @@ from typing import Optional, Union
 import numpy as np
 import torch
 
-from . import glue, kv4, quantize
+from . import glue, kv4, quantize, sampling
 from .ggml import FUSED_TYPES, Q4_K, Q6_K, TILE_ROWS, raw_row_bytes
 from .linear import (GGUFWeight, LayerWeights, QuantEmbedding, concat_rows, dispatch_matmul_gguf,
                      interleave_tiles, repack_gguf_for_gpu, split_interleaved)
@@ -244,8 +244,71 @@ def kv_cache_slots(cfg: DecoderConfig, fused: bool, kv_bits: int, kv_slots: Opti
     return slots
 
 
-class QuantDecoder:
-    """Greedy decoder over ``DecoderWeights`` with an f32 or 4-bit KV cache in HBM.
+class LayerStack:
+    """The layers of a decoder over many rows: ``cfg``, ``w`` (``DecoderWeights``) and ``device``,
+    and ``_attend_rows`` of the subclass, which holds the cache."""
+
+    cfg: DecoderConfig
+    w: DecoderWeights
+    device: torch.device
+
+    def _attend_rows(self, l: int, qkv: torch.Tensor, pos: torch.Tensor, att: torch.Tensor,
+                     held: int) -> None:
+        """Attention of layer l's rows ``[q | k | v]`` into ``att``."""
+        raise NotImplementedError
+
+    def _proj(self, x: torch.Tensor, w: GGUFWeight, label: str) -> torch.Tensor:
+        M = x.shape[0]
+        y = torch.empty(M, w.n, device=self.device)
+        dispatch_matmul_gguf(x, w, y, M, w.n, w.k, label)
+        return y
+
+    def _proj_slot(self, x: torch.Tensor, lw: LayerWeights, slot: str, label: str) -> torch.Tensor:
+        ws = parts(lw, slot)
+        if len(ws) == 1:
+            return self._proj(x, ws[0], label)
+        return torch.cat([self._proj(x, w, f"{label}{i}") for i, w in enumerate(ws)], dim=1)
+
+    def _embed(self, tok: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        e = self.w.embed
+        if isinstance(e, QuantEmbedding):
+            return e.gather(tok, out)
+        x = e.index_select(0, tok).float()
+        if out is None:
+            return x
+        out.copy_(x)
+        return out
+
+    def _layers_glue(self, x: torch.Tensor, pos: torch.Tensor, held: int = 0) -> torch.Tensor:
+        """All layers over the M rows of ``x`` (updated in place) with the glue as
+        libgguf_hip kernels; returns the rows after the final RMSNorm.  ``pos`` and ``held``
+        (the slots in use before the rows) are ``_attend_rows``'s."""
+        cfg, layers = self.cfg, self.w.layers
+        M = x.shape[0]
+        h = torch.empty_like(x)
+        att = torch.empty(M, cfg.n_heads * cfg.head_dim, device=self.device)
+        a = torch.empty(M, cfg.ffn, device=self.device)
+        glue.rmsnorm(x, layers[0].attn_norm, cfg.eps, h)
+        for l, lw in enumerate(layers):
+            qkv = self._proj_slot(h, lw, "qkv", f"L{l}-qkv")
+            self._attend_rows(l, qkv, pos, att, held)
+            glue.add_rmsnorm(x, self._proj(att, lw.o_gg, f"L{l}-o"), lw.ffn_norm, cfg.eps, h)
+            w = lw.get("gateUpI_gg")
+            if w is not None:  # tile-interleaved gate / up columns -> [gate | up] rows, one copy
+                gu = torch.empty(M, 2, cfg.ffn // TILE_ROWS, TILE_ROWS, device=self.device)
+                gu.copy_(self._proj(h, w, f"L{l}-gateUp").view(M, -1, 2, TILE_ROWS).transpose(1, 2))
+                gu = gu.view(M, 2 * cfg.ffn)
+            else:
+                gu = self._proj_slot(h, lw, "gateUp", f"L{l}-gateUp")
+            glue.swiglu(gu, a)
+            nxt = layers[l + 1].attn_norm if l + 1 < len(layers) else self.w.final_norm
+            glue.add_rmsnorm(x, self._proj(a, lw.down_gg, f"L{l}-down"), nxt, cfg.eps, h)
+        return h
+
+
+class QuantDecoder(LayerStack):
+    """Decoder of one sequence over ``DecoderWeights`` with an f32 or 4-bit KV cache in HBM; its
+    tokens are the largest logits' or drawn (``set_sampling``).
 
     ``kv_bits`` 4: ``kv_slots`` (default: enough for ``max_seq``) slots per KV head, rounded up
     to a multiple of 32; ``kv_keep``: a full cache is cut back to that many slots, of which the
@@ -287,6 +350,31 @@ class QuantDecoder:
         if kv_bits == 32:
             self.w_att = glue.attention_workspace(cfg.n_heads, cfg.n_kv_heads, hd, T, self.device)
         self.w_arg = glue.argmax_workspace(self.device)
+        self._draw = None
+
+    # -- the choice of the next token --
+    def set_sampling(self, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
+                     min_p: float = 0.0, seed: int = 0) -> None:
+        """How the next tokens are chosen (``sampling.sample``); ``temperature`` 0: the largest
+        logit.  The random numbers, one for each position, follow from ``seed``.  Steps captured
+        before keep the choice that they were captured with."""
+        if not temperature > 0:
+            self._draw = None
+            return
+        g = torch.Generator(device=self.device).manual_seed(seed)
+        self._draw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        self._u = torch.rand(self.cfg.max_seq, device=self.device, generator=g)
+        self._u_now = torch.empty(1, device=self.device)
+        self._w_draw = sampling.workspace(1, self.cfg.vocab, self.device)
+
+    def _choose(self, logits: torch.Tensor, tok: torch.Tensor, pos: torch.Tensor) -> None:
+        """The token after position ``pos`` [1] into ``tok`` [1], by ``logits`` [1, vocab]."""
+        if self._draw is None:
+            glue.argmax(logits, tok, self.w_arg)
+            return
+        # a step past the last position has NaN logits or no meaning, but no index out of range
+        torch.index_select(self._u, 0, pos.clamp(0, self._u.numel() - 1), out=self._u_now)
+        sampling.sample(logits, self._u_now, tok, self._w_draw, **self._draw)
 
     # -- the 4-bit cache --
     def _init_kv4(self, slots, keep, recent, sinks) -> None:
@@ -381,19 +469,7 @@ class QuantDecoder:
                 held = self.kv_keep
         return self._proj(h[-1:], self.w.lm_head_gg, "lm_head")
 
-    # -- one pass of all layers over M tokens at positions ``pos`` (device [M]) --
-    def _proj(self, x: torch.Tensor, w: GGUFWeight, label: str) -> torch.Tensor:
-        M = x.shape[0]
-        y = torch.empty(M, w.n, device=self.device)
-        dispatch_matmul_gguf(x, w, y, M, w.n, w.k, label)
-        return y
-
-    def _proj_slot(self, x: torch.Tensor, lw: LayerWeights, slot: str, label: str) -> torch.Tensor:
-        ws = parts(lw, slot)
-        if len(ws) == 1:
-            return self._proj(x, ws[0], label)
-        return torch.cat([self._proj(x, w, f"{label}{i}") for i, w in enumerate(ws)], dim=1)
-
+    # -- one pass of all layers over M tokens at positions ``pos`` (device [M]) as torch ops --
     def _gate_up(self, h: torch.Tensor, lw: LayerWeights, label: str):
         """(gate, up) projections of the FFN input ``h``."""
         w = lw.get("gateUpI_gg")
@@ -401,16 +477,6 @@ class QuantDecoder:
             return split_interleaved(self._proj(h, w, label))
         gu = self._proj_slot(h, lw, "gateUp", label)
         return gu[:, :self.cfg.ffn], gu[:, self.cfg.ffn:]
-
-    def _embed(self, tok: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        e = self.w.embed
-        if isinstance(e, QuantEmbedding):
-            return e.gather(tok, out)
-        x = e.index_select(0, tok).float()
-        if out is None:
-            return x
-        out.copy_(x)
-        return out
 
     def _layers(self, x: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         cfg = self.cfg
@@ -441,32 +507,6 @@ class QuantDecoder:
             a = up * torch.nn.functional.silu(gate)
             x = x + self._proj(a, lw.down_gg, f"L{l}-down")
         return x
-
-    def _layers_glue(self, x: torch.Tensor, pos: torch.Tensor, held: int = 0) -> torch.Tensor:
-        """All layers over the M rows of ``x`` (updated in place) with the glue as
-        libgguf_hip kernels; returns the rows after the final RMSNorm.  ``held``: the
-        slots of a 4-bit cache in use before the rows."""
-        cfg, layers = self.cfg, self.w.layers
-        M = x.shape[0]
-        h = torch.empty_like(x)
-        att = torch.empty(M, cfg.n_heads * cfg.head_dim, device=self.device)
-        a = torch.empty(M, cfg.ffn, device=self.device)
-        glue.rmsnorm(x, layers[0].attn_norm, cfg.eps, h)
-        for l, lw in enumerate(layers):
-            qkv = self._proj_slot(h, lw, "qkv", f"L{l}-qkv")
-            self._attend_rows(l, qkv, pos, att, held)
-            glue.add_rmsnorm(x, self._proj(att, lw.o_gg, f"L{l}-o"), lw.ffn_norm, cfg.eps, h)
-            w = lw.get("gateUpI_gg")
-            if w is not None:  # tile-interleaved gate / up columns -> [gate | up] rows, one copy
-                gu = torch.empty(M, 2, cfg.ffn // TILE_ROWS, TILE_ROWS, device=self.device)
-                gu.copy_(self._proj(h, w, f"L{l}-gateUp").view(M, -1, 2, TILE_ROWS).transpose(1, 2))
-                gu = gu.view(M, 2 * cfg.ffn)
-            else:
-                gu = self._proj_slot(h, lw, "gateUp", f"L{l}-gateUp")
-            glue.swiglu(gu, a)
-            nxt = layers[l + 1].attn_norm if l + 1 < len(layers) else self.w.final_norm
-            glue.add_rmsnorm(x, self._proj(a, lw.down_gg, f"L{l}-down"), nxt, cfg.eps, h)
-        return h
 
     def _logits(self, x_last: torch.Tensor) -> torch.Tensor:
         h = rms_norm(x_last, self.w.final_norm, self.cfg.eps)
@@ -537,7 +577,7 @@ class QuantDecoder:
                                   accumulate=True)
         glue.matmul_fused(x, W.lm_head_gg, self.b_logits, glue.PROLOGUE_RMSNORM, W.final_norm,
                           cfg.eps)
-        glue.argmax(self.b_logits, tok, self.w_arg)
+        self._choose(self.b_logits, tok, pos)
         if self.kv_bits == 32:
             pos.add_(1)
             return self.b_logits
@@ -558,7 +598,7 @@ class QuantDecoder:
 
     @torch.no_grad()
     def step(self, tok: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
-        """One greedy decode step in place: reads token ``tok`` [1] at position
+        """One decode step in place: reads token ``tok`` [1] at position
         ``pos`` [1], writes the next token into ``tok`` and advances ``pos``.
         Touches no host state, so it can be captured in a graph.  With a 4-bit cache ``pos``
         is the position after the last one; a step for which it has no slot left stores
@@ -568,7 +608,10 @@ class QuantDecoder:
         x = self._embed(tok)
         x = self._layers(x, pos)
         logits = self._logits(x)
-        tok.copy_(torch.argmax(logits, dim=-1))
+        if self._draw is None:
+            tok.copy_(torch.argmax(logits, dim=-1))
+        else:
+            self._choose(logits, tok, pos)
         pos.add_(1)
         return logits
 
@@ -598,10 +641,14 @@ class QuantDecoder:
         self._graph = g
 
     @torch.no_grad()
-    def generate(self, prompt: torch.Tensor, n_new: int, graph: bool = True) -> dict:
-        """Greedy generation: returns the new token ids and prefill / decode timings.
-        tok/s = n_new / decode wall time (prefill excluded, generate.ts:1155-1160)."""
+    def generate(self, prompt: torch.Tensor, n_new: int, graph: bool = True,
+                 temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                 seed: int = 0) -> dict:
+        """Generation, greedy or sampled (``set_sampling``): returns the new token ids and prefill /
+        decode timings.  tok/s = n_new / decode wall time (prefill excluded,
+        generate.ts:1155-1160)."""
         dev = self.device
+        self.set_sampling(temperature, top_k, top_p, min_p, seed)
         if prompt.numel() + n_new > self.cfg.max_seq:
             raise ValueError(f"prompt {prompt.numel()} + {n_new} new tokens exceed max_seq "
                              f"{self.cfg.max_seq}")
@@ -616,6 +663,8 @@ class QuantDecoder:
         t0 = time.perf_counter()
         logits = self.prefill(prompt, 0)
         tok = torch.argmax(logits, dim=-1).view(1)
+        if self._draw is not None:
+            self._choose(logits, tok, torch.full((1,), prompt.numel() - 1, dtype=torch.long, device=dev))
         torch.cuda.synchronize(dev)
         t_prefill = time.perf_counter() - t0
         pos = torch.full((1,), prompt.numel(), dtype=torch.long, device=dev)

@@ -1,4 +1,4 @@
-"""Build a ``QuantDecoder`` from a GGUF model file.
+"""Build a ``QuantDecoder`` or a ``BatchDecoder`` from a GGUF model file.
 
 The reference maps GGUF tensor names onto its layer slots when it loads a
 model (``webgpu/src/model/gguf-loader.ts``, slots of
@@ -28,6 +28,7 @@ from typing import Optional, Tuple
 import numpy as np
 import torch
 
+from .batch_decoder import BatchDecoder, check_batch
 from .decoder import DecoderConfig, DecoderWeights, QuantDecoder, glue_shapes, kv_cache_slots
 from .ggml import GGML_TYPE_NAMES
 from .gguf_file import GGUFFile, GGUFTensorInfo, arch_kv, gguf_architecture, parse_gguf_path
@@ -90,12 +91,35 @@ def load_decoder(path: str, device="cuda", max_seq: int = 2048, fused: bool = Tr
                  kv_sinks: int = 4) -> Tuple[QuantDecoder, LoadedGGUFModel]:
     """Load a llama-architecture GGUF file into a ``QuantDecoder`` on ``device``, with the
     decoder's KV cache options, which are checked before the tensors are placed."""
-    file = parse_gguf_path(path)
-    cfg = config_from_gguf(file, max_seq)
-    _check_tensors(file, cfg)
+    cfg, file = _config(path, max_seq)
     cache = dict(kv_bits=kv_bits, kv_slots=kv_slots, kv_keep=kv_keep, kv_recent=kv_recent,
                  kv_sinks=kv_sinks)
     kv_cache_slots(cfg, fused and glue_shapes(cfg), **cache)
+    weights, loaded = _weights(path, file, cfg, device, on_progress)
+    return QuantDecoder(cfg, weights, device=device, fused=fused, **cache), loaded
+
+
+def load_batch_decoder(path: str, n_seq: int, device="cuda", max_seq: int = 2048, on_progress=None,
+                       n_pages: Optional[int] = None, page: int = 16,
+                       dtype: torch.dtype = torch.float16) -> Tuple[BatchDecoder, LoadedGGUFModel]:
+    """Load a llama-architecture GGUF file into a ``BatchDecoder`` on ``device``, whose options are
+    checked before the tensors are placed."""
+    cfg, file = _config(path, max_seq)
+    check_batch(cfg, n_seq, n_pages, page, dtype)
+    weights, loaded = _weights(path, file, cfg, device, on_progress)
+    return BatchDecoder(cfg, weights, n_seq, n_pages, page, dtype, device), loaded
+
+
+def _config(path: str, max_seq: int) -> Tuple[DecoderConfig, GGUFFile]:
+    file = parse_gguf_path(path)
+    cfg = config_from_gguf(file, max_seq)
+    _check_tensors(file, cfg)
+    return cfg, file
+
+
+def _weights(path: str, file: GGUFFile, cfg: DecoderConfig, device,
+             on_progress) -> Tuple[DecoderWeights, LoadedGGUFModel]:
+    """The file's tensors on ``device`` in a decoder's slots (and ``cfg.rope_freq_factors``)."""
     dev = torch.device(device)
     perms = {}
     for l in range(cfg.n_layers):
@@ -174,5 +198,4 @@ def load_decoder(path: str, device="cuda", max_seq: int = 2048, fused: bool = Tr
     if isinstance(embed, QuantEmbedding) and (embed.n, embed.k) != (cfg.vocab, d):
         raise ValueError(f"[GGUF] token_embd.weight is [{embed.n}, {embed.k}], expected "
                          f"[{cfg.vocab}, {d}]")
-    weights = DecoderWeights(layers, vec("output_norm.weight", d), lm, embed)
-    return QuantDecoder(cfg, weights, device=dev, fused=fused, **cache), loaded
+    return DecoderWeights(layers, vec("output_norm.weight", d), lm, embed), loaded
