@@ -20,7 +20,7 @@ constexpr int kRanked = 256;   // up to so many by counting, for each, those bef
 constexpr int kFewest = 512;   // a top_k of up to so many needs no bins' masses
 constexpr int kChunks = 64;
 constexpr double kOne = 0x1p43;     // a weight of 1
-constexpr double kNothing = -44.0;  // the exponent from which on a weight is 0
+constexpr double kNothing = -44.0 * 32;  // the exponent (below) from which on a weight is 0
 
 // Larger is drawn earlier; -0 is +0, NaN and -inf are 0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -35,43 +35,48 @@ __device__ __forceinline__ uint64_t place(uint32_t key, uint32_t index) {
   return (uint64_t)key << 32 | (uint32_t)~index;
 }
 
-// 2^y of y <= 0 to within 2^-50: 2^f, |f| <= 1/2, by its Taylor series to ln(2)^11 f^11 / 11!, whose
-// rest is below 6e-15.
-__device__ __forceinline__ double pow2(double y) {
-  const double n = __builtin_rint(y), f = (y - n) * 0.69314718055994530942;
-  double p = 1.0 / 39916800;
-  p = fma(p, f, 1.0 / 3628800);
-  p = fma(p, f, 1.0 / 362880);
-  p = fma(p, f, 1.0 / 40320);
-  p = fma(p, f, 1.0 / 5040);
-  p = fma(p, f, 1.0 / 720);
-  p = fma(p, f, 1.0 / 120);
-  p = fma(p, f, 1.0 / 24);
-  p = fma(p, f, 1.0 / 6);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
-  p = fma(p, f, 1.0);
-  return __builtin_ldexp(p, (int)n);
-}
-
+// A row's weights: exponents are log2 of a token's weight, in units of 1 / 32; kLeast and below
+// (nothing to draw, too) is a weight of 0 in the sums.
+constexpr double kLeast = -60.0 * 32;
 struct Row {
-  double scale;  // log2(e) / temperature
+  double scale;  // 32 log2(e) / temperature
   float top;     // the largest logit
 };
-// log2 of a token's weight, -inf for none.
 __device__ __forceinline__ double exponent(const Row &r, uint32_t key) {
-  const float x = key_value(key);
-  if (x == r.top) return 0.0;  // infinite ones too
-  const double d = ((double)x - (double)r.top) * r.scale;
-  return key && d > -INFINITY ? d : -INFINITY;
+  const float x = key_value(key);  // of key 0 a NaN
+  const double d = x == r.top ? 0.0 : ((double)x - (double)r.top) * r.scale;  // infinite ones too
+  return d > kLeast ? d : kLeast;
 }
-__device__ __forceinline__ double weight(double e) { return e > -1000.0 ? pow2(e) : 0.0; }
-// In multiples of 2^-43: below 2^52, adding 2^52 leaves the nearest integer in the low bits.
+// 2^(y / 32): by a table (in LDS) of 2^(j / 32) and the Taylor series of 2^(f / 32), |f| <= 1/2, to its
+// fifth power, whose rest is below 3e-15.  The coefficients are held in scalar registers.
+struct Powers {
+  const double *table;
+  double c5 = 1.0 / 120, c4 = 1.0 / 24, c3 = 1.0 / 6, c2 = 0.5, ln = 0.69314718055994530942 / 32;
+  __device__ __forceinline__ explicit Powers(const double *t) : table(t) {
+    asm volatile("" : "+s"(c5), "+s"(c4), "+s"(c3), "+s"(c2), "+s"(ln));
+  }
+  // by all threads, before a barrier
+  static __device__ __forceinline__ void fill(double *table) {
+    if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x / 32.0);
+  }
+  __device__ __forceinline__ double operator()(double y) const {
+    const double n = __builtin_rint(y), f = (y - n) * ln;
+    const int k = (int)n;
+    const uint64_t t = (uint64_t)__double_as_longlong(table[k & 31]);
+    const double at = __longlong_as_double((long long)(t + ((uint64_t)(uint32_t)(k >> 5) << 52)));
+    double p = fma(c5, f, c4);
+    p = fma(p, f, c3);
+    p = fma(p, f, c2);
+    p = fma(p, f, 1.0);
+    return fma(at * f, p, at);
+  }
+};
+// A weight in multiples of 2^-43: below 2^52, adding 2^52 leaves the nearest integer in the low bits.
 __device__ __forceinline__ uint64_t fixed(double w) {
   return (uint64_t)__double_as_longlong(fma(w, kOne, 0x1p52)) & 0xFFFFFFFFFFFFFull;
 }
-__device__ __forceinline__ uint64_t mass_of(const Row &r, uint32_t key) {
-  return fixed(weight(exponent(r, key)));
+__device__ __forceinline__ uint64_t mass_of(const Row &r, const Powers &pow2, uint32_t key) {
+  return fixed(pow2(exponent(r, key)));
 }
 
 // Sums and maxima over lanes by DPP shifts within rows of 16, then the rows' ends.  A lane without a
@@ -228,7 +233,7 @@ __device__ __forceinline__ Bins bins_of(const SampleArgs &a, int row, const Chun
   b.t = a.temperature ? steady(a.temperature + row) : a.temperature_all;
   b.first = wave_max(c.first);
   const uint32_t least = wave_max(c.least);
-  b.r.scale = 1.4426950408889634074 / (double)b.t;
+  b.r.scale = 32 * 1.4426950408889634074 / (double)b.t;
   b.r.top = key_value((uint32_t)(b.first >> 32));
   const double range = fmin(-exponent(b.r, ~least), -kNothing);
   b.per = range > 0.0 ? (kBins - 1) / range : 0.0;
@@ -250,6 +255,7 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a, 
   __shared__ uint64_t partm[kWaves];
   __shared__ __align__(16) uint16_t order[T * kThreads];
   __shared__ uint32_t wanted, fewest;
+  __shared__ double table[32];
   const int row = blockIdx.y, tid = threadIdx.x, i0 = blockIdx.x * T * kThreads;
   const float *x = a.logits + row * a.ld;
   constexpr int L = T < 8 ? T : 8;  // tokens of a thread in flight
@@ -265,6 +271,8 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a, 
   const bool counts_only = few(top_k);
   for (int k = tid; k < kBins; k += kThreads) count[k] = 0, mass[k] = 0;
   if (tid == 0) fewest = ~0u;
+  Powers::fill(table);
+  const Powers pow2(table);
   const Bins b = bins_of(a, row, own);
   if (!b.first || !(b.t > 0.f)) return;  // nothing to draw, or no draw
   __syncthreads();
@@ -279,7 +287,7 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a, 
     const int k = bin_of(b, e);
     rank[j] = atomicAdd(&count[k], 1u) | (uint32_t)k << 16;
     if (counts_only) continue;
-    const double v = weight(e);
+    const double v = pow2(e);
     const uint64_t m = fixed(v);
     if (m) atomicAdd(&mass[k], (unsigned long long)m);
     if (v >= (double)min_p) large += m;
@@ -329,7 +337,8 @@ struct Goal {
     return count ? c >= count : (more ? (double)m > mass : (double)m >= mass);
   }
 };
-__device__ Found find_by_digits(const SampleArgs &a, int row, const Row &r, const Goal &enough,
+__device__ Found find_by_digits(const SampleArgs &a, int row, const Row &r, const Powers &pow2,
+                                const Goal &enough,
                                 uint32_t *count, unsigned long long *mass, uint32_t *part,
                                 uint64_t *partm, Found *found) {
   const float *x = a.logits + row * a.ld;
@@ -348,7 +357,7 @@ __device__ Found find_by_digits(const SampleArgs &a, int row, const Row &r, cons
       if (sh + bits < 64 && (p >> (sh + bits)) != (prefix >> (sh + bits))) continue;
       const int k = (int)(p >> sh) & ((1 << bits) - 1);
       atomicAdd(&count[k], 1u);
-      const uint64_t m = mass_of(r, key);
+      const uint64_t m = mass_of(r, pow2, key);
       if (m) atomicAdd(&mass[k], (unsigned long long)m);
     }
     __syncthreads();
@@ -369,7 +378,7 @@ __device__ Found find_by_digits(const SampleArgs &a, int row, const Row &r, cons
     above = s_above;
     __syncthreads();
   }
-  return {prefix, above_m + mass_of(r, (uint32_t)(prefix >> 32))};
+  return {prefix, above_m + mass_of(r, pow2, (uint32_t)(prefix >> 32))};
 }
 
 // Tokens in order: those of a run of bins, or of a part of one.
@@ -389,6 +398,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
   __shared__ Found found;
   __shared__ int found_bin;
   __shared__ uint32_t appended;
+  __shared__ double table[32];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, chunks = cut.chunks;
   const float *x = a.logits + row * a.ld;
   const int64_t lists = (int64_t)row * chunks;
@@ -397,6 +407,8 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
   const float min_p = a.min_p ? steady(a.min_p + row) : a.min_p_all;
   float u = steady(a.u + row);
   u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
+  Powers::fill(table);
+  const Powers pow2(table);
   // the row's bins: half of the threads take every other chunk
   const Chunk own = chunk_of(w, row, chunks);
   uint64_t large = w.large[lists + min(lane, chunks - 1)];
@@ -510,7 +522,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       const int i = tid + j * kThreads;
-      if (i < in.n) next[i] = mass_of(b.r, (uint32_t)(list[i] >> 32));
+      if (i < in.n) next[i] = mass_of(b.r, pow2, (uint32_t)(list[i] >> 32));
     }
     __syncthreads();
 #pragma unroll
@@ -560,7 +572,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
     for (int j = tid; j < of.n; j += kThreads) {
       const uint32_t key = (uint32_t)(list[j] >> 32), k = (hi - key) / per;
       atomicAdd(&counts[k], 1u);
-      atomicAdd(&masses[k], (unsigned long long)mass_of(b.r, key));
+      atomicAdd(&masses[k], (unsigned long long)mass_of(b.r, pow2, key));
     }
     __syncthreads();
     const uint32_t cs = tid < kBins ? counts[tid] : 0;
@@ -592,7 +604,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
       Sorted of{before, k ? (uint64_t)mass[k - 1] : 0, (int)(count[k] - before)};
       if (all) of = {0, 0, (int)count[k]};
       if (by_digits || of.n > kSorted)
-        return find_by_digits(a, row, b.r, enough, counts, masses, part, partm, &found);
+        return find_by_digits(a, row, b.r, pow2, enough, counts, masses, part, partm, &found);
       gather(all ? 0 : k, k, of.n);
       if (!all && of.n > kRanked) of = narrow(of, enough);
       sort(of.n);
@@ -619,7 +631,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
           large = 0;
           const int n = all ? in.n : a.vocab;
           for (int i = tid; i < n; i += kThreads) {
-            const double v = weight(exponent(b.r, all ? (uint32_t)(list[i] >> 32) : order_key(x[i])));
+            const double v = pow2(exponent(b.r, all ? (uint32_t)(list[i] >> 32) : order_key(x[i])));
             if (v >= (double)min_p) large += fixed(v);
           }
           large = wave_sum(large);
@@ -645,7 +657,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
   }
   if (tid == 0) {
     a.out[row] = (uint32_t)~(uint32_t)f.place;
-    if (a.probs) a.probs[row] = (float)((double)mass_of(b.r, (uint32_t)(f.place >> 32)) / (double)total);
+    if (a.probs) a.probs[row] = (float)((double)mass_of(b.r, pow2, (uint32_t)(f.place >> 32)) / (double)total);
   }
 }
 
