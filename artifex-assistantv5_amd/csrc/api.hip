@@ -924,7 +924,7 @@ int gguf_hip_paged_grow(void *kv, int32_t *tables, const int64_t *lengths, int32
   if (n_layers <= 0 || n_layers > 65535)
     return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: %d layers not in 1..65535", n_layers);
   if (!kv || !tables || !lengths || !refs || !rows || !room) return null_pointer();
-  if (!aligned(kv, 16) || !aligned(tables, 4) || !aligned(lengths, 8) || !aligned(refs, 4) ||
+  if (!aligned(kv, 16) || !aligned(tables, 4) || !aligned(lengths, 8) || !aligned(refs, 16) ||
       !aligned(rows, 8) || !aligned(room, 8))
     return misaligned_pages();
   if ((rc = check_paged_work("paged_grow", work, work_bytes, need))) return rc;
@@ -956,7 +956,7 @@ int gguf_hip_paged_compact(void *kv, const int32_t *tables, const int32_t *refs,
   if (n_layers <= 0 || n_layers > 65535)
     return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged: %d layers not in 1..65535", n_layers);
   if (!kv || !tables || !refs || !tables_out || !refs_out || !live) return null_pointer();
-  if (!aligned(kv, 16) || !aligned(tables, 4) || !aligned(refs, 4) || !aligned(tables_out, 4) ||
+  if (!aligned(kv, 16) || !aligned(tables, 4) || !aligned(refs, 16) || !aligned(tables_out, 4) ||
       !aligned(refs_out, 4) || !aligned(live, 8))
     return misaligned_pages();
   if (partly(tables, tables_out, 4 * columns * n_seq) || partly(refs, refs_out, 4 * n_pages))

@@ -303,11 +303,33 @@ __device__ __forceinline__ int sum_before(int v, int *part, int &all) {
   return before + run - v;
 }
 
+// Of the M pages from i0 on (below n), those whose refs are as asked: a bit each.  A thread of the
+// kernels below takes one, 16 of a pool of more than four turns: 40000 pages are then three turns.
+constexpr int kFewPages = 4 * kGrowThreads;
+template <int M, typename F>
+__device__ __forceinline__ uint32_t pages_by(const int32_t *refs, int i0, int n, F is) {
+  uint32_t mask = 0;
+  if constexpr (M == 1) {
+    if (i0 < n) mask = is(refs[i0]);
+  } else if (i0 + M <= n) {
+    int4 v[M / 4];
+#pragma unroll
+    for (int j = 0; j < M / 4; ++j) v[j] = *(const int4 *)(refs + i0 + 4 * j);
+#pragma unroll
+    for (int j = 0; j < M / 4; ++j)
+      mask |= (uint32_t)(is(v[j].x) | is(v[j].y) << 1 | is(v[j].z) << 2 | is(v[j].w) << 3) << (4 * j);
+  } else {
+    for (int j = 0; i0 + j < n; ++j) mask |= (uint32_t)is(refs[i0 + j]) << j;
+  }
+  return mask;
+}
+
 // refs as the atomics of earlier turns left it (they act behind the first cache).
 __device__ __forceinline__ int32_t current(const int32_t *p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+template <int M>
 __global__ __launch_bounds__(kGrowThreads) void paged_grow_kernel(PagedPool c, int32_t *tables,
                                                                   const int64_t *lengths,
                                                                   int32_t *refs,
@@ -315,7 +337,7 @@ __global__ __launch_bounds__(kGrowThreads) void paged_grow_kernel(PagedPool c, i
                                                                   int64_t *room, GrowJob *jobs) {
   __shared__ int ends[kGrowSeqs];        // entries of the sequences up to this one
   __shared__ int32_t held[kGrowThreads];  // the turn's pages that others hold too, -1: none
-  __shared__ int32_t free_[2 * kGrowThreads];
+  __shared__ int32_t free_[kGrowThreads];
   __shared__ int part[kGrowWaves];
   const int tid = threadIdx.x;
   const int64_t slots = (int64_t)c.columns << c.shift;
@@ -340,7 +362,7 @@ __global__ __launch_bounds__(kGrowThreads) void paged_grow_kernel(PagedPool c, i
     total += all;
   }
   __syncthreads();
-  int at = 0, have = 0, used = 0;  // refs read up to `at`; free_[used .. have) are free
+  int at = 0;  // no page below is free
   for (int e0 = 0; e0 < total; e0 += kGrowThreads) {
     const int e = e0 + tid;
     int s = 0, column = 0, refcount = 0;
@@ -375,34 +397,30 @@ __global__ __launch_bounds__(kGrowThreads) void paged_grow_kernel(PagedPool c, i
     const bool needs = e < total && (p < 0 || copies);
     int wanted;
     const int k = sum_before(needs, part, wanted);
-    // free pages for this turn, in order
-    if (have - used < wanted) {
-      __syncthreads();
-      int32_t keep = 0;
-      if (tid < have - used) keep = free_[used + tid];
-      __syncthreads();
-      if (tid < have - used) free_[tid] = keep;
-      have -= used;
-      used = 0;
-      while (have < wanted && at < c.n_pages) {
-        const int i = at + tid;
-        const bool is_free = i < c.n_pages && current(&refs[i]) <= 0;
+    // the first free pages, in order: as many as are wanted, or all that there are
+    int got = 0;
+    if (wanted) {
+      if (e0) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // not as the turn before read them
+      while (at < c.n_pages) {
+        const int i0 = at + tid * M;
+        uint32_t mask = pages_by<M>(refs, i0, c.n_pages, [](int32_t n) { return n <= 0; });
         int found;
-        const int rank = sum_before(is_free, part, found);
-        if (is_free) free_[have + rank] = i;
-        have += found;
-        at += kGrowThreads;
+        int rank = got + sum_before(__popc(mask), part, found);
+        for (; mask && rank < wanted; mask &= mask - 1) free_[rank++] = i0 + __builtin_ctz(mask);
+        if (got + found >= wanted) break;  // (the others of these pages are for the next turn)
+        got += found;
+        at += kGrowThreads * M;
       }
+      if (at < c.n_pages) got = wanted;
       __syncthreads();
     }
-    const int got = min(wanted, have - used);
     // an entry that keeps its page since the others leave it: if they all could
     const bool fails = (needs && k >= got) || (refcount > 1 && !copies && k > got);
     if (fails) {
       const int64_t n = lengths[s], start = (int64_t)column << c.shift;
       atomicMin((long long *)&room[s], (long long)(start < n ? n : start));
     } else if (needs) {
-      const int32_t f = free_[used + k];
+      const int32_t f = free_[k];
       tables[(int64_t)s * c.columns + column] = f;
       refs[f] = 1;
       if (copies) {
@@ -415,7 +433,7 @@ __global__ __launch_bounds__(kGrowThreads) void paged_grow_kernel(PagedPool c, i
         }
       }
     }
-    used += got;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // refs are what the next turn goes by
     __syncthreads();
   }
 }
@@ -448,27 +466,32 @@ __host__ __device__ __forceinline__ CompactWork compact_work(void *work, int n_p
   return {w, w + 4, w + 4 + n_pages, w + 4 + n_pages + half};
 }
 
+template <int M>
 __global__ __launch_bounds__(kGrowThreads) void paged_compact_plan_kernel(
     PagedPool c, const int32_t *refs, int32_t *refs_out, int64_t *live, CompactWork w) {
   __shared__ int part[kGrowWaves];
   const int tid = threadIdx.x;
+  auto used = [](int32_t r) { return r > 0; };
   int mine = 0, n;
-  for (int i = tid; i < c.n_pages; i += kGrowThreads) mine += refs[i] > 0;
+  for (int i0 = tid * M; i0 < c.n_pages; i0 += kGrowThreads * M)
+    mine += __popc(pages_by<M>(refs, i0, c.n_pages, used));
   sum_before(mine, part, n);
   int holes = 0, moves = 0;
-  for (int i0 = 0; i0 < c.n_pages; i0 += kGrowThreads) {
-    const int i = i0 + tid;
-    const int32_t r = i < c.n_pages ? refs[i] : 0;
-    const bool hole = i < n && r <= 0, move = i >= n && i < c.n_pages && r > 0;
+  for (int i1 = 0; i1 < c.n_pages; i1 += kGrowThreads * M) {
+    const int i0 = i1 + tid * M, below = min(max(n - i0, 0), M), in = min(max(c.n_pages - i0, 0), M);
+    const uint32_t mask = i0 < c.n_pages ? pages_by<M>(refs, i0, c.n_pages, used) : 0u;
+    const uint32_t low = (1u << below) - 1u;
+    uint32_t hole = ~mask & low, move = mask & ~low;  // (n is at most the number of pages)
     int all;
-    const int k = sum_before(hole | move << 16, part, all);
-    if (hole) w.dst[holes + (k & 0xFFFF)] = i;
-    if (move) w.src[moves + (k >> 16)] = i;
+    const int k = sum_before(__popc(hole) | __popc(move) << 16, part, all);
+    int h = holes + (k & 0xFFFF), m = moves + (k >> 16);
+    for (; hole; hole &= hole - 1) w.dst[h++] = i0 + __builtin_ctz(hole);
+    for (; move; move &= move - 1) w.src[m++] = i0 + __builtin_ctz(move);
     holes += all & 0xFFFF;
     moves += all >> 16;
-    if (i < c.n_pages) {
-      w.to[i] = i;
-      if (refs_out != refs) refs_out[i] = r;
+    for (int j = 0; j < in; ++j) {
+      w.to[i0 + j] = i0 + j;
+      if (refs_out != refs) refs_out[i0 + j] = refs[i0 + j];
     }
   }
   __syncthreads();
@@ -497,18 +520,18 @@ __global__ __launch_bounds__(kThreads) void paged_compact_move_kernel(
   const int64_t units = c.page_values / 8, layer = (int64_t)blockIdx.y * c.n_pages;
   constexpr int U = 4, kPiece = U * kThreads;
   const int pieces = (int)((units + kPiece - 1) / kPiece);
-  const uint4 *kv = (const uint4 *)c.kv;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 *kv = (u32x4 *)c.kv;
   for (int64_t x = blockIdx.x; x < (int64_t)moves * pieces; x += gridDim.x) {
     const int m = (int)(x / pieces), at = (int)(x % pieces) * kPiece + threadIdx.x;
-    const uint4 *src = kv + (layer + w.src[m]) * units;
-    uint4 *dst = (uint4 *)kv + (layer + w.dst[m]) * units;
-    uint4 v[U];
+    const u32x4 *src = kv + (layer + w.src[m]) * units;
+    u32x4 *dst = kv + (layer + w.dst[m]) * units;
+    u32x4 v[U];  // past the end: the last again, not stored
+#pragma unroll
+    for (int i = 0; i < U; ++i) v[i] = __builtin_nontemporal_load(src + min(at + i * kThreads, (int)units - 1));
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      if (at + i * kThreads < units) v[i] = src[at + i * kThreads];
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (at + i * kThreads < units) dst[at + i * kThreads] = v[i];
+      if (at + i * kThreads < units) __builtin_nontemporal_store(v[i], dst + at + i * kThreads);
   }
 }
 
@@ -588,8 +611,14 @@ hipError_t launch_paged_grow(const PagedPool &c, int32_t *tables, const int64_t 
                              int32_t *refs, const int64_t *rows, int64_t *room, void *work,
                              hipStream_t s) {
   GrowJob *jobs = (GrowJob *)work;
-  hipLaunchKernelGGL(paged_grow_kernel, dim3(1), dim3(kGrowThreads), 0, s, c, tables, lengths, refs,
-                     rows, room, jobs);
+  auto plan = [&](auto *kernel) {
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(kGrowThreads), 0, s, c, tables, lengths, refs, rows, room,
+                       jobs);
+  };
+  if (c.n_pages <= kFewPages)
+    plan(paged_grow_kernel<1>);
+  else
+    plan(paged_grow_kernel<16>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(paged_grow_copy_kernel, dim3(c.n_seq, 4, c.n_layers), dim3(kThreads), 0, s, c,
@@ -603,8 +632,13 @@ hipError_t launch_paged_compact(const PagedPool &c, const int32_t *tables, const
                                 int32_t *tables_out, int32_t *refs_out, int64_t *live, void *work,
                                 hipStream_t s) {
   const CompactWork w = compact_work(work, c.n_pages);
-  hipLaunchKernelGGL(paged_compact_plan_kernel, dim3(1), dim3(kGrowThreads), 0, s, c, refs, refs_out,
-                     live, w);
+  auto plan = [&](auto *kernel) {
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(kGrowThreads), 0, s, c, refs, refs_out, live, w);
+  };
+  if (c.n_pages <= kFewPages)
+    plan(paged_compact_plan_kernel<1>);
+  else
+    plan(paged_compact_plan_kernel<16>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   int x = 2048 / c.n_layers;

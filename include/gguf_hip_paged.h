@@ -106,6 +106,7 @@ int gguf_hip_paged_fork(const int32_t *tables, const int64_t *lengths, const int
  * are copied in all n_layers layers.  A sequence for which no free page is left gets no further
  * ones.  room[s]: the end of the slots that the sequence may now write, lengths[s] at least (0
  * where lengths[s] < 0); it is lengths[s] where rows[s] <= 0.  lengths is not changed.
+ * refs is 16-byte aligned.
  * Two launches.  work: gguf_hip_paged_grow_workspace bytes, 16-byte aligned, no initial value;
  * calls that share it must not overlap. */
 int gguf_hip_paged_grow(void *kv, int32_t *tables, const int64_t *lengths, int32_t *refs,
@@ -120,7 +121,7 @@ int64_t gguf_hip_paged_grow_workspace(int64_t n_pages, int page, int64_t columns
  * move, in order, into the free ones below n, in order; the others stay.  All n_layers layers
  * move alike; the bytes of the pages that were left stay.  Table entries and refs follow, to
  * tables_out and refs_out (each the same array as its input or one that overlaps no other);
- * live[0] (device int64) is n.  Two launches.  work: gguf_hip_paged_compact_workspace bytes,
+ * live[0] (device int64) is n.  refs is 16-byte aligned.  Two launches.  work: gguf_hip_paged_compact_workspace bytes,
  * 16-byte aligned, no initial value; calls that share it must not overlap. */
 int gguf_hip_paged_compact(void *kv, const int32_t *tables, const int32_t *refs,
                            int32_t *tables_out, int32_t *refs_out, int64_t *live, int n_layers,

@@ -380,6 +380,19 @@ def test_grow_many_sequences_and_entries(paged):
     _grow_case(paged, rng, tables, lengths.tolist(), refs, rng.integers(-1, 70, n).tolist(), 16, 1, kv=1)
 
 
+@pytest.mark.parametrize("free", [[39999], [3, 16383, 16384, 16385, 39000], list(range(20000, 22300))])
+def test_grow_in_a_large_pool(paged, free):
+    """The lowest free pages wherever they are, over several turns of entries; too few at the end."""
+    rng = np.random.default_rng(len(free))
+    refs = np.full(40000, 2, np.int32)                 # held elsewhere too
+    refs[free] = 0
+    refs[free[0]] = -1                                 # counts as free
+    n = 1100
+    tables = np.full((n, 3), -1, np.int32)
+    tables[::2, 0] = rng.choice(np.flatnonzero(refs > 0), n // 2)
+    _grow_case(paged, rng, tables, [5] * n, refs, [30] * n, 16, 1, kv=1)
+
+
 @pytest.mark.parametrize("spare", [0, 1, 2, 5, 9])
 def test_grow_when_the_pool_runs_out(paged, spare):
     """Sequences in order get what is left; a page that its other holders could not leave stays
@@ -395,7 +408,7 @@ def test_grow_when_the_pool_runs_out(paged, spare):
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("n_pages,share,layers,page,hd", [(1, 1.0, 1, 16, 64), (50, 0.0, 2, 16, 64),
                                                           (50, 0.5, 2, 32, 128),
-                                                          (3001, 0.3, 1, 16, 64),
+                                                          (3001, 0.3, 1, 16, 64), (40003, 0.4, 1, 16, 64),
                                                           (300, 0.97, 3, 16, 256)])
 def test_compact(paged, in_place, n_pages, share, layers, page, hd):
     rng = np.random.default_rng(n_pages)
