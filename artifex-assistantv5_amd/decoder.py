@@ -350,22 +350,24 @@ class QuantDecoder(LayerStack):
         if kv_bits == 32:
             self.w_att = glue.attention_workspace(cfg.n_heads, cfg.n_kv_heads, hd, T, self.device)
         self.w_arg = glue.argmax_workspace(self.device)
-        self._draw = None
+        self._draw = self._u = None
 
     # -- the choice of the next token --
     def set_sampling(self, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
                      min_p: float = 0.0, seed: int = 0) -> None:
         """How the next tokens are chosen (``sampling.sample``); ``temperature`` 0: the largest
         logit.  The random numbers, one for each position, follow from ``seed``.  Steps captured
-        before keep the choice that they were captured with."""
+        before keep the settings that they were captured with, and read the new random numbers."""
         if not temperature > 0:
             self._draw = None
             return
         g = torch.Generator(device=self.device).manual_seed(seed)
         self._draw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
-        self._u = torch.rand(self.cfg.max_seq, device=self.device, generator=g)
-        self._u_now = torch.empty(1, device=self.device)
-        self._w_draw = sampling.workspace(1, self.cfg.vocab, self.device)
+        if self._u is None:
+            self._u = torch.empty(self.cfg.max_seq, device=self.device)
+            self._u_now = torch.empty(1, device=self.device)
+            self._w_draw = sampling.workspace(1, self.cfg.vocab, self.device)
+        self._u.copy_(torch.rand(self.cfg.max_seq, device=self.device, generator=g))
 
     def _choose(self, logits: torch.Tensor, tok: torch.Tensor, pos: torch.Tensor) -> None:
         """The token after position ``pos`` [1] into ``tok`` [1], by ``logits`` [1, vocab]."""

@@ -17,7 +17,8 @@
  * (device int64): the slots in use.  Slot t holds the token at RoPE position t.  refs[p]
  * (device int32): how many table entries hold page p; 0 is a free page.
  * Optional, device int64: room[s]: slots from room[s] on are not written (the end of what
- * gguf_hip_paged_grow gave the sequence, so that a page which others hold is never written).
+ * gguf_hip_paged_grow gave the sequence, so that a page which others hold is never written;
+ * without it the caller sees to that).
  *
  * Supported: head_dim 64, 128 or 256; n_heads 1..8 times n_kv_heads; f32 rows
  * qkv = [q (n_heads * head_dim) | k | v (n_kv_heads * head_dim each)] with a row stride

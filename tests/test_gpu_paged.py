@@ -467,3 +467,194 @@ def test_refusals(paged):
         paged.compact(kv, t, r, n, paged.compact_workspace(kv, t))
     with pytest.raises(ValueError, match="workspace"):
         paged.compact(kv, t, r, n[:1].clone(), torch.empty(16, dtype=torch.uint8, device="cuda"))
+
+
+def test_pages_past_4_gib(paged):
+    """Pages whose bytes lie past 2^32, in every call."""
+    heads, kv, hd, page, n_pages = 8, 8, 128, 64, 20000       # 262144 bytes a page: 5.2 GB
+    rng = np.random.default_rng(11)
+    dev = torch.empty(n_pages, 2, kv, page, hd, dtype=torch.bfloat16, device="cuda")
+    last = n_pages - 8
+    small = _pool(rng, 8, kv, page, hd, torch.bfloat16)
+    dev[last:] = small.cuda()
+    tables = np.array([[last + 7, last + 2, last + 5], [last + 1, last + 4, last]], np.int32)
+    lengths = [130, 64]
+    cos, sin = _tables(192, hd)
+    qkv = rng.standard_normal((2, (heads + 2 * kv) * hd)).astype(np.float32)
+    t, n = _cuda(tables), _i64(lengths)
+    out = torch.empty(2, heads * hd, device="cuda")
+    args = (_cuda(qkv), n, t, _cuda(cos), _cuda(sin), dev)
+    paged.attention(*args, out, heads, paged.attention_workspace(dev, t, heads))
+    want_pool, want, bound = _reference(small, tables - last, lengths, qkv, cos, sin, heads, kv, hd)
+    assert torch.equal(_bits(dev[last:]), _bits(want_pool))
+    err = np.abs(out.cpu().double().numpy().reshape(want.shape) - want)
+    assert (err <= bound).all(), (err / bound).max()
+    k, v = (torch.zeros(2, kv, 131, hd, device="cuda") for _ in range(2))
+    paged.load(dev, t, n + 1, k, v)
+    for s, m in enumerate(lengths):
+        a, b, _ = model.rows(want_pool, tables[s] - last, m + 1, 3)
+        assert np.array_equal(k[s, 3, :m + 1].cpu().double().numpy(), a)
+        assert np.array_equal(v[s, 3, :m + 1].cpu().double().numpy(), b)
+    more = rng.standard_normal((40, (heads + 2 * kv) * hd)).astype(np.float32)
+    paged.append(_cuda(more), n + 1, t, *args[3:], heads)      # 20 rows each
+    for s, m in enumerate(lengths):
+        for i in range(20):
+            _store(want_pool, tables[s] - last, m + 1 + i, more[20 * s + i], cos, sin, heads, kv, hd)
+    assert torch.equal(_bits(dev[last:]), _bits(want_pool))
+    refs = torch.zeros(n_pages, dtype=torch.int32, device="cuda")
+    refs[t.flatten().long()] = 1
+    refs[last + 3] = 2                                         # a shared page, copied to page 0
+    t[0, 2] = last + 3
+    refs[last + 5] = 0
+    room = torch.empty_like(n)
+    paged.grow(dev, t, n, refs, _i64([1, 0]), room, paged.grow_workspace(dev, t))
+    assert t[0].tolist() == [last + 7, last + 2, 0] and room.tolist() == [192, 64]
+    assert torch.equal(_bits(dev[0, :, :, :16]), _bits(want_pool[3, :, :, :16]))
+    live = _i64([0])
+    paged.compact(dev, t, refs, live, paged.compact_workspace(dev, t))
+    order = [0, 1, 2, 3, 4, 7]                                 # of the last eight: moved to 1 .. 6
+    assert int(live) == 7 and torch.equal(_bits(dev[1:7]), _bits(want_pool[order]))
+    assert t.tolist() == [[6, 3, 0], [2, 5, 1]]
+
+
+def test_captured_calls(paged):
+    """Attention, forks, room and compaction in one graph, replayed with other lengths, tables and
+    rows, eager work between, against the same calls made eagerly."""
+    rng = np.random.default_rng(21)
+    heads, kv, hd, page, seqs, columns, n_pages = 8, 2, 128, 16, 6, 80, 300
+    cos, sin = (_cuda(x) for x in _tables(columns * page, hd))
+
+    class Side:
+        pass
+
+    sides = []
+    for _ in "ab":
+        x = Side()
+        x.kv = paged.empty(n_pages, kv, hd, page, n_layers=2)
+        x.t, x.n, x.r = paged.empty_tables(seqs, columns, n_pages)
+        x.rows, x.room, x.parents, x.live = (torch.zeros(m, dtype=torch.int64, device="cuda")
+                                             for m in (seqs, seqs, seqs, 1))
+        x.q = torch.zeros(seqs, (heads + 2 * kv) * hd, device="cuda")
+        x.out = torch.zeros(2, seqs, heads * hd, device="cuda")
+        x.w = paged.attention_workspace(x.kv[0], x.t, heads)
+        x.wg, x.wc = paged.grow_workspace(x.kv, x.t), paged.compact_workspace(x.kv, x.t)
+        sides.append(x)
+
+    def calls(x):
+        paged.fork(x.t, x.n, x.r, x.parents)
+        paged.grow(x.kv, x.t, x.n, x.r, x.rows, x.room, x.wg)
+        for l in range(2):
+            paged.attention(x.q, x.n, x.t, cos, sin, x.kv[l], x.out[l], heads, x.w, room=x.room)
+        torch.minimum(x.n + x.rows, x.room, out=x.n)
+        paged.compact(x.kv, x.t, x.r, x.live, x.wc)
+
+    a, b = sides
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for x in sides:
+            x.parents.copy_(torch.arange(seqs))
+        calls(a)                                          # nothing takes part: rows are 0
+        calls(b)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        calls(a)
+    torch.cuda.synchronize()
+    for step in range(40):
+        q = torch.from_numpy(rng.standard_normal(tuple(a.q.shape)).astype(np.float32))
+        parents = torch.arange(seqs)
+        if step % 5 == 4:
+            parents = torch.from_numpy(rng.integers(0, seqs, seqs))
+        if step % 11 == 10:
+            parents[int(rng.integers(0, seqs))] = -1
+        rows = torch.from_numpy(rng.integers(0, 2, seqs))
+        for x in sides:
+            x.q.copy_(q)
+            x.parents.copy_(parents)
+            x.rows.copy_(rows)
+            if step % 7 == 3:                             # a prompt's rows, eagerly
+                m = _i64([30 * int(i == step % seqs) for i in range(seqs)])
+                paged.grow(x.kv, x.t, x.n, x.r, m, x.room, x.wg)
+                more = torch.ones(30, x.q.shape[1], device="cuda") * (step + 1)
+                at = _i64([0] * (step % seqs + 1) + [30] * (seqs - step % seqs))
+                for l in range(2):
+                    paged.append(more, x.n, x.t, cos, sin, x.kv[l], heads, starts=at, room=x.room)
+                torch.minimum(x.n + m, x.room, out=x.n)
+        g.replay()
+        calls(b)
+        torch.cuda.synchronize()
+        for u, v in zip((a.t, a.n, a.r, a.room, a.live, a.out), (b.t, b.n, b.r, b.room, b.live, b.out)):
+            assert torch.equal(u, v), step
+        assert torch.equal(_bits(a.kv), _bits(b.kv)), step
+    held = b.t[b.t >= 0].long()
+    assert int(b.n.max()) > 3 * page and torch.equal(torch.bincount(held, minlength=n_pages), b.r.long())
+
+
+def test_two_streams_at_once(paged):
+    """Calls on two streams with workspaces of their own do not meet."""
+    rng = np.random.default_rng(5)
+    heads, kv, hd, page, n = 16, 4, 128, 16, 3000
+    columns = n // page + 1
+    cos, sin = (_cuda(x) for x in _tables(n + 1, hd))
+    sets = []
+    for i in range(2):
+        tables = _cuda(np.random.default_rng(i).permutation(columns)[None].astype(np.int32))
+        kv_ = _pool(rng, columns, kv, page, hd, torch.float16).cuda()
+        q = _cuda(rng.standard_normal((1, (heads + 2 * kv) * hd)).astype(np.float32))
+        sets.append((q, _i64([n]), tables, cos, sin, kv_, heads, paged.attention_workspace(kv_, tables, heads)))
+    alone = []
+    for q, m, t, c, s, kv_, h, w in sets:
+        out = torch.empty(1, heads * hd, device="cuda")
+        alone.append(paged.attention(q, m, t, c, s, kv_, out, h, w))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    outs = [[torch.empty(1, heads * hd, device="cuda") for _ in range(30)] for _ in sets]
+    torch.cuda.synchronize()
+    for j in range(30):
+        for i, (q, m, t, c, s, kv_, h, w) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                paged.attention(q, m, t, c, s, kv_, outs[i][j], h, w)
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in outs[i]:
+            assert torch.equal(out, alone[i])
+
+
+def test_large_batches_by_norm(paged):
+    """Random caches at the sizes that the kernels are made for, against float64 on the device: the
+    norm of the errors below 2^-15 of the outputs' (a part of an operand left out is six times
+    that)."""
+    for seed, (seqs, heads, kv, hd, page, high, dtype) in enumerate([
+            (150, 8, 2, 64, 16, 700, torch.float16), (24, 32, 8, 128, 32, 3000, torch.bfloat16),
+            (1, 32, 8, 128, 64, 100000, torch.float16), (5, 16, 2, 256, 16, 5000, torch.bfloat16),
+            (40, 20, 4, 128, 16, 1500, torch.bfloat16)]):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        lengths = torch.randint(0, high, (seqs,), device="cuda", generator=g)
+        lengths[0] = high - 1
+        columns = high // page + 1
+        n_pages = seqs * columns
+        tables = torch.randperm(n_pages, device="cuda", generator=g).view(seqs, columns).int()
+        pool = torch.randn(n_pages, 2, kv, page, hd, device="cuda", generator=g).to(dtype)
+        qkv = torch.randn(seqs, (heads + 2 * kv) * hd, device="cuda", generator=g)
+        qkv[:, :heads * hd] *= 2
+        cos, sin = (_cuda(x) for x in _tables(high + 1, hd))
+        out = torch.empty(seqs, heads * hd, device="cuda")
+        paged.attention(qkv, lengths, tables, cos, sin, pool, out, heads,
+                        paged.attention_workspace(pool, tables, heads))
+        err = norm = 0.0
+        for s in range(seqs):
+            n = int(lengths[s]) + 1
+            got = pool[tables[s, :-(-n // page)].long()].double()
+            k = got[:, 0].transpose(0, 1).reshape(kv, -1, hd)[:, :n]
+            v = got[:, 1].reshape(-1, kv, page // 16, hd, 16).transpose(-1, -2)
+            v = v.reshape(-1, kv, page, hd).transpose(0, 1).reshape(kv, -1, hd)[:, :n]
+            q = qkv[s, :heads * hd].double().view(heads, hd)
+            z = torch.complex(q[:, :hd // 2], q[:, hd // 2:]) * torch.complex(cos[n - 1].double(),
+                                                                             sin[n - 1].double())
+            q = torch.cat([z.real, z.imag], 1).view(kv, heads // kv, hd)
+            p = torch.softmax(q @ k.transpose(1, 2).contiguous() / math.sqrt(hd), -1)
+            want = (p @ v).reshape(-1)
+            err += float((out[s].double() - want).square().sum())
+            norm += float(want.square().sum())
+        assert err < (2.0 ** -15) ** 2 * norm, (seed, (err / norm) ** 0.5)

@@ -205,3 +205,81 @@ def test_refusals(sampling):
                 dict(probs=out), dict(logits=x.expand(5, 2, 10)), dict(logits=x[:, :0])):
         with pytest.raises(ValueError):
             call(**bad)
+
+
+def test_captured_with_device_settings(sampling):
+    """One graph of two calls that share a workspace, replayed with other logits, random numbers and
+    settings, eager calls between."""
+    rows, vocab = 5, 20000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, u = torch.zeros(2, rows, vocab, device="cuda"), torch.zeros(2, rows, device="cuda")
+    t, p, m = (torch.ones(rows, device="cuda") for _ in range(3))
+    k = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    out = torch.zeros(2, rows, dtype=torch.int64, device="cuda")
+    work, other = sampling.workspace(rows, vocab), sampling.workspace(rows, vocab)
+
+    def calls(to, w):
+        for i in range(2):
+            sampling.sample(x[i], u[i], to[i], w, t, k, p, m)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        calls(out, work)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(out, work)
+    for step in range(12):
+        x.copy_(torch.randn(x.shape, device="cuda", generator=g) * (1 + step % 3))
+        u.copy_(torch.rand(u.shape, device="cuda", generator=g))
+        t.copy_(torch.rand(rows, device="cuda", generator=g) * 1.5 - 0.1)
+        k.copy_(torch.randint(-5, 900, (rows,), device="cuda", generator=g))
+        p.copy_(torch.rand(rows, device="cuda", generator=g) + 0.2)
+        m.copy_(torch.rand(rows, device="cuda", generator=g) * 0.2 - 0.1)
+        graph.replay()
+        want = torch.full_like(out, -1)
+        calls(want, other)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), step
+        for i in range(2):
+            for r in range(rows):
+                w = expected(x[i, r].cpu().numpy().astype(np.float64), float(u[i, r]), float(t[r]),
+                             int(k[r]), float(p[r]), float(m[r]))
+                assert int(out[i, r]) == w[0]
+
+
+def test_a_workspace_serves_fewer_rows(sampling):
+    """A workspace of many rows serves calls of any fewer, which are cut otherwise."""
+    work = sampling.workspace(64, 151936)
+    assert work.numel() < 64 * 151936 * 4                   # less than the logits
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x, u = torch.randn(64, 151936, device="cuda", generator=g), torch.rand(64, device="cuda", generator=g)
+    out = torch.zeros(64, dtype=torch.int64, device="cuda")
+    sampling.sample(x, u, out, work, top_p=0.9)
+    for rows in (1, 3, 27, 28, 40):
+        got = torch.zeros(rows, dtype=torch.int64, device="cuda")
+        sampling.sample(x[:rows], u[:rows].contiguous(), got, work, top_p=0.9)
+        assert torch.equal(got, out[:rows])
+
+
+@pytest.mark.parametrize("m", [0.0, 0.4, 1.0])
+def test_more_equal_logits_than_are_sorted(sampling, m):
+    """Tens of thousands of equal logits at every border, few and many of them asked for."""
+    rng = np.random.default_rng(9)
+    vocab = 60000
+    x = rng.integers(0, 3, (14, vocab)).astype(np.float32)        # three values, 20000 of each
+    x[7:] -= 1e4 * (rng.random((7, vocab)) < 0.5)                 # half of them of weight zero
+    k = np.array([0, 1, 5, 512, 513, 25000, 59999] * 2)
+    p = np.array([1.0, 0.9, 0.5, 0.999, 0.3, 0.7, 0.95] * 2, np.float32)
+    check(sampling, x, rng.random(14), t=np.linspace(0.4, 3, 14).astype(np.float32), k=k, p=p, m=m)
+
+
+def test_many_of_many(sampling):
+    """top_k of thousands over a large vocabulary, narrow and wide rows, outliers at both ends."""
+    rng = np.random.default_rng(10)
+    x = (rng.standard_normal((9, 151936)) * np.array([[0.01, 0.1, 0.5, 1, 2, 4, 8, 1, 1]]).T)
+    x = x.astype(np.float32)
+    x[7, 77], x[8, 5] = 60, -1e30
+    for k, p in ((4097, 1.0), (10000, 0.97), (150000, 0.999999), (513, 0.5)):
+        check(sampling, x, rng.random(9), t=0.9, k=k, p=p)
