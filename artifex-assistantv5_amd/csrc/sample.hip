@@ -7,6 +7,10 @@
 //   bins     each chunk's bins: their tokens' indices in the order of the bins, and their masses
 //   draw     a workgroup per row: the chunks' bins added up, the limits, the draw
 // All sums are of 64-bit integers, so that neither the chunks nor timing matter.
+//
+// One row of 151936 tokens: 3.5 + 5.4 + 11 us, launches and chains of loads and barriers.  48 rows, of
+// which 16 without top_k: 10.4 (29 MB, 2.8 TB/s) + 19 (the vector unit, most of it in 64 bits) + 20 (two
+// bins put in order, one workgroup per row).
 #include "paged.hpp"
 
 namespace gguf {
