@@ -12,7 +12,7 @@ constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------------------
 // Storing rows: a wave takes one row and 256 / HD units (K or V of a KV head) side by side.  Bound: the
-// chain of loads that finds a row's place; 133 rows of six sequences, 4 heads of 64, 3.6 us.
+// chain of loads that finds a row's place; 146 rows of six sequences, 4 heads of 64, 3.6 us.
 // ---------------------------------------------------------------------------
 template <int HD, bool BF>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c,
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c,
 // Storing prompts: a wave takes the rows of one block of 16 slots, K or V of one KV head.  V's 16
 // slots of a channel are 32 bytes, which a lane has from its loads of the 16 rows; K's rows go as
 // they come.  Bound: the chain that finds a block's rows and page, then their bytes, since one
-// generation of waves takes them all; 3281 rows of five sequences, 8 heads of 128, 40 MB: 15 us (a
+// generation of waves takes them all; 3714 rows of five sequences, 8 heads of 128, 46 MB: 15 us (a
 // wave for K and V both 17, V's values one by one 26).
 // ---------------------------------------------------------------------------
 // The rows of sequence s that are stored: rows first .. first + n - 1 of qkv in slots from `slot` on.
@@ -191,7 +191,7 @@ __device__ __forceinline__ float paged_value(uint32_t bits16) {
 
 // ---------------------------------------------------------------------------
 // Reading rows back: a workgroup per block of 16 slots of a KV head.  Bound: the f32 rows written, past
-// the caches, which hold no call's rows; 6400 slots of 8 heads of 128, 79 MB: 14.7 us, 5.3 TB/s.
+// the caches, which hold no call's rows; 6104 slots of 8 heads of 128, 75 MB: 14.7 us, 5.1 TB/s.
 // ---------------------------------------------------------------------------
 template <int HD, bool BF>
 __global__ __launch_bounds__(HD) void paged_load_kernel(PagedCache c, float *__restrict__ ko,
@@ -477,7 +477,7 @@ __global__ __launch_bounds__(kThreads) void paged_grow_copy_kernel(PagedPool c,
 
 // ---------------------------------------------------------------------------
 // Compaction: a workgroup finds the moves, the second launch makes them: 236 pages of 4 MB in 32
-// layers, 2.0 GB read and written in 386 us, 5.1 TB/s; eight sequences' 66 pages 2.8 + 4.4 us.
+// layers, 2.0 GB read and written in 386 us, 5.1 TB/s; 74 pages of four layers 2.8 + 4.4 us.
 // ---------------------------------------------------------------------------
 struct CompactWork {
   int32_t *count, *to, *src, *dst;  // moves; where each page goes; the moves
@@ -580,8 +580,8 @@ __global__ __launch_bounds__(kThreads) void paged_compact_move_kernel(
 
 hipError_t launch_paged_append(const PagedCache &c, const float *qkv, int64_t ldq, int64_t n_rows,
                                const int64_t *starts, hipStream_t s) {
-  // By blocks where the sequences' rows fill some, and there are enough of them: 3281 rows of five
-  // sequences, 8 heads of 128, a row at a time 26 us, by blocks 15; 133 rows of six, 4 heads of 64,
+  // By blocks where the sequences' rows fill some, and there are enough of them: 3714 rows of five
+  // sequences, 8 heads of 128, a row at a time 26 us, by blocks 15; 146 rows of six, 4 heads of 64,
   // 3.6 and 4.8.
   if (n_rows >= 16 * (int64_t)c.n_seq && n_rows * c.nkv >= 4096) {
     const dim3 blocks((unsigned)(n_rows / 16 + 2 * c.n_seq), (unsigned)((2 * c.nkv + 3) / 4));
