@@ -609,7 +609,8 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
       all = !by_digits && (count[k] <= kRanked || (few(top_k) && count[k] <= kSorted));
       Sorted of{before, k ? (uint64_t)mass[k - 1] : 0, (int)(count[k] - before)};
       if (all) of = {0, 0, (int)count[k]};
-      if (by_digits || of.n > kSorted)
+      // (where the bins have no masses, those before this one are not known without `all`)
+      if (by_digits || of.n > kSorted || (few(top_k) && !all))
         return find_by_digits(a, row, b.r, pow2, enough, counts, masses, part, partm, &found);
       gather(all ? 0 : k, k, of.n);
       if (!all && of.n > kRanked) of = narrow(of, enough);

@@ -283,3 +283,17 @@ def test_many_of_many(sampling):
     x[7, 77], x[8, 5] = 60, -1e30
     for k, p in ((4097, 1.0), (10000, 0.97), (150000, 0.999999), (513, 0.5)):
         check(sampling, x, rng.random(9), t=0.9, k=k, p=p)
+
+
+@pytest.mark.parametrize("alike", [3700, 3797, 4096])
+def test_a_full_bin_behind_others(sampling, alike):
+    """A few hundred tokens, then as many equal ones as are just sorted, the top_k-th among them: what
+    lies before them counts."""
+    rng = np.random.default_rng(alike)
+    x = np.full((6, 20000), -5.0, np.float32)
+    for r in range(6):
+        at = rng.permutation(20000)
+        x[r, at[:300]] = 4 + 2 * rng.random(300)
+        x[r, at[300:300 + alike]] = 3
+    check(sampling, x, np.array([0.0, 0.2, 0.5, 0.9, 0.99, 0.9999]), k=np.array([299, 300, 301, 400, 512, 505]),
+          p=np.array([1.0, 0.9, 1.0, 0.99, 1.0, 0.999], np.float32), m=np.array([0, 0, 0.01, 0, 0, 0.02], np.float32))
