@@ -345,6 +345,7 @@ __global__ __launch_bounds__(kGrowThreads) void paged_grow_kernel(PagedPool c, i
   __shared__ int ends[kGrowSeqs];        // entries of the sequences up to this one
   __shared__ int32_t held[kGrowThreads];  // the turn's pages that others hold too, -1: none
   __shared__ int32_t free_[kGrowThreads];
+  __shared__ int copy_[kGrowThreads];  // which of the turn's needs a copy is, -1: no copy
   __shared__ int part[kGrowWaves];
   const int tid = threadIdx.x;
   const int64_t slots = (int64_t)c.columns << c.shift;
@@ -404,6 +405,7 @@ __global__ __launch_bounds__(kGrowThreads) void paged_grow_kernel(PagedPool c, i
     const bool needs = e < total && (p < 0 || copies);
     int wanted;
     const int k = sum_before(needs, part, wanted);
+    copy_[tid] = copies ? k : -1;
     // the first free pages, in order: as many as are wanted, or all that there are
     int got = 0;
     if (wanted) {
@@ -422,7 +424,9 @@ __global__ __launch_bounds__(kGrowThreads) void paged_grow_kernel(PagedPool c, i
       __syncthreads();
     }
     // an entry that keeps its page since the others leave it: if they all could
-    const bool fails = (needs && k >= got) || (refcount > 1 && !copies && k > got);
+    bool fails = needs && k >= got;
+    if (refcount > 1 && !copies && k > got)
+      for (int j = 0; j < tid; ++j) fails |= held[j] == p && copy_[j] >= got;
     if (fails) {
       const int64_t n = lengths[s], start = (int64_t)column << c.shift;
       atomicMin((long long *)&room[s], (long long)(start < n ? n : start));

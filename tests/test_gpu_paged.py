@@ -405,6 +405,17 @@ def test_grow_when_the_pool_runs_out(paged, spare):
     _grow_case(paged, rng, tables, [20, 20, 32, 25, 16, 20], refs, [1, 1, 1, 30, 40, 1], 16, 2)
 
 
+@pytest.mark.parametrize("spare", [1, 2, 3])
+def test_grow_keeps_what_the_others_left(paged, spare):
+    """Sequences 0 and 3 hold one page each with 2 and 4; 1 takes what the pool has left.  Where 0 could
+    leave its page, 2 keeps it alone, whatever the pool holds then; so do 3 and 4."""
+    rng = np.random.default_rng(spare)
+    tables = np.array([[0, -1, -1], [1, -1, -1], [0, -1, -1], [2, -1, -1], [2, -1, -1]], np.int32)
+    refs = np.zeros(3 + spare, np.int32)
+    refs[:3] = (2, 1, 2)
+    _grow_case(paged, rng, tables, [7, 16, 9, 3, 12], refs, [1, 32, 1, 2, 3], 16, 2)
+
+
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("n_pages,share,layers,page,hd", [(1, 1.0, 1, 16, 64), (50, 0.0, 2, 16, 64),
                                                           (50, 0.5, 2, 32, 128),
