@@ -927,6 +927,8 @@ int gguf_hip_paged_grow(void *kv, int32_t *tables, const int64_t *lengths, int32
   if (!aligned(kv, 16) || !aligned(tables, 4) || !aligned(lengths, 8) || !aligned(refs, 16) ||
       !aligned(rows, 8) || !aligned(room, 8))
     return misaligned_pages();
+  if (room == lengths || room == rows || partly(lengths, room, 8 * n_seq) || partly(rows, room, 8 * n_seq))
+    return fail(GGUF_HIP_ERR_SHAPE, "[gguf-hip] paged_grow: room overlaps lengths or rows");
   if ((rc = check_paged_work("paged_grow", work, work_bytes, need))) return rc;
   const int64_t head = (int64_t)page * head_dim;
   const gguf::PagedPool c{(uint16_t *)kv, n_layers, (int)n_pages, page, page_shift(page),

@@ -68,7 +68,8 @@ int gguf_hip_paged_append(const float *qkv, int64_t ldqkv, int64_t n_rows, const
  * bytes, 16-byte aligned, no initial value; calls that share it must not overlap.  Results do
  * not depend on timing.  f32-grade: K and V enter the matrix cores as they are, queries and
  * probabilities as two f16 parts each (22 bits of each product down to 2^-13 of a row's
- * largest, below that 2^-35 of it) or three bf16 parts (24 bits). */
+ * largest, below that 2^-35 of it) or three bf16 parts (24 bits).  Since a part may be zero, a
+ * head that sees an infinite K or V may be NaN where exact sums would not be. */
 int gguf_hip_paged_attention(const float *qkv, int64_t ldqkv, const int64_t *lengths,
                              const int64_t *room, const int32_t *tables, const float *cos_table,
                              const float *sin_table, int64_t rope_rows, void *kv, int dtype,
@@ -106,8 +107,8 @@ int gguf_hip_paged_fork(const int32_t *tables, const int64_t *lengths, const int
  * page in its place, and if the page has slots in use by the sequence, their blocks of 16 slots
  * are copied in all n_layers layers.  A sequence for which no free page is left gets no further
  * ones.  room[s]: the end of the slots that the sequence may now write, lengths[s] at least (0
- * where lengths[s] < 0); it is lengths[s] where rows[s] <= 0.  lengths is not changed.
- * refs is 16-byte aligned.
+ * where lengths[s] < 0); it is lengths[s] where rows[s] <= 0.  lengths is not changed, and room
+ * must not overlap it or rows.  refs is 16-byte aligned.
  * Two launches.  work: gguf_hip_paged_grow_workspace bytes, 16-byte aligned, no initial value;
  * calls that share it must not overlap. */
 int gguf_hip_paged_grow(void *kv, int32_t *tables, const int64_t *lengths, int32_t *refs,

@@ -183,6 +183,14 @@ def test_grow_and_compact_refusals(lib, native, call, names):
         assert call(lib, refs_out=C - 4) == native.ERR_SHAPE
 
 
+def test_grow_refuses_room_over_its_inputs(lib, native):
+    """rows may be lengths (both are only read), room neither nor a part of them."""
+    for over in (dict(room=B), dict(room=B + 8), dict(rows=A + 64, room=A + 64),
+                 dict(rows=A + 64, room=A + 56)):
+        assert _grow(lib, **over) == native.ERR_SHAPE, over
+    assert "room overlaps" in native.last_error(lib)
+
+
 def test_python_refusals_without_device_tensors(pkg):
     """What the Python layer can tell before the library is called."""
     paged = importlib.import_module("artifex-assistantv5_amd.paged")
