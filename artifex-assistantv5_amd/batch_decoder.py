@@ -174,7 +174,8 @@ class BatchDecoder(LayerStack):
     @torch.no_grad()
     def prefill(self, tokens: torch.Tensor, seq: int) -> torch.Tensor:
         """Run ``tokens`` (device int64 [M]) behind what sequence ``seq`` holds, and return the last
-        one's logits [1, vocab].  ValueError if they do not fit ``max_seq`` or the pool."""
+        one's logits [1, vocab].  ValueError if they do not fit ``max_seq`` or the pool; then nothing
+        has changed."""
         m = tokens.numel()
         if not 0 <= seq < self.n_seq:
             raise ValueError(f"sequence {seq} not in 0..{self.n_seq - 1}")
@@ -185,8 +186,11 @@ class BatchDecoder(LayerStack):
             raise ValueError(f"sequence of {held + m} exceeds max_seq {self.cfg.max_seq}")
         rows = torch.zeros_like(self.rows)
         rows[seq] = m
+        table, refs = self.tables[seq].clone(), self.refs.clone()
         self._grow(rows)
         if int(self.room[seq]) < held + m:
+            self.tables[seq] = table
+            self.refs.copy_(refs)
             raise ValueError(f"the pool of {self.kv.shape[1]} pages has no room for {m} more rows")
         self._prompt = seq
         try:
@@ -240,9 +244,11 @@ class BatchDecoder(LayerStack):
             if p.numel() + n_new - 1 > self.cfg.max_seq:
                 raise ValueError(f"prompt {p.numel()} + {n_new} new tokens exceed max_seq "
                                  f"{self.cfg.max_seq}")
-        page, columns = self.kv.shape[-2], lambda m: -(-m // self.kv.shape[-2])  # noqa: E731
-        need = sum(p.numel() // page + samples * (columns(p.numel() + n_new - 1) - p.numel() // page)
-                   for p in prompts)
+        page = self.kv.shape[-2]
+        need = 0
+        for p in prompts:  # the pages that a prompt's continuations share, and their own
+            shared = p.numel() // page if n_new > 1 else -(-p.numel() // page)
+            need += shared + samples * (-(-(p.numel() + n_new - 1) // page) - shared)
         if need > self.kv.shape[1]:
             raise ValueError(f"the sequences need {need} pages, the pool has {self.kv.shape[1]}")
         self.set_sampling(**choice)
@@ -271,5 +277,5 @@ class BatchDecoder(LayerStack):
         torch.cuda.synchronize(dev)
         t_decode = time.perf_counter() - t1
         return {"tokens": out.t(), "probs": probs.t(), "prefill_s": t_prefill, "decode_s": t_decode,
-                "decode_steps": n_new - 1, "tok_s": n * max(n_new - 1, 1) / t_decode,
+                "decode_steps": n_new - 1, "tok_s": n * (n_new - 1) / t_decode,
                 "prefill_tok_s": sum(p.numel() for p in prompts) / t_prefill}

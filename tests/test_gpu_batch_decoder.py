@@ -197,6 +197,26 @@ def test_captured_step_reads_new_settings(dec, batch):
                 x.rows.fill_(1)
 
 
+@pytest.mark.parametrize("n_seq", [33, 40])
+def test_more_sequences_than_one_pass_of_the_projections(dec, batch, paged, n_seq):
+    """Above 32 rows the projections take another kernel; resting sequences (NaN rows) are no other
+    sequence's."""
+    cfg, w = _model(dec, max_seq=64)
+    m, ref = batch.BatchDecoder(cfg, w, n_seq), FromCache(cfg, w)
+    on = [0, 7, n_seq - 1]
+    for s in on:
+        m.prefill(_tokens(cfg, 5 + s, s), s)
+        m.rows[s] = 1
+    for step in range(3):
+        tok, before = m.tok.tolist(), m.lengths.tolist()
+        logits = m.step()
+        for s in range(n_seq):
+            if s in on:
+                assert _rel(logits[s], ref.token(tok[s], before[s], _cached(paged, m, s))) < 1e-4
+            else:
+                assert torch.isnan(logits[s]).all() and int(m.lengths[s]) == 0
+
+
 def test_stop(dec, batch):
     cfg, w = _model(dec, max_seq=80)
     m = batch.BatchDecoder(cfg, w, 4)
@@ -249,6 +269,32 @@ def test_pool_and_positions_end(dec, batch):
         large.prefill(_tokens(cfg, 0, 0), 0)
     with pytest.raises(ValueError, match="not in"):
         large.prefill(_tokens(cfg, 1, 0), 3)
+
+
+def test_a_prompt_that_the_pool_refuses(dec, batch):
+    """It leaves the pages as they were, shared ones too, so that the others go on."""
+    cfg, w = _model(dec, max_seq=128)
+    m = batch.BatchDecoder(cfg, w, 3, n_pages=6)
+    m.prefill(_tokens(cfg, 20, 1), 0)
+    m.fork([0, 0, -1])
+    before = [t.clone() for t in (m.tables, m.refs, m.lengths)]
+    with pytest.raises(ValueError, match="no room"):
+        m.prefill(_tokens(cfg, 80, 2), 1)
+    for t, old in zip((m.tables, m.refs, m.lengths), before):
+        assert torch.equal(t, old)
+    m.rows.copy_(torch.tensor([1, 1, 0]))
+    for _ in range(25):                 # to 45 slots: 1 + 2 + 2 pages
+        assert torch.isfinite(m.step()[:2]).all()
+    assert m.lengths.tolist() == [45, 45, 0] and int((m.refs > 0).sum()) == 5
+
+
+def test_generate_the_first_token_alone(dec, batch):
+    """Continuations of one token share all of their prompt's pages."""
+    cfg, w = _model(dec, max_seq=64)
+    m = batch.BatchDecoder(cfg, w, 4, n_pages=2)
+    got = m.generate([_tokens(cfg, 20, 1)], 1, samples=4)
+    assert got["tokens"].shape == (4, 1) and len(set(got["tokens"][:, 0].tolist())) == 1
+    assert got["tok_s"] == 0 and got["decode_steps"] == 0 and int(m.refs.max()) == 4
 
 
 def test_a_stream_of_the_caller(dec, batch):
