@@ -8,8 +8,8 @@
 //   draw     a workgroup per row: the chunks' bins added up, the limits, the draw
 // All sums are of 64-bit integers, so that neither the chunks nor timing matter.
 //
-// One row of 151936 tokens: 3.5 + 5.4 + 11 us, launches and chains of loads and barriers.  48 rows, of
-// which 16 without top_k: 10.4 (29 MB, 2.8 TB/s) + 19 (the vector unit, most of it in 64 bits) + 20 (two
+// One row of 151936 tokens: 3.3 + 5.0 + 11.9 us, launches and chains of loads and barriers.  48 rows, of
+// which 16 without top_k: 7.8 (29 MB, 3.7 TB/s) + 16 (the vector unit, most of it in 64 bits) + 19 (two
 // bins put in order, one workgroup per row).
 #include "paged.hpp"
 
@@ -18,7 +18,7 @@ namespace gguf {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kBins = 512;     // the last one holds the tokens of weight 0
+constexpr int kBins = 512;     // the last one for tokens of weight 0, which are in none
 constexpr int kSorted = 4096;  // tokens that a workgroup puts in order
 constexpr int kRanked = 256;   // up to so many by counting, for each, those before it
 constexpr int kFewest = 512;   // a top_k of up to so many needs no bins' masses
@@ -195,16 +195,18 @@ __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleArgs a, Work
   __shared__ uint32_t partl[kWaves];
   const int row = blockIdx.y, tid = threadIdx.x, i0 = blockIdx.x * T * kThreads;
   const float *x = a.logits + row * a.ld;
-  uint64_t first = 0;
-  uint32_t least = 0;
+  float high = -INFINITY, low = INFINITY;  // of those above -inf
+  int at = 0;
 #pragma unroll
   for (int j = 0; j < T; ++j) {
-    const int i = i0 + j * kThreads + tid;
-    const uint32_t k = i < a.vocab ? order_key(x[i]) : 0u;
-    const uint64_t p = place(k, i);
-    first = k && p > first ? p : first;
-    least = k && ~k > least ? ~k : least;
+    const int i = min(i0 + j * kThreads + tid, a.vocab - 1);  // past the end: the last again
+    const float y = x[i];
+    at = y > high ? i : at;
+    high = y > high ? y : high;
+    low = y > -INFINITY && y < low ? y : low;
   }
+  uint64_t first = high > -INFINITY ? place(order_key(high), at) : 0;
+  uint32_t least = high > -INFINITY ? ~order_key(low) : 0u;
   first = wave_max(first);
   least = wave_max(least);
   if ((tid & 63) == 0) part[tid >> 6] = first, partl[tid >> 6] = least;
@@ -245,11 +247,6 @@ __device__ __forceinline__ Bins bins_of(const SampleArgs &a, int row, const Chun
   b.per = range > 0.0 ? (kBins - 1) / range : 0.0;
   return b;
 }
-__device__ __forceinline__ int bin_of(const Bins &b, double e) {
-  if (!(e > kNothing)) return kBins - 1;
-  const int k = (int)(-e * b.per);
-  return k < kBins - 2 ? k : kBins - 2;
-}
 // Where the first top_k tokens are all that counts, their masses are taken from them alone.
 __device__ __forceinline__ bool few(int32_t top_k) { return top_k > 0 && top_k <= kFewest; }
 
@@ -282,15 +279,20 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a, 
   const Bins b = bins_of(a, row, own);
   if (!b.first || !(b.t > 0.f)) return;  // nothing to draw, or no draw
   __syncthreads();
-  uint32_t rank[T];  // bin and place in it
+  uint32_t rank[T];  // bin and place in it; a token of weight 0 has none
   uint64_t large = 0;
+  const bool endless = b.r.top == INFINITY;
+  const double top = endless ? 0.0 : (double)b.r.top;
 #pragma unroll
   for (int j = 0; j < T; ++j) {
-    const int i = i0 + j * kThreads + tid;
-    if (i >= a.vocab) break;
     if (j && j % L == 0) load(j);
-    const double e = exponent(b.r, order_key(y[j % L]));
-    const int k = bin_of(b, e);
+    if (j % L == 0 && endless)  // as logits of 0 and of less than any
+#pragma unroll
+      for (int l = 0; l < L; ++l) y[l] = y[l] == INFINITY ? 0.f : -INFINITY;
+    const double e = ((double)y[j % L] - top) * b.r.scale;  // as `exponent`
+    rank[j] = ~0u;
+    if (!(e > kNothing) || i0 + j * kThreads + tid >= a.vocab) continue;
+    const int k = min((int)(-e * b.per), kBins - 2);
     rank[j] = atomicAdd(&count[k], 1u) | (uint32_t)k << 16;
     if (counts_only) continue;
     const double v = pow2(e);
@@ -319,7 +321,7 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a, 
   // put together here: written one by one, the indices took most of the kernel's time
 #pragma unroll
   for (int j = 0; j < T; ++j) {
-    if (i0 + j * kThreads + tid >= a.vocab) break;
+    if (rank[j] == ~0u) continue;
     order[count[rank[j] >> 16] + (rank[j] & 0xFFFFu)] = (uint16_t)(j * kThreads + tid);
   }
   __syncthreads();
@@ -424,12 +426,21 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Wor
     const int64_t at = lists * kBins + tid % kBins;
     const uint32_t *bin = (const uint32_t *)w.bin + at;
     const uint64_t *mass = w.mass + at;
-    const int half = tid / kBins;
-#pragma unroll 16
-    for (int l = half; l < chunks; l += 2) c += bin[l * kBins] & 0xFFFFu;
-    if (!few(top_k))
-#pragma unroll 16
-      for (int l = half; l < chunks; l += 2) m += mass[l * kBins];
+    constexpr int L = 8;  // chunks in flight
+    for (int l0 = tid / kBins; l0 < chunks; l0 += 2 * L) {
+      uint32_t cl[L];
+      uint64_t ml[L] = {};
+#pragma unroll
+      for (int j = 0; j < L; ++j) cl[j] = bin[min(l0 + 2 * j, chunks - 1) * kBins] & 0xFFFFu;
+      if (!few(top_k))
+#pragma unroll
+        for (int j = 0; j < L; ++j) ml[j] = mass[min(l0 + 2 * j, chunks - 1) * kBins];
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        c += l0 + 2 * j < chunks ? cl[j] : 0;
+        m += l0 + 2 * j < chunks ? ml[j] : 0;
+      }
+    }
   }
   const Bins b = bins_of(a, row, own);
   if (!b.first || !(b.t > 0.f)) {  // the bins have not been made
