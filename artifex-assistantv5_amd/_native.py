@@ -11,6 +11,8 @@ is no fallback path.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import struct
 
@@ -178,6 +180,25 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     if path is None:
         _lib = lib
     return lib
+
+
+_tensors = None
+
+
+def direct():
+    """The module of calls straight from tensors (csrc/tensors.cpp), which return False where their
+    arguments do not fit; raises if it is missing."""
+    global _tensors
+    if _tensors is None:
+        lib = load_library()
+        path = os.path.join(os.path.dirname(LIB_PATH), "_tensors.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is not built; run `python artifex-assistantv5_amd/build.py`")
+        loader = importlib.machinery.ExtensionFileLoader("_tensors", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_tensors", loader))
+        module.bind(*(ctypes.cast(getattr(lib, name), _vp).value for name in PACKED))
+        _tensors = module
+    return _tensors
 
 
 def last_error(lib=None) -> str:

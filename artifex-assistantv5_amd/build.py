@@ -1,4 +1,4 @@
-"""Build ``libgguf_hip.so`` in-tree with hipcc for gfx950.
+"""Build ``libgguf_hip.so`` in-tree with hipcc for gfx950, and ``_tensors.so`` beside it.
 
 ``python -m`` is awkward for a hyphenated package, so run it as a script:
 ``python artifex-assistantv5_amd/build.py`` (or call ``build()``).
@@ -9,16 +9,19 @@ next to this file, where ``_native.py`` loads it from.
 from __future__ import annotations
 
 import concurrent.futures
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libgguf_hip.so")
+TENSORS = os.path.join(HERE, "_tensors.so")  # csrc/tensors.cpp, a module of host code
 # every .hip file of csrc/ (the decode kernels are one translation unit per
 # ggml type, decode_<type>.hip, so that they compile in parallel)
 SOURCES = sorted(f for f in os.listdir(CSRC) if f.endswith(".hip"))
@@ -54,12 +57,31 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _build_tensors() -> str:
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    tmp = TENSORS + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__", f"-I{os.path.join(ROOT, 'include')}",
+           *(f"-isystem{os.path.join(torch, 'include', *d)}"
+             for d in ((), ("torch", "csrc", "api", "include"))),
+           f"-isystem{sysconfig.get_paths()['include']}", os.path.join(CSRC, "tensors.cpp"), "-o", tmp,
+           f"-L{os.path.join(torch, 'lib')}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode:
+        print(res.stdout + res.stderr, file=sys.stderr)
+        raise RuntimeError("g++ failed for tensors.cpp")
+    os.replace(tmp, TENSORS)
+    return TENSORS
+
+
 def build(verbose: bool = False) -> str:
     """Compile every HIP source and link ``libgguf_hip.so``; returns its path."""
     os.makedirs(BUILD, exist_ok=True)
     workers = max(1, min(len(SOURCES), len(os.sched_getaffinity(0))))
     with concurrent.futures.ThreadPoolExecutor(max_workers=workers) as ex:
+        tensors = ex.submit(_build_tensors)
         objs = list(ex.map(lambda s: _compile(s, verbose), SOURCES))
+        tensors.result()
     tmp = LIB + ".tmp"
     # Export the C ABI only: kernel stubs and helpers bind locally, so two
     # builds of the library in one process cannot interpose each other.

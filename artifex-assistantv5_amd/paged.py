@@ -33,7 +33,7 @@ from . import _native
 BLOCK = 16
 PAGES = (16, 32, 64, 128, 256)
 _DTYPES = {torch.float16: _native.PAGED_F16, torch.bfloat16: _native.PAGED_BF16}
-_call = _native.call
+_call, _direct = _native.call, _native.direct
 
 
 def pool_bytes(n_pages: int, n_kv_heads: int, head_dim: int, page: int = 16) -> int:
@@ -76,7 +76,8 @@ def _pool(kv: torch.Tensor, layers: bool = False):
     return device, n_layers, n_pages, n_kv, page, hd
 
 
-# Checks in as few steps as they need: a call of several of them costs more than its launches.
+# The calls below are made straight from the tensors where these fit (``_native.direct``); what
+# follows there says what does not, and makes those calls whose device is not the current one.
 def _array(name: str, t: torch.Tensor, dtype, shape, device: int) -> int:
     if (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == device):
         return t.data_ptr()
@@ -131,6 +132,8 @@ def append(qkv: torch.Tensor, lengths: torch.Tensor, tables: torch.Tensor, cos: 
     goes to slot ``lengths[s] + i``; rows outside every sequence, without a page, past the tables
     or ``room[s]`` (``grow``) are not stored, nor those of a sequence of negative length.
     ``lengths`` is the caller's to advance.  One launch."""
+    if _direct().append(qkv, lengths, tables, cos, sin, kv, n_heads, starts, room):
+        return kv
     dev, _, n_pages, n_kv, page, hd = _pool(kv)
     qp, ld = _row_matrix("qkv", qkv, -1, (n_heads + 2 * n_kv) * hd, dev)
     n_seq, columns, tp = _tables(tables, dev)
@@ -160,6 +163,8 @@ def attention(qkv: torch.Tensor, lengths: torch.Tensor, tables: torch.Tensor, co
     Row s is stored in slot ``lengths[s]`` and attends to slots ``0 .. lengths[s]``, of which those
     without a page are not seen.  A sequence whose row cannot be stored (negative length, no page,
     past the tables or ``room[s]``) takes no part: nothing of it is written."""
+    if _direct().attention(qkv, lengths, tables, cos, sin, kv, out, n_heads, work, room):
+        return out
     dev, _, n_pages, n_kv, page, hd = _pool(kv)
     n_seq, columns, tp = _tables(tables, dev)
     qp, ld = _row_matrix("qkv", qkv, n_seq, (n_heads + 2 * n_kv) * hd, dev)
@@ -178,6 +183,8 @@ def load(kv: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, k_out: t
     ``k_out`` / ``v_out`` ``[n_seq, n_kv_heads, out_slots, head_dim]``.  Rows from ``lengths[s]`` on,
     and of slots without a page, are not written.  For one sequence this is the layout of
     ``glue.attention_prefill``'s caches.  One launch."""
+    if _direct().load(kv, tables, lengths, k_out, v_out):
+        return
     dev, _, n_pages, n_kv, page, hd = _pool(kv)
     n_seq, columns, tp = _tables(tables, dev)
     shape = (n_seq, n_kv, k_out.shape[-2] if k_out.dim() > 1 else 0, hd)
@@ -196,6 +203,8 @@ def fork(tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, parent
     it is, a parent outside the sequences (-1) frees it.  In place, or into the ``*_out`` tensors,
     which must not overlap the inputs.  No page is copied: ``grow`` does that before a shared one
     is written.  One launch, or two where ``refs_out`` is another tensor and large."""
+    if _direct().fork(tables, lengths, refs, parents, tables_out, lengths_out, refs_out):
+        return
     dev = tables.get_device()
     if dev < 0 or refs.dim() != 1:
         raise ValueError("paged: tables must be a device tensor, refs [n_pages]")
@@ -228,6 +237,8 @@ def grow(kv: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, refs: to
     entries hold too, into whose new page the blocks of 16 slots in use are copied.  ``room[s]``
     becomes the end of the slots that the sequence may write, ``lengths[s]`` at least: less than
     was asked for where the pool has no free page left.  Two launches."""
+    if _direct().grow(kv, tables, lengths, refs, rows, room, work):
+        return
     dev, n_layers, n_pages, n_kv, page, hd = _pool(kv, layers=True)
     n_seq, columns, tp = _tables(tables, dev)
     n = (n_seq,)
@@ -255,6 +266,8 @@ def compact(kv: torch.Tensor, tables: torch.Tensor, refs: torch.Tensor, live: to
     here) of the pool: those behind them, in order, into the free ones among them, in order.
     ``tables`` and ``refs`` follow, in place or into the ``*_out`` tensors, which must not overlap
     the inputs.  Two launches."""
+    if _direct().compact(kv, tables, refs, live, work, tables_out, refs_out):
+        return
     dev, n_layers, n_pages, n_kv, page, hd = _pool(kv, layers=True)
     n_seq, columns, tp = _tables(tables, dev)
     pages = (n_pages,)

@@ -50,6 +50,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, out: torch.Tensor, work: torch
     the first of the largest.  ``probs`` (f32 ``[rows]``): the drawn tokens' probabilities among
     the kept ones.  ``work``: from ``workspace``, for calls that do not overlap.  Allocates and
     synchronises nothing."""
+    if _native.direct().sample(logits, u, out, work, temperature, top_k, top_p, min_p, probs):
+        return out
     dev = logits.get_device()
     if logits.dim() != 2 or logits.dtype is not torch.float32 or dev < 0:
         raise ValueError("sample: logits must be float32 device rows [rows, vocab]")
