@@ -8,8 +8,8 @@
 //   draw     a workgroup per row: the chunks' bins added up, the limits, the draw
 // All sums are of 64-bit integers, so that neither the chunks nor timing matter.
 //
-// One row of 151936 tokens: 3.3 + 5.0 + 11.9 us, launches and chains of loads and barriers.  48 rows, of
-// which 16 without top_k: 7.8 (29 MB, 3.7 TB/s) + 16 (the vector unit, most of it in 64 bits) + 19 (two
+// One row of 151936 tokens: 3.1 + 5.0 + 11.9 us, launches and chains of loads and barriers.  48 rows, of
+// which 16 without top_k: 7 (29 MB, 4.1 TB/s) + 15.5 (the vector unit, most of it in 64 bits) + 19 (two
 // bins put in order, one workgroup per row).
 #include "paged.hpp"
 
@@ -162,7 +162,7 @@ struct Cut {
   int chunk, chunks;  // tokens of a chunk, chunks of a row
 };
 // Small chunks while they do not fill the chip (us of a replayed call of 48 rows of 151936 tokens:
-// 16 tokens a thread 48.3, eight 51.7, four 57.5).
+// 16 tokens a thread 40.4, eight 43.4).
 constexpr int64_t kSmall = 4 * kThreads * 1024;  // tokens of a call
 Cut cut(int64_t vocab, bool small) {
   const int chunk = (small ? 4 : 16) * kThreads;
