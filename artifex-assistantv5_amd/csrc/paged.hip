@@ -74,8 +74,9 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c,
 // Storing prompts: a wave takes the rows of one block of 16 slots, K or V of one KV head.  V's 16
 // slots of a channel are 32 bytes, which a lane has from its loads of the 16 rows; K's rows go as
 // they come.  Bound: the chain that finds a block's rows and page, then their bytes, since one
-// generation of waves takes them all; 3714 rows of five sequences, 8 heads of 128, 46 MB: 15 us (a
-// wave for K and V both 17, V's values one by one 26).
+// generation of waves takes them all; 3714 rows of five sequences, 8 heads of 128, 46 MB: 13 us, 3.5 TB/s
+// (the page looked up before the rows are requested, and K's row by row: 15; a wave for K and V both
+// 17, V's values one by one 26).
 // ---------------------------------------------------------------------------
 // The rows of sequence s that are stored: rows first .. first + n - 1 of qkv in slots from `slot` on.
 struct Stretch {
@@ -126,23 +127,32 @@ __global__ __launch_bounds__(kThreads) void paged_append_blocks_kernel(
   if (s < 0) return;
   const int slot0 = (x.slot & ~15) + 16 * block;     // of the block
   const int j0 = max(x.slot - slot0, 0), j1 = min(x.slot + x.n - slot0, 16);  // its slots
-  const int32_t page = c.tables[(int64_t)s * c.columns + (slot0 >> c.shift)];
-  if ((uint32_t)page >= (uint32_t)c.n_pages) return;
+  const int32_t page = c.tables[(int64_t)s * c.columns + (slot0 >> c.shift)];  // needed by the stores
   const float *rows = qkv + (int64_t)(x.first + (slot0 - x.slot)) * ldq + (int64_t)c.nh * HD;  // of slot0
   const int j_in = slot0 & (c.page - 1);
   if (!(u & 1)) {  // K: 64 / LANES rows at a time
     const float *k = rows + (int64_t)h * HD;
-    uint16_t *ko = c.kv + paged_k_at(c, page, h, j_in);
-#pragma unroll 8
-    for (int i = 0; i < 16; i += SIDE) {
-      const int j = i + lane / LANES, at = min(max(j, j0), j1 - 1);
-      Kv4Row<HD> row;
-      row.load(k + at * ldq, q);
-      row.load_turn(c.cs + (int64_t)(slot0 + at) * (HD / 2), c.sn + (int64_t)(slot0 + at) * (HD / 2), q);
-      float t[4];
-      paged_turn<HD>(row, q, true, t);
-      const uint2 w = paged_round<BF>(t);
-      if (j >= j0 && j < j1) *(uint2 *)(ko + j * HD + 4 * q) = w;
+    constexpr int N = 16 / SIDE < 8 ? 16 / SIDE : 8;  // rows of a lane in flight
+#pragma unroll
+    for (int i0 = 0; i0 < 16; i0 += N * SIDE) {
+      Kv4Row<HD> row[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int at = min(max(i0 + i * SIDE + lane / LANES, j0), j1 - 1);
+        row[i].load(k + at * ldq, q);
+        row[i].load_turn(c.cs + (int64_t)(slot0 + at) * (HD / 2), c.sn + (int64_t)(slot0 + at) * (HD / 2), q);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if ((uint32_t)page >= (uint32_t)c.n_pages) return;
+      uint16_t *ko = c.kv + paged_k_at(c, page, h, j_in) + 4 * q;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int j = i0 + i * SIDE + lane / LANES;
+        float t[4];
+        paged_turn<HD>(row[i], q, true, t);
+        const uint2 w = paged_round<BF>(t);
+        if (j >= j0 && j < j1) *(uint2 *)(ko + j * HD) = w;
+      }
     }
     return;
   }
@@ -162,6 +172,8 @@ __global__ __launch_bounds__(kThreads) void paged_append_blocks_kernel(
       y[j][0] = w.x, y[j][1] = w.y, y[j][2] = w.z, y[j][3] = w.w;
     }
   }
+  __builtin_amdgcn_sched_barrier(0);
+  if ((uint32_t)page >= (uint32_t)c.n_pages) return;
   uint16_t *vo = c.kv + paged_v_at(c, page, h, j_in) + 16 * CH * lane;
 #pragma unroll
   for (int e = 0; e < CH; ++e) {
@@ -585,7 +597,7 @@ __global__ __launch_bounds__(kThreads) void paged_compact_move_kernel(
 hipError_t launch_paged_append(const PagedCache &c, const float *qkv, int64_t ldq, int64_t n_rows,
                                const int64_t *starts, hipStream_t s) {
   // By blocks where the sequences' rows fill some, and there are enough of them: 3714 rows of five
-  // sequences, 8 heads of 128, a row at a time 26 us, by blocks 15; 146 rows of six, 4 heads of 64,
+  // sequences, 8 heads of 128, a row at a time 26 us, by blocks 13; 146 rows of six, 4 heads of 64,
   // 3.6 and 4.8.
   if (n_rows >= 16 * (int64_t)c.n_seq && n_rows * c.nkv >= 4096) {
     const dim3 blocks((unsigned)(n_rows / 16 + 2 * c.n_seq), (unsigned)((2 * c.nkv + 3) / 4));
