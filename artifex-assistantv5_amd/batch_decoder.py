@@ -49,7 +49,8 @@ class BatchDecoder(LayerStack):
     ``max_seq`` tokens) of ``page`` slots in ``dtype``.
 
     A sequence for which the pool has no page, or past ``max_seq``, stores nothing in a step: its
-    logits are NaN, its token 0 and its length stays."""
+    logits are NaN, its ``tok`` is 0 and its length stays.  The token that it was to store waits for
+    the first step with room for it, unless ``tok`` has been given another one (not 0) by then."""
 
     def __init__(self, cfg: DecoderConfig, weights: DecoderWeights, n_seq: int,
                  n_pages: Optional[int] = None, page: int = 16,
@@ -63,6 +64,7 @@ class BatchDecoder(LayerStack):
         self.tables, self.lengths, self.refs = paged.empty_tables(n_seq, columns, n_pages, dev)
         i64 = lambda n: torch.zeros(n, dtype=torch.int64, device=dev)  # noqa: E731
         self.rows, self.room, self.tok = i64(n_seq), i64(n_seq), i64(n_seq)
+        self._waiting = i64(n_seq)          # tokens of sequences that had no room, 0: none
         self.live = i64(1)
         self.cos, self.sin = rope_tables(dataclasses.replace(cfg, max_seq=self.slots), dev)
         # one layer's rows of a sequence in f32, for the attention of a prompt
@@ -108,9 +110,10 @@ class BatchDecoder(LayerStack):
             self._u = torch.empty(self.slots, n, device=dev)
         self._u.copy_(torch.rand(self._u.shape, device=dev, generator=g))
 
-    def _choose(self, logits: torch.Tensor, takes: torch.Tensor) -> None:
+    def _choose(self, logits: torch.Tensor, takes: torch.Tensor, stored: torch.Tensor) -> None:
         """The tokens after the last slots of the sequences for which ``takes`` (int64, 0 or 1),
-        by ``logits`` [n_seq, vocab]."""
+        by ``logits`` [n_seq, vocab].  Where ``stored`` is 0 they are no draws, which ``stop``
+        could end."""
         at = (self.lengths - 1).clamp_(0, self.slots - 1)
         u = self._u[at, self._seq]
         tok = torch.empty_like(self.tok)
@@ -121,13 +124,13 @@ class BatchDecoder(LayerStack):
         self.tok.copy_(torch.where(on, tok, self.tok))
         self.probs.copy_(torch.where(on, probs, self.probs))
         if self._stop is not None:
-            self.rows.mul_((self.tok != self._stop) | ~on)
+            self.rows.mul_((self.tok != self._stop) | (stored == 0))
 
     # -- the cache --
     def reset(self) -> None:
         """No sequence holds anything, none takes part."""
         self.tables.fill_(-1)
-        for t in (self.lengths, self.refs, self.rows, self.room, self.tok):
+        for t in (self.lengths, self.refs, self.rows, self.room, self.tok, self._waiting):
             t.zero_()
 
     @torch.no_grad()
@@ -138,7 +141,7 @@ class BatchDecoder(LayerStack):
         paged.fork(self.tables, self.lengths, self.refs, p)
         ok = (p >= 0) & (p < self.n_seq)
         src = torch.where(ok, p, 0)
-        for t in (self.tok, self.rows, self.probs):
+        for t in (self.tok, self._waiting, self.rows, self.probs):
             t.copy_(torch.where(ok, t[src], torch.zeros_like(t)))
 
     @torch.no_grad()
@@ -199,7 +202,14 @@ class BatchDecoder(LayerStack):
         finally:
             self._prompt = None
         self.lengths[seq] += m
+        s = slice(seq, seq + 1)
+        self.tok[s] = self._next_tok()[s]
+        self._waiting[s] = 0
         return self._proj(h[-1:], self.w.lm_head_gg, "lm_head")
+
+    def _next_tok(self) -> torch.Tensor:
+        """The tokens that the next step reads."""
+        return torch.where(self.tok != 0, self.tok, self._waiting)
 
     @torch.no_grad()
     def step(self) -> torch.Tensor:
@@ -207,10 +217,13 @@ class BatchDecoder(LayerStack):
         next slot and the one after it takes its place.  Returns the logits [n_seq, vocab], NaN
         where a sequence did not take part.  Touches no host state, so it can be captured."""
         self._grow(self.rows)
-        h = self._layers_glue(self._embed(self.tok), self.lengths)
+        tok = self._next_tok()
+        h = self._layers_glue(self._embed(tok), self.lengths)
         logits = self._proj(h, self.w.lm_head_gg, "lm_head")
-        torch.minimum(self.lengths + self.rows, self.room, out=self.lengths)  # those that were stored
-        self._choose(logits, self.rows)
+        stored = torch.minimum(self.lengths + self.rows, self.room) - self.lengths
+        self.lengths.add_(stored)
+        self._waiting.copy_(torch.where(self.rows > 0, tok * (1 - stored), self._waiting))
+        self._choose(logits, self.rows, stored)
         return logits
 
     @torch.no_grad()
@@ -261,7 +274,7 @@ class BatchDecoder(LayerStack):
         parents = [s // samples * samples if s < n else s for s in range(self.n_seq)]
         self.fork(parents)
         self.rows[:n] = 1
-        self._choose(first, self.rows)
+        self._choose(first, self.rows, self.rows)
         del first
         out = torch.empty(n_new, n, dtype=torch.int64, device=dev)
         probs = torch.empty(n_new, n, device=dev)

@@ -35,3 +35,142 @@ def test_pages(batch):
 def test_refusals(batch, over, args, match):
     with pytest.raises(ValueError, match=match):
         batch.check_batch(_config(**over), *args)
+
+
+class Host:
+    """A BatchDecoder on the CPU: pages by the loops of paged_model.py, greedy tokens, and logits that
+    follow from a sequence's stored tokens."""
+
+    def __new__(cls, batch, monkeypatch, n_seq, n_pages, vocab=61, max_seq=70):
+        import types
+
+        import numpy as np
+        import paged_model
+
+        cfg = _config(vocab=vocab, max_seq=max_seq)
+        for name in ("attention_workspace", "grow_workspace", "compact_workspace"):
+            monkeypatch.setattr(batch.paged, name, lambda *a: None)
+        monkeypatch.setattr(batch.sampling, "workspace", lambda *a: None)
+        m = batch.BatchDecoder(cfg, types.SimpleNamespace(lm_head_gg=None), n_seq, n_pages,
+                               device="cpu")
+        stored = {}  # per sequence, by slot
+
+        def grow(kv, tables, lengths, refs, rows, room, work):
+            t, r, end, _ = paged_model.grow(tables.numpy(), lengths.numpy(), refs.numpy(),
+                                            rows.tolist(), kv.shape[-2])
+            for to, new in ((tables, t), (refs, r), (room, end)):
+                to.copy_(torch.from_numpy(new))
+
+        def fork(tables, lengths, refs, parents):
+            new = paged_model.fork(tables.numpy(), lengths.numpy(), refs.numpy(), parents.tolist())
+            for to, x in zip((tables, lengths, refs), new):
+                to.copy_(torch.from_numpy(x))
+            old = {s: dict(x) for s, x in stored.items()}
+            for s, p in enumerate(parents.tolist()):
+                stored[s] = dict(old.get(p, {}))
+
+        def layers(x, pos, held=0):
+            out = []
+            for i, tok in enumerate(x[:, 0].long().tolist()):
+                s = i if m._prompt is None else m._prompt
+                at = int(m.lengths[s]) + (0 if m._prompt is None else i)
+                takes = m._prompt is not None or (int(m.rows[s]) and int(m.room[s]) > at)
+                if takes:
+                    stored.setdefault(s, {})[at] = tok
+                history = [stored[s][j] for j in range(at + 1)] if takes else []
+                seed = hash(tuple(history)) % 2 ** 32
+                row = np.random.default_rng(seed).standard_normal(vocab)
+                out.append(torch.from_numpy(row if takes else row * float("nan")))
+            return torch.stack(out).float()
+
+        def sample(logits, u, out, work, *settings, probs):
+            gone = torch.isnan(logits).all(-1)
+            out.copy_(torch.where(gone, 0, logits.nan_to_num(-1e9).argmax(-1)))
+            probs.copy_((~gone).float())
+
+        monkeypatch.setattr(batch.paged, "grow", grow)
+        monkeypatch.setattr(batch.paged, "fork", fork)
+        monkeypatch.setattr(batch.sampling, "sample", sample)
+        m._embed, m._layers_glue, m._proj = lambda t: t.view(-1, 1).float(), layers, lambda h, w, n: h
+        m.stored = stored
+        return m
+
+
+def _start(m, lengths):
+    for s, n in enumerate(lengths):
+        m.prefill(torch.arange(1, n + 1), s)
+    m.tok.copy_(torch.arange(11, 11 + len(lengths)))
+    m.rows.fill_(1)
+
+
+def test_a_sequence_without_a_page_goes_on_with_its_token(batch, monkeypatch):
+    """Sequence 1 needs its second page when the pool is full; once another sequence has gone it goes
+    on as in a pool that had the room, from the very token that it could not store."""
+    with monkeypatch.context() as mp:
+        want = Host(batch, mp, 3, 15)
+        _start(want, (15, 14, 40))
+        for _ in range(13):
+            want.step()
+    m = Host(batch, monkeypatch, 3, 5)   # 1 + 1 + 3: no page is free
+    _start(m, (15, 14, 40))
+    for step in range(6):
+        logits = m.step()
+        assert torch.isnan(logits[:2]).all(-1).tolist() == [step >= 1, step >= 2]
+    assert m.lengths.tolist() == [16, 16, 46]
+    assert m.tok[:2].tolist() == [0, 0] and m.rows.tolist() == [1, 1, 1]
+    m.fork([0, 1, -1])
+    for _ in range(10):
+        assert torch.isfinite(m.step()[:2]).all()
+    assert m.lengths.tolist() == [26, 26, 0]
+    for s in range(2):
+        assert m.stored[s] == {j: want.stored[s][j] for j in range(26)}
+        assert int(m.tok[s]) == want.stored[s][26]
+
+
+def test_a_waiting_token_is_forked_replaced_and_freed(batch, monkeypatch):
+    m = Host(batch, monkeypatch, 4, 4)
+    _start(m, (16, 16, 16, 15))
+    m.step()
+    m.step()                          # 0, 1 and 2 wait with 11, 12 and 13; 3 waits since this step
+    waits = m.stored[3][15]
+    assert waits == 14 and m.tok.tolist() == [0, 0, 0, 0]
+    m.fork([0, 0, 2, -1])             # 1 becomes a fork of 0; two pages are free now
+    m.tok[2] = 33
+    m.step()                          # 0 and 1 get them
+    assert m.stored[0][16] == 11 and m.stored[1][16] == 11 and m.lengths.tolist() == [17, 17, 16, 0]
+    assert int(m.tok[0]) == int(m.tok[1]) != 0
+    m.fork([0, -1, 2, -1])
+    m.step()
+    assert m.stored[2][16] == 33
+    m.fork([-1, 1, 2, -1])
+    m.prefill(torch.arange(1, 4), 1)  # in a sequence that was freed nothing waits
+    m.rows[1] = 1
+    assert int(m.tok[1]) == 0
+    m.step()
+    assert m.stored[1] == {0: 1, 1: 2, 2: 3, 3: 0}
+
+
+def test_a_prompt_behind_a_waiting_token(batch, monkeypatch):
+    """The token shows again, and is stored behind the prompt, as one that had not waited."""
+    m = Host(batch, monkeypatch, 2, 2)
+    _start(m, (16, 16))
+    m.step()
+    assert m.tok.tolist() == [0, 0]
+    m.fork([0, -1])
+    m.prefill(torch.arange(1, 4), 0)
+    assert m.tok.tolist() == [11, 0] and m.lengths.tolist() == [19, 0]
+    m.tok[0] = 0                      # token 0 is a token like another now
+    m.step()
+    assert m.stored[0][19] == 0
+
+
+def test_stop_ends_no_sequence_that_waits(batch, monkeypatch):
+    """Token 0 of a sequence without room is not a draw of the stop token 0."""
+    m = Host(batch, monkeypatch, 2, 2)
+    m.set_sampling(stop=0)
+    _start(m, (16, 12))
+    m.step()
+    assert m.tok[0] == 0 and m.rows.tolist() == [1, 1]
+    m.fork([0, -1])
+    m.step()
+    assert m.stored[0][16] == 11

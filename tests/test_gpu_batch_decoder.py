@@ -353,3 +353,39 @@ def test_a_model_file(batch, tmp_path):
     assert torch.equal(a["tokens"], b["tokens"]) and torch.equal(a["probs"], b["probs"])
     with pytest.raises(ValueError, match="sequences"):
         gmodel.load_batch_decoder(p, 0)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_sequence_that_had_no_page_goes_on(dec, batch, graph):
+    """Sequences that stall in a full pool go on, once another one has gone, with the logits, tokens
+    and probabilities of a decoder that always had room, bit for bit; the stop token 0 does not end
+    them while they wait."""
+    cfg, w = _model(dec, max_seq=64)
+    small, large = batch.BatchDecoder(cfg, w, 3, n_pages=5), batch.BatchDecoder(cfg, w, 3)
+    for m in (small, large):
+        m.set_sampling(temperature=1.0, seed=3, stop=0)
+        for s, n in ((0, 15), (1, 14), (2, 40)):
+            m.prefill(_tokens(cfg, n, s), s)
+        m.rows.fill_(1)
+        m.tok.copy_(torch.tensor([5, 6, 7]))
+    want, step = [], small.capture().replay if graph else small.step
+    for _ in range(20):
+        logits = large.step()
+        want.append((logits[:2].clone(), large.tok[:2].clone(), large.probs[:2].clone()))
+    assert large.rows[:2].tolist() == [1, 1]  # neither has drawn the stop token
+    at = [0, 0]
+    for turn in range(16):
+        if turn == 5:                         # pages of 1 + 1 + 3; 0 and 1 have waited since 1 and 2
+            assert small.lengths.tolist()[:2] == [16, 16] and small.rows.tolist()[:2] == [1, 1]
+            assert small.tok.tolist()[:2] == [0, 0] and small.probs.tolist()[:2] == [0, 0]
+            small.fork([0, 1, -1])
+        got = step()
+        got = small._logits if graph else got
+        for s in range(2):
+            if turn < 5 and turn > s:
+                assert torch.isnan(got[s]).all()
+                continue
+            logits, tok, probs = (x[s] for x in want[at[s]])
+            assert torch.equal(got[s], logits) and small.tok[s] == tok and small.probs[s] == probs
+            at[s] += 1
+    assert at == [12, 13]
