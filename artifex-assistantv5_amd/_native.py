@@ -187,7 +187,7 @@ _tensors = None
 
 def direct():
     """The module of calls straight from tensors (csrc/tensors.cpp), which return False where their
-    arguments do not fit; raises if it is missing."""
+    arguments do not fit and raise by ``check`` where the call failed; raises if it is missing."""
     global _tensors
     if _tensors is None:
         lib = load_library()
@@ -197,6 +197,7 @@ def direct():
         loader = importlib.machinery.ExtensionFileLoader("_tensors", path)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_tensors", loader))
         module.bind(*(ctypes.cast(getattr(lib, name), _vp).value for name in PACKED))
+        module.on_failure(check)
         _tensors = module
     return _tensors
 

@@ -2,8 +2,10 @@
 //
 // Each function takes the arguments of its namesake in paged.py or sampling.py, all of them, checks
 // what that one checks, and calls the entry point on the current stream.  It returns True if the call
-// has been made, else False with nothing done: the Python function then makes its own checks, which
-// name what is wrong, and the calls whose device is not the current one.
+// has been made, and False with nothing done where the arguments do not fit: the Python function then
+// makes its own checks, which name what is wrong, and the calls whose device is not the current one.
+// A call that failed otherwise may have launched some of its kernels, so it is not to be made again:
+// it raises what `on_failure` was given for that.
 //
 // Checks in Python, tensor by tensor, and the arguments' packing cost 4 us a call, more than the smaller
 // kernels take.  us of calls from Python, before and with these: attention over 300 slots 10.4, 8.5; 146
@@ -31,6 +33,7 @@ struct Entries {
 } entry;
 constexpr int kEntries = sizeof(Entries) / sizeof(void *);
 PyObject *current_device, *current_stream;
+PyObject *failure;  // called with an entry point's code, raises
 
 using at::ScalarType;
 
@@ -164,26 +167,31 @@ struct Tables {
   }
 };
 
-// The call, if everything fits, without the interpreter's lock; no exception passes.
+// The call, if everything fits, without the interpreter's lock; no exception of C++ passes.
+constexpr int kRefused = 1;  // no code of an entry point
 template <typename F>
 PyObject *guarded(F make) {
-  bool done = false;
+  int rc = kRefused;
   try {
-    done = make();
+    rc = make();
   } catch (...) {
   }
   if (PyErr_Occurred()) PyErr_Clear();
-  return PyBool_FromLong(done);
+  if (rc == GGUF_HIP_OK || rc == kRefused) return PyBool_FromLong(rc == GGUF_HIP_OK);
+  PyObject *r = failure ? PyObject_CallFunction(failure, "i", rc) : nullptr;
+  Py_XDECREF(r);
+  if (!PyErr_Occurred()) PyErr_Format(PyExc_RuntimeError, "a call failed with %d", rc);
+  return nullptr;
 }
 template <typename E, typename... T>
-bool launch(Args &x, E call, T... args) {
+int launch(Args &x, E call, T... args) {
   void *stream = x.stream();
-  if (!x.ok) return false;
+  if (!x.ok) return kRefused;
   int rc;
   Py_BEGIN_ALLOW_THREADS;
   rc = call(args..., stream);
   Py_END_ALLOW_THREADS;
-  return rc == GGUF_HIP_OK;
+  return rc <= GGUF_HIP_ERR_TYPE && rc >= GGUF_HIP_ERR_BYTES ? kRefused : rc;  // by its own checks
 }
 
 PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t n) {
@@ -319,10 +327,19 @@ PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// What a failed call raises by: called with its code.
+PyObject *on_failure(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 1 || !PyCallable_Check(args[0])) return PyErr_Format(PyExc_TypeError, "one callable");
+  Py_INCREF(args[0]);
+  Py_XDECREF(failure);
+  failure = args[0];
+  Py_RETURN_NONE;
+}
+
 #define FUNCTION(name) {#name, (PyCFunction)(void *)name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FUNCTION(append), FUNCTION(attention), FUNCTION(load),   FUNCTION(fork),
                          FUNCTION(grow),   FUNCTION(compact),   FUNCTION(sample), FUNCTION(bind),
-                         {nullptr, nullptr, 0, nullptr}};
+                         FUNCTION(on_failure), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, methods};
 
 }  // namespace

@@ -38,3 +38,10 @@ def test_missing_module(native, monkeypatch, tmp_path):
     monkeypatch.setattr(native, "LIB_PATH", str(tmp_path / "libgguf_hip.so"))
     with pytest.raises(RuntimeError, match="is not built"):
         native.direct()
+
+
+def test_on_failure(native):
+    for args in ((), (1,), (native.check, native.check)):
+        with pytest.raises(TypeError, match="one callable"):
+            native.direct().on_failure(*args)
+    native.direct().on_failure(native.check)

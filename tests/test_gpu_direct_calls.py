@@ -183,3 +183,45 @@ def test_streams_and_threads(native, ops):
     a = _args(ops, "attention")
     ops["paged"].attention(*a)
     assert all(torch.equal(got[k], a[6]) for k in range(4))
+
+
+@pytest.fixture
+def answers(native):
+    """Entry points that do nothing but return a code, and count their calls."""
+    import ctypes
+
+    signatures = {**native.PAGED_SIGNATURES, **native.SAMPLE_SIGNATURES}
+    state = dict(rc=0, calls=0)
+
+    def answer(*args):
+        state["calls"] += 1
+        return state["rc"]
+
+    stubs = [ctypes.CFUNCTYPE(signatures[n][0], *signatures[n][1])(answer) for n in native.PACKED]
+    lib, direct = native.load_library(), native.direct()
+    address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
+    direct.bind(*map(address, stubs))
+    yield state
+    direct.bind(*(address(getattr(lib, n)) for n in native.PACKED))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_call_that_failed_is_not_made_again(native, ops, answers, name):
+    """A HIP error may come after the first of two launches: it is raised, and nothing more is done."""
+    args = _args(ops, name)
+    before = [x.clone() if isinstance(x, torch.Tensor) else x for x in args]
+    for rc in (native.ERR_HIP, -99):
+        answers.update(rc=rc, calls=0)
+        with pytest.raises(native.GGUFHipError) as e:
+            _call(ops, name, args)
+        assert e.value.code == rc and answers["calls"] == 1
+        for x, old in zip(args, before):
+            if isinstance(x, torch.Tensor) and x.dtype is not torch.uint8:
+                assert torch.equal(x, old)
+    f = getattr(native.direct(), name)
+    for rc in (native.ERR_TYPE, native.ERR_SHAPE, native.ERR_NULL, native.ERR_ALIGN, native.ERR_DTYPE,
+               native.ERR_BYTES):
+        answers.update(rc=rc, calls=0)
+        assert f(*args) is False and answers["calls"] == 1
+    answers.update(rc=0, calls=0)
+    assert f(*args) is True and answers["calls"] == 1
