@@ -351,6 +351,7 @@ class QuantDecoder(LayerStack):
             self.w_att = glue.attention_workspace(cfg.n_heads, cfg.n_kv_heads, hd, T, self.device)
         self.w_arg = glue.argmax_workspace(self.device)
         self._draw = self._u = None
+        self._chosen: dict = {}             # set_sampling's arguments
 
     # -- the choice of the next token --
     def set_sampling(self, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
@@ -358,6 +359,12 @@ class QuantDecoder(LayerStack):
         """How the next tokens are chosen (``sampling.sample``); ``temperature`` 0: the largest
         logit.  The random numbers, one for each position, follow from ``seed``.  Steps captured
         before keep the settings that they were captured with, and read the new random numbers."""
+        choice = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, seed=seed)
+        self._set_sampling(**choice)
+        self._chosen = choice
+
+    def _set_sampling(self, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
+                      min_p: float = 0.0, seed: int = 0) -> None:
         if not temperature > 0:
             self._draw = None
             return
@@ -644,13 +651,15 @@ class QuantDecoder(LayerStack):
 
     @torch.no_grad()
     def generate(self, prompt: torch.Tensor, n_new: int, graph: bool = True,
-                 temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
-                 seed: int = 0) -> dict:
-        """Generation, greedy or sampled (``set_sampling``): returns the new token ids and prefill /
-        decode timings.  tok/s = n_new / decode wall time (prefill excluded,
+                 temperature: Optional[float] = None, top_k: Optional[int] = None,
+                 top_p: Optional[float] = None, min_p: Optional[float] = None,
+                 seed: Optional[int] = None) -> dict:
+        """Generation, greedy or sampled: returns the new token ids and prefill / decode timings.
+        What is not given of the settings is what ``set_sampling`` chose; what is given holds until
+        the next call of either.  tok/s = n_new / decode wall time (prefill excluded,
         generate.ts:1155-1160)."""
         dev = self.device
-        self.set_sampling(temperature, top_k, top_p, min_p, seed)
+        given = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, seed=seed)
         if prompt.numel() + n_new > self.cfg.max_seq:
             raise ValueError(f"prompt {prompt.numel()} + {n_new} new tokens exceed max_seq "
                              f"{self.cfg.max_seq}")
@@ -658,6 +667,7 @@ class QuantDecoder(LayerStack):
                 and prompt.numel() + n_new > self.kv_slots + 1):
             raise ValueError(f"prompt {prompt.numel()} + {n_new} new tokens exceed the cache's "
                              f"{self.kv_slots} slots (kv_keep bounds it)")
+        self._set_sampling(**{**self._chosen, **{k: v for k, v in given.items() if v is not None}})
         if self.kv_bits == 32:
             self.k_cache.zero_()
             self.v_cache.zero_()

@@ -389,3 +389,28 @@ def test_a_sequence_that_had_no_page_goes_on(dec, batch, graph):
             assert torch.equal(got[s], logits) and small.tok[s] == tok and small.probs[s] == probs
             at[s] += 1
     assert at == [12, 13]
+
+
+@pytest.mark.parametrize("kw", [{}, dict(fused=False), dict(kv_bits=4)])
+def test_generate_by_the_settings_chosen_before(dec, kw):
+    """What generate is not given is what set_sampling chose; what it is given is not kept."""
+    cfg, w = _model(dec)
+    m = dec.QuantDecoder(cfg, w, **kw)
+    prompt = _tokens(cfg, 12, 9)
+    run = lambda **choice: m.generate(prompt, 30, **choice)["tokens"]  # noqa: E731
+    greedy = run()
+    drawn = run(temperature=1.0, top_p=0.95, seed=1)
+    other = run(temperature=1.0, top_p=0.95, seed=2)
+    assert not torch.equal(drawn, greedy) and not torch.equal(drawn, other)
+    m.set_sampling(temperature=1.0, top_p=0.95, seed=1)
+    assert torch.equal(run(), drawn) and torch.equal(run(graph=False), drawn)
+    assert torch.equal(run(seed=2), other) and torch.equal(run(temperature=0.0), greedy)
+    with pytest.raises(ValueError, match="max_seq"):
+        m.generate(prompt, cfg.max_seq, temperature=0.0)
+    assert m._draw is None               # as run() above left it: a refused call changes nothing
+    assert torch.equal(run(), drawn)
+    with pytest.raises(ValueError, match="max_seq"):
+        m.generate(prompt, cfg.max_seq, temperature=0.0)
+    assert m._draw == dict(temperature=1.0, top_k=0, top_p=0.95, min_p=0.0)
+    m.set_sampling()
+    assert torch.equal(run(), greedy)
