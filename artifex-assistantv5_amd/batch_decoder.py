@@ -78,7 +78,8 @@ class BatchDecoder(LayerStack):
         self._seq = torch.arange(n_seq, device=dev)
         self._logits = None
         self._prompt = None                 # the sequence whose prompt runs; None: a step
-        self.set_sampling()
+        self._set_sampling()
+        self._chosen: dict = {}             # set_sampling's arguments
 
     # -- the choice of the tokens --
     def set_sampling(self, temperature: Setting = 0.0, top_k: Setting = 0, top_p: Setting = 1.0,
@@ -87,6 +88,12 @@ class BatchDecoder(LayerStack):
         each.  The random numbers follow from ``seed``.  A sequence whose token is ``stop`` rests
         from then on.  Steps captured before read these settings too, except whether there is a
         ``stop``."""
+        self._set_sampling(temperature, top_k, top_p, min_p, seed, stop)
+        self._chosen = dict(temperature=self._temperature.clone(), top_k=self._top_k.clone(),
+                            top_p=self._top_p.clone(), min_p=self._min_p.clone(), seed=seed, stop=stop)
+
+    def _set_sampling(self, temperature: Setting = 0.0, top_k: Setting = 0, top_p: Setting = 1.0,
+                      min_p: Setting = 0.0, seed: int = 0, stop: Optional[int] = None) -> None:
         dev, n = self.device, self.n_seq
 
         def each(name, v, dtype):
@@ -247,8 +254,9 @@ class BatchDecoder(LayerStack):
                  graph: bool = True, **choice) -> dict:
         """``samples`` continuations of each prompt (device int64 [M]), ``n_new`` tokens each, from
         an empty cache; ``choice``: ``set_sampling``'s arguments, for sequence ``i * samples + j``
-        the j-th continuation of prompt i.  Returns their tokens [sequences, n_new] (after ``stop``:
-        ``stop``), the probabilities they were drawn with, and prefill / decode timings."""
+        the j-th continuation of prompt i, which hold until the next call of either; those that are
+        not given are what ``set_sampling`` chose.  Returns their tokens [sequences, n_new] (after
+        ``stop``: ``stop``), the probabilities they were drawn with, and prefill / decode timings."""
         dev, n = self.device, len(prompts) * samples
         if samples < 1 or n_new < 1 or not 0 < n <= self.n_seq:
             raise ValueError(f"{len(prompts)} prompts of {samples} continuations of {n_new} tokens for "
@@ -264,7 +272,7 @@ class BatchDecoder(LayerStack):
             need += shared + samples * (-(-(p.numel() + n_new - 1) // page) - shared)
         if need > self.kv.shape[1]:
             raise ValueError(f"the sequences need {need} pages, the pool has {self.kv.shape[1]}")
-        self.set_sampling(**choice)
+        self._set_sampling(**{**self._chosen, **choice})
         self.reset()
         torch.cuda.synchronize(dev)
         t0 = time.perf_counter()

@@ -174,3 +174,32 @@ def test_stop_ends_no_sequence_that_waits(batch, monkeypatch):
     m.fork([0, -1])
     m.step()
     assert m.stored[0][16] == 11
+
+
+def _settings(m):
+    return [t.tolist() for t in (m._temperature, m._top_k, m._top_p, m._min_p, m._u)] + [m._stop]
+
+
+def test_generate_by_the_settings_chosen_before(batch, monkeypatch):
+    """What generate is not given is what set_sampling chose; what it is given is not kept."""
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    m = Host(batch, monkeypatch, 3, 15)
+    run = lambda **choice: m.generate([torch.arange(1, 9)], 3, graph=False, **choice)  # noqa: E731
+    plain = _settings(m)
+    run()
+    assert _settings(m) == plain
+    run(temperature=2.0, top_k=3, stop=5)
+    assert m._temperature.tolist() == [2.0] * 3 and m._top_k.tolist() == [3] * 3 and m._stop == 5
+    run()
+    assert _settings(m) == plain
+    warm = torch.tensor([0.5, 1.0, 2.0])
+    m.set_sampling(temperature=warm, top_p=0.5, min_p=[0.0, 0.25, 0.5], seed=3, stop=7)
+    chosen = _settings(m)
+    warm.zero_()                      # the caller's own afterwards
+    for given, changed in (({}, {}), (dict(top_k=9, stop=None), {1: [9] * 3, 5: None}), ({}, {}),
+                           (dict(temperature=0.0), {0: [0.0] * 3}), ({}, {})):
+        run(**given)
+        assert _settings(m) == [changed.get(i, x) for i, x in enumerate(chosen)]
+    m.set_sampling()
+    run()
+    assert _settings(m) == plain
