@@ -86,8 +86,8 @@ class BatchDecoder(LayerStack):
                      min_p: Setting = 0.0, seed: int = 0, stop: Optional[int] = None) -> None:
         """How the next tokens are chosen (``sampling.sample``): values for all sequences or one for
         each.  The random numbers follow from ``seed``.  A sequence whose token is ``stop`` rests
-        from then on.  Steps captured before read these settings too, except whether there is a
-        ``stop``."""
+        from then on.  Steps captured before read these settings too, but for a ``stop`` where they
+        were captured without any."""
         self._set_sampling(temperature, top_k, top_p, min_p, seed, stop)
         self._chosen = dict(temperature=self._temperature.clone(), top_k=self._top_k.clone(),
                             top_p=self._top_p.clone(), min_p=self._min_p.clone(), seed=seed, stop=stop)
@@ -111,6 +111,9 @@ class BatchDecoder(LayerStack):
         self._top_p = each("top_p", top_p, torch.float32)
         self._min_p = each("min_p", min_p, torch.float32)
         self._stop = stop
+        stop_tok = torch.full((1,), -1 if stop is None else stop, dtype=torch.int64, device=dev)
+        old = getattr(self, "_stop_tok", None)
+        self._stop_tok = stop_tok if old is None else old.copy_(stop_tok)  # what captured steps read
         # a row of random numbers for each position; two sequences at one position have their own
         g = torch.Generator(device=dev).manual_seed(seed)
         if getattr(self, "_u", None) is None:
@@ -131,7 +134,7 @@ class BatchDecoder(LayerStack):
         self.tok.copy_(torch.where(on, tok, self.tok))
         self.probs.copy_(torch.where(on, probs, self.probs))
         if self._stop is not None:
-            self.rows.mul_((self.tok != self._stop) | (stored == 0))
+            self.rows.mul_((self.tok != self._stop_tok) | (stored == 0))
 
     # -- the cache --
     def reset(self) -> None:

@@ -414,3 +414,41 @@ def test_generate_by_the_settings_chosen_before(dec, kw):
     assert m._draw == dict(temperature=1.0, top_k=0, top_p=0.95, min_p=0.0)
     m.set_sampling()
     assert torch.equal(run(), greedy)
+
+
+def test_captured_step_reads_a_new_stop(dec, batch):
+    """A step captured with a stop token rests at another one that is set later, and at none."""
+    cfg, w = _model(dec, max_seq=96)
+    m = batch.BatchDecoder(cfg, w, 2)
+    first = [m.prefill(_tokens(cfg, n, n), s)[0].argmax() for s, n in ((0, 9), (1, 14))]
+    m.fork([0, 1])
+
+    def begin():
+        m.reset()
+        for s, n in ((0, 9), (1, 14)):
+            m.prefill(_tokens(cfg, n, n), s)
+        m.tok.copy_(torch.stack(first))
+        m.rows.fill_(1)
+
+    def free(n):                              # tokens of n steps without a stop
+        begin()
+        m.set_sampling(temperature=1.0, seed=4)
+        return torch.stack([m.tok.clone() for _ in range(n) if m.step() is not None])
+
+    tok = free(12)
+    a, b = tok[3, 0], tok[8, 1]
+    assert not (tok[:3] == a).any() and not (tok[:8, 1] == b).any() and a != b
+    begin()
+    m.set_sampling(temperature=1.0, seed=4, stop=int(a))
+    graph = m.capture()
+    for stop in (int(a), int(b), None, int(b)):
+        begin()
+        m.set_sampling(temperature=1.0, seed=4, stop=stop)
+        rests = [False, False]
+        for t in range(12):
+            graph.replay()
+            for s in range(2):
+                if not rests[s]:
+                    assert m.tok[s] == tok[t, s]
+                    rests[s] = stop is not None and int(tok[t, s]) == stop
+                assert int(m.rows[s]) == (not rests[s])
