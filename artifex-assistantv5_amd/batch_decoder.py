@@ -100,25 +100,20 @@ class BatchDecoder(LayerStack):
             t = torch.as_tensor(v, dtype=dtype).to(dev)
             if t.dim() > 1 or (t.dim() == 1 and t.shape[0] != n):
                 raise ValueError(f"{name} must be one value, or one for each of {n} sequences")
-            t = t.expand(n).contiguous()
-            old = getattr(self, "_" + name, None)
-            if old is None:
-                return t.clone()
-            return old.copy_(t)
+            return t.expand(n).contiguous()
 
-        self._temperature = each("temperature", temperature, torch.float32)
-        self._top_k = each("top_k", top_k, torch.int32)
-        self._top_p = each("top_p", top_p, torch.float32)
-        self._min_p = each("min_p", min_p, torch.float32)
-        self._stop = stop
-        stop_tok = torch.full((1,), -1 if stop is None else stop, dtype=torch.int64, device=dev)
-        old = getattr(self, "_stop_tok", None)
-        self._stop_tok = stop_tok if old is None else old.copy_(stop_tok)  # what captured steps read
         # a row of random numbers for each position; two sequences at one position have their own
         g = torch.Generator(device=dev).manual_seed(seed)
-        if getattr(self, "_u", None) is None:
-            self._u = torch.empty(self.slots, n, device=dev)
-        self._u.copy_(torch.rand(self._u.shape, device=dev, generator=g))
+        new = dict(_temperature=each("temperature", temperature, torch.float32),
+                   _top_k=each("top_k", top_k, torch.int32),
+                   _top_p=each("top_p", top_p, torch.float32),
+                   _min_p=each("min_p", min_p, torch.float32),
+                   _stop_tok=torch.full((1,), -1 if stop is None else stop, dtype=torch.int64, device=dev),
+                   _u=torch.rand(self.slots, n, device=dev, generator=g))
+        for name, t in new.items():  # all of them fit; in place, for steps captured before
+            old = getattr(self, name, None)
+            setattr(self, name, t.clone() if old is None else old.copy_(t))
+        self._stop = stop
 
     def _choose(self, logits: torch.Tensor, takes: torch.Tensor, stored: torch.Tensor) -> None:
         """The tokens after the last slots of the sequences for which ``takes`` (int64, 0 or 1),

@@ -203,3 +203,18 @@ def test_generate_by_the_settings_chosen_before(batch, monkeypatch):
     m.set_sampling()
     run()
     assert _settings(m) == plain
+
+
+@pytest.mark.parametrize("wrong", [dict(top_k=[1, 2]), dict(top_p=[[0.5]] * 3), dict(min_p="x"),
+                                   dict(seed="x"), dict(stop="x")])
+def test_refused_settings_change_nothing(batch, monkeypatch, wrong):
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    m = Host(batch, monkeypatch, 3, 15)
+    m.set_sampling(temperature=0.5, top_k=7, seed=2, stop=4)
+    before = _settings(m)
+    with pytest.raises((ValueError, TypeError, RuntimeError)):
+        m.set_sampling(**{**dict(temperature=[1.0, 2.0, 3.0], seed=9, stop=8), **wrong})
+    assert _settings(m) == before
+    m.generate([torch.arange(1, 9)], 2, graph=False, temperature=2.0)
+    m.generate([torch.arange(1, 9)], 2, graph=False)
+    assert _settings(m) == before
