@@ -260,6 +260,8 @@ class BatchDecoder(LayerStack):
             raise ValueError(f"{len(prompts)} prompts of {samples} continuations of {n_new} tokens for "
                              f"{self.n_seq} sequences")
         for p in prompts:
+            if p.numel() == 0:
+                raise ValueError("an empty prompt has no logits")
             if p.numel() + n_new - 1 > self.cfg.max_seq:
                 raise ValueError(f"prompt {p.numel()} + {n_new} new tokens exceed max_seq "
                                  f"{self.cfg.max_seq}")

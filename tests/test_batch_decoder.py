@@ -218,3 +218,15 @@ def test_refused_settings_change_nothing(batch, monkeypatch, wrong):
     m.generate([torch.arange(1, 9)], 2, graph=False, temperature=2.0)
     m.generate([torch.arange(1, 9)], 2, graph=False)
     assert _settings(m) == before
+
+
+def test_generate_refuses_an_empty_prompt_before_it_clears(batch, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    m = Host(batch, monkeypatch, 2, 10)
+    _start(m, (16, 5))
+    before = [t.clone() for t in (m.tables, m.lengths, m.refs, m.rows, m.tok)] + _settings(m)
+    with pytest.raises(ValueError, match="empty"):
+        m.generate([torch.arange(1, 9), torch.arange(0)], 2, graph=False, temperature=2.0)
+    after = [m.tables, m.lengths, m.refs, m.rows, m.tok] + _settings(m)
+    for x, old in zip(after, before):
+        assert torch.equal(x, old) if isinstance(x, torch.Tensor) else x == old
