@@ -21,7 +21,7 @@ from typing import Optional, Sequence, Union
 
 import torch
 
-from . import glue, paged, sampling
+from . import _native, glue, paged, sampling
 from .decoder import DecoderConfig, DecoderWeights, LayerStack, glue_shapes, rope_tables
 
 Setting = Union[float, int, Sequence, torch.Tensor]
@@ -41,6 +41,14 @@ def check_batch(cfg: DecoderConfig, n_seq: int, n_pages: Optional[int], page: in
     columns = -(-cfg.max_seq // page)
     n_pages = n_seq * columns if n_pages is None else n_pages
     paged.pool_bytes(n_pages, cfg.n_kv_heads, cfg.head_dim, page)
+    if not 1 <= cfg.n_layers <= 65535:
+        raise ValueError(f"BatchDecoder: {cfg.n_layers} layers not in 1..65535")
+    # what the calls over its sequences, of a prompt and of a draw take
+    lib = _native.load_library()
+    heads = (cfg.n_heads, cfg.n_kv_heads, cfg.head_dim)
+    _native.check(lib.gguf_hip_paged_attention_workspace(page, columns, n_seq, *heads), lib)
+    _native.check(lib.gguf_hip_attention_workspace(*heads, columns * page), lib)
+    _native.check(lib.gguf_hip_sample_workspace(n_seq, cfg.vocab), lib)
     return columns, n_pages
 
 

@@ -230,3 +230,28 @@ def test_generate_refuses_an_empty_prompt_before_it_clears(batch, monkeypatch):
     after = [m.tables, m.lengths, m.refs, m.rows, m.tok] + _settings(m)
     for x, old in zip(after, before):
         assert torch.equal(x, old) if isinstance(x, torch.Tensor) else x == old
+
+
+@pytest.mark.parametrize("over,args,match", [
+    (dict(n_heads=32, n_kv_heads=32), (4096, 8192, 16, torch.float16), "4096 sequences of 32 KV heads"),
+    (dict(max_seq=1 << 23), (1, 8192, 16, torch.float16), "524288 columns"),
+    (dict(vocab=(1 << 20) + 1), (3, None, 16, torch.float16), "vocabulary"),
+    (dict(n_layers=65536), (3, None, 16, torch.float16), "65536 layers"),
+    (dict(max_seq=0), (3, 8, 16, torch.float16), "columns"),
+    (dict(max_seq=(1 << 20) + 1), (1, 8192, 16, torch.float16), "max_seq 1048592 out of range"),
+    (dict(n_heads=64, n_kv_heads=64, head_dim=256, max_seq=1 << 18), (1, 8192, 16, torch.float16),
+     "cache of one layer too large"),
+])
+def test_refuses_what_no_call_would_take(batch, monkeypatch, over, args, match):
+    """Before a tensor is placed: neither the decoder nor a file's loader makes any."""
+    with pytest.raises(ValueError, match=match):
+        batch.check_batch(_config(**over), *args)
+    monkeypatch.setattr(torch, "zeros", None)
+    monkeypatch.setattr(torch, "full", None)
+    with pytest.raises(ValueError, match=match):
+        batch.BatchDecoder(_config(**over), None, *args)
+
+
+def test_takes_the_largest(batch):
+    cfg = _config(n_heads=16, n_kv_heads=15 + 1, max_seq=1 << 20, vocab=1 << 20)
+    assert batch.check_batch(cfg, 4095, 8192, 256, torch.float16) == (1 << 12, 8192)
