@@ -74,14 +74,7 @@ def _build_tensors() -> str:
     return TENSORS
 
 
-def build(verbose: bool = False) -> str:
-    """Compile every HIP source and link ``libgguf_hip.so``; returns its path."""
-    os.makedirs(BUILD, exist_ok=True)
-    workers = max(1, min(len(SOURCES), len(os.sched_getaffinity(0))))
-    with concurrent.futures.ThreadPoolExecutor(max_workers=workers) as ex:
-        tensors = ex.submit(_build_tensors)
-        objs = list(ex.map(lambda s: _compile(s, verbose), SOURCES))
-        tensors.result()
+def _link(objs: list) -> None:
     tmp = LIB + ".tmp"
     # Export the C ABI only: kernel stubs and helpers bind locally, so two
     # builds of the library in one process cannot interpose each other.
@@ -95,6 +88,18 @@ def build(verbose: bool = False) -> str:
         print(res.stdout + res.stderr, file=sys.stderr)
         raise RuntimeError("hipcc link failed")
     os.replace(tmp, LIB)
+
+
+def build(verbose: bool = False) -> str:
+    """Compile every HIP source and link ``libgguf_hip.so``; returns its path.  ``_tensors.so`` is
+    built beside it; where that fails, the library, which needs hipcc alone, is there and this
+    raises."""
+    os.makedirs(BUILD, exist_ok=True)
+    workers = max(1, min(len(SOURCES), len(os.sched_getaffinity(0))))
+    with concurrent.futures.ThreadPoolExecutor(max_workers=workers) as ex:
+        tensors = ex.submit(_build_tensors)
+        _link(list(ex.map(lambda s: _compile(s, verbose), SOURCES)))
+        tensors.result()
     return LIB
 
 

@@ -45,3 +45,25 @@ def test_on_failure(native):
         with pytest.raises(TypeError, match="one callable"):
             native.direct().on_failure(*args)
     native.direct().on_failure(native.check)
+
+
+def test_the_library_is_linked_where_the_module_cannot_be_built(pkg, monkeypatch, tmp_path):
+    """A host with hipcc alone (no g++, no headers of Python's or torch's) still gets the C ABI."""
+    build = importlib.import_module("artifex-assistantv5_amd.build")
+    lib = tmp_path / "libgguf_hip.so"
+    monkeypatch.setattr(build, "LIB", str(lib))
+    monkeypatch.setattr(build, "BUILD", str(tmp_path / "_build"))
+    monkeypatch.setattr(build, "hipcc", lambda: "hipcc")
+    monkeypatch.setattr(build, "_compile", lambda src, verbose: str(tmp_path / src))
+
+    def run(cmd, **kw):
+        if cmd[0] == "g++":
+            raise FileNotFoundError("g++")
+        with open(cmd[cmd.index("-o") + 1], "w") as f:
+            f.write("linked")
+        return build.subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    with pytest.raises(FileNotFoundError, match="g\\+\\+"):
+        build.build()
+    assert lib.read_text() == "linked"
