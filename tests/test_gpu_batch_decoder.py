@@ -452,3 +452,40 @@ def test_captured_step_reads_a_new_stop(dec, batch):
                     assert m.tok[s] == tok[t, s]
                     rests[s] = stop is not None and int(tok[t, s]) == stop
                 assert int(m.rows[s]) == (not rests[s])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_draws_are_the_definitions(dec, batch, dtype):
+    """Each token after a prompt, after forks and in steps is the float64 rule's of the sequence's own
+    logits, settings and random number.  Its probability is rounded once, and weights are multiples
+    of 2^-43 of a sum that is 1 at least: 2^-24 of it and (1 + 512) 2^-44."""
+    from test_gpu_sampling import expected
+
+    cfg, w = _model(dec, max_seq=96)
+    m, e = (batch.BatchDecoder(cfg, w, 6, dtype=dtype) for _ in "ab")
+    kw = dict(temperature=[0.6, 1.0, 1.5, 0.0, 2.0, 1.2], top_k=[0, 40, 0, 5, 3, 0],
+              top_p=[0.7, 1.0, 0.95, 0.5, 0.6, 1.0], min_p=[0.0, 0.02, 0.1, 0.0, 0.0, 0.3])
+    prompts = [_tokens(cfg, 20, 1), _tokens(cfg, 9, 2)]
+
+    def check(logits, tok, probs, lengths, seed):
+        u = torch.rand(m.slots, 6, device="cuda",
+                       generator=torch.Generator(device="cuda").manual_seed(seed)).cpu().numpy()
+        for s in range(6):
+            t, p, q = (float(np.float32(kw[n][s])) for n in ("temperature", "top_p", "min_p"))
+            want, prob, _ = expected(logits[s].cpu().numpy(), u[lengths[s] - 1, s], t, kw["top_k"][s], p, q)
+            assert int(tok[s]) == want, s
+            assert abs(float(probs[s]) - prob) <= prob * 2.0 ** -24 + 513 * 2.0 ** -44, s
+
+    first = torch.cat([e.prefill(p, 3 * i).expand(3, -1) for i, p in enumerate(prompts)])
+    got = m.generate(prompts, 1, samples=3, seed=11, **kw)
+    check(first, got["tokens"][:, 0], got["probs"][:, 0], [20] * 3 + [9] * 3, 11)
+    drawn = set()
+    for step in range(25):
+        if step == 9:
+            m.set_sampling(seed=12, **kw)
+        if step == 14:
+            m.fork([2, 1, 0, 3, 5, 4])
+        logits = m.step()
+        check(logits, m.tok, m.probs, m.lengths.tolist(), 11 if step < 9 else 12)
+        drawn.update(m.tok.tolist())
+    assert len(drawn) > 30
