@@ -124,8 +124,8 @@ class BatchDecoder(LayerStack):
         self._stop = stop
 
     def _choose(self, logits: torch.Tensor, takes: torch.Tensor, stored: torch.Tensor) -> None:
-        """The tokens after the last slots of the sequences for which ``takes`` (int64, 0 or 1),
-        by ``logits`` [n_seq, vocab].  Where ``stored`` is 0 they are no draws, which ``stop``
+        """The tokens after the last slots of the sequences for which ``takes`` (bool), by ``logits``
+        [n_seq, vocab].  Where ``stored`` is 0 they are no draws, which ``stop``
         could end."""
         at = (self.lengths - 1).clamp_(0, self.slots - 1)
         u = self._u[at, self._seq]
@@ -133,9 +133,8 @@ class BatchDecoder(LayerStack):
         probs = torch.empty_like(self.probs)
         sampling.sample(logits, u, tok, self.w_draw, self._temperature, self._top_k, self._top_p,
                         self._min_p, probs=probs)
-        on = takes > 0
-        self.tok.copy_(torch.where(on, tok, self.tok))
-        self.probs.copy_(torch.where(on, probs, self.probs))
+        torch.where(takes, tok, self.tok, out=self.tok)
+        torch.where(takes, probs, self.probs, out=self.probs)
         if self._stop is not None:
             self.rows.mul_((self.tok != self._stop_tok) | (stored == 0))
 
@@ -233,10 +232,12 @@ class BatchDecoder(LayerStack):
         tok = self._next_tok()
         h = self._layers_glue(self._embed(tok), self.lengths)
         logits = self._proj(h, self.w.lm_head_gg, "lm_head")
-        stored = torch.minimum(self.lengths + self.rows, self.room) - self.lengths
+        stored = torch.minimum(self.rows, self.room - self.lengths)
         self.lengths.add_(stored)
-        self._waiting.copy_(torch.where(self.rows > 0, tok * (1 - stored), self._waiting))
-        self._choose(logits, self.rows, stored)
+        takes = self.rows > 0
+        # tok where it was not stored, 0 where it was
+        torch.where(takes, torch.addcmul(tok, tok, stored, value=-1), self._waiting, out=self._waiting)
+        self._choose(logits, takes, stored)
         return logits
 
     @torch.no_grad()
@@ -290,7 +291,7 @@ class BatchDecoder(LayerStack):
         parents = [s // samples * samples if s < n else s for s in range(self.n_seq)]
         self.fork(parents)
         self.rows[:n] = 1
-        self._choose(first, self.rows, self.rows)
+        self._choose(first, self.rows > 0, self.rows)
         del first
         out = torch.empty(n_new, n, dtype=torch.int64, device=dev)
         probs = torch.empty(n_new, n, device=dev)
