@@ -93,8 +93,10 @@ class BatchDecoder(LayerStack):
     def set_sampling(self, temperature: Setting = 0.0, top_k: Setting = 0, top_p: Setting = 1.0,
                      min_p: Setting = 0.0, seed: int = 0, stop: Optional[int] = None) -> None:
         """How the next tokens are chosen (``sampling.sample``): values for all sequences or one for
-        each.  The random numbers follow from ``seed``.  A sequence whose token is ``stop`` rests
-        from then on.  Steps captured before read these settings too, but for a ``stop`` where they
+        each.  A sequence whose token is ``stop`` rests from then on.  The random numbers follow from
+        ``seed``, one for each position of each sequence: the same seed gives the same ones again,
+        also to another prompt that takes a sequence's place, and another seed gives all sequences
+        new ones.  Steps captured before read these settings too, but for a ``stop`` where they
         were captured without any."""
         self._set_sampling(temperature, top_k, top_p, min_p, seed, stop)
         self._chosen = dict(temperature=self._temperature.clone(), top_k=self._top_k.clone(),
@@ -125,8 +127,7 @@ class BatchDecoder(LayerStack):
 
     def _choose(self, logits: torch.Tensor, takes: torch.Tensor, stored: torch.Tensor) -> None:
         """The tokens after the last slots of the sequences for which ``takes`` (bool), by ``logits``
-        [n_seq, vocab].  Where ``stored`` is 0 they are no draws, which ``stop``
-        could end."""
+        [n_seq, vocab].  Where ``stored`` is 0 they are no draws, which ``stop`` could end."""
         at = (self.lengths - 1).clamp_(0, self.slots - 1)
         u = self._u[at, self._seq]
         tok = torch.empty_like(self.tok)

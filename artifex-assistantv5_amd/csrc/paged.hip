@@ -242,8 +242,8 @@ __global__ __launch_bounds__(HD) void paged_load_kernel(PagedCache c, float *__r
 // ---------------------------------------------------------------------------
 // Forks.  A workgroup takes `stripe` columns of every table: it reads all of them before it writes
 // any, so that the tables may be their own output.  Pages that a sequence had before are not counted
-// again, so that a common beginning costs no atomics.  Bound: a launch; 16 tables of 66 columns over
-// 400 pages 1.9 us, in one workgroup with the counts' copy.
+// again, so that a common beginning costs no atomics.  Bound: a launch and the chain of loads, copies
+// and atomics; 16 tables of 66 columns 3.4 us, four of 14 1.9, in one workgroup with the counts' copy.
 // ---------------------------------------------------------------------------
 constexpr int kForkThreads = 1024, kForkWords = 16384;
 
@@ -295,8 +295,8 @@ __global__ __launch_bounds__(kForkThreads) void paged_fork_kernel(
 // Room for new rows.  One workgroup walks the entries (sequence, column) in order, 1024 at a
 // time: what an entry needs follows from refs, which the entries before it have brought up to
 // date, and from the entries of its own turn that hold the same page.  The n-th need takes the
-// n-th free page.  A second launch copies the pages.  Bound: the chain of barriers and loads, 4.9 us
-// for 16 sequences.
+// n-th free page.  A second launch copies the pages.  Bound: the chain of barriers and loads, 5.8 us
+// for 16 sequences, 4.9 for four.
 // ---------------------------------------------------------------------------
 constexpr int kGrowThreads = 1024, kGrowWaves = kGrowThreads / 64;
 constexpr int kGrowSeqs = 4096;
@@ -596,9 +596,11 @@ __global__ __launch_bounds__(kThreads) void paged_compact_move_kernel(
 
 hipError_t launch_paged_append(const PagedCache &c, const float *qkv, int64_t ldq, int64_t n_rows,
                                const int64_t *starts, hipStream_t s) {
-  // By blocks where the sequences' rows fill some, and there are enough of them: 3714 rows of five
-  // sequences, 8 heads of 128, a row at a time 26 us, by blocks 13; 146 rows of six, 4 heads of 64,
-  // 3.6 and 4.8.
+  // By blocks where the sequences' rows fill some, and there are enough of them (us, a row at a time /
+  // by blocks): 8 heads of 128, four sequences of 64, 128 and 512 rows 4.9 / 5.5, 6.8 / 5.9 and 16 / 8.5,
+  // 3714 rows of five 26 / 13; 4 heads of 64, four of 128, 256 and 512 rows 4.0 / 4.4, 4.8 / 4.4 and
+  // 6.7 / 5.0; one head of 256, where the border is lower, four of 256 and 512 5.0 / 5.6 and 7.0 / 5.8.
+  // Many sequences of one block each are the rule's worst: 32 of 16 rows, 8 heads of 128, 7.1 / 9.0.
   if (n_rows >= 16 * (int64_t)c.n_seq && n_rows * c.nkv >= 4096) {
     const dim3 blocks((unsigned)(n_rows / 16 + 2 * c.n_seq), (unsigned)((2 * c.nkv + 3) / 4));
     PAGED_DISPATCH(c, hipLaunchKernelGGL((paged_append_blocks_kernel<HD, BF>), blocks, dim3(kThreads),

@@ -41,8 +41,10 @@ __device__ __forceinline__ int32_t page_of(const PagedCache &c, int64_t s, int s
 }
 
 // How the units of a list are cut: `per` for each workgroup, `n` of them at most S.  Every workgroup
-// of the call gets about the same number, whatever the sequences' lengths: all lists' units over
-// `wgs` workgroups, in whole turns of a workgroup's W waves, and no fewer than eight.
+// of the call gets about the same number: all lists' units over `wgs` workgroups, in whole turns of a
+// workgroup's W waves, and no fewer than eight.  But for S, which goes by the number of lists (`plan`):
+// a sequence much longer than the others is on S workgroups a list, each with more than the others'.
+// 130000 slots beside 31 sequences of 300 take 174 us, alone 97.
 constexpr int kLeastUnits = 8;
 struct Cut {
   int S, wgs, W;
@@ -121,7 +123,8 @@ __device__ __forceinline__ float4_t mfma(uint4 a, uint4 b, float4_t c, std::true
                                                  __builtin_bit_cast(bhalf8_t, b), c, 0, 0, 0);
 }
 
-// 16 bytes; STREAM: past the caches, since no other wave reads them.
+// 16 bytes; STREAM: past the caches (`plan` says when).  No other wave of the list reads them; those of
+// sequences that share the page do.
 template <bool STREAM>
 __device__ __forceinline__ uint4 load16(const uint16_t *p) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -195,7 +198,7 @@ __device__ __forceinline__ float all_parts(float v) {
 // Bound: HBM (4 head_dim bytes per slot and list) where lists are long: 130000 slots of 8 lists, 128
 // channels, 533 MB: 89 us, 6.0 TB/s (a 1 GB copy reads and writes 4.7 together); 32 sequences of 37 ..
 // 8191 slots, 475 MB: 98, 4.8 TB/s, the uneven ends of their lists.  A short list waits for its chain of
-// loads (length, page, rows): 300 slots 8.6 us.
+// loads (length, page, rows): 300 slots 9.0 us.
 template <int HD, bool BF, int C, int W, int WPS, bool STREAM>
 __global__ __launch_bounds__(64 * W, WPS) void paged_attention_kernel(PagedCache c, PagedAttn a,
                                                                       float *__restrict__ rec,
@@ -565,9 +568,10 @@ Plan plan(int page, int64_t columns, int n_seq, int nkv, int hd) {
   Plan p;
   p.lists = (int64_t)n_seq * nkv;
   const int64_t units = (columns * page + kUnit - 1) / kUnit;
-  // a list of two turns is not cut: one launch, and nothing to join
+  // a list of two turns is not cut: one launch, and nothing to join.  What counts is what a table holds,
+  // which the host knows: 300 slots 8.9 us of a table of 512 slots, 11.3 of one of 2048.
   const bool whole = units <= 16;
-  // (300 slots: 4 waves and the join's launch 7.8 + 2.9 us, 8 waves 8.6)
+  // (300 slots: 4 waves and the join's launch 7.8 + 2.9 us, 8 waves 9.0)
   p.cut.W = whole && units > 8 ? 8 : 4;
   // Workgroups at a time, as many as fit (us, 32 sequences of 37 .. 8191 slots / 32 of 4000 / 130000
   // slots): 512 109 / 101 / 99, 768 104 / 104 / 100, 1024 105 / 106 / 104, 1536 106 / 116 / 115.
@@ -576,9 +580,12 @@ Plan plan(int page, int64_t columns, int n_seq, int nkv, int hd) {
   // sequences of different lengths: up to four times the workgroups that equal ones would take
   const int64_t want = (4 * p.cut.wgs + p.lists - 1) / p.lists;
   p.cut.S = (int)(want < most ? want : most);
-  // Tables of more than the last cache holds (256 MB) are read past the caches: 130000 slots of 8
-  // lists 110 us, so 101, 32 sequences of 4000 112 and 102, a list of 6000 slots, whose pages the
-  // caches still hold from the call before, 11.6 and 13.9.
+  // Tables of more than the last cache holds (256 MB) are read past the caches (us, 8 lists a sequence,
+  // cached / past them): 130000 slots 101 / 93, 32 sequences of 4000 103 / 96.  What the caches still
+  // hold from the call before is read faster from there: a list of 6000 slots 11.6 / 13.9.  That goes
+  // for large tables with little in them, and with pages that sequences share, too, which the rule does
+  // not see: 32 sequences of 300 slots 17.8 / 21.1, 16 and 32 of 8100 of which 8000 are shared 50 / 61
+  // and 85 / 109.
   p.stream = p.lists * columns * page * hd * 4 > (int64_t)256 << 20;
   return p;
 }

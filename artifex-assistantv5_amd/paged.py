@@ -76,8 +76,9 @@ def _pool(kv: torch.Tensor, layers: bool = False):
     return device, n_layers, n_pages, n_kv, page, hd
 
 
-# The calls below are made straight from the tensors where these fit (``_native.direct``); what
-# follows there says what does not, and makes those calls whose device is not the current one.
+# The calls below are made straight from the tensors where these fit (``_native.direct``, which raises
+# if a call fails); what follows there says what does not fit, and makes those calls whose device is
+# not the current one.
 def _array(name: str, t: torch.Tensor, dtype, shape, device: int) -> int:
     if (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == device):
         return t.data_ptr()
