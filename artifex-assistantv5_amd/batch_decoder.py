@@ -64,11 +64,11 @@ class BatchDecoder(LayerStack):
                  n_pages: Optional[int] = None, page: int = 16,
                  dtype: torch.dtype = torch.float16, device="cuda"):
         columns, n_pages = check_batch(cfg, n_seq, n_pages, page, dtype)
-        dev = self.device = torch.device(device)
         self.cfg, self.w, self.n_seq = cfg, weights, n_seq
         self.slots = columns * page
-        self.kv = paged.empty(n_pages, cfg.n_kv_heads, cfg.head_dim, page, dtype, dev,
+        self.kv = paged.empty(n_pages, cfg.n_kv_heads, cfg.head_dim, page, dtype, device,
                               n_layers=cfg.n_layers)
+        dev = self.device = self.kv.device  # with its index: what is current may change
         self.tables, self.lengths, self.refs = paged.empty_tables(n_seq, columns, n_pages, dev)
         i64 = lambda n: torch.zeros(n, dtype=torch.int64, device=dev)  # noqa: E731
         self.rows, self.room, self.tok = i64(n_seq), i64(n_seq), i64(n_seq)
@@ -84,7 +84,7 @@ class BatchDecoder(LayerStack):
         self.w_draw = sampling.workspace(n_seq, cfg.vocab, dev)
         self.probs = torch.zeros(n_seq, device=dev)
         self._seq = torch.arange(n_seq, device=dev)
-        self._logits = None
+        self._logits = self._side = None
         self._prompt = None                 # the sequence whose prompt runs; None: a step
         self._set_sampling()
         self._chosen: dict = {}             # set_sampling's arguments
@@ -244,16 +244,18 @@ class BatchDecoder(LayerStack):
     @torch.no_grad()
     def capture(self) -> "torch.cuda.CUDAGraph":
         """A HIP graph of ``step``; the cache and the sequences are as they were before."""
-        s = torch.cuda.Stream(device=self.device)
-        s.wait_stream(torch.cuda.current_stream(self.device))
+        if self._side is None:  # of this device, whichever is current or was captured on first
+            self._side = torch.cuda.Stream(device=self.device)
+        s, now = self._side, torch.cuda.current_stream(self.device)
+        s.wait_stream(now)
         rows = self.rows.clone()
         with torch.cuda.stream(s):
             self.rows.zero_()
             self.step()                    # warm-up outside the graph, in which no sequence takes part
             self.rows.copy_(rows)
-        torch.cuda.current_stream(self.device).wait_stream(s)
+        now.wait_stream(s)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with torch.cuda.device(self.device), torch.cuda.graph(graph, stream=s):
             self._logits = self.step()
         return graph
 

@@ -255,3 +255,53 @@ def test_refuses_what_no_call_would_take(batch, monkeypatch, over, args, match):
 def test_takes_the_largest(batch):
     cfg = _config(n_heads=16, n_kv_heads=15 + 1, max_seq=1 << 20, vocab=1 << 20)
     assert batch.check_batch(cfg, 4095, 8192, 256, torch.float16) == (1 << 12, 8192)
+
+
+def test_captures_on_its_own_device(batch, monkeypatch):
+    """Another device is current, and the process captured there first: the step runs on a stream of
+    the decoder's device both times."""
+    import contextlib
+
+    current = [0]
+    streams = {}                              # the current stream of each device
+
+    class Stream:
+        def __init__(self, device=None):
+            self.device = torch.device(device if device is not None else f"cuda:{current[0]}")
+
+        def wait_stream(self, other):
+            assert other.device == self.device
+
+    @contextlib.contextmanager
+    def on_device(d):
+        before, current[0] = current[0], torch.device(d).index
+        yield
+        current[0] = before
+
+    @contextlib.contextmanager
+    def on_stream(s):
+        with on_device(s.device):
+            before = streams.get(s.device)
+            streams[s.device] = s
+            yield
+            streams[s.device] = before
+
+    default = Stream("cuda:0")                # what a first capture on device 0 left
+
+    @contextlib.contextmanager
+    def graph(g, stream=None):
+        s = default if stream is None else stream
+        with on_stream(s):
+            s.captures = True
+            yield
+            s.captures = False
+
+    m = Host(batch, monkeypatch, 2, 10)
+    m.device = torch.device("cuda:1")
+    for name, f in dict(Stream=Stream, device=on_device, stream=on_stream, graph=graph, CUDAGraph=object,
+                        current_stream=lambda d: streams.get(torch.device(d)) or Stream(d)).items():
+        monkeypatch.setattr(torch.cuda, name, f)
+    seen = []
+    m.step = lambda: seen.append((current[0], getattr(streams.get(m.device), "captures", False)))
+    m.capture()
+    assert seen == [(1, False), (1, True)] and current == [0]

@@ -489,3 +489,10 @@ def test_draws_are_the_definitions(dec, batch, dtype):
         check(logits, m.tok, m.probs, m.lengths.tolist(), 11 if step < 9 else 12)
         drawn.update(m.tok.tolist())
     assert len(drawn) > 30
+
+
+def test_the_device_has_its_index(dec, batch):
+    """A decoder made on "cuda" stays on the device that was current then."""
+    cfg, w = _model(dec)
+    m = batch.BatchDecoder(cfg, w, 2, device="cuda")
+    assert m.device == torch.device("cuda", torch.cuda.current_device())
